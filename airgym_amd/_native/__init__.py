@@ -27,6 +27,8 @@ AG_FLAG_FIX_TIME_OUTS = 1 << 2
 AG_FLAG_STAGGER_PHASE = 1 << 3
 AG_NUM_REWARD_TERMS = 11
 
+AG_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # ag_dtype
+
 AG_ERR_UNKNOWN_TASK = -2
 AG_ERR_UNKNOWN_CTL = -3
 AG_ERR_UNSUPPORTED = -6
@@ -126,6 +128,48 @@ class AgLossEpilogue(ctypes.Structure):
         ("e_clip", ctypes.c_float), ("critic_coef", ctypes.c_float), ("bounds_loss_coef", ctypes.c_float),
         ("clip_value", ctypes.c_int), ("bound_type", ctypes.c_int), ("tile_rows", ctypes.c_int), ("partial_tiles", ctypes.c_int),
     ]
+
+
+class AgConvArgs(ctypes.Structure):
+    """ag_conv_args (include/airgym_hip.h)"""
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [(n, ctypes.c_int) for n in ("dtype", "B", "T", "D", "W", "silu")] + \
+        [(n, ctypes.c_void_p) for n in ("x_dev", "weight_dev", "bias_dev", "state_in_dev", "lengths_dev", "resets_dev")] + \
+        [(n, ctypes.c_longlong) for n in ("x_sb", "x_st", "r_sb", "r_st")] + [(n, ctypes.c_void_p) for n in ("y_dev", "state_out_dev")]
+
+
+class AgConvGrads(ctypes.Structure):
+    """ag_conv_grads (include/airgym_hip.h)"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("dy_dev", ctypes.c_void_p), ("dstate_out_dev", ctypes.c_void_p),
+                ("dy_sb", ctypes.c_longlong), ("dy_st", ctypes.c_longlong)] + \
+        [(n, ctypes.c_void_p) for n in ("dx_dev", "dweight_dev", "dbias_dev", "dstate_dev", "workspace_dev")] + \
+        [("workspace_bytes", ctypes.c_longlong)]
+
+
+class AgScanArgs(ctypes.Structure):
+    """ag_scan_args (include/airgym_hip.h)"""
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [(n, ctypes.c_int) for n in ("dtype", "B", "T", "D", "N", "G", "softplus")] + \
+        [(n, ctypes.c_void_p) for n in ("u_dev", "delta_dev", "z_dev", "Bm_dev", "Cm_dev", "A_dev", "Dskip_dev", "delta_bias_dev",
+                                        "state_in_dev", "lengths_dev", "resets_dev")] + \
+        [(n, ctypes.c_longlong) for n in ("u_sb", "u_st", "delta_sb", "delta_st", "z_sb", "z_st", "b_sb", "b_st", "b_sg", "c_sb", "c_st",
+                                          "c_sg", "r_sb", "r_st")] + \
+        [(n, ctypes.c_void_p) for n in ("out_dev", "state_out_dev", "ckpt_dev", "workspace_dev")] + [("workspace_bytes", ctypes.c_longlong)]
+
+
+class AgScanGrads(ctypes.Structure):
+    """ag_scan_grads (include/airgym_hip.h)"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("dout_dev", ctypes.c_void_p), ("dout_sb", ctypes.c_longlong),
+                ("dout_st", ctypes.c_longlong)] + \
+        [(n, ctypes.c_void_p) for n in ("dstate_out_dev", "du_dev", "ddelta_dev", "dz_dev", "dBm_dev", "dCm_dev", "dA_dev", "dDskip_dev",
+                                        "ddelta_bias_dev", "dstate_in_dev", "workspace_dev")] + [("workspace_bytes", ctypes.c_longlong)]
+
+
+class AgTokenLossArgs(ctypes.Structure):
+    """ag_token_loss_args (include/airgym_hip.h)"""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("dtype", ctypes.c_int), ("V", ctypes.c_int)] + \
+        [(n, ctypes.c_longlong) for n in ("R0", "R1", "s0", "s1")] + \
+        [(n, ctypes.c_void_p) for n in ("logits_dev", "actions_dev", "old_logp_dev", "advantages_dev", "ref_logp_dev", "mask_dev")] + \
+        [(n, ctypes.c_float) for n in ("e_clip", "kl_coef", "entropy_coef")] + \
+        [(n, ctypes.c_void_p) for n in ("stats_dev", "dlogits_dev", "workspace_dev")] + [("workspace_bytes", ctypes.c_longlong)]
 
 
 class AgInputLayerArgs(ctypes.Structure):
@@ -280,6 +324,19 @@ SYMBOLS = [
     ("ag_ppo_loss_max_blocks", ctypes.c_int, []),
     ("ag_ppo_loss", ctypes.c_int, [_P] * 9 + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                    ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, ctypes.POINTER(ctypes.c_int), _P]),
+    ("ag_causal_conv_fwd", ctypes.c_int, [ctypes.POINTER(AgConvArgs), _P]),
+    ("ag_causal_conv_workspace_bytes", ctypes.c_longlong, [ctypes.c_int] * 4),
+    ("ag_causal_conv_bwd", ctypes.c_int, [ctypes.POINTER(AgConvArgs), ctypes.POINTER(AgConvGrads), _P]),
+    ("ag_causal_conv_step", ctypes.c_int, [_P, ctypes.c_longlong, _P, _P, _P, _P, _P] + [ctypes.c_int] * 5 + [_P]),
+    ("ag_selective_scan_ckpt_floats", ctypes.c_longlong, [ctypes.c_int] * 4),
+    ("ag_selective_scan_workspace_bytes", ctypes.c_longlong, [ctypes.c_int] * 6),
+    ("ag_selective_scan_fwd", ctypes.c_int, [ctypes.POINTER(AgScanArgs), _P]),
+    ("ag_selective_scan_bwd", ctypes.c_int, [ctypes.POINTER(AgScanArgs), ctypes.POINTER(AgScanGrads), _P]),
+    ("ag_selective_scan_step", ctypes.c_int, [ctypes.POINTER(AgScanArgs), _P]),
+    ("ag_token_policy_loss_workspace_bytes", ctypes.c_longlong, [ctypes.c_longlong, ctypes.c_int]),
+    ("ag_token_policy_loss", ctypes.c_int, [ctypes.POINTER(AgTokenLossArgs), _P]),
+    ("ag_scale_by", ctypes.c_int, [_P, ctypes.c_longlong, ctypes.c_int, _P, _P]),
+    ("ag_token_logp", ctypes.c_int, [_P] + [ctypes.c_longlong] * 4 + [ctypes.c_int, ctypes.c_int, _P, _P, _P, _P]),
 ]
 
 # include/airgym_hip_debug.h: present in the experiments build only

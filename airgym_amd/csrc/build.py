@@ -1,5 +1,5 @@
 #!/usr/bin/env python3
-"""Build libairgym_hip.so for gfx950 with hipcc (no cmake; 24 translation units compiled in parallel).
+"""Build libairgym_hip.so for gfx950 with hipcc (no cmake; 27 translation units compiled in parallel).
 
     python airgym_amd/csrc/build.py [--force] [--jobs N] [--experiments]
 
@@ -23,8 +23,13 @@ ARCH = "gfx950"
 
 HIPCC = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
 COMMON = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-fno-gpu-rdc", "-Wall", "-Wno-unused-function"]
+# No v_pk_{add,mul,fma}_f32 in the sequence operators: some forms of them have returned wrong values now and then on this part, with
+# no error and not reliably in tests.  The older units keep their instruction selection: a seeded training run of theirs is chaotic
+# in the last bit, and their learning regressions are gates on such runs.  (The host pass does not know the feature and says so.)
+UNPACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+HOST_PASS_NOTE = "'-packed-fp32-ops' is not a recognized feature for this target"
 
-HEADERS = ["env_math.hpp", "planning_math.hpp", "kernel_args.hpp", "rollout_math.hpp", "handle.hpp", "split_common.hpp", "ppo_loss_math.hpp",
+HEADERS = ["env_math.hpp", "planning_math.hpp", "kernel_args.hpp", "rollout_math.hpp", "handle.hpp", "split_common.hpp", "ppo_loss_math.hpp", "seq_common.hpp",
            os.path.join("..", "..", "include", "airgym_hip.h")]
 
 
@@ -56,6 +61,8 @@ def units(experiments=False):
         # rolled and the tiles go to scratch (576 B per lane, 186 us instead of ~75 at M = 65 536) - hence the raised threshold
         flags = ["-ffp-contract=on"] if name == "rollout_kernels" else (["-mllvm", "-pragma-unroll-threshold=100000"] if name == "mlp_chain" else [])
         out.append((os.path.join(od, name + ".o"), name + ".hip", flags + list(x)))
+    for name in ("causal_conv", "selective_scan", "policy_loss"):
+        out.append((os.path.join(od, name + ".o"), name + ".hip", UNPACKED_FP32 + list(x)))
     # mixed_precision: the three matrix-core sources once more with ONE bf16 plane per operand (one MFMA per product, f32
     # accumulate); their compute entry points are exported with the suffix _bf16 (split_common.hpp)
     for name in ("split_gemm", "split_wgrad", "mlp_chain", "first_layer"):
@@ -69,7 +76,8 @@ def units(experiments=False):
 def compile_one(obj, src, defs, extra):
     cmd = COMMON + extra + defs + ["-c", os.path.join(HERE, src), "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
-    return obj, r.returncode, (r.stdout + r.stderr).strip(), " ".join(cmd)
+    log = "\n".join(line for line in (r.stdout + r.stderr).splitlines() if HOST_PASS_NOTE not in line)
+    return obj, r.returncode, log.strip(), " ".join(cmd)
 
 
 def build(force=False, jobs=None, extra=(), verbose=True, experiments=False, tag=None):

@@ -1,0 +1,68 @@
+// seq_common.hpp - element types and scalar functions shared by the sequence operators (causal_conv.hip, selective_scan.hip,
+// policy_loss.hip).  Activations come in float32, bfloat16 or float16; every product and sum is formed in float32 and rounded
+// once, to nearest, where a result is stored in its type.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/airgym_hip.h"
+
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+typedef _Float16 f16_t;
+typedef __bf16 bf16_t;
+
+template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
+template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }
+
+// N consecutive elements moved with one load / store when the address allows it (the caller has checked that it is aligned)
+template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp
+__device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }       // v_log_f32: 1 ulp
+__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }        // v_rcp_f32: 1 ulp
+__device__ __forceinline__ float exp_hw(float x) { return exp2_hw(x * kLog2e); }
+__device__ __forceinline__ float sigmoid(float x) { return rcp_hw(1.0f + exp_hw(-x)); }
+
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in [0, 1].  log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the odd series up to
+// s^15 leaves (1/9)^8 / 17 < 2e-9, and - unlike log(1 + e) - it keeps its RELATIVE accuracy where e is small (steps of 1e-3 and less
+// are what the scan's time step usually is).
+__device__ __forceinline__ float softplus(float x) {
+    const float e = exp_hw(-__builtin_fabsf(x));
+    const float s = e * rcp_hw(2.0f + e), q = s * s;
+    float p = 2.0f / 15.0f;
+    p = __builtin_fmaf(p, q, 2.0f / 13.0f);
+    p = __builtin_fmaf(p, q, 2.0f / 11.0f);
+    p = __builtin_fmaf(p, q, 2.0f / 9.0f);
+    p = __builtin_fmaf(p, q, 2.0f / 7.0f);
+    p = __builtin_fmaf(p, q, 2.0f / 5.0f);
+    p = __builtin_fmaf(p, q, 2.0f / 3.0f);
+    p = __builtin_fmaf(p, q, 2.0f);
+    return __builtin_fmaf(p, s, fmaxf(x, 0.0f));
+}
+
+// steps of sequence b that count: all T, or its length clamped to what the buffers hold
+__device__ __forceinline__ int seq_len(const int* lengths, int b, int T) {
+    if (!lengths) return T;
+    const int n = lengths[b];
+    return n < 0 ? 0 : (n > T ? T : n);
+}
+
+inline int seq_status() { return hipGetLastError() == hipSuccess ? AG_OK : AG_ERR_HIP; }
+
+}  // namespace
+
+// run CALL with `T` bound to the element type of an ag_dtype; AG_ERR_UNSUPPORTED for any other value
+#define AG_FOR_DTYPE(dtype, CALL)                              \
+    do {                                                       \
+        switch (dtype) {                                       \
+            case AG_F32: { using T = float; CALL; } break;     \
+            case AG_BF16: { using T = bf16_t; CALL; } break;   \
+            case AG_F16: { using T = f16_t; CALL; } break;     \
+            default: return AG_ERR_UNSUPPORTED;                \
+        }                                                      \
+    } while (0)

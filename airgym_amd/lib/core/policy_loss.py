@@ -1,0 +1,121 @@
+"""Clipped policy loss with a KL term over rows of logits (csrc/policy_loss.hip): what `fused_ppo_loss` (fused_loss.py) is to a
+Gaussian head, for a policy that answers with a choice - a discrete head, a token of a vocabulary.
+
+    lp = log softmax(logits)[action]    r = exp(lp - old_logp)    d = ref_logp - lp
+    row = max(-A r, -A clip(r, 1 - e_clip, 1 + e_clip)) + kl_coef (exp(d) - d - 1) - entropy_coef H
+
+averaged over the rows that `mask` counts.  exp(d) - d - 1 is the non-negative estimate of KL(policy || reference) from the action
+taken.  One pass writes the loss and its gradient: a forward under autograd already holds d loss / d logits, the backward only scales
+it (by nothing at all if the loss is the graph's root)."""
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from airgym_amd import _native as N
+from airgym_amd.lib.core.native_call import activations, flags_of, on_device_of, ptr, require, stream_of
+
+STATS = ("policy_loss", "kl", "entropy", "old_kl", "clip_frac", "rows")
+
+
+def _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, want_grad):
+    lib = N.load()
+    r0, r1, v = logits.shape
+    stats = torch.empty(8, dtype=torch.float32, device=logits.device)
+    grad = torch.empty(r0, r1, v, dtype=logits.dtype, device=logits.device) if want_grad else None
+    n = lib.ag_token_policy_loss_workspace_bytes(r0 * r1, v)
+    ws = torch.empty(n, dtype=torch.uint8, device=logits.device)
+    a = N.AgTokenLossArgs(ctypes.sizeof(N.AgTokenLossArgs), N.AG_DTYPES[logits.dtype], v, r0, r1, logits.stride(0), logits.stride(1),
+                          logits.data_ptr(), actions.data_ptr(), old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(mask),
+                          *coefs, stats.data_ptr(), ptr(grad), ws.data_ptr(), n)
+    with on_device_of(logits):
+        N.check(lib.ag_token_policy_loss(ctypes.byref(a), stream_of(logits)), "ag_token_policy_loss")
+    return stats, grad
+
+
+class _TokenPolicyLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, coefs):
+        stats, grad = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, ctx.needs_input_grad[0])
+        ctx.save_for_backward(logits, actions, old_logp, advantages, ref_logp, mask)
+        ctx.coefs, ctx.grad = coefs, grad
+        loss, rest = stats[0], stats[1:7]
+        ctx.mark_non_differentiable(rest)
+        return loss, rest
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss, _):
+        saved = ctx.saved_tensors
+        # the gradient is handed over, not kept: autograd may go on to add to it in place.  A second pass over a retained graph forms
+        # it again.
+        grad, ctx.grad = ctx.grad, None
+        if grad is None:
+            _, grad = _launch(*saved, ctx.coefs, True)
+        scale = dloss.to(torch.float32).contiguous()
+        with on_device_of(grad):
+            N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], scale.data_ptr(), stream_of(grad)),
+                    "ag_scale_by")
+        return grad, None, None, None, None, None, None
+
+
+def _rows(logits, actions):
+    """logits as [R0, R1, V] (a view where their strides allow), the leading shape and the actions as dense int64."""
+    require(isinstance(logits, torch.Tensor) and logits.dim() >= 2, "logits: expected [..., V]")
+    lead, v = tuple(logits.shape[:-1]), logits.shape[-1]
+    require(v >= 1, "logits: no choices")
+    logits = activations("logits", logits, logits.shape)
+    require(isinstance(actions, torch.Tensor) and actions.dtype == torch.int64 and tuple(actions.shape) == lead
+            and actions.device == logits.device, f"actions: expected int64 {list(lead)} on {logits.device}")
+    if len(lead) == 1:
+        logits = logits.unsqueeze(0)
+    elif len(lead) > 2:
+        logits = logits.reshape(-1, lead[-1], v)
+    return logits, lead, actions.contiguous()
+
+
+def _per_row(name, t, lead, device):
+    if t is None:
+        return None
+    require(isinstance(t, torch.Tensor) and t.dtype == torch.float32 and tuple(t.shape) == lead and t.device == device,
+            f"{name}: expected float32 {list(lead)} on {device}")
+    require(not (torch.is_grad_enabled() and t.requires_grad), f"{name}: the loss has gradients for the logits only; detach it")
+    return t.contiguous()
+
+
+def policy_loss(logits, actions, old_logp, advantages, *, ref_logp=None, mask=None, e_clip=0.2, kl_coef=0.0, entropy_coef=0.0):
+    """logits [..., V] (float32, bfloat16 or float16), actions int64 [...], old_logp, advantages and ref_logp float32 [...], mask bool
+    or uint8 [...] (None: every row counts) -> (loss, stats), float32: the loss to call backward() on and
+    [policy loss, KL term, entropy, KL of the old policy, fraction of clipped rows, rows counted], each a mean over the rows counted.
+
+    Rows that do not count are not read: whatever their logits, actions and numbers are, they add nothing and get a gradient of zero.
+    If no row counts, loss, statistics and gradients are zero.  Logits of -inf are choices that are not available.  An action outside
+    [0, V) in a row that counts gives NaN."""
+    logits, lead, actions = _rows(logits, actions)
+    dev = logits.device
+    old_logp, advantages, ref_logp = (_per_row(n, t, lead, dev) for n, t in (("old_logp", old_logp), ("advantages", advantages),
+                                                                              ("ref_logp", ref_logp)))
+    require(old_logp is not None and advantages is not None, "old_logp and advantages are needed")
+    mask = flags_of("mask", mask, lead, dev)
+    mask = None if mask is None else mask.contiguous()
+    require(e_clip >= 0.0, f"e_clip: {e_clip} is negative")
+    require(ref_logp is not None or kl_coef == 0.0, "kl_coef: the KL term needs ref_logp")
+    if logits.numel() == 0:
+        return logits.sum().float(), torch.zeros(6, device=dev)
+    return _TokenPolicyLoss.apply(logits, actions, old_logp, advantages, ref_logp, mask, (float(e_clip), float(kl_coef), float(entropy_coef)))
+
+
+def action_logp(logits, actions):
+    """log softmax(logits)[action] and the entropy of every row, float32 [...]: what a rollout stores as old_logp and what a reference
+    policy's logits give as ref_logp.  No gradients.  An action outside [0, V) gives NaN."""
+    require(not (torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad),
+            "action_logp has no backward pass: detach the logits (policy_loss trains)")
+    logits, lead, actions = _rows(logits, actions)
+    logp = torch.empty(lead, dtype=torch.float32, device=logits.device)
+    entropy = torch.empty_like(logp)
+    if logits.numel():
+        r0, r1, v = logits.shape
+        with on_device_of(logits):
+            N.check(N.load().ag_token_logp(logits.data_ptr(), r0, r1, logits.stride(0), logits.stride(1), v, N.AG_DTYPES[logits.dtype],
+                                           actions.data_ptr(), logp.data_ptr(), entropy.data_ptr(), stream_of(logits)), "ag_token_logp")
+    return logp, entropy

@@ -1,0 +1,152 @@
+"""Selective state space scan on the HIP kernels of csrc/selective_scan.hip, for sequences and for single steps.
+
+    dt = softplus(delta + delta_bias)
+    h[b, d, n] <- exp(dt[d] A[d, n]) h[b, d, n] + dt[d] B[n] u[d]        y[d] = sum_n C[n] h[d, n] + D[d] u[d]
+    out = y z sigmoid(z)                                                  (y without z)
+
+The state before step 0 is `initial_state` (zeros if None); `resets[b, t]` clears it before step t (an episode ended), `lengths[b]` is
+where a padded sequence ends: later steps give zeros, get no gradient and leave the state alone."""
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from airgym_amd import _native as N
+from airgym_amd.lib.core.native_call import (activations, flags_of, in_place_state, lengths_of, no_gradient, on_device_of, parameter, ptr,
+                                             require, stream_of)
+
+MAX_STATES = 32
+
+
+def _fill(u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus):
+    """The argument block of sequences [B, T, ...]."""
+    b, T, d = u.shape
+    a = N.AgScanArgs(ctypes.sizeof(N.AgScanArgs), N.AG_DTYPES[u.dtype], b, T, d, A.shape[1], B.shape[2], softplus, u.data_ptr(),
+                     delta.data_ptr(), ptr(z), B.data_ptr(), C.data_ptr(), A.data_ptr(), ptr(D), ptr(bias), ptr(state), ptr(lengths),
+                     ptr(resets), u.stride(0), u.stride(1), delta.stride(0), delta.stride(1))
+    if z is not None:
+        a.z_sb, a.z_st = z.stride(0), z.stride(1)
+    a.b_sb, a.b_st, a.b_sg = B.stride(0), B.stride(1), B.stride(2)
+    a.c_sb, a.c_st, a.c_sg = C.stride(0), C.stride(1), C.stride(2)
+    if resets is not None:
+        a.r_sb, a.r_st = resets.stride()
+    return a
+
+
+def _workspace(n, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus, want_state):
+        lib = N.load()
+        b, T, d = u.shape
+        n = A.shape[1]
+        out = torch.empty(b, T, d, dtype=u.dtype, device=u.device)
+        last = torch.empty(b, d, n, dtype=torch.float32, device=u.device) if want_state else None
+        ckpt = None
+        if any(ctx.needs_input_grad):
+            ckpt = torch.empty(lib.ag_selective_scan_ckpt_floats(b, T, d, n), dtype=torch.float32, device=u.device)
+        bytes_ = lib.ag_selective_scan_workspace_bytes(b, T, d, n, B.shape[2], 0)
+        ws = _workspace(bytes_, u.device)
+        a = _fill(u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus)
+        a.out_dev, a.state_out_dev, a.workspace_dev, a.workspace_bytes = out.data_ptr(), ptr(last), ptr(ws), bytes_
+        a.ckpt_dev = ptr(ckpt)
+        with on_device_of(u):
+            N.check(lib.ag_selective_scan_fwd(ctypes.byref(a), stream_of(u)), "ag_selective_scan_fwd")
+        ctx.save_for_backward(u, delta, A, B, C, D, z, bias, state, lengths, resets, ckpt)
+        ctx.softplus = softplus
+        ctx.set_materialize_grads(False)
+        return out, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlast):
+        u, delta, A, B, C, D, z, bias, state, lengths, resets, ckpt = ctx.saved_tensors
+        lib = N.load()
+        b, T, d = u.shape
+        n, G = A.shape[1], B.shape[2]
+
+        def like(t):        # dense gradient of t
+            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+        dout = torch.zeros(b, T, d, dtype=u.dtype, device=u.device) if dout is None else activations("dout", dout, u.shape, u)
+        dlast = None if dlast is None else dlast.contiguous()
+        du, ddelta, dA, dB, dC, dD, dz, dbias, dstate = (like(t) for t in (u, delta, A, B, C, D, z, bias, state))
+        bytes_ = lib.ag_selective_scan_workspace_bytes(b, T, d, n, G, 1)
+        ws = _workspace(bytes_, u.device)
+        a = _fill(u, delta, A, B, C, D, z, bias, state, lengths, resets, ctx.softplus)
+        a.ckpt_dev = ptr(ckpt)
+        g = N.AgScanGrads(ctypes.sizeof(N.AgScanGrads), dout.data_ptr(), dout.stride(0), dout.stride(1), ptr(dlast), du.data_ptr(),
+                          ddelta.data_ptr(), ptr(dz), dB.data_ptr(), dC.data_ptr(), dA.data_ptr(), ptr(dD), ptr(dbias), ptr(dstate),
+                          ptr(ws), bytes_)
+        with on_device_of(u):
+            N.check(lib.ag_selective_scan_bwd(ctypes.byref(a), ctypes.byref(g), stream_of(u)), "ag_selective_scan_bwd")
+        return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate, None, None, None, None
+
+
+def _parameters(A, D, delta_bias, d, device):
+    require(isinstance(A, torch.Tensor) and A.dim() == 2, "A: expected [D, N]")
+    n = A.shape[1]
+    require(1 <= n <= MAX_STATES, f"A: 1 to {MAX_STATES} states per channel, got {n}")
+    return parameter("A", A, (d, n), device), parameter("D", D, (d,), device), parameter("delta_bias", delta_bias, (d,), device)
+
+
+def _shared(name, t, lead, n, u):
+    """B or C as [..., G, N]; [..., N] is one group."""
+    require(isinstance(t, torch.Tensor) and t.dim() in (len(lead) + 1, len(lead) + 2), f"{name}: expected {list(lead)} + [N] or [G, N]")
+    if t.dim() == len(lead) + 1:
+        t = t.unsqueeze(-2)
+    groups = t.shape[-2]
+    require(groups >= 1 and u.shape[-1] % groups == 0, f"{name}: {u.shape[-1]} channels do not split into {groups} groups")
+    return activations(name, t, (*lead, groups, n), u)
+
+
+def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_softplus=True, initial_state=None, lengths=None,
+                   resets=None, return_state=False):
+    """u, delta, z [B, T, D] and B, C [B, T, G, N] (or [B, T, N]) in one of float32, bfloat16, float16, with any batch, time and group
+    strides; A [D, N], D [D], delta_bias [D] and initial_state [B, D, N] float32; lengths int32 [B]; resets bool or uint8 [B, T].
+    G groups of D / G consecutive channels share B and C.  -> out [B, T, D], and with return_state the state [B, D, N] (float32) after
+    each sequence's last step.  Gradients reach every floating-point argument, also through the returned state."""
+    require(isinstance(u, torch.Tensor) and u.dim() == 3, "u: expected [B, T, D]")
+    b, T, d = u.shape
+    u = activations("u", u, u.shape)
+    delta = activations("delta", delta, u.shape, u)
+    z = None if z is None else activations("z", z, u.shape, u)
+    A, D, delta_bias = _parameters(A, D, delta_bias, d, u.device)
+    B, C = _shared("B", B, (b, T), A.shape[1], u), _shared("C", C, (b, T), A.shape[1], u)
+    require(B.shape == C.shape, f"B and C: {tuple(B.shape)} and {tuple(C.shape)}")
+    state = parameter("initial_state", initial_state, (b, d, A.shape[1]), u.device)
+    lengths, resets = lengths_of(lengths, b, u.device), flags_of("resets", resets, (b, T), u.device)
+    if u.numel() == 0:
+        out = u.clone()
+        last = torch.zeros(b, d, A.shape[1], dtype=torch.float32, device=u.device) if state is None else state.clone()
+    else:
+        out, last = _SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, state, lengths, resets, int(bool(delta_softplus)), return_state)
+    return (out, last) if return_state else out
+
+
+def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=None, *, delta_softplus=True, resets=None):
+    """One step: u, delta, z [B, D], B, C [B, G, N] (or [B, N]) -> out [B, D]; state [B, D, N] (float32, contiguous) is moved on in
+    place.  resets [B] clears a row's state first.  No gradients."""
+    require(isinstance(u, torch.Tensor) and u.dim() == 2, "u: expected [B, D]")
+    b, d = u.shape
+    no_gradient("selective_scan_step", u, delta, A, B, C, D, z, delta_bias)
+    u = activations("u", u, u.shape)
+    delta = activations("delta", delta, u.shape, u)
+    z = None if z is None else activations("z", z, u.shape, u)
+    A, D, delta_bias = _parameters(A, D, delta_bias, d, u.device)
+    B, C = _shared("B", B, (b,), A.shape[1], u), _shared("C", C, (b,), A.shape[1], u)
+    require(B.shape == C.shape, f"B and C: {tuple(B.shape)} and {tuple(C.shape)}")
+    state = in_place_state("state", state, (b, d, A.shape[1]), torch.float32, u.device)
+    resets = flags_of("resets", resets, (b,), u.device)
+    out = torch.empty(b, d, dtype=u.dtype, device=u.device)
+    if u.numel() == 0:
+        return out
+    one = lambda t: None if t is None else t.unsqueeze(1)      # noqa: E731
+    a = _fill(one(u), one(delta), A, one(B), one(C), D, one(z), delta_bias, state, None, one(resets), int(bool(delta_softplus)))
+    a.out_dev, a.state_out_dev = out.data_ptr(), state.data_ptr()
+    with on_device_of(u):
+        N.check(N.load().ag_selective_scan_step(ctypes.byref(a), stream_of(u)), "ag_selective_scan_step")
+    return out

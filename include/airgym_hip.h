@@ -792,6 +792,138 @@ int ag_planning_render_now(ag_handle h);
  * encoder (lib/network/vae_image_encoder.py:34-53) re-encode only when the image changed. */
 int ag_planning_last_step_rendered(ag_handle h);
 
+/* ---- Sequence operators --------------------------------------------------------------------------------
+ * A policy with memory (short causal convolution + selective state space scan, over a horizon of steps or one step at a time)
+ * and the clipped policy loss over rows of logits.  The reference has no counterpart (its recurrent-state plumbing, 'states' in
+ * lib/agent/a2c_continuous.py:76, is never filled).
+ * Activations are float32, bfloat16 or float16 (ag_dtype); parameters, scan states and statistics are float32.  Sequences are
+ * [B, T, ...] with element strides for batch and time (the channel stride is 1), so a [T, B, ...] rollout buffer is read where it
+ * lies.  lengths_dev int32 [B] (or NULL = T everywhere; clamped to [0, T]): steps from there on are not read, their outputs and
+ * gradients are zero and they leave the state alone.  resets_dev u8 [B, T] (or NULL): a non-zero flag clears the state BEFORE that
+ * step (an episode ended there).  B, T >= 1; all pointers are device pointers on the current device. */
+typedef enum ag_dtype { AG_F32 = 0, AG_BF16 = 1, AG_F16 = 2 } ag_dtype;
+
+/* Causal depthwise convolution of W taps, 2 <= W <= 8:
+ *   p[b,t,d] = bias[d] + sum_k weight[d,k] x[b, t-W+1+k, d],  y = silu ? p sigmoid(p) : p
+ * where x before step 0 is state_in [B, W-1, D] (oldest first; NULL = zeros) and taps that lie before the last reset are zero.
+ * state_out [B, W-1, D] (or NULL): the last W-1 inputs after the sequence's last step, the next call's state_in. */
+typedef struct ag_conv_args {
+    uint32_t struct_size;              /* = sizeof(ag_conv_args), ABI guard */
+    int dtype, B, T, D, W, silu;
+    const void* x_dev;                 /* [B, T, D], strides x_sb, x_st, 1 */
+    const float* weight_dev;           /* [D, W] */
+    const float* bias_dev;             /* [D] or NULL */
+    const void* state_in_dev;          /* [B, W-1, D] or NULL */
+    const int* lengths_dev;            /* [B] or NULL */
+    const unsigned char* resets_dev;   /* [B, T], strides r_sb, r_st, or NULL */
+    long long x_sb, x_st, r_sb, r_st;
+    void* y_dev;                       /* forward: [B, T, D] contiguous */
+    void* state_out_dev;               /* forward: [B, W-1, D] or NULL */
+} ag_conv_args;
+/* Gradients given dy [B, T, D] (strides dy_sb, dy_st, 1) and, optionally, dstate_out [B, W-1, D].  The parameter gradients are summed
+ * over rows in a fixed order through workspace_dev (ag_causal_conv_workspace_bytes, 16-byte aligned).  y_dev and state_out_dev of args
+ * are not used. */
+typedef struct ag_conv_grads {
+    uint32_t struct_size;              /* = sizeof(ag_conv_grads), ABI guard */
+    const void* dy_dev;
+    const void* dstate_out_dev;        /* [B, W-1, D] or NULL */
+    long long dy_sb, dy_st;
+    void* dx_dev;                      /* [B, T, D] contiguous */
+    float* dweight_dev;                /* [D, W] */
+    float* dbias_dev;                  /* [D] or NULL */
+    void* dstate_dev;                  /* [B, W-1, D] or NULL */
+    void* workspace_dev;
+    long long workspace_bytes;
+} ag_conv_grads;
+int ag_causal_conv_fwd(const ag_conv_args* args, void* stream);
+long long ag_causal_conv_workspace_bytes(int B, int T, int D, int W);
+int ag_causal_conv_bwd(const ag_conv_args* args, const ag_conv_grads* grads, void* stream);
+/* one step for B sequences: x, y [B, D] (x rows x_sb apart), state_dev [B, W-1, D] moved on in place, resets_dev u8 [B] or NULL */
+int ag_causal_conv_step(const void* x_dev, long long x_sb, void* state_dev, const float* weight_dev, const float* bias_dev,
+                        const unsigned char* resets_dev, void* y_dev, int dtype, int B, int D, int W, int silu, void* stream);
+
+/* Selective state space scan, 1 <= N <= 32 states per channel, G groups of D / G channels that share B and C:
+ *   dt = softplus ? log(1 + exp(delta + delta_bias)) : delta + delta_bias
+ *   h[d,n] <- exp(dt[d] A[d,n]) h[d,n] + dt[d] B[g(d),n] u[d],   y[d] = sum_n C[g(d),n] h[d,n] + Dskip[d] u[d]
+ *   out = z ? y z sigmoid(z) : y
+ * ckpt_dev (training): ag_selective_scan_ckpt_floats(B, T, D, N) floats, the states the backward restarts from.
+ * workspace_dev: ag_selective_scan_workspace_bytes bytes, 16-byte aligned (NULL when that is 0). */
+typedef struct ag_scan_args {
+    uint32_t struct_size;              /* = sizeof(ag_scan_args), ABI guard */
+    int dtype, B, T, D, N, G, softplus;
+    const void *u_dev, *delta_dev, *z_dev;   /* [B, T, D]; z NULL = no gate */
+    const void *Bm_dev, *Cm_dev;       /* [B, T, G, N], strides sb, st, sg, 1 */
+    const float* A_dev;                /* [D, N] */
+    const float* Dskip_dev;            /* [D] or NULL (0) */
+    const float* delta_bias_dev;       /* [D] or NULL (0) */
+    const float* state_in_dev;         /* [B, D, N] or NULL (zeros) */
+    const int* lengths_dev;            /* [B] or NULL */
+    const unsigned char* resets_dev;   /* [B, T], strides r_sb, r_st, or NULL */
+    long long u_sb, u_st, delta_sb, delta_st, z_sb, z_st, b_sb, b_st, b_sg, c_sb, c_st, c_sg, r_sb, r_st;
+    void* out_dev;                     /* forward: [B, T, D] contiguous */
+    float* state_out_dev;              /* forward: [B, D, N] or NULL (may be state_in_dev) */
+    float* ckpt_dev;                   /* written by the forward, read by the backward; NULL: forward without backward */
+    void* workspace_dev;
+    long long workspace_bytes;
+} ag_scan_args;
+/* Gradients given dout [B, T, D] and, optionally, dstate_out [B, D, N] of the final state.  Sums over rows and channels are formed
+ * in a fixed order: the same inputs give the same bits.  out_dev, state_out_dev and the workspace of args are not used. */
+typedef struct ag_scan_grads {
+    uint32_t struct_size;              /* = sizeof(ag_scan_grads), ABI guard */
+    const void* dout_dev;              /* strides dout_sb, dout_st, 1 */
+    long long dout_sb, dout_st;
+    const float* dstate_out_dev;       /* [B, D, N] or NULL */
+    void *du_dev, *ddelta_dev;         /* [B, T, D] contiguous */
+    void* dz_dev;                      /* [B, T, D] contiguous; NULL iff z is */
+    void *dBm_dev, *dCm_dev;           /* [B, T, G, N] contiguous */
+    float* dA_dev;                     /* [D, N] */
+    float *dDskip_dev, *ddelta_bias_dev;   /* [D] or NULL */
+    float* dstate_in_dev;              /* [B, D, N] or NULL */
+    void* workspace_dev;
+    long long workspace_bytes;
+} ag_scan_grads;
+long long ag_selective_scan_ckpt_floats(int B, int T, int D, int N);
+long long ag_selective_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward);
+int ag_selective_scan_fwd(const ag_scan_args* args, void* stream);
+int ag_selective_scan_bwd(const ag_scan_args* args, const ag_scan_grads* grads, void* stream);
+/* one step for B sequences (args.T = 1; time strides, lengths, ckpt and workspace unused): state_in_dev -> state_out_dev, which may
+ * be the same buffer */
+int ag_selective_scan_step(const ag_scan_args* args, void* stream);
+
+/* Clipped policy loss with a KL term over rows of logits [R0, R1, V] (strides s0, s1, 1); R = R0 R1 rows:
+ *   lp = x[action] - log sum exp x,  r = exp(lp - old_logp),  d = ref_logp - lp,  H = -sum p log p
+ *   row loss = max(-A r, -A clip(r, 1 - e_clip, 1 + e_clip)) + kl_coef (exp(d) - d - 1) - entropy_coef H
+ * averaged over the rows with mask != 0 (mask NULL: all; none: loss 0, gradients 0).  Rows that do not count are neither read nor
+ * checked; their gradient is zero.  An action outside [0, V) in a row that counts makes that row's results NaN.
+ * Logits of -inf are choices that are not available: probability 0, gradient 0.
+ *   stats_dev [8] = {loss, policy loss, KL term, entropy, KL of the old policy to this one (r - 1 - log r), fraction of rows whose r
+ *       left the clip range, rows counted, 0}
+ *   dlogits_dev [R, V] contiguous in the logits' type, or NULL
+ *   workspace_dev: ag_token_policy_loss_workspace_bytes(R, V) bytes, 16-byte aligned. */
+typedef struct ag_token_loss_args {
+    uint32_t struct_size;              /* = sizeof(ag_token_loss_args), ABI guard */
+    int dtype, V;
+    long long R0, R1, s0, s1;
+    const void* logits_dev;
+    const long long* actions_dev;      /* int64 [R] */
+    const float* old_logp_dev;         /* [R] */
+    const float* advantages_dev;       /* [R] */
+    const float* ref_logp_dev;         /* [R] or NULL (no KL term) */
+    const unsigned char* mask_dev;     /* u8 [R] or NULL */
+    float e_clip, kl_coef, entropy_coef;
+    float* stats_dev;                  /* [8] */
+    void* dlogits_dev;
+    void* workspace_dev;
+    long long workspace_bytes;
+} ag_token_loss_args;
+long long ag_token_policy_loss_workspace_bytes(long long R, int V);
+int ag_token_policy_loss(const ag_token_loss_args* args, void* stream);
+/* x *= *scale_dev in place over n elements; a factor of exactly 1 touches nothing (the gradient of a loss that is the graph's root) */
+int ag_scale_by(void* x_dev, long long n, int dtype, const float* scale_dev, void* stream);
+/* log-probability of each row's action and the row's entropy: logp_dev, entropy_dev f32 [R] (entropy NULL: not written) */
+int ag_token_logp(const void* logits_dev, long long R0, long long R1, long long s0, long long s1, int V, int dtype,
+                  const long long* actions_dev, float* logp_dev, float* entropy_dev, void* stream);
+
 /* Benchmark / diagnostic knobs are not part of this interface nor of the shipped library: see airgym_hip_debug.h
  * (experiments build, `python airgym_amd/csrc/build.py --experiments`). */
 

@@ -1,0 +1,551 @@
+"""The sequence operators (causal convolution, selective scan, clipped policy loss) against float64 restatements.
+
+Tolerances.  u = 2^-24 is half a step of float32.  An output that is a sum along a path of n roundings differs from the exact one by
+at most n u times the sum of the terms' magnitudes; that sum is what the same function gives for the inputs' absolute values
+(`size`: its largest entry).  n is counted per operator below, with the hardware exponential, logarithm and reciprocal at 2 u each.
+An output stored in its type adds half a step of the type, finfo.eps / 2 of its value."""
+import pytest
+import torch
+
+from oracle import sequence_ref as ref
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def close(name, got, want, n, size):
+    """|got - want| <= n u size + half a step of got's type; NaN nowhere."""
+    got64 = got.detach().double().cpu()
+    assert got64.shape == want.shape, (name, got64.shape, want.shape)
+    half = 0.0 if got.dtype == torch.float32 else torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    room = n * U * float(size) + half * (want.abs() * (1 + n * U) + n * U * float(size)) + tiny
+    off = (got64 - want).abs()
+    assert torch.isfinite(got64).all(), f"{name}: not finite"
+    assert bool((off <= room).all()), f"{name}: off by {float((off - room).max() + 0):.3g} over the bound, max error {float(off.max()):.3g}, size {float(size):.3g}"
+
+
+def leaves(*tensors):
+    return [None if t is None else t.detach().double().cpu().requires_grad_() for t in tensors]
+
+
+def largest(t):
+    return 0.0 if t is None or t.numel() == 0 else float(t.abs().max())
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+# ------------------------------------------------------------------------------------------------ causal convolution
+CONV = [  # B, T, D, W, silu, lengths, resets, state
+    (1, 1, 1, 2, True, None, 0.0, False),
+    (2, 1, 5, 8, True, None, 0.0, True),
+    (3, 2, 64, 4, True, [2, 0, 1], 0.0, True),
+    (2, 24, 33, 4, True, None, 0.2, True),
+    (3, 70, 40, 4, False, [70, 33, 32], 0.0, True),
+    (2, 65, 130, 3, True, [64, 65], 0.1, True),
+    (1, 200, 16, 5, True, None, 0.02, False),
+    (4, 31, 8, 8, True, [0, 31, 7, 3], 0.3, True),
+    (2, 40, 24, 7, True, None, 1.0, True),
+    (2, 129, 512, 4, True, [129, 100], 0.0, True),
+]
+
+
+def conv_case(case, dtype, seed=0):
+    B, T, D, W, silu, lengths, p, with_state = case
+    g = gen(seed)
+    x = torch.randn(B, T, 2 * D, generator=g).to(dtype)
+    weight, bias = torch.randn(D, W, generator=g) / W ** 0.5, torch.randn(D, generator=g) * 0.1
+    state = torch.randn(B, W - 1, D, generator=g).to(dtype) if with_state else None
+    resets = (torch.rand(B, T, generator=g) < p) if p else None
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    dy, dlast = torch.randn(B, T, D, generator=g).to(dtype), torch.randn(B, W - 1, D, generator=g).to(dtype)
+    if ln is not None:
+        for b, n in enumerate(lengths):
+            x[b, n:] = float("nan")              # what stands behind a sequence's end has no effect
+            dy[b, n:] = float("nan")
+    return x[..., D:], weight, bias, state, ln, resets, dy, dlast, silu
+
+
+def conv_reference(x, weight, bias, state, ln, resets, dy, dlast, silu):
+    xs, dys = torch.nan_to_num(x.double()), torch.nan_to_num(dy.double())
+    lv = leaves(xs, weight, bias, state)
+    y, last = ref.causal_conv(lv[0], lv[1], lv[2], lv[3], silu, ln, resets)
+    live = [t for t in lv if t is not None]
+    grads = torch.autograd.grad([y, last], live, [dys, dlast.double()], allow_unused=True)
+    it = iter([torch.zeros_like(t) if v is None else v for t, v in zip(live, grads)])
+    return y.detach(), last.detach(), [None if t is None else next(it) for t in lv]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", CONV, ids=lambda c: "x".join(map(str, c[:4])))
+def test_causal_conv_and_gradients(case, dtype):
+    from airgym_amd.lib.network.causal_conv import causal_conv
+    x, weight, bias, state, ln, resets, dy, dlast, silu = conv_case(case, DTYPES[dtype])
+    y64, last64, g64 = conv_reference(x, weight, bias, state, ln, resets, dy, dlast, silu)
+    B, T, D, W = case[:4]
+    dev = [None if t is None else t.cuda().detach().requires_grad_(t.is_floating_point()) for t in (x, weight, bias, state)]
+    rs, lc = (None if t is None else t.cuda() for t in (resets, ln))
+    y, last = causal_conv(*dev[:3], activation="silu" if silu else None, initial_state=dev[3], lengths=lc, resets=rs, return_state=True)
+    assert torch.equal(last.cpu().double(), last64)                     # copies
+    # p: W products and sums and the bias, W + 1 roundings of terms whose magnitudes add up to `size`; silu: |y| <= |p|, slope < 1.1,
+    # and exp, sum, reciprocal, product at 2 + 1 + 2 + 1 u (times |p| in the exponent, |p| e^-|p| < 1)
+    size = W * largest(weight) * max(largest(torch.nan_to_num(x)), largest(state)) + largest(bias)
+    close("y", y, y64, 1.1 * (W + 1) + 8, size)
+    live = [t for t in dev if t is not None]
+    got = torch.autograd.grad([y, last], live, [dy.cuda(), dlast.cuda()])
+    got = dict(zip([n for n, t in zip(("dx", "dweight", "dbias", "dstate"), dev) if t is not None], got))
+    # dp = dy s (1 + p (1 - s)): slope of the factor < 1, magnitude < 1.1, 10 roundings and p's error; dx sums W of them (and dlast),
+    # the parameters' gradients B T of them, each weighted with an input, in any order
+    ddp = largest(torch.nan_to_num(dy)) * ((W + 1) * max(size, 1.0) + 10)
+    mdy = 1.1 * largest(torch.nan_to_num(dy))
+    xin = max(largest(torch.nan_to_num(x)), largest(state))
+    bound_dx = W * largest(weight) * (ddp + (W + 1) * mdy) + largest(dlast)
+    for name in ("dx", "dstate"):
+        if name in got:
+            close(name, got[name], g64[0 if name == "dx" else 3], 1, bound_dx)
+    rows = B * T
+    close("dweight", got["dweight"], g64[1], 1, rows * xin * (ddp + (rows + 1) * mdy))
+    close("dbias", got["dbias"], g64[2], 1, rows * (ddp + rows * mdy))
+
+
+def test_causal_conv_reads_time_major_buffers_and_flags_where_they_lie():
+    from airgym_amd.lib.network.causal_conv import causal_conv
+    g = gen(3)
+    x = torch.randn(24, 6, 40, generator=g).cuda()                      # [T, B, D]
+    resets = (torch.rand(24, 6, generator=g) < 0.2).to(torch.uint8).cuda()
+    weight = torch.randn(40, 4, generator=g).cuda()
+    a = causal_conv(x.transpose(0, 1), weight, resets=resets.t())
+    b = causal_conv(x.transpose(0, 1).contiguous(), weight, resets=resets.t().contiguous().bool())
+    assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,D,W", [(1, 1, 2), (3, 5, 8), (130, 65, 4), (7, 256, 3)])
+def test_causal_conv_steps_are_the_sequence(B, D, W, dtype):
+    """The step form does the sequence form's arithmetic: same order of the same operations, so the same bits."""
+    from airgym_amd.lib.network.causal_conv import causal_conv, causal_conv_step
+    g, T = gen(B), 9
+    x = torch.randn(B, T, D, generator=g).to(DTYPES[dtype]).cuda()
+    weight, bias = torch.randn(D, W, generator=g).cuda(), torch.randn(D, generator=g).cuda()
+    state = torch.randn(B, W - 1, D, generator=g).to(DTYPES[dtype]).cuda()
+    resets = (torch.rand(B, T, generator=g) < 0.3).cuda()
+    y, last = causal_conv(x, weight, bias, initial_state=state, resets=resets, return_state=True)
+    run = state.clone()
+    for t in range(T):
+        yt = causal_conv_step(x[:, t], run, weight, bias, resets=resets[:, t])
+        assert torch.equal(yt, y[:, t]), t
+    assert torch.equal(run, last)
+
+
+# ------------------------------------------------------------------------------------------------ selective scan
+SCAN = [  # B, T, D, N, G, lengths, resets, state, z, D, bias, softplus
+    (1, 1, 1, 1, 1, None, 0.0, False, False, False, False, True),
+    (2, 1, 65, 16, 1, None, 0.0, True, True, True, True, True),
+    (3, 2, 6, 3, 2, [0, 1, 2], 0.0, True, True, True, True, True),
+    (2, 16, 64, 16, 1, None, 0.0, True, True, True, True, True),
+    (2, 17, 70, 13, 1, [17, 16], 0.1, True, True, False, True, True),
+    (3, 24, 128, 16, 1, None, 0.1, True, True, True, True, True),
+    (2, 40, 96, 32, 3, [33, 40], 0.0, True, True, True, True, True),
+    (2, 33, 36, 8, 4, None, 0.05, False, True, True, False, True),
+    (1, 100, 20, 4, 1, None, 0.0, True, False, True, True, False),
+    (5, 19, 130, 16, 2, [0, 19, 3, 16, 17], 0.2, True, True, True, True, True),
+    (2, 30, 40, 20, 1, None, 1.0, True, True, True, True, True),
+]
+NAMES = ("u", "delta", "A", "B", "C", "D", "z", "bias", "state")
+
+
+def scan_case(case, dtype, seed=0):
+    B, T, D, N, G, lengths, p, with_state, with_z, with_d, with_bias, softplus = case
+    g = gen(seed)
+
+    def r(*s):
+        return torch.randn(*s, generator=g)
+
+    t = dict(u=r(B, T, D).to(dtype), delta=(0.5 * r(B, T, D)).to(dtype), A=-torch.rand(D, N, generator=g) * 4 - 0.1,
+             B=r(B, T, G, 2 * N)[..., :N].to(dtype), C=r(B, T, G, 2 * N)[..., N:].to(dtype), D=r(D) if with_d else None,
+             z=r(B, T, 2 * D)[..., D:].to(dtype) if with_z else None, bias=r(D) - 2 if with_bias else None,
+             state=r(B, D, N) if with_state else None)
+    if not softplus:
+        t["delta"] = t["delta"].abs()
+        t["bias"] = None if t["bias"] is None else t["bias"].abs()
+    resets = (torch.rand(B, T, generator=g) < p) if p else None
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32)
+    dy, dlast = r(B, T, D).to(dtype), r(B, D, N)
+    if ln is not None:
+        for b, n in enumerate(lengths):
+            for v in (t["u"], t["delta"], t["B"], t["C"], t["z"], dy):
+                if v is not None:
+                    v[b, n:] = float("nan")
+    return t, ln, resets, dy, dlast, softplus
+
+
+def scan_reference(t, ln, resets, dy, dlast, softplus, absolute=False):
+    def clean(v):
+        return None if v is None else torch.nan_to_num(v.double())
+    t = {k: clean(v) for k, v in t.items()}
+    dy, dlast = clean(dy), clean(dlast)
+    if absolute:        # what the sums' terms add up to without their signs (the decays stay what they are)
+        t = {k: v if v is None or k in ("A", "delta", "bias") else v.abs() for k, v in t.items()}
+        dy, dlast = dy.abs(), dlast.abs()
+    lv = leaves(*(t[k] for k in NAMES))
+    out, last = ref.selective_scan(*lv, softplus=softplus, lengths=ln, resets=resets)
+    live = [v for v in lv if v is not None]
+    grads = torch.autograd.grad([out, last], live, [dy, dlast], allow_unused=True)
+    it = iter([torch.zeros_like(v) if w is None else w for v, w in zip(live, grads)])
+    return out.detach(), last.detach(), {k: next(it) for k, v in zip(NAMES, lv) if v is not None}
+
+
+def scan_roundings(T, N):
+    """Per step the state meets the time step (softplus: about 12), the decay's argument and exponential (2 + 2 + |dt A| 14, |dt A| < 8
+    here: the time step's own error is in the exponent), two products and a sum; T of them in a row at most.  Reading it out adds N + 1
+    sums, the gate 8."""
+    return T * (12 + 4 + 8 * 14 + 3) + N + 9
+
+
+def check_scan(t, ln, resets, dy, dlast, softplus, n, rows):
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    out64, last64, g64 = scan_reference(t, ln, resets, dy, dlast, softplus)
+    size_o, size_l, size_g = scan_reference(t, ln, resets, dy, dlast, softplus, absolute=True)
+    dev = {k: None if v is None else v.cuda().detach().requires_grad_() for k, v in t.items()}
+    out, last = selective_scan(dev["u"], dev["delta"], dev["A"], dev["B"], dev["C"], dev["D"], dev["z"], dev["bias"], delta_softplus=softplus,
+                               initial_state=dev["state"], lengths=None if ln is None else ln.cuda(),
+                               resets=None if resets is None else resets.cuda(), return_state=True)
+    close("out", out, out64, n, largest(size_o))
+    close("state", last, last64, n, largest(size_l))
+    live = [k for k in NAMES if dev[k] is not None]
+    got = torch.autograd.grad([out, last], [dev[k] for k in live], [dy.cuda(), dlast.cuda()])
+    for k, v in zip(live, got):
+        # forward and reverse recurrence, then a sum over at most `rows` rows; ddelta and dA take the difference of two such paths
+        size = max(largest(size_g[k]), largest(g64[k]), *((largest(size_g["u"]) * 8,) if k in ("delta", "bias") else ()))
+        close("d" + k, v, g64[k], 2 * n + rows, size)
+    return out, last
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", SCAN, ids=lambda c: "x".join(map(str, c[:5])))
+def test_selective_scan_and_gradients(case, dtype):
+    t, ln, resets, dy, dlast, softplus = scan_case(case, DTYPES[dtype])
+    check_scan(t, ln, resets, dy, dlast, softplus, scan_roundings(case[1], case[3]), case[0] * case[1] + case[2])
+
+
+def test_a_reset_clears_a_state_that_is_not_finite():
+    from airgym_amd.lib.network.selective_scan import selective_scan, selective_scan_step
+    case = (2, 20, 40, 16, 1, None, 0.0, True, True, True, True, True)
+    t, _, _, dy, _, _ = scan_case(case, torch.float32)
+    resets = torch.zeros(2, 20, dtype=torch.bool)
+    resets[:, 0] = True
+    dev = {k: v.cuda().requires_grad_() for k, v in t.items()}
+    poisoned = torch.full((2, 40, 16), float("inf"), device="cuda").requires_grad_()
+    args = [dev[k] for k in NAMES[:-1]]
+    a = selective_scan(*args, initial_state=poisoned, resets=resets.cuda())
+    b = selective_scan(*args)
+    assert torch.equal(a, b)
+    ga = torch.autograd.grad(a, args + [poisoned], dy.cuda())
+    gb = torch.autograd.grad(b, args, dy.cuda())
+    for x, y in zip(ga, gb):
+        assert torch.equal(x, y)
+    assert not ga[-1].any()
+    with torch.no_grad():
+        state = poisoned.detach().clone()
+        one = [dev["u"][:, 0], dev["delta"][:, 0], dev["A"], dev["B"][:, 0], dev["C"][:, 0], state, dev["D"], dev["z"][:, 0], dev["bias"]]
+        assert torch.isfinite(selective_scan_step(*one, resets=resets[:, 0].cuda())).all() and torch.isfinite(state).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,D,N,G", [(1, 1, 1, 1), (3, 6, 3, 2), (5, 130, 16, 1), (2, 64, 8, 1), (3, 33, 32, 1), (2, 48, 13, 3)])
+def test_selective_scan_steps_against_float64(B, D, N, G, dtype):
+    from airgym_amd.lib.network.selective_scan import selective_scan_step
+    T = 5
+    t, _, resets, _, _, _ = scan_case((B, T, D, N, G, None, 0.3, True, True, True, True, True), DTYPES[dtype], seed=B)
+    d64 = {k: v.double() for k, v in t.items()}
+    out64, last64 = ref.selective_scan(*(d64[k] for k in NAMES), resets=resets)
+    a64 = {k: v if k in ("A", "delta", "bias") else v.abs() for k, v in d64.items()}
+    size_o, size_l = ref.selective_scan(*(a64[k] for k in NAMES), resets=resets)
+    dev = {k: v.cuda() for k, v in t.items()}
+    state = dev["state"].clone()
+    for i in range(T):
+        y = selective_scan_step(dev["u"][:, i], dev["delta"][:, i], dev["A"], dev["B"][:, i], dev["C"][:, i], state, dev["D"],
+                                dev["z"][:, i], dev["bias"], resets=resets[:, i].cuda())
+        close(f"step {i}", y, out64[:, i], scan_roundings(T, N), largest(size_o))
+    close("state", state, last64, scan_roundings(T, N), largest(size_l))
+
+
+def test_scan_inputs_that_are_expanded_or_time_major():
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    g = gen(5)
+    T, B, D, N = 20, 3, 48, 16
+    u = torch.randn(T, B, D, generator=g).cuda()
+    delta = torch.randn(B, T, 1, generator=g).cuda().requires_grad_()           # one time step for all channels
+    Bm = torch.randn(1, T, N, generator=g).cuda().requires_grad_()              # shared by the batch
+    C = torch.randn(B, T, N, generator=g).cuda()
+    A = -torch.rand(D, N, generator=g).cuda()
+    dy = torch.randn(B, T, D, generator=g).cuda()
+    a = selective_scan(u.transpose(0, 1), delta.expand(B, T, D), A, Bm.expand(B, T, N), C)
+    ga = torch.autograd.grad(a, (delta, Bm), dy)
+    full, bfull = delta.detach().expand(B, T, D).contiguous().requires_grad_(), Bm.detach().expand(B, T, N).contiguous().requires_grad_()
+    b = selective_scan(u.transpose(0, 1).contiguous(), full, A, bfull, C)
+    gb = torch.autograd.grad(b, (full, bfull), dy)
+    assert torch.equal(a, b)
+    assert torch.equal(ga[0], gb[0].sum(-1, keepdim=True)) and torch.equal(ga[1], gb[1].sum(0, keepdim=True))
+
+
+def test_gradients_against_differences():
+    """Directional derivatives of the float64 restatement, central differences with step 1e-5 (error ~1e-10 of third derivatives of order
+    one, far below the gradients' own bound)."""
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    case = (2, 21, 12, 16, 1, [21, 15], 0.1, True, True, True, True, True)
+    t, ln, resets, dy, dlast, _ = scan_case(case, torch.float32, seed=7)
+    t = {k: torch.nan_to_num(v) for k, v in t.items()}
+    dy = torch.nan_to_num(dy)
+    dev = {k: v.cuda().requires_grad_() for k, v in t.items()}
+    out, last = selective_scan(*(dev[k] for k in NAMES[:-1]), initial_state=dev["state"], lengths=ln.cuda(), resets=resets.cuda(),
+                               return_state=True)
+    grads = dict(zip(NAMES, torch.autograd.grad([out, last], [dev[k] for k in NAMES], [dy.cuda(), dlast.cuda()])))
+    _, _, size = scan_reference(t, ln, resets, dy, dlast, True, absolute=True)
+
+    def value(**change):
+        v = {k: x.double() for k, x in t.items()} | change
+        o, s = ref.selective_scan(*(v[k] for k in NAMES), lengths=ln, resets=resets)
+        return float((o * dy.double()).sum() + (s * dlast.double()).sum())
+
+    for k in NAMES:
+        v = torch.randn(t[k].shape, generator=gen(11), dtype=torch.float64)
+        eps = 1e-5
+        diff = (value(**{k: t[k].double() + eps * v}) - value(**{k: t[k].double() - eps * v})) / (2 * eps)
+        along = float((grads[k].double().cpu() * v).sum())
+        room = (2 * scan_roundings(21, 16) + 54) * U * max(largest(size[k]), 8 * largest(size["u"])) * float(v.abs().sum()) + 1e-7 * abs(diff) + 1e-6
+        assert abs(diff - along) <= room, (k, diff, along, room)
+
+
+# ------------------------------------------------------------------------------------------------ clipped policy loss
+LOSS = [(1, 1), (1, 2), (3, 5), (70, 21), (64, 64), (33, 257), (5, 1000), (7, 4099), (3, 33001)]
+
+
+def loss_case(R, V, dtype, masked, minus_inf, seed=0):
+    g = gen(seed + R + V)
+    logits = (2 * torch.randn(R, V + 3, generator=g)).to(dtype)[:, :V]
+    actions = torch.randint(0, V, (R,), generator=g)
+    if minus_inf and V > 2:
+        off = torch.rand(R, V, generator=g) < 0.3
+        off[torch.arange(R), actions] = False
+        logits = logits.masked_fill(off, -float("inf"))
+    lp = torch.log_softmax(logits.double(), 1).gather(1, actions[:, None])[:, 0]
+    moved = torch.randn(R, generator=g).double() * 0.2
+    for e in (1.2, 0.8):            # the border itself has two right gradients
+        border = torch.tensor(e).double().log()
+        moved = torch.where((moved - border).abs() < 1e-3, moved + 3e-3, moved)
+    old, refl = (lp - moved).float(), (lp + 0.2 * torch.randn(R, generator=g).double()).float()
+    adv = torch.randn(R, generator=g)
+    mask = (torch.rand(R, generator=g) < 0.6) if masked else None
+    if masked:
+        mask[0] = True
+        bad = ~mask
+        logits[bad] = float("nan")
+        actions[bad] = -100
+        old[bad], adv[bad], refl[bad] = float("inf"), float("nan"), float("nan")
+    return logits, actions, old, adv, refl, mask
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("masked,minus_inf", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("R,V", LOSS)
+def test_policy_loss_and_gradient(R, V, masked, minus_inf, dtype):
+    from airgym_amd.lib.core.policy_loss import action_logp, policy_loss
+    logits, actions, old, adv, refl, mask = loss_case(R, V, DTYPES[dtype], masked, minus_inf)
+    coefs = dict(e_clip=0.2, kl_coef=0.1, entropy_coef=0.01)
+    x = logits.double().requires_grad_()
+    loss64, stats64 = ref.policy_loss(x, actions, old.double(), adv.double(), refl.double(), mask, **coefs)
+    (g64,) = torch.autograd.grad(loss64, x)
+    leaf = logits.cuda().requires_grad_()
+    loss, stats = policy_loss(leaf, actions.cuda(), old.cuda(), adv.cuda(), ref_logp=refl.cuda(), mask=None if mask is None else mask.cuda(),
+                              **coefs)
+    (g,) = torch.autograd.grad(loss, leaf)
+    on = torch.ones(R, dtype=torch.bool) if mask is None else mask
+    # lse: exponent (argument |x - m| < 20: 20 + 2) and the sum's order (<= 2 log2 V + V / 256 links here), logarithm, two differences
+    # of numbers below 20; everything downstream multiplies by at most 3 (ratio) (|A| + 1) and adds 10 of its own
+    n = 20 * 3 + 2 * 17 + V / 256 + 60
+    size = 3 * (largest(adv[on]) + 1) * 10
+    close("loss", loss, loss64.detach(), n, size)
+    close("stats", stats[[0, 1, 2, 3, 5]], stats64[[0, 1, 2, 3, 5]], n, size)
+    assert float(stats[4]) == pytest.approx(float(stats64[4]), abs=1e-6)
+    close("dlogits", g, g64, n, size / int(on.sum()))
+    assert not g[~on.cuda()].any()
+    lp, H = action_logp(logits.cuda()[on.cuda()], actions.cuda()[on.cuda()])
+    ls = torch.log_softmax(logits[on].double(), 1)
+    close("logp", lp, ls.gather(1, actions[on][:, None])[:, 0], n, 20)
+    close("entropy", H, -(ls.exp() * ls.clamp(min=-1e30)).sum(1), n, 20)
+
+
+def test_policy_loss_of_rows_that_do_not_count_at_all():
+    from airgym_amd.lib.core.policy_loss import policy_loss
+    logits = torch.full((6, 40), float("nan"), device="cuda").requires_grad_()
+    bad = torch.full((6,), float("nan"), device="cuda")
+    loss, stats = policy_loss(logits, torch.full((6,), 99, device="cuda"), bad, bad, mask=torch.zeros(6, dtype=torch.bool, device="cuda"))
+    (g,) = torch.autograd.grad(loss, logits)
+    assert float(loss) == 0.0 and not stats.any() and not g.any()
+
+
+def test_policy_loss_action_out_of_range_is_nan_and_reads_nothing_outside():
+    from airgym_amd.lib.core.policy_loss import action_logp, policy_loss
+    logits = torch.randn(4, 10, device="cuda").requires_grad_()
+    actions = torch.tensor([1, 10, 3, -1], device="cuda")
+    zero = torch.zeros(4, device="cuda")
+    loss, _ = policy_loss(logits, actions, zero, zero + 1)
+    (g,) = torch.autograd.grad(loss, logits)
+    assert torch.isnan(loss) and torch.isnan(g[[1, 3]]).all() and torch.isfinite(g[[0, 2]]).all()
+    lp, _ = action_logp(logits.detach(), actions)
+    assert torch.isnan(lp[[1, 3]]).all() and torch.isfinite(lp[[0, 2]]).all()
+
+
+def test_policy_loss_scaled_and_backward_twice():
+    from airgym_amd.lib.core.policy_loss import policy_loss
+    g = gen(2)
+    logits = torch.randn(3, 7, 300, generator=g).cuda().requires_grad_()
+    actions = torch.randint(0, 300, (3, 7), generator=g).cuda()
+    old, adv = torch.full((3, 7), -5.0).cuda(), torch.randn(3, 7, generator=g).cuda()
+    loss, _ = policy_loss(logits, actions, old, adv, entropy_coef=0.1)
+    first = torch.autograd.grad(loss, logits, retain_graph=True)[0].clone()
+    again = torch.autograd.grad(3.0 * loss, logits, retain_graph=True)[0]
+    assert torch.equal(again, 3.0 * first)
+    logits.grad = None
+    loss.backward(retain_graph=True)
+    loss.backward()
+    assert torch.equal(logits.grad, first + first)
+    flat = logits.detach().reshape(21, 300).requires_grad_()
+    l2, _ = policy_loss(flat, actions.reshape(21), old.reshape(21), adv.reshape(21), entropy_coef=0.1)
+    assert torch.equal(l2, loss) and torch.equal(torch.autograd.grad(l2, flat)[0].view_as(first), first)
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs, refusals
+def _together(x, p, resets, actions, old, adv):
+    """conv -> scan -> head -> loss, as a policy with memory is trained."""
+    from airgym_amd.lib.core.policy_loss import policy_loss
+    from airgym_amd.lib.network.causal_conv import causal_conv
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    h = causal_conv(x, p["w"], p["b"], resets=resets)
+    bc = h @ p["wbc"]
+    y = selective_scan(h, h @ p["wd"], -torch.exp(p["alog"]), bc[..., :16], bc[..., 16:], p["D"], x, p["dbias"], resets=resets)
+    loss, stats = policy_loss(y @ p["head"], actions, old, adv, entropy_coef=0.01)
+    return loss, stats
+
+
+def _together_inputs(seed):
+    g = gen(seed)
+    B, T, D, V = 6, 24, 64, 21
+    p = dict(w=torch.randn(D, 4, generator=g) / 2, b=torch.zeros(D), wbc=torch.randn(D, 32, generator=g) / 8, wd=torch.randn(D, D, generator=g) / 8,
+             alog=torch.log(torch.arange(1, 17).float()).repeat(D, 1), D=torch.ones(D), dbias=torch.full((D,), -3.0),
+             head=torch.randn(D, V, generator=g) / 8)
+    x, resets = torch.randn(B, T, D, generator=g), torch.rand(B, T, generator=g) < 0.1
+    actions, old, adv = torch.randint(0, V, (B, T), generator=g), torch.full((B, T), -3.0), torch.randn(B, T, generator=g)
+    return {k: v.cuda().requires_grad_() for k, v in p.items()}, [t.cuda() for t in (x, resets, actions, old, adv)]
+
+
+def test_all_operators_together_on_another_stream():
+    p, data = _together_inputs(0)
+    loss, _ = _together(data[0], p, *data[1:])
+    want = torch.autograd.grad(loss, list(p.values()))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loss2, _ = _together(data[0], p, *data[1:])
+        got = torch.autograd.grad(loss2, list(p.values()))
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert torch.equal(loss, loss2)
+    for k, a, b in zip(p, want, got):
+        assert torch.equal(a, b), k
+
+
+def test_all_operators_together_captured_and_replayed():
+    """Forward and backward as one graph; every replay against the eager result on the same inputs, with eager work in between."""
+    p, data = _together_inputs(1)
+    names = list(p)
+    static = [t.clone() for t in data]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        loss, _ = _together(static[0], p, *static[1:])
+        torch.autograd.grad(loss, [p[k] for k in names])
+        del loss
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        gl, _ = _together(static[0], p, *static[1:])
+        gg = torch.autograd.grad(gl, [p[k] for k in names])
+    for seed in range(2, 6):
+        _, fresh = _together_inputs(seed)
+        for a, b in zip(static, fresh):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [gl.clone()] + [t.clone() for t in gg]
+        loss, _ = _together(fresh[0], p, *fresh[1:])
+        want = [loss.detach()] + list(torch.autograd.grad(loss, [p[k] for k in names]))
+        for k, a, b in zip(["loss"] + names, got, want):
+            assert torch.equal(a, b), (seed, k)
+
+
+def test_refusals():
+    from airgym_amd.lib.core.policy_loss import action_logp, policy_loss
+    from airgym_amd.lib.network.causal_conv import causal_conv, causal_conv_step
+    from airgym_amd.lib.network.selective_scan import selective_scan, selective_scan_step
+    c = dict(device="cuda")
+    x, w = torch.zeros(2, 5, 8, **c), torch.zeros(8, 4, **c)
+    bad = [
+        lambda: causal_conv(x.cpu(), w), lambda: causal_conv(x.double(), w), lambda: causal_conv(x[0], w),
+        lambda: causal_conv(x, w[:, :1]), lambda: causal_conv(x, torch.zeros(8, 9, **c)), lambda: causal_conv(x, w.half()),
+        lambda: causal_conv(x, torch.zeros(7, 4, **c)), lambda: causal_conv(x, w, torch.zeros(7, **c)),
+        lambda: causal_conv(x, w, activation="relu"), lambda: causal_conv(x, w, initial_state=torch.zeros(2, 4, 8, **c)),
+        lambda: causal_conv(x, w, initial_state=torch.zeros(2, 3, 8, **c).half()), lambda: causal_conv(x, w, lengths=torch.zeros(2, **c)),
+        lambda: causal_conv(x, w, lengths=torch.zeros(3, dtype=torch.int32, **c)), lambda: causal_conv(x, w, resets=torch.zeros(2, 5, **c)),
+        lambda: causal_conv(x, w, lengths=torch.zeros(2, dtype=torch.int32)),
+        lambda: causal_conv_step(x[:, 0], torch.zeros(2, 8, 3, **c), w), lambda: causal_conv_step(x[:, 0], torch.zeros(3, 2, 8, **c).transpose(0, 1), w),
+        lambda: causal_conv_step(x[:, 0], torch.zeros(2, 3, 8, **c), w.clone().requires_grad_()),
+    ]
+    A, B = torch.zeros(8, 16, **c), torch.zeros(2, 5, 16, **c)
+    h = torch.zeros(2, 8, 16, **c)
+    bad += [
+        lambda: selective_scan(x, x[:, :4], A, B, B), lambda: selective_scan(x, x.half(), A, B, B), lambda: selective_scan(x, x, A[:7], B, B),
+        lambda: selective_scan(x, x, torch.zeros(8, 33, **c), B, B), lambda: selective_scan(x, x, A.half(), B, B),
+        lambda: selective_scan(x, x, A, B, B[..., :8]), lambda: selective_scan(x, x, A, torch.zeros(2, 5, 3, 16, **c), torch.zeros(2, 5, 3, 16, **c)),
+        lambda: selective_scan(x, x, A, torch.zeros(2, 5, 2, 16, **c), B), lambda: selective_scan(x, x, A, B, B, torch.zeros(9, **c)),
+        lambda: selective_scan(x, x, A, B, B, initial_state=h.half()), lambda: selective_scan(x, x, A, B, B, initial_state=h[:1]),
+        lambda: selective_scan(x, x, A, B.cpu(), B), lambda: selective_scan(x, x, A, B, B, resets=torch.zeros(5, 2, dtype=torch.bool, **c)),
+        lambda: selective_scan_step(x[:, 0], x[:, 0], A, B[:, 0], B[:, 0], h.half()),
+        lambda: selective_scan_step(x[:, 0], x[:, 0], A, B[:, 0], B[:, 0], torch.zeros(2, 16, 8, **c).transpose(1, 2)),
+        lambda: selective_scan_step(x[:, 0], x[:, 0], A.clone().requires_grad_(), B[:, 0], B[:, 0], h),
+    ]
+    lo, ac, f = torch.zeros(3, 9, **c), torch.zeros(3, dtype=torch.int64, **c), torch.zeros(3, **c)
+    bad += [
+        lambda: policy_loss(lo.cpu(), ac, f, f), lambda: policy_loss(lo, ac.int(), f, f), lambda: policy_loss(lo, ac, f.half(), f),
+        lambda: policy_loss(lo, ac, f, f[:2]), lambda: policy_loss(lo, ac, f, f, mask=f), lambda: policy_loss(lo, ac, f, f, kl_coef=0.1),
+        lambda: policy_loss(lo, ac, f, f, e_clip=-0.1), lambda: policy_loss(lo, ac, f.clone().requires_grad_(), f),
+        lambda: policy_loss(lo.double(), ac, f, f), lambda: policy_loss(lo[0], ac, f, f), lambda: policy_loss(lo, ac, None, f),
+        lambda: action_logp(lo.clone().requires_grad_(), ac), lambda: action_logp(lo, ac[:2]),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            print("not refused:", i)
+
+
+def test_empty_batches():
+    from airgym_amd.lib.core.policy_loss import action_logp, policy_loss
+    from airgym_amd.lib.network.causal_conv import causal_conv, causal_conv_step
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    c = dict(device="cuda")
+    w, A, s = torch.zeros(8, 4, **c), torch.zeros(8, 16, **c), torch.randn(2, 3, 8, **c)
+    y, last = causal_conv(torch.zeros(2, 0, 8, **c), w, initial_state=s, return_state=True)
+    assert y.shape == (2, 0, 8) and torch.equal(last, s)
+    assert causal_conv_step(torch.zeros(0, 8, **c), torch.zeros(0, 3, 8, **c), w).shape == (0, 8)
+    h = torch.randn(2, 8, 16, **c)
+    e = torch.zeros(2, 0, 8, **c)
+    out, last = selective_scan(e, e, A, torch.zeros(2, 0, 16, **c), torch.zeros(2, 0, 16, **c), initial_state=h, return_state=True)
+    assert out.shape == (2, 0, 8) and torch.equal(last, h)
+    lo = torch.zeros(0, 9, **c).requires_grad_()
+    loss, _ = policy_loss(lo, torch.zeros(0, dtype=torch.int64, **c), torch.zeros(0, **c), torch.zeros(0, **c))
+    loss.backward()
+    assert float(loss) == 0.0 and action_logp(lo.detach(), torch.zeros(0, dtype=torch.int64, **c))[0].shape == (0,)
