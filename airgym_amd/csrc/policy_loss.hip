@@ -4,22 +4,24 @@
 //   row loss = max(-A r, -A clip(r)) + kl (e^d - d - 1) - ent H,   r = e^{lp - old},  d = ref - lp
 //   d loss / d x_j = f (delta_ja - p_j) + ent p_j (log p_j + H),   f = [-A r if the unclipped side is the larger] + kl (1 - e^d)
 //
-// One workgroup per row: a first sweep forms the maximum and, against it, the two sums (each thread against a maximum of its own,
-// joined at the end); a second one, which finds the row in the cache, writes the gradient.  Logits of -inf have probability 0; where
-// 0 times their infinite log-probability would appear, the log-probability is held at -1e30 instead.
+// Read once, write once: a row is held in registers, 16 bytes per access, between the sums and the gradient - by 1 to 64 lanes of a
+// wave (short rows), by a workgroup of 256 or 1024 threads, or, beyond what registers hold, read a second time from the cache.
+// Every wave sums against a maximum of its own and the waves' results are joined.  Memory bounds it: about 20 issue slots per element
+// are some 2 T elements/s over the chip, more than arrives.
+// Logits of -inf have probability 0.  Their infinite log-probability would meet it as 0 times inf: a wave that finds its second sum
+// NaN forms it again with the log-probability held at -1e30, and so does the gradient.
 #include "seq_common.hpp"
 
 namespace {
 
-constexpr int kThreads = 256;
 constexpr float kFloor = -1e30f;
 constexpr int kSums = 5;               // policy loss, KL term, entropy, KL of the old policy, clipped
 
 struct LossArgs {
     const void* logits; const long long* actions; const float *old_logp, *adv, *ref_logp; const unsigned char* mask;
     void* dlogits; const float* count;
-    float* rows;                       // [R, kSums] per-row terms
-    float *logp, *entropy;
+    float* partials;                   // [workgroups, kSums] sums of the rows' terms
+    float *logp, *entropy;             // the log-probability form: these instead
     long long R1, s0, s1, R;
     int V;
     float e_clip, kl_coef, entropy_coef;
@@ -31,125 +33,383 @@ __device__ __forceinline__ float safe_max(float m) { return m == -__builtin_inff
 
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
     const float m = fmaxf(a.m, b.m), base = safe_max(m);
-    const float da = fmaxf(a.m - base, kFloor), dbb = fmaxf(b.m - base, kFloor);
-    const float ea = exp_hw(da), eb = exp_hw(dbb);
+    const float da = fmaxf(a.m - base, kFloor), db = fmaxf(b.m - base, kFloor);
+    const float ea = exp_hw(da), eb = exp_hw(db);
     // t shifts with the base: sum e^{x-m} (x-m) = e^{a.m-m} (a.t + (a.m-m) a.s)
-    return Sums{m, a.s * ea + b.s * eb, ea * (a.t + da * a.s) + eb * (b.t + dbb * b.s)};
+    return Sums{m, a.s * ea + b.s * eb, ea * (a.t + da * a.s) + eb * (b.t + db * b.s)};
 }
 
-__device__ __forceinline__ Sums wave_join(Sums v) {
+template <typename T> __device__ __forceinline__ const T* row_of(const LossArgs& a, long long row) {
+    return (const T*)a.logits + (row / a.R1) * a.s0 + (row % a.R1) * a.s1;
+}
+
+// what a row's sums say: base and logarithm of the softmax, entropy, log-probability, and the two factors of its gradient
+struct Row {
+    float base, logS, H, lp, f, ent;
+    bool inf;                          // some logits are -inf
+};
+
+__device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, bool inf, float xa, long long row) {
+    Row r;
+    r.inf = inf;
+    r.base = safe_max(v.m);
+    r.logS = log2_hw(v.s) * kLn2;
+    r.H = r.logS - v.t / v.s;
+    r.lp = (xa - r.base) - r.logS;
+    r.f = r.ent = 0.0f;
+    if (a.logp) return r;
+    const float adv = a.adv[row], ratio = expf(r.lp - a.old_logp[row]);
+    const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
+    float f = plain >= held || plain != plain ? plain : 0.0f;
+    if (a.ref_logp) f -= a.kl_coef * expm1f(a.ref_logp[row] - r.lp);
+    const float n = 1.0f / a.count[0];
+    r.f = f * n;
+    r.ent = a.entropy_coef * n;
+    return r;
+}
+
+// the row's share of the statistics (one lane needs it)
+__device__ __forceinline__ void row_terms(const LossArgs& a, const Row& r, long long row, float* term) {
+    const float adv = a.adv[row], moved = r.lp - a.old_logp[row], ratio = expf(moved);
+    const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
+    term[0] = plain != plain ? plain : fmaxf(plain, held);
+    const float d = a.ref_logp ? a.ref_logp[row] - r.lp : 0.0f;
+    term[1] = expm1f(d) - d;
+    term[2] = r.H;
+    term[3] = expm1f(moved) - moved;
+    term[4] = ratio < 1.0f - a.e_clip || ratio > 1.0f + a.e_clip ? 1.0f : 0.0f;
+}
+
+// f (delta - p) + ent p (log p + H) without the delta, from d = x - base
+__device__ __forceinline__ float grad_of(const Row& r, float d) {
+    if (r.inf) d = fmaxf(d, kFloor);
+    const float p = exp2_hw((d - r.logS) * kLog2e);
+    return p * __builtin_fmaf(r.ent, d + (r.H - r.logS), -r.f);
+}
+
+// one element's share of the sums
+__device__ __forceinline__ void add_to(Sums& v, float x, float base) {
+    const float d = x - base, e = exp_hw(d);
+    v.s += e;
+    v.t = __builtin_fmaf(e, d, v.t);
+}
+
+// ---- short rows: L lanes of a wave per row, up to 8 elements a lane ------------------------------------------------------
+constexpr int kShortThreads = 256, kPerLane = 8, kShortLanes = 16;
+
+template <typename T, int L>
+__global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArgs a) {
+    constexpr int kRows = kShortThreads / L;
+    __shared__ float part[kShortThreads / 64][kSums];
+    const int l = threadIdx.x % L;
+    const long long row = (long long)blockIdx.x * kRows + threadIdx.x / L;
+    const bool there = row < a.R, on = there && !(a.mask && !a.mask[row]);
+    float x[kPerLane], xa = __builtin_nanf(""), t[kSums] = {0, 0, 0, 0, 0};
+    Row r;
+    int act = -1;
+    if (on) {
+        const T* p = row_of<T>(a, row);
+        const long long av = a.actions[row];
+        act = av >= 0 && av < a.V ? (int)av : -1;
+        Sums v{-__builtin_inff(), 0.0f, 0.0f};
 #pragma unroll
-    for (int o = 32; o; o >>= 1) v = join(v, Sums{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.t, o)});
-    return v;
+        for (int k = 0; k < kPerLane; k++) {
+            const int j = l + k * L;
+            x[k] = j < a.V ? to_f32(p[j]) : -__builtin_inff();
+            v.m = fmaxf(v.m, x[k]);
+        }
+        if (act >= 0) xa = to_f32(p[act]);
+#pragma unroll
+        for (int o = L / 2; o; o >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, o));
+        const float base = safe_max(v.m);
+        bool inf = false;
+#pragma unroll
+        for (int k = 0; k < kPerLane; k++)
+            if (l + k * L < a.V) {
+                const float d = x[k] - base, e = exp_hw(d);
+                inf |= d == -__builtin_inff();
+                v.s += e;
+                v.t = __builtin_fmaf(e, fmaxf(d, kFloor), v.t);
+            }
+#pragma unroll
+        for (int o = L / 2; o; o >>= 1) v.s += __shfl_xor(v.s, o), v.t += __shfl_xor(v.t, o);
+        r = finish_row(a, v, inf, xa, row);
+        if (a.logp) {
+            if (l == 0) {
+                a.logp[row] = r.lp;
+                if (a.entropy) a.entropy[row] = r.H;
+            }
+        } else if (l == 0) row_terms(a, r, row, t);
+    }
+    if (a.logp) return;
+    if (a.dlogits && there) {
+        T* dx = (T*)a.dlogits + row * a.V;
+#pragma unroll
+        for (int k = 0; k < kPerLane; k++) {
+            const int j = l + k * L;
+            if (j < a.V) {
+                float g = 0.0f;
+                if (on) g = grad_of(r, x[k] - r.base) + (j == act ? r.f : 0.0f);
+                dx[j] = from_f32<T>(g);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSums; k++) {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) t[k] += __shfl_xor(t[k], o);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][k] = t[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < kSums) {
+        float s = part[0][threadIdx.x];
+#pragma unroll
+        for (int i = 1; i < kShortThreads / 64; i++) s += part[i][threadIdx.x];
+        a.partials[(long long)blockIdx.x * kSums + threadIdx.x] = s;
+    }
 }
 
-// a row's loss terms and the two coefficients of its gradient
-struct Row { float lse, H, f, ent; };
+// ---- long rows: a workgroup per row -----------------------------------------------------------------------------------------
+// 16 bytes of logits, kept as they came.  Rows of an odd width start anywhere: the access is aligned to the element only.
+template <typename T> struct Vec {
+    static constexpr int E = 16 / sizeof(T);
+    uint32_t w[4];
+    __device__ __forceinline__ float at(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t v = w[i / 2];
+        if (__is_same(T, bf16_t)) return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
+        return (float)__builtin_bit_cast(f16_t, (uint16_t)(i & 1 ? v >> 16 : v));
+    }
+    __device__ __forceinline__ void set(const float* x) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (sizeof(T) == 4) w[k] = __float_as_uint(x[k]);
+            else {
+                typedef T pair __attribute__((ext_vector_type(2)));
+                typedef float two __attribute__((ext_vector_type(2)));
+                const two f = {x[(2 * k) % E], x[(2 * k + 1) % E]};
+                w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, pair));
+            }
+        }
+    }
+};
+template <> __device__ __forceinline__ void Vec<float>::set(const float* x) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) w[k] = __float_as_uint(x[k]);
+}
+typedef uint32_t words_any2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t words_any4 __attribute__((ext_vector_type(4), aligned(4)));
+template <int N> struct Words { using type = words_any2; };
+template <> struct Words<4> { using type = words_any4; };
+template <typename T> __device__ __forceinline__ Vec<T> load_vec(const T* p) {
+    const auto v = *(const typename Words<sizeof(T)>::type*)p;
+    return Vec<T>{{v[0], v[1], v[2], v[3]}};
+}
+template <typename T> __device__ __forceinline__ void store_vec(T* p, const Vec<T>& c) {
+    using W = typename Words<sizeof(T)>::type;
+    *(W*)p = W{c.w[0], c.w[1], c.w[2], c.w[3]};
+}
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void token_loss_kernel(LossArgs a) {
-    __shared__ Sums part[kThreads / 64];
+// NV > 0: the row is held in NV accesses per thread.  NV = 0: it is longer than that, and read again for the gradient.
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
+    constexpr int E = 16 / sizeof(T), kWaves = THREADS / 64, kKeep = NV ? NV : 1;
+    __shared__ Sums part[kWaves];
+    __shared__ int has_inf[kWaves];
     const long long row = blockIdx.x;
-    const T* x = (const T*)a.logits + (row / a.R1) * a.s0 + (row % a.R1) * a.s1;
+    const T* x = row_of<T>(a, row);
     T* dx = a.dlogits ? (T*)a.dlogits + row * a.V : nullptr;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int full = a.V / E, nq = NV ? NV : (full + THREADS - 1) / THREADS;      // whole accesses of the row, per thread
+    const int tail = full * E + threadIdx.x;                                        // the elements behind them: one per thread
     if (a.mask && !a.mask[row]) {
-        if (dx)
-            for (int j = threadIdx.x; j < a.V; j += kThreads) dx[j] = from_f32<T>(0.0f);
-        if (threadIdx.x < kSums && a.rows) a.rows[row * kSums + threadIdx.x] = 0.0f;
+        const Vec<T> zero{{0, 0, 0, 0}};
+        if (dx) {
+            for (int q = threadIdx.x; q < full; q += THREADS) store_vec(dx + q * E, zero);
+            if (tail < a.V) dx[tail] = from_f32<T>(0.0f);
+        }
+        if (threadIdx.x < kSums) a.partials[row * kSums + threadIdx.x] = 0.0f;
         return;
     }
+    const long long av = a.actions[row];
+    const int act = av >= 0 && av < a.V ? (int)av : -1;
+    const float xa = act >= 0 ? to_f32(x[act]) : __builtin_nanf("");
+    Vec<T> c[kKeep];
     Sums v{-__builtin_inff(), 0.0f, 0.0f};
-    for (int j = threadIdx.x; j < a.V; j += kThreads) {
-        const float xv = to_f32(x[j]);
-        const float m = fmaxf(v.m, xv);
-        if (m != v.m) v = join(v, Sums{m, 0.0f, 0.0f});
-        const float e = exp_hw(xv - safe_max(v.m));
-        v.s += e;
-        v.t = __builtin_fmaf(e, fmaxf(xv - safe_max(v.m), kFloor), v.t);
-    }
-    v = wave_join(v);
-    if (lane == 0) part[w] = v;
-    __syncthreads();
-    v = part[0];
+    bool inf = false;
+    // The row stays as it came: without this the compiler keeps the 16-bit types' float forms from one pass over it to the next, two
+    // registers for one.
+    auto as_it_came = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 1; i < kThreads / 64; i++) v = join(v, part[i]);
-    const float logS = log2_hw(v.s) * kLn2, base = safe_max(v.m), H = logS - v.t / v.s;
-    const long long act = a.actions[row];
-    const float lp = act >= 0 && act < a.V ? (to_f32(x[act]) - base) - logS : __builtin_nanf("");
+        for (int k = 0; k < kKeep; k++) asm volatile("" : "+v"(c[k].w[0]), "+v"(c[k].w[1]), "+v"(c[k].w[2]), "+v"(c[k].w[3]));
+    };
+    // the sums of what c (and xt) holds against the wave's maximum m, joined to what the wave has
+    auto sum_up = [&](int k0, float xt) __attribute__((always_inline)) {
+        float m = xt;
+#pragma unroll
+        for (int k = 0; k < kKeep; k++)
+            if ((k0 + k) * THREADS + (int)threadIdx.x < full)
+#pragma unroll
+                for (int i = 0; i < E; i++) m = fmaxf(m, c[k].at(i));
+#pragma unroll
+        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        Sums u{m, 0.0f, 0.0f};
+        const float base = safe_max(m);
+        as_it_came();
+#pragma unroll
+        for (int k = 0; k < kKeep; k++)
+            if ((k0 + k) * THREADS + (int)threadIdx.x < full)
+#pragma unroll
+                for (int i = 0; i < E; i++) add_to(u, c[k].at(i), base);
+        if (u.t != u.t) {              // some x - base are -inf (or NaN, which stays)
+            inf = true;
+            u.t = 0.0f;
+            as_it_came();
+#pragma unroll
+            for (int k = 0; k < kKeep; k++)
+                if ((k0 + k) * THREADS + (int)threadIdx.x < full)
+#pragma unroll
+                    for (int i = 0; i < E; i++) {
+                        const float d = c[k].at(i) - base;
+                        u.t = __builtin_fmaf(exp_hw(d), fmaxf(d, kFloor), u.t);
+                    }
+        }
+        if (k0 == 0 && tail < a.V) {
+            const float d = xt - base, e = exp_hw(d);
+            inf |= d == -__builtin_inff();
+            u.s += e;
+            u.t = __builtin_fmaf(e, fmaxf(d, kFloor), u.t);
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) u.s += __shfl_xor(u.s, o), u.t += __shfl_xor(u.t, o);
+        v = NV ? u : join(v, u);
+    };
+    const float xt = tail < a.V ? to_f32(x[tail]) : -__builtin_inff();
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int k = 0; k < kKeep; k++) {
+            const int q = threadIdx.x + k * THREADS;
+            if (q < full) c[k] = load_vec(x + q * E);
+        }
+        sum_up(0, xt);
+    } else {
+        for (int k = 0; k < nq; k++) {
+            const int q = threadIdx.x + k * THREADS;
+            if (q < full) c[0] = load_vec(x + q * E);
+            sum_up(k, k ? -__builtin_inff() : xt);
+        }
+    }
+    const bool any = __any(inf);
+    if (lane == 0) part[w] = v, has_inf[w] = any;
+    __syncthreads();
+    v = part[lane % kWaves];
+    const bool row_inf = __any(has_inf[lane % kWaves]);
+#pragma unroll
+    for (int o = kWaves / 2; o; o >>= 1) v = join(v, Sums{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.t, o)});
+    const Row r = finish_row(a, v, row_inf, xa, row);
     if (a.logp) {
         if (threadIdx.x == 0) {
-            a.logp[row] = lp;
-            if (a.entropy) a.entropy[row] = H;
+            a.logp[row] = r.lp;
+            if (a.entropy) a.entropy[row] = r.H;
         }
         return;
     }
-    const float adv = a.adv[row], moved = lp - a.old_logp[row], r = expf(moved);
-    const float rc = fminf(fmaxf(r, 1.0f - a.e_clip), 1.0f + a.e_clip);
-    const float plain = -adv * r, held = -adv * rc;
-    float kl = 0.0f, f = plain >= held || !(plain == plain) ? plain : 0.0f;
-    if (a.ref_logp) {
-        const float d = a.ref_logp[row] - lp, em = expm1f(d);
-        kl = em - d;
-        f -= a.kl_coef * em;
-    }
-    if (threadIdx.x == 0) {
-        float* t = a.rows + row * kSums;
-        t[0] = plain != plain ? plain : fmaxf(plain, held);
-        t[1] = kl;
-        t[2] = H;
-        t[3] = expm1f(moved) - moved;
-        t[4] = r < 1.0f - a.e_clip || r > 1.0f + a.e_clip ? 1.0f : 0.0f;
-    }
+    if (threadIdx.x == 0) row_terms(a, r, row, a.partials + row * kSums);
     if (!dx) return;
-    const float n = 1.0f / a.count[0], ent = a.entropy_coef * n;
-    f *= n;
-    for (int j = threadIdx.x; j < a.V; j += kThreads) {
-        const float lj = fmaxf((to_f32(x[j]) - base) - logS, kFloor), xj = to_f32(x[j]);
-        const float p = exp_hw((xj - base) - logS);
-        float gj = p * (ent * (lj + H) - f);
-        if (j == act) gj += f;
-        if (lp != lp) gj = lp;
-        dx[j] = from_f32<T>(gj);
+    const int aq = act >= 0 ? act / E : -1, ai = act % E;
+    auto gradient = [&](int q, const Vec<T>& held) __attribute__((always_inline)) {
+        if (q >= full) return;
+        float g[E];
+#pragma unroll
+        for (int i = 0; i < E; i++) g[i] = grad_of(r, held.at(i) - r.base);
+        if (q == aq)
+#pragma unroll
+            for (int i = 0; i < E; i++) g[i] += i == ai ? r.f : 0.0f;
+        Vec<T> out;
+        out.set(g);
+        store_vec(dx + q * E, out);
+    };
+    if constexpr (NV > 0) {
+        as_it_came();
+#pragma unroll
+        for (int k = 0; k < kKeep; k++) gradient(threadIdx.x + k * THREADS, c[k]);
+    } else {
+        for (int q = threadIdx.x; q < full; q += THREADS) gradient(q, load_vec(x + q * E));
     }
+    if (tail < a.V) dx[tail] = from_f32<T>(grad_of(r, xt - r.base) + (tail == act ? r.f : 0.0f));
 }
 
-// number of rows that count, at least 1
+// {max(rows that count, 1), rows that count}
 __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, long long R, float* count) {
     __shared__ int part[16];
     int c = 0;
-    for (long long i = threadIdx.x; i < R; i += 1024) c += mask ? mask[i] != 0 : 1;
+    if (mask) {
+        const long long head = (16 - ((uintptr_t)mask & 15)) & 15, n16 = R > head ? (R - head) / 16 : 0;
+        const uint4* m = (const uint4*)(mask + head);
+        for (long long i = threadIdx.x; i < n16; i += 1024) {
+            const uint4 v = m[i];
+            const unsigned q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; k++) {      // bytes that are not zero: bit 7 of (b | (b & 0x7f) + 0x7f)
+                const unsigned nz = (q[k] | ((q[k] & 0x7f7f7f7fu) + 0x7f7f7f7fu)) & 0x80808080u;
+                c += __popc(nz);
+            }
+        }
+        if (threadIdx.x < head && threadIdx.x < R) c += mask[threadIdx.x] != 0;
+        const long long tail = head + n16 * 16 + threadIdx.x;      // at most 15 bytes
+        if (tail < R) c += mask[tail] != 0;
+    }
     for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = c;
     __syncthreads();
     if (threadIdx.x == 0) {
-        int s = 0;
+        long long s = mask ? 0 : R;
         for (int i = 0; i < 16; i++) s += part[i];
         count[0] = s > 0 ? (float)s : 1.0f;
         count[1] = (float)s;
     }
 }
 
-__global__ __launch_bounds__(1024) void stats_kernel(const float* rows, long long R, const float* count, float kl_coef, float ent_coef,
-                                                     float* stats) {
-    __shared__ double part[16][kSums];
-    double s[kSums] = {0, 0, 0, 0, 0};
-    for (long long i = threadIdx.x; i < R; i += 1024)
-        for (int k = 0; k < kSums; k++) s[k] += rows[i * kSums + k];
+// The rows' terms summed in a fixed order, in double: kStatsRows of them per workgroup, then those sums by one workgroup (which, for
+// few rows, takes the terms themselves).  One workgroup over 65 536 rows took 45 us, the two stages take 7.
+constexpr int kStatsRows = 1024;
+
+template <typename S>
+__device__ __forceinline__ void sum_rows(const S* rows, long long n, double* s, double (*part)[kSums]) {
+#pragma unroll
+    for (int k = 0; k < kSums; k++) s[k] = 0.0;
+    for (long long i = threadIdx.x; i < n; i += 256)
+#pragma unroll
+        for (int k = 0; k < kSums; k++) s[k] += (double)rows[i * kSums + k];
+#pragma unroll
     for (int k = 0; k < kSums; k++) {
         for (int o = 32; o; o >>= 1) s[k] += __shfl_xor(s[k], o);
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][k] = s[k];
     }
     __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kSums; k++) s[k] = ((part[0][k] + part[1][k]) + part[2][k]) + part[3][k];
+}
+
+__global__ __launch_bounds__(256) void stats_part_kernel(const float* rows, long long n, double* out) {
+    __shared__ double part[4][kSums];
+    double s[kSums];
+    const long long first = (long long)blockIdx.x * kStatsRows;
+    sum_rows(rows + first * kSums, min((long long)kStatsRows, n - first), s, part);
+    if (threadIdx.x == 0)
+#pragma unroll
+        for (int k = 0; k < kSums; k++) out[(long long)blockIdx.x * kSums + k] = s[k];
+}
+
+template <typename S>
+__global__ __launch_bounds__(256) void stats_kernel(const S* rows, long long n, const float* count, float kl_coef, float ent_coef, float* stats) {
+    __shared__ double part[4][kSums];
+    double s[kSums];
+    sum_rows(rows, n, s, part);
     if (threadIdx.x == 0) {
-        double t[kSums];
-        for (int k = 0; k < kSums; k++) {
-            t[k] = 0;
-            for (int i = 0; i < 16; i++) t[k] += part[i][k];
-            t[k] /= (double)count[0];
-        }
-        stats[0] = (float)(t[0] + (double)kl_coef * t[1] - (double)ent_coef * t[2]);
-        for (int k = 0; k < kSums; k++) stats[1 + k] = (float)t[k];
+#pragma unroll
+        for (int k = 0; k < kSums; k++) s[k] /= (double)count[0], stats[1 + k] = (float)s[k];
+        stats[0] = (float)(s[0] + (double)kl_coef * s[1] - (double)ent_coef * s[2]);
         stats[6] = count[1];
         stats[7] = 0.0f;
     }
@@ -164,9 +424,59 @@ __global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const flo
 
 }  // namespace
 
+// Which form takes a row of V logits.  Short rows (V <= 8 lanes' worth of a wave's 64) share a wave; beyond, a workgroup holds the
+// row: 256 threads while 8 accesses of 16 bytes per thread suffice, 1024 threads up to 16 of them, and what is longer is read twice.
+static int short_lanes(int V) {
+    int l = 1;
+    while (l * kPerLane < V) l *= 2;
+    return l;
+}
+
+template <typename T>
+static long long launch_rows(const LossArgs& a, void* stream) {
+    const hipStream_t st = (hipStream_t)stream;
+    const int lanes = short_lanes(a.V);
+    if (lanes <= kShortLanes) {
+        const int rows = kShortThreads / lanes;
+        const dim3 grid((unsigned)((a.R + rows - 1) / rows)), block(kShortThreads);
+        switch (lanes) {
+            case 1: hipLaunchKernelGGL((token_loss_short_kernel<T, 1>), grid, block, 0, st, a); break;
+            case 2: hipLaunchKernelGGL((token_loss_short_kernel<T, 2>), grid, block, 0, st, a); break;
+            case 4: hipLaunchKernelGGL((token_loss_short_kernel<T, 4>), grid, block, 0, st, a); break;
+            case 8: hipLaunchKernelGGL((token_loss_short_kernel<T, 8>), grid, block, 0, st, a); break;
+            case 16: hipLaunchKernelGGL((token_loss_short_kernel<T, 16>), grid, block, 0, st, a); break;
+            case 32: hipLaunchKernelGGL((token_loss_short_kernel<T, 32>), grid, block, 0, st, a); break;
+            default: hipLaunchKernelGGL((token_loss_short_kernel<T, 64>), grid, block, 0, st, a); break;
+        }
+        return grid.x;
+    }
+    const dim3 grid((unsigned)a.R);
+    const int q = (int)(((long long)a.V * sizeof(T) + 15) / 16);       // accesses per row
+    if (q <= 64) hipLaunchKernelGGL((token_loss_kernel<T, 64, 1>), grid, dim3(64), 0, st, a);
+    else if (q <= 128) hipLaunchKernelGGL((token_loss_kernel<T, 64, 2>), grid, dim3(64), 0, st, a);
+    else if (q <= 256) hipLaunchKernelGGL((token_loss_kernel<T, 64, 4>), grid, dim3(64), 0, st, a);
+    else if (q <= 512) hipLaunchKernelGGL((token_loss_kernel<T, 64, 8>), grid, dim3(64), 0, st, a);
+    else if (q <= 1024) hipLaunchKernelGGL((token_loss_kernel<T, 256, 4>), grid, dim3(256), 0, st, a);
+    else if (q <= 2048) hipLaunchKernelGGL((token_loss_kernel<T, 256, 8>), grid, dim3(256), 0, st, a);
+    else if (q <= 4096) hipLaunchKernelGGL((token_loss_kernel<T, 1024, 4>), grid, dim3(1024), 0, st, a);
+    else if (q <= 8192) hipLaunchKernelGGL((token_loss_kernel<T, 1024, 8>), grid, dim3(1024), 0, st, a);
+    else if (q <= 16384) hipLaunchKernelGGL((token_loss_kernel<T, 1024, 16>), grid, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((token_loss_kernel<T, 1024, 0>), grid, dim3(1024), 0, st, a);
+    return a.R;
+}
+
+static long long partial_rows(long long R, int V) {
+    const int lanes = short_lanes(V);
+    return lanes <= kShortLanes ? (R * lanes + kShortThreads - 1) / kShortThreads : R;
+}
+
+// workgroups of the first stage of the statistics; 0: one stage
+static long long stats_blocks(long long rows) { return rows > kStatsRows ? (rows + kStatsRows - 1) / kStatsRows : 0; }
+
 extern "C" long long ag_token_policy_loss_workspace_bytes(long long R, int V) {
     if (R <= 0 || V <= 0) return 0;
-    return (4 + R * kSums) * (long long)sizeof(float);
+    const long long rows = partial_rows(R, V);
+    return 16 + stats_blocks(rows) * kSums * (long long)sizeof(double) + rows * kSums * (long long)sizeof(float);
 }
 
 extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
@@ -176,13 +486,20 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     if (p->dtype < AG_F32 || p->dtype > AG_F16 || p->R0 > 0x7fffffffLL / p->R1) return AG_ERR_UNSUPPORTED;
     const long long R = p->R0 * p->R1;
     if (p->workspace_bytes < ag_token_policy_loss_workspace_bytes(R, p->V)) return AG_ERR_INVALID_ARG;
-    float* count = (float*)p->workspace_dev;
+    float* count = (float*)p->workspace_dev;                 // 4 floats, then the stages' sums, then the rows' terms
+    const long long blocks = stats_blocks(partial_rows(R, p->V));
+    double* sums = (double*)(count + 4);
     const LossArgs a{p->logits_dev, p->actions_dev, p->old_logp_dev, p->advantages_dev, p->ref_logp_dev, p->mask_dev, p->dlogits_dev, count,
-                     count + 4, nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef, p->entropy_coef};
+                     (float*)(sums + blocks * kSums), nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef, p->entropy_coef};
     hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p->mask_dev, R, count);
-    AG_FOR_DTYPE(p->dtype, hipLaunchKernelGGL((token_loss_kernel<T>), dim3((unsigned)R), dim3(kThreads), 0, (hipStream_t)stream, a));
-    hipLaunchKernelGGL(stats_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, a.rows, R, count, p->ref_logp_dev ? p->kl_coef : 0.0f,
-                       p->entropy_coef, p->stats_dev);
+    long long rows = 0;
+    AG_FOR_DTYPE(p->dtype, rows = launch_rows<T>(a, stream));
+    const float kl = p->ref_logp_dev ? p->kl_coef : 0.0f;
+    if (blocks) {
+        hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a.partials, rows, sums);
+        hipLaunchKernelGGL((stats_kernel<double>), dim3(1), dim3(256), 0, (hipStream_t)stream, sums, blocks, count, kl, p->entropy_coef, p->stats_dev);
+    } else
+        hipLaunchKernelGGL((stats_kernel<float>), dim3(1), dim3(256), 0, (hipStream_t)stream, a.partials, rows, count, kl, p->entropy_coef, p->stats_dev);
     return seq_status();
 }
 
@@ -192,7 +509,7 @@ extern "C" int ag_token_logp(const void* logits, long long R0, long long R1, lon
     if (dtype < AG_F32 || dtype > AG_F16 || R0 > 0x7fffffffLL / R1) return AG_ERR_UNSUPPORTED;
     const LossArgs a{logits, actions, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, logp, entropy, R1, s0, s1, R0 * R1, V,
                      0.0f, 0.0f, 0.0f};
-    AG_FOR_DTYPE(dtype, hipLaunchKernelGGL((token_loss_kernel<T>), dim3((unsigned)a.R), dim3(kThreads), 0, (hipStream_t)stream, a));
+    AG_FOR_DTYPE(dtype, (void)launch_rows<T>(a, stream));
     return seq_status();
 }
 
