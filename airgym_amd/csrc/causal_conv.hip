@@ -145,17 +145,16 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGrad
     out[W] = db;
 }
 
-// one thread per parameter: the partial rows in order
-__global__ __launch_bounds__(kThreads) void conv_params_kernel(const float* partials, int rows, int D, int W, float* dw, float* db) {
-    const int i = blockIdx.x * kThreads + threadIdx.x;
-    const int n = D * (W + 1);
-    if (i >= n) return;
-    float s = 0.0f;
-    for (int r = 0; r < rows; r++) s += partials[(long long)r * n + i];
-    const int d = i / (W + 1), k = i - d * (W + 1);
-    if (k < W) dw[d * W + k] = s;
-    else if (db) db[d] = s;
-}
+struct ConvParams {
+    float *dw, *db;
+    int W;
+    __device__ __forceinline__ void operator()(long long i, float s) const {
+        const long long d = i / (W + 1);
+        const int k = (int)(i - d * (W + 1));
+        if (k < W) dw[d * W + k] = s;
+        else if (db) db[d] = s;
+    }
+};
 
 template <typename T, int W>
 __global__ __launch_bounds__(kThreads) void conv_step_kernel(const T* x, long long xb, T* state, const float* weight, const float* bias,
@@ -240,9 +239,7 @@ extern "C" int ag_causal_conv_bwd(const ag_conv_args* p, const ag_conv_grads* q,
     const ConvGradArgs g{q->dy_dev, q->dstate_out_dev, q->dx_dev, q->dstate_dev, (float*)q->workspace_dev, q->dy_sb, q->dy_st, rows};
     const dim3 grid((unsigned)(((long long)rows * a.D + kThreads - 1) / kThreads));
     AG_FOR_DTYPE(p->dtype, AG_FOR_TAPS(p->W, hipLaunchKernelGGL((conv_bwd_kernel<T, W>), grid, dim3(kThreads), 0, (hipStream_t)stream, a, g)));
-    const int n = a.D * (p->W + 1);
-    hipLaunchKernelGGL(conv_params_kernel, dim3((n + kThreads - 1) / kThreads), dim3(kThreads), 0, (hipStream_t)stream, g.partials, rows, a.D,
-                       p->W, q->dweight_dev, q->dbias_dev);
+    launch_sum_rows(g.partials, rows, (long long)a.D * (p->W + 1), ConvParams{q->dweight_dev, q->dbias_dev, p->W}, stream);
     return seq_status();
 }
 

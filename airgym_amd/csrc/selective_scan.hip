@@ -3,17 +3,21 @@
 //   dt = softplus(delta + bias);  h_t = exp(dt A) h_{t-1} + dt B_t u_t;  y_t = C_t . h_t + D u_t;  out = y z sigmoid(z)
 //   (per channel d a state of N numbers; B_t, C_t shared by the channels of a group; h := 0 before a step flagged as a reset)
 //
-// Layout.  A workgroup owns 64 consecutive channels of one group and walks along time in tiles of 16 steps; wave w owns states
-// 4w .. 4w+3 of all 64 channels (lane = channel), so N = 16 is four waves.  What does not depend on the state index - softplus, the
-// products dt u, the gate - is formed once per (step, channel) by whichever wave stages that row and goes through LDS; per (step,
-// channel, state) there remain one multiply, one v_exp_f32, one multiply and two FMAs.  The sums over states (y, and in the backward
-// the two sums behind du and ddelta) are joined through LDS, in a fixed order.
+// Layout.  A workgroup owns 64 consecutive channels of one group and walks along time in tiles; wave w owns states 4w .. 4w+3 of all
+// 64 channels (lane = channel), so N = 16 is four waves.  What does not depend on the state index - softplus, the products dt u, the
+// gate - is formed once per (step, channel) by whichever wave stages that row and goes through LDS; per (step, channel, state) there
+// remain one multiply, one v_exp_f32, one multiply and two FMAs.  The sums over states (y, and in the backward the two sums behind du
+// and ddelta) are joined through LDS, in a fixed order.
 // The vector ALU bounds these kernels (v_exp_f32 takes four issue slots of the eight per state), the bytes come second.
+// Few rows.  When sequences and channels alone do not fill the chip, time is cut into chunks: a first pass finds what each chunk makes
+// of a zero state (backward: of a zero gradient) and the sum of its time steps - exp(A sum dt) is the chunk's decay -, the main pass
+// starts each chunk from those of the chunks before (behind) it.
 #include "seq_common.hpp"
 
 namespace {
 
-constexpr int kTile = 16;              // steps per tile
+constexpr int kTile = 16;              // steps per tile of the forward
+constexpr int kBack = 8;               // steps per tile of the backward, which keeps their states in registers
 constexpr int kLanes = 64;             // channels per workgroup
 
 struct ScanArgs {
@@ -24,8 +28,10 @@ struct ScanArgs {
     long long ub, ut, db, dt, zb, zt, bb, bt, bg, cb, ct, cg, rb, rt;
     void* out;
     float *s1, *ckpt;
+    float *chunk_h, *chunk_dt;         // [B, chunks, D, N], [B, chunks, D]: what a chunk makes of nothing, and its sum of dt (NaN: reset)
     int B, T, D, N, G, softplus;
-    int Dg, nb, tiles;                 // channels per group, workgroups per group, tiles of T
+    int Dg, nb;                        // channels per group, workgroups per group
+    int chunks, steps;                 // chunks of time, steps in each (a multiple of both tiles)
 };
 
 struct ScanGradArgs {
@@ -38,100 +44,180 @@ struct ScanGradArgs {
     int rows;                          // workgroups along the batch
 };
 
-// reset flags of the tile's steps as a wave-uniform bit mask
+// Which 64 channels, row of the batch and chunk a workgroup has.
+struct Place {
+    int lane, w, g, cb, row, chunk, d0, d;      // d0: first channel of the workgroup, d: the lane's (clamped when it has none)
+    bool live;
+};
+__device__ __forceinline__ Place place_of(const ScanArgs& a) {
+    Place p;
+    p.lane = threadIdx.x & 63;
+    p.w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    unsigned i = blockIdx.x;
+    p.cb = i % a.nb, i /= a.nb;
+    p.g = i % a.G, i /= a.G;
+    p.chunk = i % a.chunks;
+    p.row = i / a.chunks;
+    const int ch = p.cb * kLanes + p.lane;
+    p.live = ch < a.Dg;
+    p.d0 = p.g * a.Dg + p.cb * kLanes;
+    p.d = p.live ? p.d0 + p.lane : p.g * a.Dg + a.Dg - 1;
+    return p;
+}
+
+// reset flags of nv steps from t0 as a wave-uniform bit mask
 __device__ __forceinline__ unsigned reset_bits(const ScanArgs& a, int b, int t0, int nv, int lane) {
     if (!a.resets) return 0;
     const bool f = lane < nv && a.resets[b * a.rb + (t0 + lane) * a.rt] != 0;
-    return (unsigned)__ballot(f);
+    return __builtin_amdgcn_readfirstlane((unsigned)__ballot(f));
 }
 
 __device__ __forceinline__ float time_step(const ScanArgs& a, float raw) { return a.softplus ? softplus(raw) : raw; }
 
-template <typename T, int NG>
+// a branch that stays one: a select in its place would cost every step what only a reset needs
+#define AG_RARE(cond) if (__builtin_expect(cond, 0)) if (([]() __attribute__((always_inline)) { asm volatile(""); }(), true))
+
+// state (or gradient of a state) that chunk `chunk` starts from, folded over the chunks first .. last - 1 (step +-1) before it
+__device__ __forceinline__ void fold_chunks(const ScanArgs& a, int b, int d, int w, int first, int last, int step, const float* A2, float* h) {
+    for (int c = first; c != last; c += step) {
+        const long long at = ((long long)b * a.chunks + c) * a.D + d;
+        const float sum = a.chunk_dt[at];
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (4 * w + j < a.N) {
+                const float keep = sum == sum ? exp2_hw(sum * A2[j]) * h[j] : 0.0f;
+                h[j] = keep + a.chunk_h[at * a.N + 4 * w + j];
+            }
+    }
+}
+
+// kStates: the first pass over chunks (every chunk but the last; no outputs but chunk_h and chunk_dt).  Otherwise the scan itself.
+template <typename T, int NG, bool kStates>
 __global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
-    constexpr int kRows = kTile / NG, kStates = 4 * NG;
-    __shared__ float sdt[kTile][kLanes], sdtu[kTile][kLanes], sy[NG][kTile][kLanes];
-    __shared__ alignas(16) float sB[kTile][kStates], sC[kTile][kStates];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cb = blockIdx.x % a.nb, g = (blockIdx.x / a.nb) % a.G, b = blockIdx.x / (a.nb * a.G);
-    const int ch = cb * kLanes + lane;
-    const bool live = ch < a.Dg;
-    const int d = g * a.Dg + (live ? ch : a.Dg - 1);
+    constexpr int kRows = kTile / NG, kWide = 4 * NG;
+    __shared__ float2 sdt[kTile][kLanes];                               // dt, dt u
+    __shared__ float sy[kStates ? 1 : NG][kTile][kLanes];
+    __shared__ alignas(16) float sB[kTile][kWide], sC[kTile][kWide];
+    const Place p = place_of(a);
+    const int lane = p.lane, w = p.w, b = p.row, d = p.d;
     const int len = seq_len(a.lengths, b, a.T);
-    const T* u = (const T*)a.u + b * a.ub + d;
-    const T* delta = (const T*)a.delta + b * a.db + d;
-    const T* z = a.z ? (const T*)a.z + b * a.zb + d : nullptr;
-    const T* Bm = (const T*)a.Bm + b * a.bb + g * a.bg;
-    const T* Cm = (const T*)a.Cm + b * a.cb + g * a.cg;
-    T* out = (T*)a.out + (long long)b * a.T * a.D + d;
+    const int from = p.chunk * a.steps, to = min(from + a.steps, a.T), end = min(to, len);
+    if (kStates && p.chunk == a.chunks - 1) return;
+    const T* u = (const T*)a.u + b * a.ub;
+    const T* delta = (const T*)a.delta + b * a.db;
+    const T* z = a.z ? (const T*)a.z + b * a.zb : nullptr;
+    const T* Bm = (const T*)a.Bm + b * a.bb + p.g * a.bg;
+    const T* Cm = (const T*)a.Cm + b * a.cb + p.g * a.cg;
+    T* out = (T*)a.out + (long long)b * a.T * a.D;
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
+    const bool gate = !kStates && z;
 
     float A2[4], h[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int n = 4 * w + j;
         A2[j] = n < a.N ? a.A[(long long)d * a.N + n] * kLog2e : 0.0f;
-        h[j] = n < a.N && a.s0 ? a.s0[((long long)b * a.D + d) * a.N + n] : 0.0f;
+        h[j] = !kStates && n < a.N && a.s0 ? a.s0[((long long)b * a.D + d) * a.N + n] : 0.0f;
     }
-    const int brow = threadIdx.x / kStates, bn = threadIdx.x % kStates;
-    for (int t0 = 0; t0 < len; t0 += kTile) {
-        const int nv = min(kTile, len - t0);
-        if (a.ckpt && t0 && live)
+    if (!kStates && (from < end || (len == 0 && p.chunk == 0))) fold_chunks(a, b, d, w, 0, p.chunk, 1, A2, h);
+
+    const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
+    T ru[kRows], rd[kRows], rz[kRows], rB, rC;
+    auto load = [&](int t0) __attribute__((always_inline)) {            // the tile's rows, as they are stored
+        const int nv = end - t0;
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (4 * w + j < a.N)
-                    a.ckpt[(((long long)b * (a.tiles - 1) + t0 / kTile - 1) * a.D + d) * a.N + 4 * w + j] = h[j];
+        for (int k = 0; k < kRows; k++) {
+            const int t = t0 + w + k * NG;
+            if (w + k * NG < nv) {
+                ru[k] = (u + t * a.ut)[d];
+                rd[k] = (delta + t * a.dt)[d];
+                if (gate) rz[k] = (z + t * a.zt)[d];
+            }
+        }
+        const bool bl = brow < nv && bn < a.N;
+        rB = bl ? Bm[(t0 + brow) * a.bt + bn] : from_f32<T>(0.0f);
+        if (!kStates) rC = bl ? Cm[(t0 + brow) * a.ct + bn] : from_f32<T>(0.0f);
+    };
+    float total = 0.0f;                                                 // kStates: sum of dt over the rows this wave staged
+    bool any_cut = false;
+    if (from < end) load(from);
+    for (int t0 = from; t0 < end; t0 += kTile) {
+        const int nv = min(kTile, end - t0);
         float uu[kRows], zz[kRows];
 #pragma unroll
         for (int k = 0; k < kRows; k++) {
-            const int r = w + k * NG, t = t0 + r;
+            const int r = w + k * NG;
             float dt = 0.0f;
             uu[k] = zz[k] = 0.0f;
             if (r < nv) {
-                uu[k] = to_f32(u[t * a.ut]);
-                dt = time_step(a, to_f32(delta[t * a.dt]) + bias);
-                if (z) zz[k] = to_f32(z[t * a.zt]);
+                uu[k] = to_f32(ru[k]);
+                dt = time_step(a, to_f32(rd[k]) + bias);
+                if (gate) zz[k] = to_f32(rz[k]);
             }
-            sdt[r][lane] = dt;
-            sdtu[r][lane] = dt * uu[k];
+            if (kStates) total += dt;
+            sdt[r][lane] = make_float2(dt, dt * uu[k]);
         }
-        const bool bl = brow < nv && bn < a.N;
-        sB[brow][bn] = bl ? to_f32(Bm[(t0 + brow) * a.bt + bn]) : 0.0f;
-        sC[brow][bn] = bl ? to_f32(Cm[(t0 + brow) * a.ct + bn]) : 0.0f;
+        sB[brow][bn] = to_f32(rB);
+        if (!kStates) sC[brow][bn] = to_f32(rC);
         const unsigned cut = reset_bits(a, b, t0, nv, lane);
+        any_cut |= cut != 0;
         __syncthreads();
-#pragma unroll 4
-        for (int r = 0; r < nv; r++) {
-            if (cut >> r & 1) h[0] = h[1] = h[2] = h[3] = 0.0f;
-            const float dt = sdt[r][lane], dtu = sdtu[r][lane];
-            const float4 Bv = *(const float4*)&sB[r][4 * w], Cv = *(const float4*)&sC[r][4 * w];
-            const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
-            float y = 0.0f;
+        if (t0 + kTile < end) load(t0 + kTile);                         // in flight behind the tile's arithmetic
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                h[j] = __builtin_fmaf(exp2_hw(dt * A2[j]), h[j], dtu * B4[j]);
-                y = __builtin_fmaf(C4[j], h[j], y);
+        for (int r = 0; r < kTile; r++) {                               // steps behind nv have dt = 0: they change nothing
+            if (r % 4 == 0 && r >= nv) break;
+            if (!kStates && r % kBack == 0 && a.ckpt && t0 + r && p.live) {
+                float* c = a.ckpt + (((long long)b * ((a.T - 1) / kBack) + (t0 + r) / kBack - 1) * a.D + d) * a.N + 4 * w;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (4 * w + j < a.N) c[j] = h[j];
             }
-            sy[w][r][lane] = y;
+            AG_RARE(cut >> r & 1) h[0] = h[1] = h[2] = h[3] = 0.0f;
+            const float2 q = sdt[r][lane];
+            const float4 Bv = *(const float4*)&sB[r][4 * w];
+            const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[j] = __builtin_fmaf(exp2_hw(q.x * A2[j]), h[j], q.y * B4[j]);
+            if (!kStates) {
+                const float4 Cv = *(const float4*)&sC[r][4 * w];
+                sy[w][r][lane] = __builtin_fmaf(Cv.x, h[0], Cv.y * h[1]) + __builtin_fmaf(Cv.z, h[2], Cv.w * h[3]);
+            }
         }
         __syncthreads();
+        if (!kStates)
 #pragma unroll
-        for (int k = 0; k < kRows; k++) {
-            const int r = w + k * NG;
-            float y = skip * uu[k];
+            for (int k = 0; k < kRows; k++) {
+                const int r = w + k * NG;
+                if (r >= nv) break;
+                float y = skip * uu[k];
 #pragma unroll
-            for (int v = 0; v < NG; v++) y += sy[v][r][lane];
-            if (z) y *= zz[k] * sigmoid(zz[k]);
-            if (r < nv && live) out[(long long)(t0 + r) * a.D] = from_f32<T>(y);
+                for (int v = 0; v < NG; v++) y += sy[v][r][lane];
+                if (gate) y *= zz[k] * sigmoid(zz[k]);
+                if (p.live) (out + (long long)(t0 + r) * a.D)[d] = from_f32<T>(y);
+            }
+    }
+    if (kStates) {
+        float* sums = (float*)sdt;
+        sums[w * kLanes + lane] = total;
+        __syncthreads();
+        if (!p.live) return;
+        const long long at = ((long long)b * a.chunks + p.chunk) * a.D + d;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (4 * w + j < a.N) a.chunk_h[at * a.N + 4 * w + j] = h[j];
+        if (w == 0) {
+            float s = 0.0f;
+            for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
+            a.chunk_dt[at] = any_cut ? __builtin_nanf("") : s;
         }
+        return;
     }
-    if (live) {
-        for (int t = len + w; t < a.T; t += NG) out[(long long)t * a.D] = from_f32<T>(0.0f);
-        if (a.s1)
+    if (!p.live) return;
+    for (int t = max(from, end) + w; t < to; t += NG) (out + (long long)t * a.D)[d] = from_f32<T>(0.0f);
+    if (a.s1 && (len ? from < len && len <= to : p.chunk == 0))         // the chunk with the last step
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (4 * w + j < a.N) a.s1[((long long)b * a.D + d) * a.N + 4 * w + j] = h[j];
-    }
+        for (int j = 0; j < 4; j++)
+            if (4 * w + j < a.N) a.s1[((long long)b * a.D + d) * a.N + 4 * w + j] = h[j];
 }
 
 // Sums of 8 registers over the 64 lanes, transposed on the way so that the number of live registers halves with every step (18
@@ -164,124 +250,152 @@ __device__ __forceinline__ int sum_lanes8_order(int lane) {
 
 // Reverse pass.  g_t = C_t dy_t + a_{t+1} g_{t+1} is the gradient of h_t; with q = g_t a_t h_{t-1}:
 //   s1 = sum_n g B, s2 = sum_n q A:  du = dt s1 + D dy,  ddt = u s1 + s2;   dA += q dt;   dB = sum_d g dt u;   dC = sum_d dy h
-// The states of a tile are run again from the state the forward left before it and kept, with the decays, in registers; tiles are
-// walked backwards.  A workgroup takes every `rows`-th sequence, so that dA, dD and the bias gradient stay in registers meanwhile.
-template <typename T, int NG, bool kResets>
+// The states of a tile of 8 steps are run again from the state the forward left before it and kept, with the decays, in registers;
+// tiles are walked backwards.  16 steps per tile took 326 registers (one wave per SIMD) and five times as long.  A workgroup takes
+// every `rows`-th sequence, so that dA, dD and the bias gradient stay in registers meanwhile.
+// dB and dC are sums over channels, that is over lanes: two steps' four values at a time, transposed on the way.
+
+// kCarry: the first pass over chunks (every chunk but the first): what the chunk hands back to the one before when nothing reaches it
+// from behind, and its sum of dt.
+template <typename T, int NG, bool kCarry>
 __global__ __launch_bounds__(kLanes* NG) void scan_bwd_kernel(ScanArgs a, ScanGradArgs q) {
-    constexpr int kRows = kTile / NG, kStates = 4 * NG;
-    __shared__ float sdt[kTile][kLanes], sdtu[kTile][kLanes], sdy[kTile][kLanes];
-    __shared__ float sy[NG][kTile][kLanes], ss1[NG][kTile][kLanes], ss2[NG][kTile][kLanes];
-    __shared__ alignas(16) float sB[kTile][kStates], sC[kTile][kStates];
-    __shared__ float sdB[kTile][kStates], sdC[kTile][kStates];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int cb = blockIdx.x % a.nb, g = (blockIdx.x / a.nb) % a.G, row = blockIdx.x / (a.nb * a.G);
-    const int ch = cb * kLanes + lane;
-    const bool live = ch < a.Dg;
-    const int d = g * a.Dg + (live ? ch : a.Dg - 1);
+    constexpr int kRows = kBack / NG, kWide = 4 * NG;
+    __shared__ float2 sdt[kBack][kLanes];                               // dt, dt u
+    __shared__ float sdy[kBack][kLanes];
+    __shared__ float sy[kCarry ? 1 : NG][kBack][kLanes], ss1[kCarry ? 1 : NG][kBack][kLanes], ss2[kCarry ? 1 : NG][kBack][kLanes];
+    __shared__ alignas(16) float sBC[2][kBack][kWide], sdBC[2][kBack][kWide];
+    const Place p = place_of(a);
+    if (kCarry && p.chunk == 0) return;
+    const int lane = p.lane, w = p.w, d = p.d;
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
-    const int brow = threadIdx.x / kStates, bn = threadIdx.x % kStates;
-    float A1[4], dA[4], dD = 0.0f, dbias = 0.0f;
+    // 8 rows of B and of C: 64 NG values for 64 NG threads
+    const int bc = threadIdx.x / (kBack * kWide), brow = threadIdx.x / kWide % kBack, bn = threadIdx.x % kWide;
+    float A1[4], A2[4], dA[4], dD = 0.0f, dbias = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int n = 4 * w + j;
         A1[j] = n < a.N ? a.A[(long long)d * a.N + n] : 0.0f;
+        A2[j] = A1[j] * kLog2e;
         dA[j] = 0.0f;
     }
-    for (int b = row; b < a.B; b += q.rows) {
+    for (int b = p.row; b < a.B; b += q.rows) {
         const int len = seq_len(a.lengths, b, a.T);
-        const T* u = (const T*)a.u + b * a.ub + d;
-        const T* delta = (const T*)a.delta + b * a.db + d;
-        const T* z = a.z ? (const T*)a.z + b * a.zb + d : nullptr;
-        const T* dout = (const T*)q.dout + b * q.ob + d;
-        const T* Bm = (const T*)a.Bm + b * a.bb + g * a.bg;
-        const T* Cm = (const T*)a.Cm + b * a.cb + g * a.cg;
-        const long long o = (long long)b * a.T * a.D + d;
-        float carry[4];                          // a_{t+1} g_{t+1}
+        const int from = p.chunk * a.steps, to = min(from + a.steps, a.T);
+        const T* u = (const T*)a.u + b * a.ub;
+        const T* delta = (const T*)a.delta + b * a.db;
+        const T* z = a.z ? (const T*)a.z + b * a.zb : nullptr;
+        const T* dout = (const T*)q.dout + b * q.ob;
+        const T* BC = bc ? (const T*)a.Cm + b * a.cb + p.g * a.cg : (const T*)a.Bm + b * a.bb + p.g * a.bg;
+        const long long bct = bc ? a.ct : a.bt;
+        const long long o = (long long)b * a.T * a.D;
+        float carry[4];                                                 // a_{t+1} g_{t+1}
 #pragma unroll
         for (int j = 0; j < 4; j++)
-            carry[j] = q.ds1 && live && 4 * w + j < a.N ? q.ds1[((long long)b * a.D + d) * a.N + 4 * w + j] : 0.0f;
-        for (int tile = a.tiles - 1; tile >= 0; tile--) {
-            const int t0 = tile * kTile, nv = max(0, min(kTile, len - t0)), nt = min(kTile, a.T - t0);
+            carry[j] = !kCarry && q.ds1 && p.live && 4 * w + j < a.N ? q.ds1[((long long)b * a.D + d) * a.N + 4 * w + j] : 0.0f;
+        if (!kCarry) fold_chunks(a, b, d, w, a.chunks - 1, p.chunk, -1, A2, carry);
+        float total = 0.0f;
+        bool any_cut = false;
+        for (int t0 = from + (to - from - 1) / kBack * kBack; t0 >= from; t0 -= kBack) {
+            const int nv = max(0, min(kBack, len - t0)), nt = min(kBack, a.T - t0);
             float uu[kRows], dts[kRows], sg[kRows], zz[kRows], go[kRows];
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
                 const int r = w + k * NG, t = t0 + r;
                 uu[k] = dts[k] = sg[k] = zz[k] = go[k] = 0.0f;
                 float dy = 0.0f;
-                if (r < nv && live) {
-                    uu[k] = to_f32(u[t * a.ut]);
-                    const float raw = to_f32(delta[t * a.dt]) + bias;
+                if (r < nv && p.live) {
+                    if (!kCarry) uu[k] = to_f32((u + t * a.ut)[d]);
+                    const float raw = to_f32((delta + t * a.dt)[d]) + bias;
                     dts[k] = time_step(a, raw);
                     sg[k] = a.softplus ? sigmoid(raw) : 1.0f;
-                    go[k] = dy = to_f32(dout[t * q.ot]);
+                    go[k] = dy = to_f32((dout + t * q.ot)[d]);
                     if (z) {
-                        zz[k] = to_f32(z[t * a.zt]);
+                        zz[k] = to_f32((z + t * a.zt)[d]);
                         dy *= zz[k] * sigmoid(zz[k]);
                     }
                 }
-                sdt[r][lane] = dts[k];
-                sdtu[r][lane] = dts[k] * uu[k];
+                sdt[r][lane] = make_float2(dts[k], dts[k] * uu[k]);
                 sdy[r][lane] = dy;
+                if (kCarry) total += dts[k];
             }
-            const bool bl = brow < nv && bn < a.N;
-            sB[brow][bn] = bl ? to_f32(Bm[(t0 + brow) * a.bt + bn]) : 0.0f;
-            sC[brow][bn] = bl ? to_f32(Cm[(t0 + brow) * a.ct + bn]) : 0.0f;
+            sBC[bc][brow][bn] = brow < nv && bn < a.N ? to_f32((BC + (t0 + brow) * bct)[bn]) : 0.0f;
             const unsigned cut = reset_bits(a, b, t0, nv, lane);
+            any_cut |= cut != 0;
             __syncthreads();
+            if (kCarry) {
+#pragma unroll
+                for (int r = kBack - 1; r >= 0; r--) {
+                    const float4 Cv = *(const float4*)&sBC[1][r][4 * w];
+                    const float C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w}, dy = sdy[r][lane], dt = sdt[r][lane].x;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) carry[j] = exp2_hw(dt * A2[j]) * __builtin_fmaf(C4[j], dy, carry[j]);
+                    AG_RARE(cut >> r & 1) carry[0] = carry[1] = carry[2] = carry[3] = 0.0f;
+                }
+                __syncthreads();
+                continue;
+            }
             if (nv) {
-                float h[kTile + 1][4], e[kTile][4];
-                const float* from = tile ? a.ckpt + ((long long)b * (a.tiles - 1) + tile - 1) * a.D * a.N
-                                         : (a.s0 ? a.s0 + (long long)b * a.D * a.N : nullptr);
+                float h[kBack][4], e[kBack][4], now[4], v[8], sums = 0.0f;      // h[r]: the state step r starts from
+                const float* start = t0 ? a.ckpt + ((long long)b * ((a.T - 1) / kBack) + t0 / kBack - 1) * a.D * a.N
+                                        : (a.s0 ? a.s0 + (long long)b * a.D * a.N : nullptr);
 #pragma unroll
-                for (int j = 0; j < 4; j++) h[0][j] = from && live && 4 * w + j < a.N ? from[(long long)d * a.N + 4 * w + j] : 0.0f;
+                for (int j = 0; j < 4; j++) now[j] = start && p.live && 4 * w + j < a.N ? start[(long long)d * a.N + 4 * w + j] : 0.0f;
+                const int order = sum_lanes8_order(lane), odd = order >> 2, mine = lane & 3;
 #pragma unroll
-                for (int r = 0; r < kTile; r++) {      // steps behind nv have dt = 0: decay 1, no input
-                    const float dt = sdt[r][lane], dtu = sdtu[r][lane];
-                    const float4 Bv = *(const float4*)&sB[r][4 * w], Cv = *(const float4*)&sC[r][4 * w];
+                for (int r = 0; r < kBack; r++) {      // steps behind nv have dt = dy = 0: decay 1, no input
+                    AG_RARE(cut >> r & 1) now[0] = now[1] = now[2] = now[3] = 0.0f;
+                    const float2 s = sdt[r][lane];
+                    const float dy = sdy[r][lane];
+                    const float4 Bv = *(const float4*)&sBC[0][r][4 * w], Cv = *(const float4*)&sBC[1][r][4 * w];
                     const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
                     float y = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        const bool fresh = kResets && (cut >> r & 1);     // the state before is cleared, whatever it holds
-                        e[r][j] = fresh ? 0.0f : exp2_hw(dt * (A1[j] * kLog2e));
-                        h[r + 1][j] = __builtin_fmaf(e[r][j], fresh ? 0.0f : h[r][j], dtu * B4[j]);
-                        y = __builtin_fmaf(C4[j], h[r + 1][j], y);
+                        h[r][j] = now[j];
+                        e[r][j] = exp2_hw(s.x * A2[j]);
+                        now[j] = __builtin_fmaf(e[r][j], now[j], s.y * B4[j]);
+                        y = __builtin_fmaf(C4[j], now[j], y);
+                        v[(r & 1) * 4 + j] = dy * now[j];
                     }
                     sy[w][r][lane] = y;
+                    if (r & 1) {
+                        const float x = sum_lanes8(v, lane);
+                        sums = mine == r >> 1 ? x : sums;
+                    }
                 }
-                float sums = 0.0f;
+                if (!(lane & 4)) sdBC[1][2 * mine + odd][4 * w + (order & 3)] = sums;
 #pragma unroll
-                for (int r = kTile - 1; r >= 0; r--) {
-                    const float dt = sdt[r][lane], dtu = sdtu[r][lane], dy = sdy[r][lane];
-                    const float4 Bv = *(const float4*)&sB[r][4 * w], Cv = *(const float4*)&sC[r][4 * w];
+                for (int r = kBack - 1; r >= 0; r--) {
+                    const float2 s = sdt[r][lane];
+                    const float dy = sdy[r][lane];
+                    const float4 Bv = *(const float4*)&sBC[0][r][4 * w], Cv = *(const float4*)&sBC[1][r][4 * w];
                     const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
-                    float s1 = 0.0f, s2 = 0.0f, v[8];
+                    float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const float gr = __builtin_fmaf(C4[j], dy, carry[j]);
-                        v[j] = gr * dtu;
-                        v[4 + j] = dy * h[r + 1][j];
+                        v[(r & 1) * 4 + j] = gr * s.y;
                         s1 = __builtin_fmaf(gr, B4[j], s1);
-                        carry[j] = kResets && (cut >> r & 1) ? 0.0f : e[r][j] * gr;
-                        const float qq = kResets && (cut >> r & 1) ? 0.0f : carry[j] * h[r][j];
+                        carry[j] = e[r][j] * gr;
+                        const float qq = carry[j] * h[r][j];
                         s2 = __builtin_fmaf(qq, A1[j], s2);
-                        dA[j] = __builtin_fmaf(qq, dt, dA[j]);
+                        dA[j] = __builtin_fmaf(qq, s.x, dA[j]);
                     }
+                    AG_RARE(cut >> r & 1) carry[0] = carry[1] = carry[2] = carry[3] = 0.0f;      // h[r] is 0 there already
                     ss1[w][r][lane] = s1;
                     ss2[w][r][lane] = s2;
-                    // lanes 8g + (r & 7) keep step r's sums; eight steps later all lanes have one to store
-                    const float s = sum_lanes8(v, lane);
-                    sums = (lane & 7) == (r & 7) ? s : sums;
-                    if ((r & 7) == 0) {
-                        const int i = sum_lanes8_order(lane), rr = r + (lane & 7);
-                        (i < 4 ? sdB : sdC)[rr][4 * w + (i & 3)] = sums;
+                    if (!(r & 1)) {
+                        const float x = sum_lanes8(v, lane);
+                        sums = mine == r >> 1 ? x : sums;
                     }
                 }
+                if (!(lane & 4)) sdBC[0][2 * mine + odd][4 * w + (order & 3)] = sums;
             }
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
                 const int r = w + k * NG;
+                if (r >= nt) break;
                 float y = skip * uu[k], s1 = 0.0f, s2 = 0.0f;
                 if (r < nv) {
 #pragma unroll
@@ -294,70 +408,83 @@ __global__ __launch_bounds__(kLanes* NG) void scan_bwd_kernel(ScanArgs a, ScanGr
                     dy *= zz[k] * s;
                 }
                 const float draw = (uu[k] * s1 + s2) * sg[k];
-                if (r < nt && live) {
+                if (p.live) {
                     const long long at = o + (long long)(t0 + r) * a.D;
-                    ((T*)q.du)[at] = from_f32<T>(__builtin_fmaf(dts[k], s1, skip * dy));
-                    ((T*)q.ddelta)[at] = from_f32<T>(draw);
-                    if (z) ((T*)q.dz)[at] = from_f32<T>(dzv);
+                    ((T*)q.du + at)[d] = from_f32<T>(__builtin_fmaf(dts[k], s1, skip * dy));
+                    ((T*)q.ddelta + at)[d] = from_f32<T>(draw);
+                    if (z) ((T*)q.dz + at)[d] = from_f32<T>(dzv);
                 }
                 dD = __builtin_fmaf(dy, uu[k], dD);
                 dbias += draw;
             }
             if (brow < nt && bn < a.N) {
-                const float vB = brow < nv ? sdB[brow][bn] : 0.0f, vC = brow < nv ? sdC[brow][bn] : 0.0f;
-                const long long at = (((long long)b * a.T + t0 + brow) * a.G + g) * a.N + bn, n = (long long)a.B * a.T * a.G * a.N;
-                if (q.bc_partials) {
-                    q.bc_partials[(2 * cb) * n + at] = vB;
-                    q.bc_partials[(2 * cb + 1) * n + at] = vC;
-                } else {
-                    ((T*)q.dB)[at] = from_f32<T>(vB);
-                    ((T*)q.dC)[at] = from_f32<T>(vC);
-                }
+                const float v = brow < nv ? sdBC[bc][brow][bn] : 0.0f;
+                const long long at = (((long long)b * a.T + t0 + brow) * a.G + p.g) * a.N + bn, n = (long long)a.B * a.T * a.G * a.N;
+                if (q.bc_partials) q.bc_partials[(2 * p.cb + bc) * n + at] = v;
+                else ((T*)(bc ? q.dC : q.dB))[at] = from_f32<T>(v);
             }
         }
-        if (q.ds0 && live)
+        if (kCarry) {
+            float* sums = (float*)sdt;
+            sums[w * kLanes + lane] = total;
+            __syncthreads();
+            if (p.live) {
+                const long long at = ((long long)b * a.chunks + p.chunk) * a.D + d;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (4 * w + j < a.N) a.chunk_h[at * a.N + 4 * w + j] = carry[j];
+                if (w == 0) {
+                    float s = 0.0f;
+                    for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
+                    a.chunk_dt[at] = any_cut ? __builtin_nanf("") : s;
+                }
+            }
+            __syncthreads();
+        } else if (q.ds0 && p.live && p.chunk == 0)
 #pragma unroll
             for (int j = 0; j < 4; j++)
                 if (4 * w + j < a.N) q.ds0[((long long)b * a.D + d) * a.N + 4 * w + j] = carry[j];
     }
-    // this workgroup's row of partial parameter gradients: [rows, D, N + 2]
-    float* part = q.param_partials + ((long long)row * a.D + d) * (a.N + 2);
+    if (kCarry) return;
+    // this workgroup's row of partial parameter gradients: [rows chunks, D, N + 2]
+    float* part = q.param_partials + ((long long)(p.row * a.chunks + p.chunk) * a.D + d) * (a.N + 2);
     __syncthreads();
-    sdt[2 * w][lane] = dD, sdt[2 * w + 1][lane] = dbias;
+    float2* sums = &sdt[0][0];
+    sums[w * kLanes + lane] = make_float2(dD, dbias);
     __syncthreads();
-    if (!live) return;
+    if (!p.live) return;
 #pragma unroll
     for (int j = 0; j < 4; j++)
         if (4 * w + j < a.N) part[4 * w + j] = dA[j];
     if (w == 0) {
-        float s = 0.0f, p = 0.0f;
+        float s = 0.0f, t = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NG; v++) s += sdt[2 * v][lane], p += sdt[2 * v + 1][lane];
+        for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane].x, t += sums[v * kLanes + lane].y;
         part[a.N] = s;
-        part[a.N + 1] = p;
+        part[a.N + 1] = t;
     }
 }
 
-__global__ __launch_bounds__(256) void scan_params_kernel(const float* partials, int rows, int D, int N, float* dA, float* dD, float* dbias) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, n = (long long)D * (N + 2);
-    if (i >= n) return;
-    float s = 0.0f;
-    for (int r = 0; r < rows; r++) s += partials[r * n + i];
-    const int d = (int)(i / (N + 2)), k = (int)(i - (long long)d * (N + 2));
-    if (k < N) dA[(long long)d * N + k] = s;
-    else if (k == N) { if (dD) dD[d] = s; }
-    else if (dbias) dbias[d] = s;
-}
+struct ScanParams {
+    float *dA, *dD, *dbias;
+    int N;
+    __device__ __forceinline__ void operator()(long long i, float s) const {
+        const long long d = i / (N + 2);
+        const int k = (int)(i - d * (N + 2));
+        if (k < N) dA[d * N + k] = s;
+        else if (k == N) { if (dD) dD[d] = s; }
+        else if (dbias) dbias[d] = s;
+    }
+};
 
-template <typename T>
-__global__ __launch_bounds__(256) void scan_bc_kernel(const float* partials, int nb, long long n, T* dB, T* dC) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= 2 * n) return;
-    float s = 0.0f;
-    for (int c = 0; c < nb; c++) s += partials[c * 2 * n + i];
-    if (i < n) dB[i] = from_f32<T>(s);
-    else dC[i - n] = from_f32<T>(s);
-}
+template <typename T> struct ScanShared {
+    T *dB, *dC;
+    long long n;
+    __device__ __forceinline__ void operator()(long long i, float s) const {
+        if (i < n) dB[i] = from_f32<T>(s);
+        else dC[i - n] = from_f32<T>(s);
+    }
+};
 
 // One step: a channel's state is spread over L lanes, four numbers each, so that a wave moves 1 KB of states per access.
 template <typename T, int L>
@@ -394,9 +521,20 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     ((T*)a.out)[item] = from_f32<T>(y);
 }
 
-int tiles_of(int T) { return (T + kTile - 1) / kTile; }
 int groups_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 int channel_blocks(int D, int G) { return (D / G + kLanes - 1) / kLanes; }
+
+// Chunks of time.  1024 workgroups are four per CU; where sequences and channels give fewer, time is cut so that there are about that
+// many, in chunks of at least 64 steps (a multiple of 16): the first pass costs the chunks about as much again as the forward's states.
+struct Chunks { int count, steps; };
+Chunks chunks_of(int B, int T, int D, int G) {
+    const long long blocks = (long long)B * G * channel_blocks(D, G);
+    const long long want = (1024 + blocks - 1) / blocks;
+    long long steps = ((T + want - 1) / want + kTile - 1) / kTile * kTile;
+    if (steps < 64) steps = 64;
+    if (want == 1 || steps >= T) return Chunks{1, (T + kTile - 1) / kTile * kTile};
+    return Chunks{(int)((T + steps - 1) / steps), (int)steps};
+}
 
 // workgroups along the batch in the backward: a few per CU
 int grad_rows(int B, int D, int G) {
@@ -409,15 +547,23 @@ int check(const ag_scan_args* p) {
         return AG_ERR_INVALID_ARG;
     if (p->B <= 0 || p->T <= 0 || p->D <= 0 || p->G <= 0 || p->N <= 0 || p->D % p->G) return AG_ERR_INVALID_ARG;
     if (p->N > 32 || p->dtype < AG_F32 || p->dtype > AG_F16) return AG_ERR_UNSUPPORTED;
-    if ((long long)p->B * p->G * channel_blocks(p->D, p->G) > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
+    // the grid, with time in chunks: at most 1024 + B G channel blocks (or one per sequence and 64 channels)
+    if ((long long)p->B * p->G * channel_blocks(p->D, p->G) > 0x7fffffffLL - 4096) return AG_ERR_UNSUPPORTED;
     return AG_OK;
 }
 
 ScanArgs device_args(const ag_scan_args* p) {
+    const Chunks c = chunks_of(p->B, p->T, p->D, p->G);
     return ScanArgs{p->u_dev, p->delta_dev, p->z_dev, p->Bm_dev, p->Cm_dev, p->A_dev, p->Dskip_dev, p->delta_bias_dev, p->state_in_dev,
                     p->lengths_dev, p->resets_dev, p->u_sb, p->u_st, p->delta_sb, p->delta_st, p->z_sb, p->z_st, p->b_sb, p->b_st, p->b_sg,
-                    p->c_sb, p->c_st, p->c_sg, p->r_sb, p->r_st, p->out_dev, p->state_out_dev, p->ckpt_dev, p->B, p->T, p->D, p->N, p->G,
-                    p->softplus, p->D / p->G, channel_blocks(p->D, p->G), tiles_of(p->T)};
+                    p->c_sb, p->c_st, p->c_sg, p->r_sb, p->r_st, p->out_dev, p->state_out_dev, p->ckpt_dev, nullptr, nullptr, p->B, p->T,
+                    p->D, p->N, p->G, p->softplus, p->D / p->G, channel_blocks(p->D, p->G), c.count, c.steps};
+}
+
+// floats of chunk_h and chunk_dt
+long long chunk_floats(int B, int T, int D, int N, int G) {
+    const int c = chunks_of(B, T, D, G).count;
+    return c > 1 ? (long long)B * c * D * (N + 1) : 0;
 }
 
 }  // namespace
@@ -434,50 +580,58 @@ ScanArgs device_args(const ag_scan_args* p) {
 
 extern "C" long long ag_selective_scan_ckpt_floats(int B, int T, int D, int N) {
     if (B <= 0 || T <= 0 || D <= 0 || N <= 0) return 0;
-    return (long long)B * (tiles_of(T) - 1) * D * N;
+    return (long long)B * ((T - 1) / kBack) * D * N;
 }
 
 extern "C" long long ag_selective_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward) {
-    if (B <= 0 || T <= 0 || D <= 0 || N <= 0 || G <= 0 || D % G || !backward) return 0;
-    const int nb = channel_blocks(D, G);
-    const long long params = (long long)grad_rows(B, D, G) * D * (N + 2);
-    const long long bc = nb > 1 ? 2LL * nb * B * T * G * N : 0;
-    return (params + bc) * (long long)sizeof(float);
+    if (B <= 0 || T <= 0 || D <= 0 || N <= 0 || G <= 0 || D % G) return 0;
+    long long floats = chunk_floats(B, T, D, N, G);
+    if (backward) {
+        const int nb = channel_blocks(D, G);
+        floats += (long long)grad_rows(B, D, G) * chunks_of(B, T, D, G).count * D * (N + 2);
+        if (nb > 1) floats += 2LL * nb * B * T * G * N;
+    }
+    return floats * (long long)sizeof(float);
 }
 
 extern "C" int ag_selective_scan_fwd(const ag_scan_args* p, void* stream) {
     if (const int rc = check(p)) return rc;
     if (!p->out_dev) return AG_ERR_INVALID_ARG;
-    const ScanArgs a = device_args(p);
-    const dim3 grid((unsigned)((long long)a.B * a.G * a.nb));
-    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
+    ScanArgs a = device_args(p);
+    if (a.chunks > 1) {
+        if (!p->workspace_dev || p->workspace_bytes < ag_selective_scan_workspace_bytes(a.B, a.T, a.D, a.N, a.G, 0)) return AG_ERR_INVALID_ARG;
+        a.chunk_h = (float*)p->workspace_dev;
+        a.chunk_dt = a.chunk_h + (long long)a.B * a.chunks * a.D * a.N;
+    }
+    const dim3 grid((unsigned)((long long)a.B * a.chunks * a.G * a.nb));
+    if (a.chunks > 1)
+        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, true>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
+    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
     return seq_status();
 }
 
 extern "C" int ag_selective_scan_bwd(const ag_scan_args* p, const ag_scan_grads* s, void* stream) {
     if (const int rc = check(p)) return rc;
     if (!s || s->struct_size != sizeof(ag_scan_grads) || !s->dout_dev || !s->du_dev || !s->ddelta_dev || !s->dBm_dev || !s->dCm_dev ||
-        !s->dA_dev || !s->workspace_dev || (p->z_dev != nullptr) != (s->dz_dev != nullptr) || (p->T > kTile && !p->ckpt_dev))
+        !s->dA_dev || !s->workspace_dev || (p->z_dev != nullptr) != (s->dz_dev != nullptr) || (p->T > kBack && !p->ckpt_dev))
         return AG_ERR_INVALID_ARG;
     if (s->workspace_bytes < ag_selective_scan_workspace_bytes(p->B, p->T, p->D, p->N, p->G, 1)) return AG_ERR_INVALID_ARG;
-    const ScanArgs a = device_args(p);
+    ScanArgs a = device_args(p);
+    a.chunk_h = (float*)s->workspace_dev;
+    a.chunk_dt = a.chunk_h + (long long)a.B * a.chunks * a.D * a.N;
+    float* params = a.chunk_h + chunk_floats(a.B, a.T, a.D, a.N, a.G);
     const int rows = grad_rows(a.B, a.D, a.G);
-    float* params = (float*)s->workspace_dev;
-    float* bc = a.nb > 1 ? params + (long long)rows * a.D * (a.N + 2) : nullptr;
+    float* bc = a.nb > 1 ? params + (long long)rows * a.chunks * a.D * (a.N + 2) : nullptr;
     const ScanGradArgs q{s->dout_dev, s->dout_sb, s->dout_st, s->dstate_out_dev, s->du_dev, s->ddelta_dev, s->dz_dev, s->dBm_dev, s->dCm_dev,
                          s->dstate_in_dev, params, bc, rows};
-    const dim3 grid((unsigned)((long long)rows * a.G * a.nb));
-    if (a.resets)
+    const dim3 grid((unsigned)((long long)rows * a.chunks * a.G * a.nb));
+    if (a.chunks > 1)
         AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_bwd_kernel<T, NG, true>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a, q)));
-    else
-        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_bwd_kernel<T, NG, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a, q)));
-    const long long np = (long long)a.D * (a.N + 2);
-    hipLaunchKernelGGL(scan_params_kernel, dim3((unsigned)((np + 255) / 256)), dim3(256), 0, (hipStream_t)stream, params, rows, a.D, a.N,
-                       s->dA_dev, s->dDskip_dev, s->ddelta_bias_dev);
+    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_bwd_kernel<T, NG, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a, q)));
+    launch_sum_rows(params, rows * a.chunks, (long long)a.D * (a.N + 2), ScanParams{s->dA_dev, s->dDskip_dev, s->ddelta_bias_dev, a.N}, stream);
     if (bc) {
         const long long n = (long long)a.B * a.T * a.G * a.N;
-        AG_FOR_DTYPE(p->dtype, hipLaunchKernelGGL((scan_bc_kernel<T>), dim3((unsigned)((2 * n + 255) / 256)), dim3(256), 0, (hipStream_t)stream,
-                                                  bc, a.nb, n, (T*)s->dBm_dev, (T*)s->dCm_dev));
+        AG_FOR_DTYPE(p->dtype, launch_sum_rows(bc, a.nb, 2 * n, ScanShared<T>{(T*)s->dBm_dev, (T*)s->dCm_dev, n}, stream));
     }
     return seq_status();
 }

@@ -52,6 +52,33 @@ __device__ __forceinline__ int seq_len(const int* lengths, int b, int T) {
     return n < 0 ? 0 : (n > T ? T : n);
 }
 
+// Sums over the rows of a [rows, n] table, in a fixed order: a column per lane, `Parts` parts of the rows per column (so that a table
+// of few columns and many rows still has enough loads in flight), joined through LDS.  `out(i, sum)` puts column i's sum away.
+template <int Parts, typename Out>
+__global__ __launch_bounds__(64 * Parts) void sum_rows_kernel(const float* table, int rows, long long n, Out out) {
+    __shared__ float part[Parts][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const long long i = (long long)blockIdx.x * 64 + lane;
+    const int per = (rows + Parts - 1) / Parts, first = w * per, last = first + per < rows ? first + per : rows;
+    float s = 0.0f;
+    if (i < n)
+#pragma unroll 8
+        for (int r = first; r < last; r++) s += table[(long long)r * n + i];
+    part[w][lane] = s;
+    __syncthreads();
+    if (w || i >= n) return;
+#pragma unroll
+    for (int k = 1; k < Parts; k++) s += part[k][lane];
+    out(i, s);
+}
+
+template <typename Out>
+inline void launch_sum_rows(const float* table, int rows, long long n, Out out, void* stream) {
+    const dim3 grid((unsigned)((n + 63) / 64));
+    if (rows > 64) hipLaunchKernelGGL((sum_rows_kernel<16, Out>), grid, dim3(1024), 0, (hipStream_t)stream, table, rows, n, out);
+    else hipLaunchKernelGGL((sum_rows_kernel<4, Out>), grid, dim3(256), 0, (hipStream_t)stream, table, rows, n, out);
+}
+
 inline int seq_status() { return hipGetLastError() == hipSuccess ? AG_OK : AG_ERR_HIP; }
 
 }  // namespace

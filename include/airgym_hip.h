@@ -861,7 +861,7 @@ typedef struct ag_scan_args {
     const unsigned char* resets_dev;   /* [B, T], strides r_sb, r_st, or NULL */
     long long u_sb, u_st, delta_sb, delta_st, z_sb, z_st, b_sb, b_st, b_sg, c_sb, c_st, c_sg, r_sb, r_st;
     void* out_dev;                     /* forward: [B, T, D] contiguous */
-    float* state_out_dev;              /* forward: [B, D, N] or NULL (may be state_in_dev) */
+    float* state_out_dev;              /* forward: [B, D, N], not state_in_dev, or NULL */
     float* ckpt_dev;                   /* written by the forward, read by the backward; NULL: forward without backward */
     void* workspace_dev;
     long long workspace_bytes;

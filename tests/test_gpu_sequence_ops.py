@@ -153,6 +153,12 @@ SCAN = [  # B, T, D, N, G, lengths, resets, state, z, D, bias, softplus
     (1, 100, 20, 4, 1, None, 0.0, True, False, True, True, False),
     (5, 19, 130, 16, 2, [0, 19, 3, 16, 17], 0.2, True, True, True, True, True),
     (2, 30, 40, 20, 1, None, 1.0, True, True, True, True, True),
+    # long enough, with few enough rows, for time to be cut into chunks
+    (1, 300, 20, 16, 1, None, 0.0, True, True, True, True, True),
+    (3, 200, 12, 8, 2, [200, 64, 0], 0.0, True, True, True, True, True),
+    (2, 260, 9, 3, 1, [129, 260], 0.01, True, True, True, True, True),
+    (1, 129, 8, 32, 1, None, 0.05, False, False, True, True, True),
+    (2, 192, 8, 4, 1, [65, 192], 0.0, True, True, True, False, False),
 ]
 NAMES = ("u", "delta", "A", "B", "C", "D", "z", "bias", "state")
 
