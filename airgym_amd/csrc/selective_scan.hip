@@ -31,6 +31,7 @@ struct ScanArgs {
     float *chunk_h, *chunk_dt;         // [B, chunks, D, N], [B, chunks, D]: what a chunk makes of nothing, and its sum of dt (NaN: reset)
     int B, T, D, N, G, softplus;
     int Dg, nb;                        // channels per group, workgroups per group
+    int rows;                          // forward: workgroups along the batch
     int chunks, steps;                 // chunks of time, steps in each (a multiple of both tiles)
 };
 
@@ -77,21 +78,44 @@ __device__ __forceinline__ float time_step(const ScanArgs& a, float raw) { retur
 // a branch that stays one: a select in its place would cost every step what only a reset needs
 #define AG_RARE(cond) if (__builtin_expect(cond, 0)) if (([]() __attribute__((always_inline)) { asm volatile(""); }(), true))
 
+// element of a row at a lane's byte offset: the row is wave-uniform, so the access is a scalar base plus 32 bits per lane
+template <typename T> __device__ __forceinline__ T get(const T* row, unsigned bytes) { return *(const T*)((const char*)row + bytes); }
+template <typename T> __device__ __forceinline__ void put(T* row, unsigned bytes, T v) { *(T*)((char*)row + bytes) = v; }
+
+// a lane's four states in a row of N, zero where there are none: one access where the row is whole
+typedef float four_any4 __attribute__((ext_vector_type(4), aligned(4)));
+__device__ __forceinline__ void load4(const float* row, int w, int N, float* x) {
+    if (N % 4 == 0 && 4 * w < N) {
+        const four_any4 v = *(const four_any4*)(row + 4 * w);
+        x[0] = v[0], x[1] = v[1], x[2] = v[2], x[3] = v[3];
+    } else
+#pragma unroll
+        for (int j = 0; j < 4; j++) x[j] = 4 * w + j < N ? row[4 * w + j] : 0.0f;
+}
+__device__ __forceinline__ void store4(float* row, int w, int N, const float* x) {
+    if (N % 4 == 0 && 4 * w < N) *(four_any4*)(row + 4 * w) = four_any4{x[0], x[1], x[2], x[3]};
+    else
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (4 * w + j < N) row[4 * w + j] = x[j];
+}
+__device__ __forceinline__ void zero4(float* x) { x[0] = x[1] = x[2] = x[3] = 0.0f; }
+
 // state (or gradient of a state) that chunk `chunk` starts from, folded over the chunks first .. last - 1 (step +-1) before it
 __device__ __forceinline__ void fold_chunks(const ScanArgs& a, int b, int d, int w, int first, int last, int step, const float* A2, float* h) {
     for (int c = first; c != last; c += step) {
         const long long at = ((long long)b * a.chunks + c) * a.D + d;
         const float sum = a.chunk_dt[at];
+        float x[4];
+        load4(a.chunk_h + at * a.N, w, a.N, x);
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (4 * w + j < a.N) {
-                const float keep = sum == sum ? exp2_hw(sum * A2[j]) * h[j] : 0.0f;
-                h[j] = keep + a.chunk_h[at * a.N + 4 * w + j];
-            }
+        for (int j = 0; j < 4; j++) h[j] = (sum == sum ? exp2_hw(sum * A2[j]) * h[j] : 0.0f) + x[j];
     }
 }
 
 // kStates: the first pass over chunks (every chunk but the last; no outputs but chunk_h and chunk_dt).  Otherwise the scan itself.
+// A workgroup takes every `rows`-th sequence; while a tile is worked on, the next one's inputs - of the same sequence or the next - are
+// on their way.
 template <typename T, int NG, bool kStates>
 __global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
     constexpr int kRows = kTile / NG, kWide = 4 * NG;
@@ -99,125 +123,126 @@ __global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
     __shared__ float sy[kStates ? 1 : NG][kTile][kLanes];
     __shared__ alignas(16) float sB[kTile][kWide], sC[kTile][kWide];
     const Place p = place_of(a);
-    const int lane = p.lane, w = p.w, b = p.row, d = p.d;
-    const int len = seq_len(a.lengths, b, a.T);
-    const int from = p.chunk * a.steps, to = min(from + a.steps, a.T), end = min(to, len);
+    const int lane = p.lane, w = p.w, d = p.d;
     if (kStates && p.chunk == a.chunks - 1) return;
-    const T* u = (const T*)a.u + b * a.ub;
-    const T* delta = (const T*)a.delta + b * a.db;
-    const T* z = a.z ? (const T*)a.z + b * a.zb : nullptr;
-    const T* Bm = (const T*)a.Bm + b * a.bb + p.g * a.bg;
-    const T* Cm = (const T*)a.Cm + b * a.cb + p.g * a.cg;
-    T* out = (T*)a.out + (long long)b * a.T * a.D;
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
-    const bool gate = !kStates && z;
+    const bool gate = !kStates && a.z;
+    const int from = p.chunk * a.steps, to = min(from + a.steps, a.T);
 
-    float A2[4], h[4];
+    float A2[4];
+    load4(a.A + (long long)d * a.N, w, a.N, A2);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int n = 4 * w + j;
-        A2[j] = n < a.N ? a.A[(long long)d * a.N + n] * kLog2e : 0.0f;
-        h[j] = !kStates && n < a.N && a.s0 ? a.s0[((long long)b * a.D + d) * a.N + n] : 0.0f;
-    }
-    if (!kStates && (from < end || (len == 0 && p.chunk == 0))) fold_chunks(a, b, d, w, 0, p.chunk, 1, A2, h);
-
+    for (int j = 0; j < 4; j++) A2[j] *= kLog2e;
     const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
+    const unsigned at = (unsigned)d * (unsigned)sizeof(T);
+    const long long bat = brow * a.bt + bn, cat = brow * a.ct + bn;
     T ru[kRows], rd[kRows], rz[kRows], rB, rC;
-    auto load = [&](int t0) __attribute__((always_inline)) {            // the tile's rows, as they are stored
-        const int nv = end - t0;
-#pragma unroll
-        for (int k = 0; k < kRows; k++) {
-            const int t = t0 + w + k * NG;
-            if (w + k * NG < nv) {
-                ru[k] = (u + t * a.ut)[d];
-                rd[k] = (delta + t * a.dt)[d];
-                if (gate) rz[k] = (z + t * a.zt)[d];
-            }
-        }
-        const bool bl = brow < nv && bn < a.N;
-        rB = bl ? Bm[(t0 + brow) * a.bt + bn] : from_f32<T>(0.0f);
-        if (!kStates) rC = bl ? Cm[(t0 + brow) * a.ct + bn] : from_f32<T>(0.0f);
-    };
-    float total = 0.0f;                                                 // kStates: sum of dt over the rows this wave staged
-    bool any_cut = false;
-    if (from < end) load(from);
-    for (int t0 = from; t0 < end; t0 += kTile) {
-        const int nv = min(kTile, end - t0);
-        float uu[kRows], zz[kRows];
+    auto load = [&](int b, int t0, int nv) __attribute__((always_inline)) {      // a tile's rows, as they are stored
+        const T* u = (const T*)a.u + (b * a.ub + t0 * a.ut);
+        const T* delta = (const T*)a.delta + (b * a.db + t0 * a.dt);
+        const T* z = (const T*)a.z + (b * a.zb + t0 * a.zt);
 #pragma unroll
         for (int k = 0; k < kRows; k++) {
             const int r = w + k * NG;
-            float dt = 0.0f;
-            uu[k] = zz[k] = 0.0f;
             if (r < nv) {
-                uu[k] = to_f32(ru[k]);
-                dt = time_step(a, to_f32(rd[k]) + bias);
-                if (gate) zz[k] = to_f32(rz[k]);
-            }
-            if (kStates) total += dt;
-            sdt[r][lane] = make_float2(dt, dt * uu[k]);
-        }
-        sB[brow][bn] = to_f32(rB);
-        if (!kStates) sC[brow][bn] = to_f32(rC);
-        const unsigned cut = reset_bits(a, b, t0, nv, lane);
-        any_cut |= cut != 0;
-        __syncthreads();
-        if (t0 + kTile < end) load(t0 + kTile);                         // in flight behind the tile's arithmetic
-#pragma unroll
-        for (int r = 0; r < kTile; r++) {                               // steps behind nv have dt = 0: they change nothing
-            if (r % 4 == 0 && r >= nv) break;
-            if (!kStates && r % kBack == 0 && a.ckpt && t0 + r && p.live) {
-                float* c = a.ckpt + (((long long)b * ((a.T - 1) / kBack) + (t0 + r) / kBack - 1) * a.D + d) * a.N + 4 * w;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (4 * w + j < a.N) c[j] = h[j];
-            }
-            AG_RARE(cut >> r & 1) h[0] = h[1] = h[2] = h[3] = 0.0f;
-            const float2 q = sdt[r][lane];
-            const float4 Bv = *(const float4*)&sB[r][4 * w];
-            const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) h[j] = __builtin_fmaf(exp2_hw(q.x * A2[j]), h[j], q.y * B4[j]);
-            if (!kStates) {
-                const float4 Cv = *(const float4*)&sC[r][4 * w];
-                sy[w][r][lane] = __builtin_fmaf(Cv.x, h[0], Cv.y * h[1]) + __builtin_fmaf(Cv.z, h[2], Cv.w * h[3]);
+                ru[k] = get(u + r * a.ut, at);
+                rd[k] = get(delta + r * a.dt, at);
+                if (gate) rz[k] = get(z + r * a.zt, at);
             }
         }
-        __syncthreads();
-        if (!kStates)
+        const bool bl = brow < nv && bn < a.N;
+        rB = bl ? ((const T*)a.Bm + (b * a.bb + p.g * a.bg + t0 * a.bt))[bat] : from_f32<T>(0.0f);
+        if (!kStates) rC = bl ? ((const T*)a.Cm + (b * a.cb + p.g * a.cg + t0 * a.ct))[cat] : from_f32<T>(0.0f);
+    };
+    int loaded = -1;                                                    // sequence whose first tile is on its way
+    float total = 0.0f;                                                 // kStates: sum of dt over the rows this wave staged
+    bool any_cut = false;
+    for (int b = p.row; b < a.B; b += a.rows) {
+        const int len = seq_len(a.lengths, b, a.T), end = min(to, len);
+        T* out = (T*)a.out + (long long)b * a.T * a.D;
+        if (from < end && loaded != b) load(b, from, end - from);
+        float h[4];
+        zero4(h);
+        if (!kStates) {
+            if (a.s0) load4(a.s0 + ((long long)b * a.D + d) * a.N, w, a.N, h);
+            if (p.chunk && from < end) fold_chunks(a, b, d, w, 0, p.chunk, 1, A2, h);
+        }
+        for (int t0 = from; t0 < end; t0 += kTile) {
+            const int nv = min(kTile, end - t0);
+            float uu[kRows], zz[kRows];
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
                 const int r = w + k * NG;
-                if (r >= nv) break;
-                float y = skip * uu[k];
-#pragma unroll
-                for (int v = 0; v < NG; v++) y += sy[v][r][lane];
-                if (gate) y *= zz[k] * sigmoid(zz[k]);
-                if (p.live) (out + (long long)(t0 + r) * a.D)[d] = from_f32<T>(y);
+                float dt = 0.0f;
+                uu[k] = zz[k] = 0.0f;
+                if (r < nv) {
+                    uu[k] = to_f32(ru[k]);
+                    dt = time_step(a, to_f32(rd[k]) + bias);
+                    if (gate) zz[k] = to_f32(rz[k]);
+                }
+                if (kStates) total += dt;
+                sdt[r][lane] = make_float2(dt, dt * uu[k]);
             }
-    }
-    if (kStates) {
-        float* sums = (float*)sdt;
-        sums[w * kLanes + lane] = total;
-        __syncthreads();
-        if (!p.live) return;
-        const long long at = ((long long)b * a.chunks + p.chunk) * a.D + d;
+            sB[brow][bn] = to_f32(rB);
+            if (!kStates) sC[brow][bn] = to_f32(rC);
+            const unsigned cut = reset_bits(a, b, t0, nv, lane);
+            any_cut |= cut != 0;
+            __syncthreads();
+            int nb = b, nt = t0 + kTile, nn = end - nt;
+            if (!kStates && nn <= 0 && b + a.rows < a.B) {
+                nb = loaded = b + a.rows;
+                nt = from;
+                nn = min(to, seq_len(a.lengths, nb, a.T)) - from;
+            }
+            load(nb, nt, nn);
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (4 * w + j < a.N) a.chunk_h[at * a.N + 4 * w + j] = h[j];
-        if (w == 0) {
-            float s = 0.0f;
-            for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
-            a.chunk_dt[at] = any_cut ? __builtin_nanf("") : s;
+            for (int r = 0; r < kTile; r++) {                           // steps behind nv have dt = 0: they change nothing
+                if (r % 4 == 0 && r >= nv) break;
+                if (!kStates && r % kBack == 0 && a.ckpt && t0 + r && p.live)
+                    store4(a.ckpt + (((long long)b * ((a.T - 1) / kBack) + (t0 + r) / kBack - 1) * a.D + d) * a.N, w, a.N, h);
+                AG_RARE(cut >> r & 1) zero4(h);
+                const float2 q = sdt[r][lane];
+                const float4 Bv = *(const float4*)&sB[r][4 * w];
+                const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) h[j] = __builtin_fmaf(exp2_hw(q.x * A2[j]), h[j], q.y * B4[j]);
+                if (!kStates) {
+                    const float4 Cv = *(const float4*)&sC[r][4 * w];
+                    sy[w][r][lane] = __builtin_fmaf(Cv.x, h[0], Cv.y * h[1]) + __builtin_fmaf(Cv.z, h[2], Cv.w * h[3]);
+                }
+            }
+            __syncthreads();
+            if (!kStates)
+#pragma unroll
+                for (int k = 0; k < kRows; k++) {
+                    const int r = w + k * NG;
+                    if (r >= nv) break;
+                    float y = skip * uu[k];
+#pragma unroll
+                    for (int v = 0; v < NG; v++) y += sy[v][r][lane];
+                    if (gate) y *= zz[k] * sigmoid(zz[k]);
+                    if (p.live) put(out + (long long)(t0 + r) * a.D, at, from_f32<T>(y));
+                }
         }
-        return;
+        if (kStates) {
+            float* sums = (float*)sdt;
+            sums[w * kLanes + lane] = total;
+            __syncthreads();
+            if (!p.live) return;
+            const long long row = ((long long)b * a.chunks + p.chunk) * a.D + d;
+            store4(a.chunk_h + row * a.N, w, a.N, h);
+            if (w == 0) {
+                float s = 0.0f;
+                for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
+                a.chunk_dt[row] = any_cut ? __builtin_nanf("") : s;
+            }
+            return;                                                     // chunks: one sequence per workgroup
+        }
+        if (!p.live) continue;
+        for (int t = max(from, end) + w; t < to; t += NG) put(out + (long long)t * a.D, at, from_f32<T>(0.0f));
+        if (a.s1 && (len ? from < len && len <= to : p.chunk == 0))     // the chunk with the last step
+            store4(a.s1 + ((long long)b * a.D + d) * a.N, w, a.N, h);
     }
-    if (!p.live) return;
-    for (int t = max(from, end) + w; t < to; t += NG) (out + (long long)t * a.D)[d] = from_f32<T>(0.0f);
-    if (a.s1 && (len ? from < len && len <= to : p.chunk == 0))         // the chunk with the last step
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (4 * w + j < a.N) a.s1[((long long)b * a.D + d) * a.N + 4 * w + j] = h[j];
 }
 
 // Sums of 8 registers over the 64 lanes, transposed on the way so that the number of live registers halves with every step (18
@@ -258,7 +283,7 @@ __device__ __forceinline__ int sum_lanes8_order(int lane) {
 // kCarry: the first pass over chunks (every chunk but the first): what the chunk hands back to the one before when nothing reaches it
 // from behind, and its sum of dt.
 template <typename T, int NG, bool kCarry>
-__global__ __launch_bounds__(kLanes* NG) void scan_bwd_kernel(ScanArgs a, ScanGradArgs q) {
+__global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd_kernel(ScanArgs a, ScanGradArgs q) {
     constexpr int kRows = kBack / NG, kWide = 4 * NG;
     __shared__ float2 sdt[kBack][kLanes];                               // dt, dt u
     __shared__ float sdy[kBack][kLanes];
@@ -268,60 +293,93 @@ __global__ __launch_bounds__(kLanes* NG) void scan_bwd_kernel(ScanArgs a, ScanGr
     if (kCarry && p.chunk == 0) return;
     const int lane = p.lane, w = p.w, d = p.d;
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
-    // 8 rows of B and of C: 64 NG values for 64 NG threads
-    const int bc = threadIdx.x / (kBack * kWide), brow = threadIdx.x / kWide % kBack, bn = threadIdx.x % kWide;
-    float A1[4], A2[4], dA[4], dD = 0.0f, dbias = 0.0f;
+    const bool gate = a.z;
+    const int from = p.chunk * a.steps, to = min(from + a.steps, a.T), last = from + (to - from - 1) / kBack * kBack;
+    // 8 rows of B and of C: half of the threads have one of each
+    const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
+    const unsigned at = (unsigned)d * (unsigned)sizeof(T);
+    const long long bat = brow * a.bt + bn, cat = brow * a.ct + bn;
+    float A2[4], dA[4], dD = 0.0f, dbias = 0.0f;
+    load4(a.A + (long long)d * a.N, w, a.N, A2);
+    zero4(dA);
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int n = 4 * w + j;
-        A1[j] = n < a.N ? a.A[(long long)d * a.N + n] : 0.0f;
-        A2[j] = A1[j] * kLog2e;
-        dA[j] = 0.0f;
-    }
+    for (int j = 0; j < 4; j++) A2[j] *= kLog2e;
+
+    T ru[kRows], rd[kRows], rz[kRows], rg[kRows], rB, rC;
+    float start[4];
+    // a tile's inputs as they are stored, and the state it starts from; nv <= 0: nothing
+    auto load = [&](int b, int t0, int nv) __attribute__((always_inline)) {
+        const T* u = (const T*)a.u + (b * a.ub + t0 * a.ut);
+        const T* delta = (const T*)a.delta + (b * a.db + t0 * a.dt);
+        const T* z = (const T*)a.z + (b * a.zb + t0 * a.zt);
+        const T* dout = (const T*)q.dout + (b * q.ob + t0 * q.ot);
+#pragma unroll
+        for (int k = 0; k < kRows; k++) {
+            const int r = w + k * NG;
+            if (r < nv) {
+                if (!kCarry) ru[k] = get(u + r * a.ut, at);
+                rd[k] = get(delta + r * a.dt, at);
+                rg[k] = get(dout + r * q.ot, at);
+                if (gate) rz[k] = get(z + r * a.zt, at);
+            }
+        }
+        const bool bl = brow < kBack && brow < nv && bn < a.N;
+        if (!kCarry) rB = bl ? ((const T*)a.Bm + (b * a.bb + p.g * a.bg + t0 * a.bt))[bat] : from_f32<T>(0.0f);
+        rC = bl ? ((const T*)a.Cm + (b * a.cb + p.g * a.cg + t0 * a.ct))[cat] : from_f32<T>(0.0f);
+        if (kCarry || nv <= 0) return;
+        if (t0) load4(a.ckpt + (((long long)b * ((a.T - 1) / kBack) + t0 / kBack - 1) * a.D + d) * a.N, w, a.N, start);
+        else if (a.s0) load4(a.s0 + ((long long)b * a.D + d) * a.N, w, a.N, start);
+        else zero4(start);
+    };
+    int len = p.row < a.B ? seq_len(a.lengths, p.row, a.T) : 0;
+    if (p.row < a.B) load(p.row, last, len - last);
     for (int b = p.row; b < a.B; b += q.rows) {
-        const int len = seq_len(a.lengths, b, a.T);
-        const int from = p.chunk * a.steps, to = min(from + a.steps, a.T);
-        const T* u = (const T*)a.u + b * a.ub;
-        const T* delta = (const T*)a.delta + b * a.db;
-        const T* z = a.z ? (const T*)a.z + b * a.zb : nullptr;
-        const T* dout = (const T*)q.dout + b * q.ob;
-        const T* BC = bc ? (const T*)a.Cm + b * a.cb + p.g * a.cg : (const T*)a.Bm + b * a.bb + p.g * a.bg;
-        const long long bct = bc ? a.ct : a.bt;
         const long long o = (long long)b * a.T * a.D;
+        const int next_b = b + q.rows, next_len = next_b < a.B ? seq_len(a.lengths, next_b, a.T) : 0;
         float carry[4];                                                 // a_{t+1} g_{t+1}
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            carry[j] = !kCarry && q.ds1 && p.live && 4 * w + j < a.N ? q.ds1[((long long)b * a.D + d) * a.N + 4 * w + j] : 0.0f;
-        if (!kCarry) fold_chunks(a, b, d, w, a.chunks - 1, p.chunk, -1, A2, carry);
+        zero4(carry);
+        if (!kCarry) {
+            if (q.ds1 && p.live) load4(q.ds1 + ((long long)b * a.D + d) * a.N, w, a.N, carry);
+            fold_chunks(a, b, d, w, a.chunks - 1, p.chunk, -1, A2, carry);
+        }
         float total = 0.0f;
         bool any_cut = false;
-        for (int t0 = from + (to - from - 1) / kBack * kBack; t0 >= from; t0 -= kBack) {
+        for (int t0 = last; t0 >= from; t0 -= kBack) {
             const int nv = max(0, min(kBack, len - t0)), nt = min(kBack, a.T - t0);
-            float uu[kRows], dts[kRows], sg[kRows], zz[kRows], go[kRows];
+            float uu[kRows], dts[kRows], sg[kRows], zz[kRows], sz[kRows], go[kRows], now[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) now[j] = p.live ? start[j] : 0.0f;
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
-                const int r = w + k * NG, t = t0 + r;
+                const int r = w + k * NG;
                 uu[k] = dts[k] = sg[k] = zz[k] = go[k] = 0.0f;
+                sz[k] = 1.0f;
                 float dy = 0.0f;
                 if (r < nv && p.live) {
-                    if (!kCarry) uu[k] = to_f32((u + t * a.ut)[d]);
-                    const float raw = to_f32((delta + t * a.dt)[d]) + bias;
-                    dts[k] = time_step(a, raw);
-                    sg[k] = a.softplus ? sigmoid(raw) : 1.0f;
-                    go[k] = dy = to_f32((dout + t * q.ot)[d]);
-                    if (z) {
-                        zz[k] = to_f32((z + t * a.zt)[d]);
-                        dy *= zz[k] * sigmoid(zz[k]);
+                    if (!kCarry) uu[k] = to_f32(ru[k]);
+                    dts[k] = to_f32(rd[k]) + bias;
+                    sg[k] = 1.0f;
+                    if (a.softplus) dts[k] = softplus(dts[k], sg[k]);
+                    go[k] = dy = to_f32(rg[k]);
+                    if (gate) {
+                        zz[k] = to_f32(rz[k]);
+                        sz[k] = sigmoid(zz[k]);
+                        dy *= zz[k] * sz[k];
                     }
                 }
                 sdt[r][lane] = make_float2(dts[k], dts[k] * uu[k]);
                 sdy[r][lane] = dy;
                 if (kCarry) total += dts[k];
             }
-            sBC[bc][brow][bn] = brow < nv && bn < a.N ? to_f32((BC + (t0 + brow) * bct)[bn]) : 0.0f;
+            if (brow < kBack) {
+                if (!kCarry) sBC[0][brow][bn] = to_f32(rB);
+                sBC[1][brow][bn] = to_f32(rC);
+            }
             const unsigned cut = reset_bits(a, b, t0, nv, lane);
             any_cut |= cut != 0;
             __syncthreads();
+            const bool same = t0 > from;
+            load(same ? b : next_b, same ? t0 - kBack : last, same ? len - t0 + kBack : next_len - last);
             if (kCarry) {
 #pragma unroll
                 for (int r = kBack - 1; r >= 0; r--) {
@@ -329,21 +387,17 @@ __global__ __launch_bounds__(kLanes* NG) void scan_bwd_kernel(ScanArgs a, ScanGr
                     const float C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w}, dy = sdy[r][lane], dt = sdt[r][lane].x;
 #pragma unroll
                     for (int j = 0; j < 4; j++) carry[j] = exp2_hw(dt * A2[j]) * __builtin_fmaf(C4[j], dy, carry[j]);
-                    AG_RARE(cut >> r & 1) carry[0] = carry[1] = carry[2] = carry[3] = 0.0f;
+                    AG_RARE(cut >> r & 1) zero4(carry);
                 }
                 __syncthreads();
                 continue;
             }
             if (nv) {
-                float h[kBack][4], e[kBack][4], now[4], v[8], sums = 0.0f;      // h[r]: the state step r starts from
-                const float* start = t0 ? a.ckpt + ((long long)b * ((a.T - 1) / kBack) + t0 / kBack - 1) * a.D * a.N
-                                        : (a.s0 ? a.s0 + (long long)b * a.D * a.N : nullptr);
-#pragma unroll
-                for (int j = 0; j < 4; j++) now[j] = start && p.live && 4 * w + j < a.N ? start[(long long)d * a.N + 4 * w + j] : 0.0f;
+                float h[kBack][4], e[kBack][4], v[8], sums = 0.0f;      // h[r]: the state step r starts from
                 const int order = sum_lanes8_order(lane), odd = order >> 2, mine = lane & 3;
 #pragma unroll
                 for (int r = 0; r < kBack; r++) {      // steps behind nv have dt = dy = 0: decay 1, no input
-                    AG_RARE(cut >> r & 1) now[0] = now[1] = now[2] = now[3] = 0.0f;
+                    AG_RARE(cut >> r & 1) zero4(now);
                     const float2 s = sdt[r][lane];
                     const float dy = sdy[r][lane];
                     const float4 Bv = *(const float4*)&sBC[0][r][4 * w], Cv = *(const float4*)&sBC[1][r][4 * w];
@@ -378,10 +432,10 @@ __global__ __launch_bounds__(kLanes* NG) void scan_bwd_kernel(ScanArgs a, ScanGr
                         s1 = __builtin_fmaf(gr, B4[j], s1);
                         carry[j] = e[r][j] * gr;
                         const float qq = carry[j] * h[r][j];
-                        s2 = __builtin_fmaf(qq, A1[j], s2);
+                        s2 = __builtin_fmaf(qq, A2[j], s2);
                         dA[j] = __builtin_fmaf(qq, s.x, dA[j]);
                     }
-                    AG_RARE(cut >> r & 1) carry[0] = carry[1] = carry[2] = carry[3] = 0.0f;      // h[r] is 0 there already
+                    AG_RARE(cut >> r & 1) zero4(carry);                 // h[r] is 0 there already
                     ss1[w][r][lane] = s1;
                     ss2[w][r][lane] = s2;
                     if (!(r & 1)) {
@@ -402,48 +456,49 @@ __global__ __launch_bounds__(kLanes* NG) void scan_bwd_kernel(ScanArgs a, ScanGr
                     for (int v = 0; v < NG; v++) y += sy[v][r][lane], s1 += ss1[v][r][lane], s2 += ss2[v][r][lane];
                 }
                 float dy = go[k], dzv = 0.0f;
-                if (z) {
-                    const float s = sigmoid(zz[k]);
-                    dzv = go[k] * y * (s * (1.0f + zz[k] * (1.0f - s)));
-                    dy *= zz[k] * s;
+                if (gate) {
+                    dzv = go[k] * y * (sz[k] * (1.0f + zz[k] * (1.0f - sz[k])));
+                    dy *= zz[k] * sz[k];
                 }
-                const float draw = (uu[k] * s1 + s2) * sg[k];
+                const float draw = __builtin_fmaf(uu[k], s1, s2 * kLn2) * sg[k];      // s2 was summed with A log2(e)
                 if (p.live) {
-                    const long long at = o + (long long)(t0 + r) * a.D;
-                    ((T*)q.du + at)[d] = from_f32<T>(__builtin_fmaf(dts[k], s1, skip * dy));
-                    ((T*)q.ddelta + at)[d] = from_f32<T>(draw);
-                    if (z) ((T*)q.dz + at)[d] = from_f32<T>(dzv);
+                    const long long row = o + (long long)(t0 + r) * a.D;
+                    put((T*)q.du + row, at, from_f32<T>(__builtin_fmaf(dts[k], s1, skip * dy)));
+                    put((T*)q.ddelta + row, at, from_f32<T>(draw));
+                    if (gate) put((T*)q.dz + row, at, from_f32<T>(dzv));
                 }
                 dD = __builtin_fmaf(dy, uu[k], dD);
                 dbias += draw;
             }
-            if (brow < nt && bn < a.N) {
-                const float v = brow < nv ? sdBC[bc][brow][bn] : 0.0f;
-                const long long at = (((long long)b * a.T + t0 + brow) * a.G + p.g) * a.N + bn, n = (long long)a.B * a.T * a.G * a.N;
-                if (q.bc_partials) q.bc_partials[(2 * p.cb + bc) * n + at] = v;
-                else ((T*)(bc ? q.dC : q.dB))[at] = from_f32<T>(v);
+            if (brow < nt && bn < a.N) {                                // nt <= 8
+                const float vB = brow < nv ? sdBC[0][brow][bn] : 0.0f, vC = brow < nv ? sdBC[1][brow][bn] : 0.0f;
+                const long long i = (((long long)b * a.T + t0 + brow) * a.G + p.g) * a.N + bn, n = (long long)a.B * a.T * a.G * a.N;
+                if (q.bc_partials) {
+                    q.bc_partials[2 * p.cb * n + i] = vB;
+                    q.bc_partials[(2 * p.cb + 1) * n + i] = vC;
+                } else {
+                    ((T*)q.dB)[i] = from_f32<T>(vB);
+                    ((T*)q.dC)[i] = from_f32<T>(vC);
+                }
             }
         }
+        len = next_len;
         if (kCarry) {
             float* sums = (float*)sdt;
             sums[w * kLanes + lane] = total;
             __syncthreads();
             if (p.live) {
-                const long long at = ((long long)b * a.chunks + p.chunk) * a.D + d;
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (4 * w + j < a.N) a.chunk_h[at * a.N + 4 * w + j] = carry[j];
+                const long long row = ((long long)b * a.chunks + p.chunk) * a.D + d;
+                store4(a.chunk_h + row * a.N, w, a.N, carry);
                 if (w == 0) {
                     float s = 0.0f;
                     for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
-                    a.chunk_dt[at] = any_cut ? __builtin_nanf("") : s;
+                    a.chunk_dt[row] = any_cut ? __builtin_nanf("") : s;
                 }
             }
             __syncthreads();
         } else if (q.ds0 && p.live && p.chunk == 0)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (4 * w + j < a.N) q.ds0[((long long)b * a.D + d) * a.N + 4 * w + j] = carry[j];
+            store4(q.ds0 + ((long long)b * a.D + d) * a.N, w, a.N, carry);
     }
     if (kCarry) return;
     // this workgroup's row of partial parameter gradients: [rows chunks, D, N + 2]
@@ -536,17 +591,19 @@ Chunks chunks_of(int B, int T, int D, int G) {
     return Chunks{(int)((T + steps - 1) / steps), (int)steps};
 }
 
-// workgroups along the batch in the backward: a few per CU
-int grad_rows(int B, int D, int G) {
-    const int per = channel_blocks(D, G) * G, want = (2048 + per - 1) / per;
+// workgroups along the batch, each of which takes several sequences where there are many: two rounds of what the CUs hold (forward
+// six workgroups per CU, backward three)
+int rows_of(int B, int D, int G, int resident) {
+    const int per = channel_blocks(D, G) * G, want = (2 * 256 * resident + per - 1) / per;
     return B < want ? B : want;
 }
+int grad_rows(int B, int D, int G) { return rows_of(B, D, G, 3); }
 
 int check(const ag_scan_args* p) {
     if (!p || p->struct_size != sizeof(ag_scan_args) || !p->u_dev || !p->delta_dev || !p->Bm_dev || !p->Cm_dev || !p->A_dev)
         return AG_ERR_INVALID_ARG;
     if (p->B <= 0 || p->T <= 0 || p->D <= 0 || p->G <= 0 || p->N <= 0 || p->D % p->G) return AG_ERR_INVALID_ARG;
-    if (p->N > 32 || p->dtype < AG_F32 || p->dtype > AG_F16) return AG_ERR_UNSUPPORTED;
+    if (p->N > 32 || p->D > 1 << 28 || p->dtype < AG_F32 || p->dtype > AG_F16) return AG_ERR_UNSUPPORTED;
     // the grid, with time in chunks: at most 1024 + B G channel blocks (or one per sequence and 64 channels)
     if ((long long)p->B * p->G * channel_blocks(p->D, p->G) > 0x7fffffffLL - 4096) return AG_ERR_UNSUPPORTED;
     return AG_OK;
@@ -557,7 +614,8 @@ ScanArgs device_args(const ag_scan_args* p) {
     return ScanArgs{p->u_dev, p->delta_dev, p->z_dev, p->Bm_dev, p->Cm_dev, p->A_dev, p->Dskip_dev, p->delta_bias_dev, p->state_in_dev,
                     p->lengths_dev, p->resets_dev, p->u_sb, p->u_st, p->delta_sb, p->delta_st, p->z_sb, p->z_st, p->b_sb, p->b_st, p->b_sg,
                     p->c_sb, p->c_st, p->c_sg, p->r_sb, p->r_st, p->out_dev, p->state_out_dev, p->ckpt_dev, nullptr, nullptr, p->B, p->T,
-                    p->D, p->N, p->G, p->softplus, p->D / p->G, channel_blocks(p->D, p->G), c.count, c.steps};
+                    p->D, p->N, p->G, p->softplus, p->D / p->G, channel_blocks(p->D, p->G),
+                    c.count > 1 ? p->B : rows_of(p->B, p->D, p->G, 6), c.count, c.steps};
 }
 
 // floats of chunk_h and chunk_dt
@@ -603,7 +661,7 @@ extern "C" int ag_selective_scan_fwd(const ag_scan_args* p, void* stream) {
         a.chunk_h = (float*)p->workspace_dev;
         a.chunk_dt = a.chunk_h + (long long)a.B * a.chunks * a.D * a.N;
     }
-    const dim3 grid((unsigned)((long long)a.B * a.chunks * a.G * a.nb));
+    const dim3 grid((unsigned)((long long)a.rows * a.chunks * a.G * a.nb));
     if (a.chunks > 1)
         AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, true>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
     AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));

@@ -31,8 +31,7 @@ __device__ __forceinline__ float sigmoid(float x) { return rcp_hw(1.0f + exp_hw(
 // softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|) in [0, 1].  log1p(e) = 2 atanh(s), s = e / (2 + e) <= 1/3: the odd series up to
 // s^15 leaves (1/9)^8 / 17 < 2e-9, and - unlike log(1 + e) - it keeps its RELATIVE accuracy where e is small (steps of 1e-3 and less
 // are what the scan's time step usually is).
-__device__ __forceinline__ float softplus(float x) {
-    const float e = exp_hw(-__builtin_fabsf(x));
+__device__ __forceinline__ float softplus_from(float x, float e) {
     const float s = e * rcp_hw(2.0f + e), q = s * s;
     float p = 2.0f / 15.0f;
     p = __builtin_fmaf(p, q, 2.0f / 13.0f);
@@ -43,6 +42,13 @@ __device__ __forceinline__ float softplus(float x) {
     p = __builtin_fmaf(p, q, 2.0f / 3.0f);
     p = __builtin_fmaf(p, q, 2.0f);
     return __builtin_fmaf(p, s, fmaxf(x, 0.0f));
+}
+__device__ __forceinline__ float softplus(float x) { return softplus_from(x, exp_hw(-__builtin_fabsf(x))); }
+// ... and its slope, the sigmoid, from the same exponential
+__device__ __forceinline__ float softplus(float x, float& slope) {
+    const float e = exp_hw(-__builtin_fabsf(x)), r = rcp_hw(1.0f + e);
+    slope = x < 0.0f ? e * r : r;
+    return softplus_from(x, e);
 }
 
 // steps of sequence b that count: all T, or its length clamped to what the buffers hold
