@@ -67,20 +67,45 @@ __device__ __forceinline__ Place place_of(const ScanArgs& a) {
 }
 
 // reset flags of nv steps from t0 as a wave-uniform bit mask
-__device__ __forceinline__ unsigned reset_bits(const ScanArgs& a, int b, int t0, int nv, int lane) {
-    if (!a.resets) return 0;
-    const bool f = lane < nv && a.resets[b * a.rb + (t0 + lane) * a.rt] != 0;
+template <typename A>
+__device__ __forceinline__ unsigned reset_bits(A a, int b, int t0, int nv, int lane) {
+    const unsigned char* resets = a->resets;
+    if (!resets) return 0;
+    const bool f = lane < nv && resets[b * a->rb + (t0 + lane) * a->rt] != 0;
     return __builtin_amdgcn_readfirstlane((unsigned)__ballot(f));
 }
-
-__device__ __forceinline__ float time_step(const ScanArgs& a, float raw) { return a.softplus ? softplus(raw) : raw; }
 
 // a branch that stays one: a select in its place would cost every step what only a reset needs
 #define AG_RARE(cond) if (__builtin_expect(cond, 0)) if (([]() __attribute__((always_inline)) { asm volatile(""); }(), true))
 
-// element of a row at a lane's byte offset: the row is wave-uniform, so the access is a scalar base plus 32 bits per lane
-template <typename T> __device__ __forceinline__ T get(const T* row, unsigned bytes) { return *(const T*)((const char*)row + bytes); }
-template <typename T> __device__ __forceinline__ void put(T* row, unsigned bytes, T v) { *(T*)((char*)row + bytes) = v; }
+// Addresses.  A row's base is wave-uniform and moves on by scalar adds; a lane adds 32 bits of its own (the host has checked that a
+// tile of rows stays below 4 GB).  The argument block is read again, by scalar loads, where a sequence starts: all of its pointers and
+// strides held at once do not fit the scalar registers, and what is spilled from them costs vector instructions.
+template <typename S> using Const = const __attribute__((address_space(4))) S*;
+__device__ __forceinline__ Const<ScanArgs> scan_args() {
+    auto p = (Const<ScanArgs>)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return p;
+}
+__device__ __forceinline__ Const<ScanGradArgs> grad_args() {           // the second argument, behind the first
+    static_assert(sizeof(ScanArgs) % 8 == 0, "the argument blocks follow each other");
+    auto p = (Const<char>)__builtin_amdgcn_kernarg_segment_ptr() + sizeof(ScanArgs);
+    asm volatile("" : "+s"(p));
+    return (Const<ScanGradArgs>)p;
+}
+struct Rows {                          // rows of a [T, ...] array from some step on
+    const char* base;
+    unsigned step;                     // bytes from one row to the next
+    __device__ __forceinline__ void set(const void* p, long long at, long long stride, int size) {
+        base = (const char*)p + at * size;
+        step = (unsigned)(stride * size);
+    }
+    __device__ __forceinline__ void move(int rows) { base += (long long)rows * (long long)step; }
+};
+template <typename T> __device__ __forceinline__ T get(const Rows& x, int r, unsigned lane_bytes) {
+    return *(const T*)(x.base + (r * x.step + lane_bytes));
+}
+template <typename T> __device__ __forceinline__ void put(char* base, unsigned bytes, T v) { *(T*)(base + bytes) = v; }
 
 // a lane's four states in a row of N, zero where there are none: one access where the row is whole
 typedef float four_any4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -103,6 +128,7 @@ __device__ __forceinline__ void zero4(float* x) { x[0] = x[1] = x[2] = x[3] = 0.
 
 // state (or gradient of a state) that chunk `chunk` starts from, folded over the chunks first .. last - 1 (step +-1) before it
 __device__ __forceinline__ void fold_chunks(const ScanArgs& a, int b, int d, int w, int first, int last, int step, const float* A2, float* h) {
+#pragma unroll 1                       // eight at a time took the registers of a sixth workgroup per CU
     for (int c = first; c != last; c += step) {
         const long long at = ((long long)b * a.chunks + c) * a.D + d;
         const float sum = a.chunk_dt[at];
@@ -117,54 +143,70 @@ __device__ __forceinline__ void fold_chunks(const ScanArgs& a, int b, int d, int
 // A workgroup takes every `rows`-th sequence; while a tile is worked on, the next one's inputs - of the same sequence or the next - are
 // on their way.
 template <typename T, int NG, bool kStates>
-__global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
+__global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(ScanArgs a) {
     constexpr int kRows = kTile / NG, kWide = 4 * NG;
     __shared__ float2 sdt[kTile][kLanes];                               // dt, dt u
     __shared__ float sy[kStates ? 1 : NG][kTile][kLanes];
     __shared__ alignas(16) float sB[kTile][kWide], sC[kTile][kWide];
     const Place p = place_of(a);
-    const int lane = p.lane, w = p.w, d = p.d;
+    const int lane = p.lane, w = p.w, d = p.d, N = a.N, T_ = a.T, D = a.D;
     if (kStates && p.chunk == a.chunks - 1) return;
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
-    const bool gate = !kStates && a.z;
-    const int from = p.chunk * a.steps, to = min(from + a.steps, a.T);
+    const bool gate = !kStates && a.z, soft = a.softplus, ckpt = !kStates && a.ckpt;
+    const int from = p.chunk * a.steps, to = min(from + a.steps, T_);
 
     float A2[4];
-    load4(a.A + (long long)d * a.N, w, a.N, A2);
+    load4(a.A + (long long)d * N, w, N, A2);
 #pragma unroll
     for (int j = 0; j < 4; j++) A2[j] *= kLog2e;
     const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
     const unsigned at = (unsigned)d * (unsigned)sizeof(T);
-    const long long bat = brow * a.bt + bn, cat = brow * a.ct + bn;
+    const long long state = (long long)d * N;                          // of the lane's channel
+    Rows u, delta, z, Bm, Cm;
     T ru[kRows], rd[kRows], rz[kRows], rB, rC;
-    auto load = [&](int b, int t0, int nv) __attribute__((always_inline)) {      // a tile's rows, as they are stored
-        const T* u = (const T*)a.u + (b * a.ub + t0 * a.ut);
-        const T* delta = (const T*)a.delta + (b * a.db + t0 * a.dt);
-        const T* z = (const T*)a.z + (b * a.zb + t0 * a.zt);
+    auto sequence = [&](int b) __attribute__((always_inline)) {        // its first tile in this chunk
+        const auto k = scan_args();
+        u.set(k->u, b * k->ub + from * k->ut, k->ut, sizeof(T));
+        delta.set(k->delta, b * k->db + from * k->dt, k->dt, sizeof(T));
+        if (gate) z.set(k->z, b * k->zb + from * k->zt, k->zt, sizeof(T));
+        Bm.set(k->Bm, b * k->bb + p.g * k->bg + from * k->bt, k->bt, sizeof(T));
+        if (!kStates) Cm.set(k->Cm, b * k->cb + p.g * k->cg + from * k->ct, k->ct, sizeof(T));
+    };
+    auto load = [&](int nv) __attribute__((always_inline)) {           // a tile's rows, as they are stored; then on to the next tile's
 #pragma unroll
         for (int k = 0; k < kRows; k++) {
             const int r = w + k * NG;
             if (r < nv) {
-                ru[k] = get(u + r * a.ut, at);
-                rd[k] = get(delta + r * a.dt, at);
-                if (gate) rz[k] = get(z + r * a.zt, at);
+                ru[k] = get<T>(u, r, at);
+                rd[k] = get<T>(delta, r, at);
+                if (gate) rz[k] = get<T>(z, r, at);
             }
         }
-        const bool bl = brow < nv && bn < a.N;
-        rB = bl ? ((const T*)a.Bm + (b * a.bb + p.g * a.bg + t0 * a.bt))[bat] : from_f32<T>(0.0f);
-        if (!kStates) rC = bl ? ((const T*)a.Cm + (b * a.cb + p.g * a.cg + t0 * a.ct))[cat] : from_f32<T>(0.0f);
+        rB = rC = from_f32<T>(0.0f);
+        if (brow < nv && bn < N) {
+            rB = get<T>(Bm, brow, bn * (unsigned)sizeof(T));
+            if (!kStates) rC = get<T>(Cm, brow, bn * (unsigned)sizeof(T));
+        }
+        u.move(kTile), delta.move(kTile), Bm.move(kTile);
+        if (gate) z.move(kTile);
+        if (!kStates) Cm.move(kTile);
     };
     int loaded = -1;                                                    // sequence whose first tile is on its way
     float total = 0.0f;                                                 // kStates: sum of dt over the rows this wave staged
     bool any_cut = false;
     for (int b = p.row; b < a.B; b += a.rows) {
-        const int len = seq_len(a.lengths, b, a.T), end = min(to, len);
-        T* out = (T*)a.out + (long long)b * a.T * a.D;
-        if (from < end && loaded != b) load(b, from, end - from);
+        const auto k1 = scan_args();
+        const int len = seq_len(k1->lengths, b, T_), end = min(to, len);
+        char* out = (char*)k1->out + ((long long)b * T_ + from) * D * (long long)sizeof(T);
+        float* ck = k1->ckpt + ((long long)b * ((T_ - 1) / kBack) + from / kBack - 1) * D * N + state;
+        if (from < end && loaded != b) {
+            sequence(b);
+            load(end - from);
+        }
         float h[4];
         zero4(h);
         if (!kStates) {
-            if (a.s0) load4(a.s0 + ((long long)b * a.D + d) * a.N, w, a.N, h);
+            if (k1->s0) load4(k1->s0 + (long long)b * D * N + state, w, N, h);
             if (p.chunk && from < end) fold_chunks(a, b, d, w, 0, p.chunk, 1, A2, h);
         }
         for (int t0 = from; t0 < end; t0 += kTile) {
@@ -177,7 +219,8 @@ __global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
                 uu[k] = zz[k] = 0.0f;
                 if (r < nv) {
                     uu[k] = to_f32(ru[k]);
-                    dt = time_step(a, to_f32(rd[k]) + bias);
+                    dt = to_f32(rd[k]) + bias;
+                    if (soft) dt = softplus(dt);
                     if (gate) zz[k] = to_f32(rz[k]);
                 }
                 if (kStates) total += dt;
@@ -185,21 +228,23 @@ __global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
             }
             sB[brow][bn] = to_f32(rB);
             if (!kStates) sC[brow][bn] = to_f32(rC);
-            const unsigned cut = reset_bits(a, b, t0, nv, lane);
+            const unsigned cut = reset_bits(scan_args(), b, t0, nv, lane);
             any_cut |= cut != 0;
             __syncthreads();
-            int nb = b, nt = t0 + kTile, nn = end - nt;
-            if (!kStates && nn <= 0 && b + a.rows < a.B) {
-                nb = loaded = b + a.rows;
-                nt = from;
-                nn = min(to, seq_len(a.lengths, nb, a.T)) - from;
+            int next = end - t0 - kTile;
+            if (!kStates && next <= 0 && b + a.rows < a.B) {
+                loaded = b + a.rows;
+                sequence(loaded);
+                next = min(to, seq_len(scan_args()->lengths, loaded, T_)) - from;
             }
-            load(nb, nt, nn);
+            if (next > 0) load(next);
 #pragma unroll
             for (int r = 0; r < kTile; r++) {                           // steps behind nv have dt = 0: they change nothing
                 if (r % 4 == 0 && r >= nv) break;
-                if (!kStates && r % kBack == 0 && a.ckpt && t0 + r && p.live)
-                    store4(a.ckpt + (((long long)b * ((a.T - 1) / kBack) + (t0 + r) / kBack - 1) * a.D + d) * a.N, w, a.N, h);
+                if (r % kBack == 0 && ckpt) {
+                    if (t0 + r && p.live) store4(ck, w, N, h);
+                    ck += (long long)D * N;
+                }
                 AG_RARE(cut >> r & 1) zero4(h);
                 const float2 q = sdt[r][lane];
                 const float4 Bv = *(const float4*)&sB[r][4 * w];
@@ -212,7 +257,7 @@ __global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
                 }
             }
             __syncthreads();
-            if (!kStates)
+            if (!kStates) {
 #pragma unroll
                 for (int k = 0; k < kRows; k++) {
                     const int r = w + k * NG;
@@ -221,27 +266,33 @@ __global__ __launch_bounds__(kLanes* NG) void scan_fwd_kernel(ScanArgs a) {
 #pragma unroll
                     for (int v = 0; v < NG; v++) y += sy[v][r][lane];
                     if (gate) y *= zz[k] * sigmoid(zz[k]);
-                    if (p.live) put(out + (long long)(t0 + r) * a.D, at, from_f32<T>(y));
+                    if (p.live) put(out, r * (D * (unsigned)sizeof(T)) + at, from_f32<T>(y));
                 }
+                out += (long long)kTile * D * (long long)sizeof(T);
+            }
         }
+        const auto k2 = scan_args();
         if (kStates) {
             float* sums = (float*)sdt;
             sums[w * kLanes + lane] = total;
             __syncthreads();
             if (!p.live) return;
-            const long long row = ((long long)b * a.chunks + p.chunk) * a.D + d;
-            store4(a.chunk_h + row * a.N, w, a.N, h);
+            const long long row = ((long long)b * a.chunks + p.chunk) * D + d;
+            store4(k2->chunk_h + row * N, w, N, h);
             if (w == 0) {
                 float s = 0.0f;
                 for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
-                a.chunk_dt[row] = any_cut ? __builtin_nanf("") : s;
+                k2->chunk_dt[row] = any_cut ? __builtin_nanf("") : s;
             }
             return;                                                     // chunks: one sequence per workgroup
         }
         if (!p.live) continue;
-        for (int t = max(from, end) + w; t < to; t += NG) put(out + (long long)t * a.D, at, from_f32<T>(0.0f));
-        if (a.s1 && (len ? from < len && len <= to : p.chunk == 0))     // the chunk with the last step
-            store4(a.s1 + ((long long)b * a.D + d) * a.N, w, a.N, h);
+        if (len < to) {
+            out = (char*)k2->out + (long long)b * T_ * D * (long long)sizeof(T);
+            for (int t = max(from, end) + w; t < to; t += NG) put(out + (long long)t * D * (long long)sizeof(T), at, from_f32<T>(0.0f));
+        }
+        if (k2->s1 && (len ? from < len && len <= to : p.chunk == 0))   // the chunk with the last step
+            store4(k2->s1 + (long long)b * D * N + state, w, N, h);
     }
 }
 
@@ -291,61 +342,82 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
     __shared__ alignas(16) float sBC[2][kBack][kWide], sdBC[2][kBack][kWide];
     const Place p = place_of(a);
     if (kCarry && p.chunk == 0) return;
-    const int lane = p.lane, w = p.w, d = p.d;
+    const int lane = p.lane, w = p.w, d = p.d, N = a.N, T_ = a.T, D = a.D;
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
-    const bool gate = a.z;
-    const int from = p.chunk * a.steps, to = min(from + a.steps, a.T), last = from + (to - from - 1) / kBack * kBack;
+    const bool gate = a.z, soft = a.softplus;
+    const int from = p.chunk * a.steps, to = min(from + a.steps, T_), last = from + (to - from - 1) / kBack * kBack;
     // 8 rows of B and of C: half of the threads have one of each
     const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
     const unsigned at = (unsigned)d * (unsigned)sizeof(T);
-    const long long bat = brow * a.bt + bn, cat = brow * a.ct + bn;
+    const long long state = (long long)d * N;
     float A2[4], dA[4], dD = 0.0f, dbias = 0.0f;
-    load4(a.A + (long long)d * a.N, w, a.N, A2);
+    load4(a.A + state, w, N, A2);
     zero4(dA);
 #pragma unroll
     for (int j = 0; j < 4; j++) A2[j] *= kLog2e;
 
+    Rows u, delta, z, dout, Bm, Cm;
     T ru[kRows], rd[kRows], rz[kRows], rg[kRows], rB, rC;
     float start[4];
-    // a tile's inputs as they are stored, and the state it starts from; nv <= 0: nothing
+    auto sequence = [&](int b) __attribute__((always_inline)) {        // its last tile in this chunk
+        const auto k = scan_args();
+        const auto g = grad_args();
+        if (!kCarry) u.set(k->u, b * k->ub + last * k->ut, k->ut, sizeof(T));
+        delta.set(k->delta, b * k->db + last * k->dt, k->dt, sizeof(T));
+        if (gate) z.set(k->z, b * k->zb + last * k->zt, k->zt, sizeof(T));
+        dout.set(g->dout, b * g->ob + last * g->ot, g->ot, sizeof(T));
+        if (!kCarry) Bm.set(k->Bm, b * k->bb + p.g * k->bg + last * k->bt, k->bt, sizeof(T));
+        Cm.set(k->Cm, b * k->cb + p.g * k->cg + last * k->ct, k->ct, sizeof(T));
+    };
+    // a tile's inputs as they are stored, and the state it starts from (nv <= 0: nothing); then on to the tile before
     auto load = [&](int b, int t0, int nv) __attribute__((always_inline)) {
-        const T* u = (const T*)a.u + (b * a.ub + t0 * a.ut);
-        const T* delta = (const T*)a.delta + (b * a.db + t0 * a.dt);
-        const T* z = (const T*)a.z + (b * a.zb + t0 * a.zt);
-        const T* dout = (const T*)q.dout + (b * q.ob + t0 * q.ot);
 #pragma unroll
         for (int k = 0; k < kRows; k++) {
             const int r = w + k * NG;
             if (r < nv) {
-                if (!kCarry) ru[k] = get(u + r * a.ut, at);
-                rd[k] = get(delta + r * a.dt, at);
-                rg[k] = get(dout + r * q.ot, at);
-                if (gate) rz[k] = get(z + r * a.zt, at);
+                if (!kCarry) ru[k] = get<T>(u, r, at);
+                rd[k] = get<T>(delta, r, at);
+                rg[k] = get<T>(dout, r, at);
+                if (gate) rz[k] = get<T>(z, r, at);
             }
         }
-        const bool bl = brow < kBack && brow < nv && bn < a.N;
-        if (!kCarry) rB = bl ? ((const T*)a.Bm + (b * a.bb + p.g * a.bg + t0 * a.bt))[bat] : from_f32<T>(0.0f);
-        rC = bl ? ((const T*)a.Cm + (b * a.cb + p.g * a.cg + t0 * a.ct))[cat] : from_f32<T>(0.0f);
-        if (kCarry || nv <= 0) return;
-        if (t0) load4(a.ckpt + (((long long)b * ((a.T - 1) / kBack) + t0 / kBack - 1) * a.D + d) * a.N, w, a.N, start);
-        else if (a.s0) load4(a.s0 + ((long long)b * a.D + d) * a.N, w, a.N, start);
-        else zero4(start);
+        rB = rC = from_f32<T>(0.0f);
+        if (brow < kBack && brow < nv && bn < N) {
+            if (!kCarry) rB = get<T>(Bm, brow, bn * (unsigned)sizeof(T));
+            rC = get<T>(Cm, brow, bn * (unsigned)sizeof(T));
+        }
+        if (!kCarry && nv > 0) {
+            const auto k = scan_args();
+            if (t0) load4(k->ckpt + ((long long)b * ((T_ - 1) / kBack) + t0 / kBack - 1) * D * N + state, w, N, start);
+            else if (k->s0) load4(k->s0 + (long long)b * D * N + state, w, N, start);
+            else zero4(start);
+        }
+        if (!kCarry) u.move(-kBack), Bm.move(-kBack);
+        delta.move(-kBack), dout.move(-kBack), Cm.move(-kBack);
+        if (gate) z.move(-kBack);
     };
-    int len = p.row < a.B ? seq_len(a.lengths, p.row, a.T) : 0;
-    if (p.row < a.B) load(p.row, last, len - last);
+    int len = 0;
+    if (p.row < a.B) {
+        len = seq_len(a.lengths, p.row, T_);
+        sequence(p.row);
+        load(p.row, last, len - last);
+    }
     for (int b = p.row; b < a.B; b += q.rows) {
-        const long long o = (long long)b * a.T * a.D;
-        const int next_b = b + q.rows, next_len = next_b < a.B ? seq_len(a.lengths, next_b, a.T) : 0;
+        const auto k1 = scan_args();
+        const auto g1 = grad_args();
+        const long long o = ((long long)b * T_ + last) * D * (long long)sizeof(T);
+        char *du = (char*)g1->du + o, *ddelta = (char*)g1->ddelta + o, *dz = (char*)g1->dz + o;
+        const int next_b = b + q.rows, next_len = next_b < a.B ? seq_len(k1->lengths, next_b, T_) : 0;
         float carry[4];                                                 // a_{t+1} g_{t+1}
         zero4(carry);
         if (!kCarry) {
-            if (q.ds1 && p.live) load4(q.ds1 + ((long long)b * a.D + d) * a.N, w, a.N, carry);
+            if (g1->ds1 && p.live) load4(g1->ds1 + (long long)b * D * N + state, w, N, carry);
             fold_chunks(a, b, d, w, a.chunks - 1, p.chunk, -1, A2, carry);
         }
         float total = 0.0f;
         bool any_cut = false;
         for (int t0 = last; t0 >= from; t0 -= kBack) {
-            const int nv = max(0, min(kBack, len - t0)), nt = min(kBack, a.T - t0);
+            const int nv = max(0, min(kBack, len - t0)), nt = min(kBack, T_ - t0);
             float uu[kRows], dts[kRows], sg[kRows], zz[kRows], sz[kRows], go[kRows], now[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) now[j] = p.live ? start[j] : 0.0f;
@@ -359,7 +431,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
                     if (!kCarry) uu[k] = to_f32(ru[k]);
                     dts[k] = to_f32(rd[k]) + bias;
                     sg[k] = 1.0f;
-                    if (a.softplus) dts[k] = softplus(dts[k], sg[k]);
+                    if (soft) dts[k] = softplus(dts[k], sg[k]);
                     go[k] = dy = to_f32(rg[k]);
                     if (gate) {
                         zz[k] = to_f32(rz[k]);
@@ -375,10 +447,11 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
                 if (!kCarry) sBC[0][brow][bn] = to_f32(rB);
                 sBC[1][brow][bn] = to_f32(rC);
             }
-            const unsigned cut = reset_bits(a, b, t0, nv, lane);
+            const unsigned cut = reset_bits(scan_args(), b, t0, nv, lane);
             any_cut |= cut != 0;
             __syncthreads();
             const bool same = t0 > from;
+            if (!same && next_b < a.B) sequence(next_b);
             load(same ? b : next_b, same ? t0 - kBack : last, same ? len - t0 + kBack : next_len - last);
             if (kCarry) {
 #pragma unroll
@@ -462,47 +535,53 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
                 }
                 const float draw = __builtin_fmaf(uu[k], s1, s2 * kLn2) * sg[k];      // s2 was summed with A log2(e)
                 if (p.live) {
-                    const long long row = o + (long long)(t0 + r) * a.D;
-                    put((T*)q.du + row, at, from_f32<T>(__builtin_fmaf(dts[k], s1, skip * dy)));
-                    put((T*)q.ddelta + row, at, from_f32<T>(draw));
-                    if (gate) put((T*)q.dz + row, at, from_f32<T>(dzv));
+                    const unsigned i = r * (D * (unsigned)sizeof(T)) + at;
+                    put(du, i, from_f32<T>(__builtin_fmaf(dts[k], s1, skip * dy)));
+                    put(ddelta, i, from_f32<T>(draw));
+                    if (gate) put(dz, i, from_f32<T>(dzv));
                 }
                 dD = __builtin_fmaf(dy, uu[k], dD);
                 dbias += draw;
             }
-            if (brow < nt && bn < a.N) {                                // nt <= 8
+            const long long back = (long long)kBack * D * (long long)sizeof(T);
+            du -= back, ddelta -= back, dz -= back;
+            if (brow < nt && bn < N) {                                  // nt <= 8
+                const auto k = scan_args();
+                const auto g = grad_args();
                 const float vB = brow < nv ? sdBC[0][brow][bn] : 0.0f, vC = brow < nv ? sdBC[1][brow][bn] : 0.0f;
-                const long long i = (((long long)b * a.T + t0 + brow) * a.G + p.g) * a.N + bn, n = (long long)a.B * a.T * a.G * a.N;
-                if (q.bc_partials) {
-                    q.bc_partials[2 * p.cb * n + i] = vB;
-                    q.bc_partials[(2 * p.cb + 1) * n + i] = vC;
+                const long long i = (((long long)b * T_ + t0 + brow) * k->G + p.g) * N + bn, n = (long long)k->B * T_ * k->G * N;
+                if (g->bc_partials) {
+                    g->bc_partials[2 * p.cb * n + i] = vB;
+                    g->bc_partials[(2 * p.cb + 1) * n + i] = vC;
                 } else {
-                    ((T*)q.dB)[i] = from_f32<T>(vB);
-                    ((T*)q.dC)[i] = from_f32<T>(vC);
+                    ((T*)g->dB)[i] = from_f32<T>(vB);
+                    ((T*)g->dC)[i] = from_f32<T>(vC);
                 }
             }
         }
         len = next_len;
+        const auto k2 = scan_args();
+        const auto g2 = grad_args();
         if (kCarry) {
             float* sums = (float*)sdt;
             sums[w * kLanes + lane] = total;
             __syncthreads();
             if (p.live) {
-                const long long row = ((long long)b * a.chunks + p.chunk) * a.D + d;
-                store4(a.chunk_h + row * a.N, w, a.N, carry);
+                const long long row = ((long long)b * k2->chunks + p.chunk) * D + d;
+                store4(k2->chunk_h + row * N, w, N, carry);
                 if (w == 0) {
                     float s = 0.0f;
                     for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
-                    a.chunk_dt[row] = any_cut ? __builtin_nanf("") : s;
+                    k2->chunk_dt[row] = any_cut ? __builtin_nanf("") : s;
                 }
             }
             __syncthreads();
-        } else if (q.ds0 && p.live && p.chunk == 0)
-            store4(q.ds0 + ((long long)b * a.D + d) * a.N, w, a.N, carry);
+        } else if (g2->ds0 && p.live && p.chunk == 0)
+            store4(g2->ds0 + (long long)b * D * N + state, w, N, carry);
     }
     if (kCarry) return;
     // this workgroup's row of partial parameter gradients: [rows chunks, D, N + 2]
-    float* part = q.param_partials + ((long long)(p.row * a.chunks + p.chunk) * a.D + d) * (a.N + 2);
+    float* part = grad_args()->param_partials + ((long long)(p.row * a.chunks + p.chunk) * D + d) * (N + 2);
     __syncthreads();
     float2* sums = &sdt[0][0];
     sums[w * kLanes + lane] = make_float2(dD, dbias);
@@ -510,13 +589,13 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
     if (!p.live) return;
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (4 * w + j < a.N) part[4 * w + j] = dA[j];
+        if (4 * w + j < N) part[4 * w + j] = dA[j];
     if (w == 0) {
         float s = 0.0f, t = 0.0f;
 #pragma unroll
         for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane].x, t += sums[v * kLanes + lane].y;
-        part[a.N] = s;
-        part[a.N + 1] = t;
+        part[N] = s;
+        part[N + 1] = t;
     }
 }
 
@@ -541,29 +620,34 @@ template <typename T> struct ScanShared {
     }
 };
 
-// One step: a channel's state is spread over L lanes, four numbers each, so that a wave moves 1 KB of states per access.
+// One step: a channel's state is spread over L lanes, four numbers each, so that a wave moves 1 KB of states per access; the states
+// in and out are nearly all of the bytes.
 template <typename T, int L>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
-    const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / L;
+    const unsigned item = (unsigned)(((unsigned long long)blockIdx.x * 256 + threadIdx.x) / L), D = a.D;      // B D < 2^31
     const int part = threadIdx.x % L;
-    const bool live = item < (long long)a.B * a.D;
-    const int b = live ? (int)(item / a.D) : 0, d = live ? (int)(item - (long long)b * a.D) : 0, g = d / a.Dg;
-    const T* Bm = (const T*)a.Bm + b * a.bb + g * a.bg;
-    const T* Cm = (const T*)a.Cm + b * a.cb + g * a.cg;
-    const float uu = to_f32(((const T*)a.u)[b * a.ub + d]);
-    const float dt = time_step(a, to_f32(((const T*)a.delta)[b * a.db + d]) + (a.bias ? a.bias[d] : 0.0f));
+    const bool live = item < (unsigned)a.B * D;
+    const unsigned b = live ? item / D : 0, d = live ? item - b * D : 0, g = a.G > 1 ? d / (unsigned)a.Dg : 0;
+    const T* Bm = (const T*)a.Bm + (b * a.bb + g * a.bg);
+    const T* Cm = (const T*)a.Cm + (b * a.cb + g * a.cg);
+    const long long row = ((long long)b * D + d) * a.N;
+    float h[4], A[4];
+    zero4(h);
     const bool cut = a.resets && a.resets[b * a.rb];
+    if (a.s0 && !cut) load4(a.s0 + row, part, a.N, h);
+    load4(a.A + (long long)d * a.N, part, a.N, A);
+    const float uu = to_f32(((const T*)a.u)[b * a.ub + d]);
+    const float raw = to_f32(((const T*)a.delta)[b * a.db + d]) + (a.bias ? a.bias[d] : 0.0f);
+    const float dt = a.softplus ? softplus(raw) : raw;
     float y = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int n = 4 * part + j;
         if (n >= a.N) break;
-        const long long at = ((long long)b * a.D + d) * a.N + n;
-        float h = a.s0 && !cut ? a.s0[at] : 0.0f;
-        h = __builtin_fmaf(exp2_hw(dt * (a.A[(long long)d * a.N + n] * kLog2e)), h, dt * uu * to_f32(Bm[n]));
-        y = __builtin_fmaf(to_f32(Cm[n]), h, y);
-        if (live) a.s1[at] = h;
+        h[j] = __builtin_fmaf(exp2_hw(dt * (A[j] * kLog2e)), h[j], dt * uu * to_f32(Bm[n]));
+        y = __builtin_fmaf(to_f32(Cm[n]), h[j], y);
     }
+    if (live) store4(a.s1 + row, part, a.N, h);
     if (L > 1) y += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y), 0xB1, 0xf, 0xf, true));
     if (L > 2) y += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y), 0x4E, 0xf, 0xf, true));
     if (L > 4) y += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y), 0x141, 0xf, 0xf, true));
@@ -579,12 +663,14 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
 int groups_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 int channel_blocks(int D, int G) { return (D / G + kLanes - 1) / kLanes; }
 
-// Chunks of time.  1024 workgroups are four per CU; where sequences and channels give fewer, time is cut so that there are about that
-// many, in chunks of at least 64 steps (a multiple of 16): the first pass costs the chunks about as much again as the forward's states.
+// Chunks of time.  1536 workgroups are six per CU, what the forward's registers let in and two rounds of the backward; where sequences
+// and channels give fewer, time is cut so that there are about that many, in chunks of at least 64 steps (a multiple of 16).  Measured
+// at B = 8, T = 2047, D = 2048, bf16, ragged: 1024 workgroups 235 + 530 us (forward + backward), 1536 200 + 510, 3072 195 + 508; at B = 1,
+// T = 4096, D = 2048, where each chunk has more chunks before it to start from: 88, 100 and 98 us.
 struct Chunks { int count, steps; };
 Chunks chunks_of(int B, int T, int D, int G) {
     const long long blocks = (long long)B * G * channel_blocks(D, G);
-    const long long want = (1024 + blocks - 1) / blocks;
+    const long long want = (1536 + blocks - 1) / blocks;
     long long steps = ((T + want - 1) / want + kTile - 1) / kTile * kTile;
     if (steps < 64) steps = 64;
     if (want == 1 || steps >= T) return Chunks{1, (T + kTile - 1) / kTile * kTile};
@@ -603,8 +689,11 @@ int check(const ag_scan_args* p) {
     if (!p || p->struct_size != sizeof(ag_scan_args) || !p->u_dev || !p->delta_dev || !p->Bm_dev || !p->Cm_dev || !p->A_dev)
         return AG_ERR_INVALID_ARG;
     if (p->B <= 0 || p->T <= 0 || p->D <= 0 || p->G <= 0 || p->N <= 0 || p->D % p->G) return AG_ERR_INVALID_ARG;
-    if (p->N > 32 || p->D > 1 << 28 || p->dtype < AG_F32 || p->dtype > AG_F16) return AG_ERR_UNSUPPORTED;
-    // the grid, with time in chunks: at most 1024 + B G channel blocks (or one per sequence and 64 channels)
+    if (p->N > 32 || p->dtype < AG_F32 || p->dtype > AG_F16) return AG_ERR_UNSUPPORTED;
+    // a lane's offset within a tile's rows has 32 bits
+    const long long most = (0xffffffffLL / 4 - p->D) / kTile;
+    if (p->D > most || p->u_st > most || p->delta_st > most || p->z_st > most || p->b_st > most || p->c_st > most) return AG_ERR_UNSUPPORTED;
+    // the grid, with time in chunks: about 1536 or B G channel blocks (or one per sequence and 64 channels)
     if ((long long)p->B * p->G * channel_blocks(p->D, p->G) > 0x7fffffffLL - 4096) return AG_ERR_UNSUPPORTED;
     return AG_OK;
 }
@@ -674,6 +763,7 @@ extern "C" int ag_selective_scan_bwd(const ag_scan_args* p, const ag_scan_grads*
         !s->dA_dev || !s->workspace_dev || (p->z_dev != nullptr) != (s->dz_dev != nullptr) || (p->T > kBack && !p->ckpt_dev))
         return AG_ERR_INVALID_ARG;
     if (s->workspace_bytes < ag_selective_scan_workspace_bytes(p->B, p->T, p->D, p->N, p->G, 1)) return AG_ERR_INVALID_ARG;
+    if (s->dout_st > (0xffffffffLL / 4 - p->D) / kTile) return AG_ERR_UNSUPPORTED;
     ScanArgs a = device_args(p);
     a.chunk_h = (float*)s->workspace_dev;
     a.chunk_dt = a.chunk_h + (long long)a.B * a.chunks * a.D * a.N;
@@ -699,8 +789,8 @@ extern "C" int ag_selective_scan_step(const ag_scan_args* p, void* stream) {
     if (p->T != 1 || !p->out_dev || !p->state_out_dev) return AG_ERR_INVALID_ARG;
     const ScanArgs a = device_args(p);
     const int lanes = groups_of(p->N);
+    if ((long long)a.B * a.D > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
     const long long blocks = ((long long)a.B * a.D * lanes + 255) / 256;
-    if (blocks > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
     AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, NG>), dim3((unsigned)blocks), dim3(256), 0,
                                                                   (hipStream_t)stream, a)));
     return seq_status();

@@ -78,8 +78,25 @@ __global__ __launch_bounds__(64 * Parts) void sum_rows_kernel(const float* table
     out(i, s);
 }
 
+// ... and of a table of few rows: a column per thread
+template <typename Out>
+__global__ __launch_bounds__(256) void sum_few_rows_kernel(const float* table, int rows, long long n, Out out) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int r = 0; r < rows; r++) s += table[(long long)r * n + i];
+    out(i, s);
+}
+
+// At 256 columns x 1024 rows the split rows take 5 us where a column per thread took 236; at 3 M columns x 4 rows the plain form takes
+// half of theirs.
 template <typename Out>
 inline void launch_sum_rows(const float* table, int rows, long long n, Out out, void* stream) {
+    if (rows <= 4 || n >= (1 << 18)) {
+        hipLaunchKernelGGL((sum_few_rows_kernel<Out>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, table, rows, n, out);
+        return;
+    }
     const dim3 grid((unsigned)((n + 63) / 64));
     if (rows > 64) hipLaunchKernelGGL((sum_rows_kernel<16, Out>), grid, dim3(1024), 0, (hipStream_t)stream, table, rows, n, out);
     else hipLaunchKernelGGL((sum_rows_kernel<4, Out>), grid, dim3(256), 0, (hipStream_t)stream, table, rows, n, out);
