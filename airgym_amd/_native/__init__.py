@@ -325,7 +325,7 @@ SYMBOLS = [
     ("ag_ppo_loss", ctypes.c_int, [_P] * 9 + [ctypes.c_int, ctypes.c_int, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                    ctypes.c_int, ctypes.c_int, _P, _P, _P, _P, ctypes.POINTER(ctypes.c_int), _P]),
     ("ag_causal_conv_fwd", ctypes.c_int, [ctypes.POINTER(AgConvArgs), _P]),
-    ("ag_causal_conv_workspace_bytes", ctypes.c_longlong, [ctypes.c_int] * 4),
+    ("ag_causal_conv_workspace_bytes", ctypes.c_longlong, [ctypes.c_int] * 5),
     ("ag_causal_conv_bwd", ctypes.c_int, [ctypes.POINTER(AgConvArgs), ctypes.POINTER(AgConvGrads), _P]),
     ("ag_causal_conv_step", ctypes.c_int, [_P, ctypes.c_longlong, _P, _P, _P, _P, _P] + [ctypes.c_int] * 5 + [_P]),
     ("ag_selective_scan_ckpt_floats", ctypes.c_longlong, [ctypes.c_int] * 4),

@@ -3,146 +3,259 @@
 //   p[t] = bias + sum_k w[k] x[t-W+1+k]   (taps before the last reset are zero, before step 0 they are the state's)
 //   y[t] = p sigmoid(p)  or  p
 //
-// One thread owns a channel over a run of consecutive steps and carries the last W-1 inputs in registers, so that every input is
-// read once per run plus W-1 steps of halo.  Neighbouring lanes hold neighbouring channels.
+// One thread owns VEC neighbouring channels over a run of consecutive steps and carries the last W-1 inputs in registers, so that every
+// input is read once per run plus W-1 steps of halo.  A workgroup is lx threads along the channels by ly runs.  Memory bounds it: the
+// arithmetic is about 20 issue slots per element (half of them the sigmoid) for 4 to 8 bytes.  Hence accesses of 16 bytes where the
+// channels divide (4 bytes or single channels where not), four steps' loads at a time, and runs short enough to have many in flight.
 #include "seq_common.hpp"
 
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRun = 32;               // steps per thread
+constexpr int kAhead = 4;              // steps whose loads are issued together
 
 struct ConvArgs {
     const void* x; const float* w; const float* bias; const void* s0; const int* lengths; const unsigned char* resets;
     void* y; void* s1;
     long long xb, xt, rb, rt;
-    int B, T, D, silu, runs;
+    int B, T, D, silu;
+    int run, runs;                     // steps per thread, runs per sequence
+    int lx, ly, nx;                    // threads along channels and along runs in a workgroup, workgroups along channels
 };
 
 struct ConvGradArgs {
     const void *dy, *ds1; void* dx; void* ds0; float* partials;
     long long dyb, dyt;
-    int rows;
+    int groups;                        // workgroups along the runs = rows of partial parameter gradients
 };
 
-// input at step t of sequence b; the state's before step 0
-template <typename T, int W>
-__device__ __forceinline__ float input_at(const ConvArgs& a, int b, int t, int d) {
-    if (t >= 0) return to_f32(((const T*)a.x)[b * a.xb + t * a.xt + d]);
-    return a.s0 ? to_f32(((const T*)a.s0)[((long long)b * (W - 1) + (t + W - 1)) * a.D + d]) : 0.0f;
-}
-
-// the W-1 inputs before step t0 as the convolution sees them there: zero from the last reset in the halo backwards
-template <typename T, int W>
-__device__ __forceinline__ void load_window(const ConvArgs& a, int b, int t0, int d, float* win) {
+// the W-1 inputs before step t0 as the convolution sees them there: the state's before step 0, zero from the last reset backwards
+template <typename T, int W, int VEC>
+__device__ __forceinline__ void load_window(const ConvArgs& a, int b, int t0, int d, float (*win)[VEC]) {
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
         const int t = t0 - (W - 1) + j;
-        if (a.resets && t >= 0 && a.resets[b * a.rb + t * a.rt])
+        Vec<T, VEC> c;
+        if (t >= 0) {
+            c = load_vec<T, VEC>((const T*)a.x + (b * a.xb + t * a.xt + d));
+            if (a.resets && a.resets[b * a.rb + t * a.rt])
 #pragma unroll
-            for (int i = 0; i < j; i++) win[i] = 0.0f;
-        win[j] = input_at<T, W>(a, b, t, d);
+                for (int i = 0; i < j; i++)
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) win[i][v] = 0.0f;
+        } else if (a.s0) c = load_vec<T, VEC>((const T*)a.s0 + (((long long)b * (W - 1) + (t + W - 1)) * a.D + d));
+#pragma unroll
+        for (int v = 0; v < VEC; v++) win[j][v] = t >= 0 || a.s0 ? c.at(v) : 0.0f;
     }
 }
 
-template <typename T, int W>
-__global__ __launch_bounds__(kThreads) void conv_fwd_kernel(ConvArgs a) {
-    const long long item = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const int d = (int)(item % a.D);
-    const long long row = item / a.D;                    // (b, run)
-    if (row >= (long long)a.B * a.runs) return;
-    const int b = (int)(row / a.runs), t0 = (int)(row % a.runs) * kRun;
-    const int len = seq_len(a.lengths, b, a.T);
-    const int t1 = min(t0 + kRun, a.T), tv = min(t1, len);
-    T* y = (T*)a.y + ((long long)b * a.T) * a.D + d;
-    float w[W], win[W];
+template <typename T, int W, int VEC>
+__device__ __forceinline__ void load_taps(const ConvArgs& a, int d, float (*w)[VEC], float* bias) {
 #pragma unroll
-    for (int k = 0; k < W; k++) w[k] = a.w[(long long)d * W + k];
-    const float bias = a.bias ? a.bias[d] : 0.0f;
-    if (t0 < tv || (len == 0 && t0 == 0)) load_window<T, W>(a, b, min(t0, len), d, win);
-    for (int t = t0; t < tv; t++) {
-        if (a.resets && a.resets[b * a.rb + t * a.rt])
+    for (int v = 0; v < VEC; v++) {
 #pragma unroll
-            for (int j = 0; j < W - 1; j++) win[j] = 0.0f;
-        win[W - 1] = to_f32(((const T*)a.x)[b * a.xb + t * a.xt + d]);
-        float p = bias;
-#pragma unroll
-        for (int k = 0; k < W; k++) p = __builtin_fmaf(w[k], win[k], p);
-        y[(long long)t * a.D] = from_f32<T>(a.silu ? p * sigmoid(p) : p);
-#pragma unroll
-        for (int j = 0; j < W - 1; j++) win[j] = win[j + 1];
+        for (int k = 0; k < W; k++) w[k][v] = a.w[(long long)(d + v) * W + k];
+        bias[v] = a.bias ? a.bias[d + v] : 0.0f;
     }
-    for (int t = max(t0, tv); t < t1; t++) y[(long long)t * a.D] = from_f32<T>(0.0f);
-    // the run that holds the last step (the first run of an empty sequence) leaves the state behind
-    if (a.s1 && (len == 0 ? t0 == 0 : (t0 < len && len <= t0 + kRun))) {
-        T* s1 = (T*)a.s1 + ((long long)b * (W - 1)) * a.D + d;
+}
+
+template <typename T, int W, int VEC>
+__global__ __launch_bounds__(kThreads) void conv_fwd_kernel(ConvArgs a) {
+    const int tx = threadIdx.x % a.lx, ty = threadIdx.x / a.lx;
+    const int d = ((int)(blockIdx.x % a.nx) * a.lx + tx) * VEC;
+    const long long row = (long long)(blockIdx.x / a.nx) * a.ly + ty;           // (b, run)
+    if (ty >= a.ly || d >= a.D || row >= (long long)a.B * a.runs) return;
+    const int b = (int)(row / a.runs), t0 = (int)(row - (long long)b * a.runs) * a.run;
+    const int len = seq_len(a.lengths, b, a.T);
+    const int t1 = min(t0 + a.run, a.T), tv = min(t1, len);
+    const T* x = (const T*)a.x + (b * a.xb + d);
+    T* y = (T*)a.y + ((long long)b * a.T * a.D + d);
+    float w[W][VEC], bias[VEC], win[W][VEC];
+    load_taps<T, W, VEC>(a, d, w, bias);
+    if (t0 < tv || (len == 0 && t0 == 0)) load_window<T, W, VEC>(a, b, min(t0, len), d, win);
+    for (int t = t0; t < tv; t += kAhead) {
+        Vec<T, VEC> c[kAhead];
+        unsigned char cut[kAhead];
 #pragma unroll
-        for (int j = 0; j < W - 1; j++) s1[(long long)j * a.D] = from_f32<T>(win[j]);
+        for (int i = 0; i < kAhead; i++) {
+            cut[i] = 0;
+            if (t + i < tv) {
+                c[i] = load_vec<T, VEC>(x + (t + i) * a.xt);
+                if (a.resets) cut[i] = a.resets[b * a.rb + (t + i) * a.rt];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) {
+            if (t + i >= tv) break;
+            float p[VEC];
+#pragma unroll
+            for (int v = 0; v < VEC; v++) {
+                win[W - 1][v] = c[i].at(v);
+                p[v] = bias[v];
+            }
+            if (cut[i])
+#pragma unroll
+                for (int j = 0; j < W - 1; j++)
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) win[j][v] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < W; k++)
+#pragma unroll
+                for (int v = 0; v < VEC; v++) p[v] = __builtin_fmaf(w[k][v], win[k][v], p[v]);
+            if (a.silu)
+#pragma unroll
+                for (int v = 0; v < VEC; v++) p[v] *= sigmoid(p[v]);
+            Vec<T, VEC> o;
+            o.set(p);
+            store_vec<T, VEC>(y + (long long)(t + i) * a.D, o);
+#pragma unroll
+            for (int j = 0; j < W - 1; j++)
+#pragma unroll
+                for (int v = 0; v < VEC; v++) win[j][v] = win[j + 1][v];
+        }
+    }
+    const float none[VEC] = {};
+    Vec<T, VEC> zero;
+    zero.set(none);
+    for (int t = max(t0, tv); t < t1; t++) store_vec<T, VEC>(y + (long long)t * a.D, zero);
+    // the run that holds the last step (the first run of an empty sequence) leaves the state behind
+    if (a.s1 && (len == 0 ? t0 == 0 : (t0 < len && len <= t0 + a.run))) {
+        T* s1 = (T*)a.s1 + ((long long)b * (W - 1) * a.D + d);
+#pragma unroll
+        for (int j = 0; j < W - 1; j++) {
+            Vec<T, VEC> o;
+            o.set(win[j]);
+            store_vec<T, VEC>(s1 + (long long)j * a.D, o);
+        }
     }
 }
 
 // dp[t] = dy[t] act'(p[t]);  dx[t] = sum_k w[k] dp[t+W-1-k], the later step not behind a reset after t.  The thread walks on W-1
-// steps past its run for the contributions of later steps; those steps' own parameter gradients belong to the next run.
-template <typename T, int W>
+// steps past its run for the contributions of later steps; those steps' own parameter gradients belong to the next run.  A workgroup
+// takes every `groups`-th block of runs, and adds up its own runs' parameter gradients.
+template <typename T, int W, int VEC>
 __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGradArgs g) {
-    const long long item = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const int d = (int)(item % a.D);
-    const long long lane_row = item / a.D;
-    if (lane_row >= g.rows) return;
-    float w[W], dw[W], db = 0.0f;
+    __shared__ float sums[kThreads];
+    const int tx = threadIdx.x % a.lx, ty = threadIdx.x / a.lx;
+    const int dx0 = ((int)(blockIdx.x % a.nx) * a.lx + tx) * VEC, group = blockIdx.x / a.nx;
+    const bool live = ty < a.ly && dx0 < a.D;
+    const int d = live ? dx0 : 0;
+    float w[W][VEC], bias[VEC], dw[W + 1][VEC];
+    load_taps<T, W, VEC>(a, d, w, bias);
 #pragma unroll
-    for (int k = 0; k < W; k++) w[k] = a.w[(long long)d * W + k], dw[k] = 0.0f;
-    const float bias = a.bias ? a.bias[d] : 0.0f;
-    for (long long row = lane_row; row < (long long)a.B * a.runs; row += g.rows) {
-        const int b = (int)(row / a.runs), t0 = (int)(row % a.runs) * kRun, t1 = min(t0 + kRun, a.T);
-        const int len = seq_len(a.lengths, b, a.T);
-        T* dx = (T*)g.dx + ((long long)b * a.T) * a.D + d;
-        float win[W], acc[W];                      // inputs and their gradients, oldest first
+    for (int k = 0; k <= W; k++)
 #pragma unroll
-        for (int j = 0; j < W; j++) acc[j] = 0.0f;
-        load_window<T, W>(a, b, t0, d, win);       // beyond the length: read but not used (dp = 0 there)
-        int alive = W;                             // taps that reach back over no reset since the run's start
-        for (int t = t0; t < t1 + W - 1; t++) {
-            float dp = 0.0f;
-            win[W - 1] = 0.0f;
-            if (t < len) {
-                if (a.resets && a.resets[b * a.rb + t * a.rt]) {
-                    alive = 1;
+        for (int v = 0; v < VEC; v++) dw[k][v] = 0.0f;
+    const long long rows = (long long)a.B * a.runs;
+    if (live)
+        for (long long row = (long long)group * a.ly + ty; row < rows; row += (long long)g.groups * a.ly) {
+            const int b = (int)(row / a.runs), t0 = (int)(row - (long long)b * a.runs) * a.run, t1 = min(t0 + a.run, a.T);
+            const int len = seq_len(a.lengths, b, a.T);
+            const T* x = (const T*)a.x + (b * a.xb + d);
+            const T* dy = (const T*)g.dy + (b * g.dyb + d);
+            T* dx = (T*)g.dx + ((long long)b * a.T * a.D + d);
+            float win[W][VEC], acc[W][VEC];        // inputs and their gradients, oldest first
 #pragma unroll
-                    for (int j = 0; j < W - 1; j++) win[j] = 0.0f;
-                }
-                win[W - 1] = to_f32(((const T*)a.x)[b * a.xb + t * a.xt + d]);
-                float p = bias;
+            for (int j = 0; j < W; j++)
 #pragma unroll
-                for (int k = 0; k < W; k++) p = __builtin_fmaf(w[k], win[k], p);
-                dp = to_f32(((const T*)g.dy)[b * g.dyb + t * g.dyt + d]);
-                if (a.silu) {
-                    const float s = sigmoid(p);
-                    dp *= s * (1.0f + p * (1.0f - s));
-                }
-                if (t < t1) {
-                    db += dp;
+                for (int v = 0; v < VEC; v++) acc[j][v] = 0.0f;
+            load_window<T, W, VEC>(a, b, t0, d, win);      // beyond the length: read but not used (dp = 0 there)
+            int alive = W;                         // taps that reach back over no reset since the run's start
+            for (int t = t0; t < t1 + W - 1; t += kAhead) {
+                Vec<T, VEC> cx[kAhead], cg[kAhead];
+                unsigned char cut[kAhead];
 #pragma unroll
-                    for (int k = 0; k < W; k++) dw[k] = __builtin_fmaf(dp, win[k], dw[k]);
+                for (int i = 0; i < kAhead; i++) {
+                    cut[i] = 0;
+                    if (t + i < min(len, t1 + W - 1)) {
+                        cx[i] = load_vec<T, VEC>(x + (t + i) * a.xt);
+                        cg[i] = load_vec<T, VEC>(dy + (t + i) * g.dyt);
+                        if (a.resets) cut[i] = a.resets[b * a.rb + (t + i) * a.rt];
+                    }
                 }
 #pragma unroll
-                for (int k = 0; k < W; k++) acc[k] = k >= W - alive ? __builtin_fmaf(w[k], dp, acc[k]) : acc[k];
-                alive = min(alive + 1, W);
+                for (int i = 0; i < kAhead; i++) {
+                    const int ti = t + i;
+                    if (ti >= t1 + W - 1) break;
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) win[W - 1][v] = 0.0f;
+                    if (ti < len) {
+                        float p[VEC], dp[VEC];
+                        if (cut[i]) {
+                            alive = 1;
+#pragma unroll
+                            for (int j = 0; j < W - 1; j++)
+#pragma unroll
+                                for (int v = 0; v < VEC; v++) win[j][v] = 0.0f;
+                        }
+#pragma unroll
+                        for (int v = 0; v < VEC; v++) {
+                            win[W - 1][v] = cx[i].at(v);
+                            p[v] = bias[v];
+                            dp[v] = cg[i].at(v);
+                        }
+                        if (a.silu) {
+#pragma unroll
+                            for (int k = 0; k < W; k++)
+#pragma unroll
+                                for (int v = 0; v < VEC; v++) p[v] = __builtin_fmaf(w[k][v], win[k][v], p[v]);
+#pragma unroll
+                            for (int v = 0; v < VEC; v++) {
+                                const float s = sigmoid(p[v]);
+                                dp[v] *= s * (1.0f + p[v] * (1.0f - s));
+                            }
+                        }
+                        if (ti < t1) {
+#pragma unroll
+                            for (int v = 0; v < VEC; v++) {
+                                dw[W][v] += dp[v];
+#pragma unroll
+                                for (int k = 0; k < W; k++) dw[k][v] = __builtin_fmaf(dp[v], win[k][v], dw[k][v]);
+                            }
+                        }
+#pragma unroll
+                        for (int k = 0; k < W; k++)
+                            if (k >= W - alive)
+#pragma unroll
+                                for (int v = 0; v < VEC; v++) acc[k][v] = __builtin_fmaf(w[k][v], dp[v], acc[k][v]);
+                        alive = min(alive + 1, W);
+                    }
+                    const int done = ti - (W - 1);         // this input has met every step that reads it
+                    if (g.ds1 && ti >= len && done < len && len - 1 - done < alive - 1) {      // ... and is part of the state left behind
+                        const auto c = load_vec<T, VEC>((const T*)g.ds1 + (((long long)b * (W - 1) + (ti - len)) * a.D + d));
+#pragma unroll
+                        for (int v = 0; v < VEC; v++) acc[0][v] += c.at(v);
+                    }
+                    Vec<T, VEC> o;
+                    o.set(acc[0]);
+                    if (done >= t0) store_vec<T, VEC>(dx + (long long)done * a.D, o);
+                    else if (t0 == 0 && g.ds0) store_vec<T, VEC>((T*)g.ds0 + (((long long)b * (W - 1) + ti) * a.D + d), o);
+#pragma unroll
+                    for (int v = 0; v < VEC; v++) {
+#pragma unroll
+                        for (int j = 0; j < W - 1; j++) win[j][v] = win[j + 1][v], acc[j][v] = acc[j + 1][v];
+                        acc[W - 1][v] = 0.0f;
+                    }
+                }
             }
-            const int done = t - (W - 1);          // this input has met every step that reads it
-            if (g.ds1 && t >= len && done < len && len - 1 - done < alive - 1)      // ... and is part of the state left behind
-                acc[0] += to_f32(((const T*)g.ds1)[((long long)b * (W - 1) + (t - len)) * a.D + d]);
-            if (done >= t0) dx[(long long)done * a.D] = from_f32<T>(acc[0]);
-            else if (t0 == 0 && g.ds0) ((T*)g.ds0)[((long long)b * (W - 1) + t) * a.D + d] = from_f32<T>(acc[0]);
-#pragma unroll
-            for (int j = 0; j < W - 1; j++) win[j] = win[j + 1], acc[j] = acc[j + 1];
-            acc[W - 1] = 0.0f;
         }
-    }
-    float* out = g.partials + (lane_row * a.D + d) * (W + 1);
+    // the workgroup's runs added up in order; one row of partial gradients [groups, D, W + 1]
+    float* out = g.partials + ((long long)group * a.D + d) * (W + 1);
 #pragma unroll
-    for (int k = 0; k < W; k++) out[k] = dw[k];
-    out[W] = db;
+    for (int k = 0; k <= W; k++)
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            if (a.ly > 1) {
+                __syncthreads();
+                sums[threadIdx.x] = dw[k][v];
+                __syncthreads();
+            }
+            if (live && ty == 0) {
+                float s = dw[k][v];
+                for (int j = 1; j < a.ly; j++) s += sums[j * a.lx + tx];
+                out[v * (W + 1) + k] = s;
+            }
+        }
 }
 
 struct ConvParams {
@@ -177,25 +290,46 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(const T* x, long lo
     for (int j = 0; j < W - 1; j++) s[(long long)j * D] = win[j + 1];
 }
 
-int runs_of(int T) { return (T + kRun - 1) / kRun; }
+// How the work is laid out, from sizes alone: channels per thread, threads along the channels, steps per run.
+struct Plan { int vec, lx, ly, nx, run, runs; };
+Plan plan_of(long long B, int T, int D, int wide) {
+    Plan p;
+    // 16 bytes per access (8 for the backward's 16-bit types, which carry gradients too); channels that do not divide move two or one
+    p.vec = D % wide == 0 ? wide : D % 2 == 0 ? 2 : 1;
+    const int dv = D / p.vec;
+    p.lx = dv < kThreads ? dv : kThreads;
+    p.ly = kThreads / p.lx;
+    p.nx = (dv + p.lx - 1) / p.lx;
+    // whole sequences per thread if that makes 4096 waves (16 per CU) or sequences are short; else runs of 16 steps and more
+    const long long threads = B * dv;
+    long long runs = (262144 + threads - 1) / threads;
+    long long run = (T + runs - 1) / runs;
+    run = (run + kAhead - 1) / kAhead * kAhead;
+    p.run = (int)(run < 16 ? 16 : run);
+    p.runs = (T + p.run - 1) / p.run;
+    return p;
+}
 
-// rows of partial parameter gradients: enough threads to fill the chip, and no more rows than there are runs
-int grad_rows(long long B, int T, int D) {
-    const long long all = B * runs_of(T), want = (262144 + D - 1) / D;
-    return (int)(all < want ? all : want);
+constexpr int wide_fwd(int size) { return 16 / size; }
+constexpr int wide_bwd(int) { return 4; }
+
+// workgroups along the runs in the backward, each with one row of partial gradients
+int grad_groups(const Plan& p, long long B) {
+    const long long blocks = (B * p.runs + p.ly - 1) / p.ly, want = (1024 + p.nx - 1) / p.nx;
+    return (int)(blocks < want ? blocks : want);
 }
 
 int check(const ag_conv_args* p) {
     if (!p || p->struct_size != sizeof(ag_conv_args) || !p->x_dev || !p->weight_dev) return AG_ERR_INVALID_ARG;
     if (p->B <= 0 || p->T <= 0 || p->D <= 0) return AG_ERR_INVALID_ARG;
     if (p->W < 2 || p->W > 8 || p->dtype < AG_F32 || p->dtype > AG_F16) return AG_ERR_UNSUPPORTED;
-    if (((long long)p->B * runs_of(p->T) * p->D + kThreads - 1) / kThreads > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
+    if ((long long)p->B * (p->T / 16 + 1) > 0x7fffffffLL / ((p->D + kThreads - 1) / kThreads)) return AG_ERR_UNSUPPORTED;
     return AG_OK;
 }
 
-ConvArgs device_args(const ag_conv_args* p) {
+ConvArgs device_args(const ag_conv_args* p, const Plan& l) {
     return ConvArgs{p->x_dev, p->weight_dev, p->bias_dev, p->state_in_dev, p->lengths_dev, p->resets_dev, p->y_dev, p->state_out_dev,
-                    p->x_sb, p->x_st, p->r_sb, p->r_st, p->B, p->T, p->D, p->silu, runs_of(p->T)};
+                    p->x_sb, p->x_st, p->r_sb, p->r_st, p->B, p->T, p->D, p->silu, l.run, l.runs, l.lx, l.ly, l.nx};
 }
 
 }  // namespace
@@ -214,32 +348,46 @@ ConvArgs device_args(const ag_conv_args* p) {
         }                                                                \
     } while (0)
 
+// run CALL with VEC bound to the plan's channels per thread
+#define AG_FOR_VEC(vec, WIDE, CALL)                            \
+    do {                                                       \
+        if (vec == WIDE) { constexpr int VEC = WIDE; CALL; }   \
+        else if (vec == 2) { constexpr int VEC = 2; CALL; }    \
+        else { constexpr int VEC = 1; CALL; }                  \
+    } while (0)
+
 extern "C" int ag_causal_conv_fwd(const ag_conv_args* p, void* stream) {
     if (const int rc = check(p)) return rc;
     if (!p->y_dev) return AG_ERR_INVALID_ARG;
-    const ConvArgs a = device_args(p);
-    const long long items = (long long)a.B * a.runs * a.D;
-    const dim3 grid((unsigned)((items + kThreads - 1) / kThreads));
-    AG_FOR_DTYPE(p->dtype, AG_FOR_TAPS(p->W, hipLaunchKernelGGL((conv_fwd_kernel<T, W>), grid, dim3(kThreads), 0, (hipStream_t)stream, a)));
+    const int size = p->dtype == AG_F32 ? 4 : 2;
+    const Plan l = plan_of(p->B, p->T, p->D, wide_fwd(size));
+    const ConvArgs a = device_args(p, l);
+    const dim3 grid((unsigned)(((long long)a.B * a.runs + l.ly - 1) / l.ly * l.nx));
+    AG_FOR_DTYPE(p->dtype, AG_FOR_TAPS(p->W, AG_FOR_VEC(l.vec, wide_fwd(sizeof(T)), hipLaunchKernelGGL((conv_fwd_kernel<T, W, VEC>), grid,
+                                                                                     dim3(kThreads), 0, (hipStream_t)stream, a))));
     return seq_status();
 }
 
-extern "C" long long ag_causal_conv_workspace_bytes(int B, int T, int D, int W) {
-    if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 8) return 0;
-    return (long long)grad_rows(B, T, D) * D * (W + 1) * (long long)sizeof(float);
+extern "C" long long ag_causal_conv_workspace_bytes(int B, int T, int D, int W, int dtype) {
+    if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 8 || dtype < AG_F32 || dtype > AG_F16) return 0;
+    const int size = dtype == AG_F32 ? 4 : 2;
+    return (long long)grad_groups(plan_of(B, T, D, wide_bwd(size)), B) * D * (W + 1) * (long long)sizeof(float);
 }
 
 extern "C" int ag_causal_conv_bwd(const ag_conv_args* p, const ag_conv_grads* q, void* stream) {
     if (const int rc = check(p)) return rc;
     if (!q || q->struct_size != sizeof(ag_conv_grads) || !q->dy_dev || !q->dx_dev || !q->dweight_dev || !q->workspace_dev)
         return AG_ERR_INVALID_ARG;
-    if (q->workspace_bytes < ag_causal_conv_workspace_bytes(p->B, p->T, p->D, p->W)) return AG_ERR_INVALID_ARG;
-    const ConvArgs a = device_args(p);
-    const int rows = grad_rows(a.B, a.T, a.D);
-    const ConvGradArgs g{q->dy_dev, q->dstate_out_dev, q->dx_dev, q->dstate_dev, (float*)q->workspace_dev, q->dy_sb, q->dy_st, rows};
-    const dim3 grid((unsigned)(((long long)rows * a.D + kThreads - 1) / kThreads));
-    AG_FOR_DTYPE(p->dtype, AG_FOR_TAPS(p->W, hipLaunchKernelGGL((conv_bwd_kernel<T, W>), grid, dim3(kThreads), 0, (hipStream_t)stream, a, g)));
-    launch_sum_rows(g.partials, rows, (long long)a.D * (p->W + 1), ConvParams{q->dweight_dev, q->dbias_dev, p->W}, stream);
+    if (q->workspace_bytes < ag_causal_conv_workspace_bytes(p->B, p->T, p->D, p->W, p->dtype)) return AG_ERR_INVALID_ARG;
+    const int size = p->dtype == AG_F32 ? 4 : 2;
+    const Plan l = plan_of(p->B, p->T, p->D, wide_bwd(size));
+    const ConvArgs a = device_args(p, l);
+    const ConvGradArgs g{q->dy_dev, q->dstate_out_dev, q->dx_dev, q->dstate_dev, (float*)q->workspace_dev, q->dy_sb, q->dy_st,
+                         grad_groups(l, a.B)};
+    const dim3 grid((unsigned)(g.groups * l.nx));
+    AG_FOR_DTYPE(p->dtype, AG_FOR_TAPS(p->W, AG_FOR_VEC(l.vec, wide_bwd(sizeof(T)), hipLaunchKernelGGL((conv_bwd_kernel<T, W, VEC>), grid,
+                                                                                     dim3(kThreads), 0, (hipStream_t)stream, a, g))));
+    launch_sum_rows(g.partials, g.groups, (long long)a.D * (p->W + 1), ConvParams{q->dweight_dev, q->dbias_dev, p->W}, stream);
     return seq_status();
 }
 

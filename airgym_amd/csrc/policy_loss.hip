@@ -170,46 +170,6 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
 }
 
 // ---- long rows: a workgroup per row -----------------------------------------------------------------------------------------
-// 16 bytes of logits, kept as they came.  Rows of an odd width start anywhere: the access is aligned to the element only.
-template <typename T> struct Vec {
-    static constexpr int E = 16 / sizeof(T);
-    uint32_t w[4];
-    __device__ __forceinline__ float at(int i) const {
-        if (sizeof(T) == 4) return __uint_as_float(w[i]);
-        const uint32_t v = w[i / 2];
-        if (__is_same(T, bf16_t)) return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
-        return (float)__builtin_bit_cast(f16_t, (uint16_t)(i & 1 ? v >> 16 : v));
-    }
-    __device__ __forceinline__ void set(const float* x) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (sizeof(T) == 4) w[k] = __float_as_uint(x[k]);
-            else {
-                typedef T pair __attribute__((ext_vector_type(2)));
-                typedef float two __attribute__((ext_vector_type(2)));
-                const two f = {x[(2 * k) % E], x[(2 * k + 1) % E]};
-                w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, pair));
-            }
-        }
-    }
-};
-template <> __device__ __forceinline__ void Vec<float>::set(const float* x) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) w[k] = __float_as_uint(x[k]);
-}
-typedef uint32_t words_any2 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t words_any4 __attribute__((ext_vector_type(4), aligned(4)));
-template <int N> struct Words { using type = words_any2; };
-template <> struct Words<4> { using type = words_any4; };
-template <typename T> __device__ __forceinline__ Vec<T> load_vec(const T* p) {
-    const auto v = *(const typename Words<sizeof(T)>::type*)p;
-    return Vec<T>{{v[0], v[1], v[2], v[3]}};
-}
-template <typename T> __device__ __forceinline__ void store_vec(T* p, const Vec<T>& c) {
-    using W = typename Words<sizeof(T)>::type;
-    *(W*)p = W{c.w[0], c.w[1], c.w[2], c.w[3]};
-}
-
 // NV > 0: the row is held in NV accesses per thread.  NV = 0: it is longer than that, and read again for the gradient.
 template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
@@ -223,7 +183,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     const int full = a.V / E, nq = NV ? NV : (full + THREADS - 1) / THREADS;      // whole accesses of the row, per thread
     const int tail = full * E + threadIdx.x;                                        // the elements behind them: one per thread
     if (a.mask && !a.mask[row]) {
-        const Vec<T> zero{{0, 0, 0, 0}};
+        const Vec<T, E> zero{{0, 0, 0, 0}};
         if (dx) {
             for (int q = threadIdx.x; q < full; q += THREADS) store_vec(dx + q * E, zero);
             if (tail < a.V) dx[tail] = from_f32<T>(0.0f);
@@ -234,7 +194,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     const long long av = a.actions[row];
     const int act = av >= 0 && av < a.V ? (int)av : -1;
     const float xa = act >= 0 ? to_f32(x[act]) : __builtin_nanf("");
-    Vec<T> c[kKeep];
+    Vec<T, E> c[kKeep];
     Sums v{-__builtin_inff(), 0.0f, 0.0f};
     bool inf = false;
     // The row stays as it came: without this the compiler keeps the 16-bit types' float forms from one pass over it to the next, two
@@ -289,13 +249,13 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
 #pragma unroll
         for (int k = 0; k < kKeep; k++) {
             const int q = threadIdx.x + k * THREADS;
-            if (q < full) c[k] = load_vec(x + q * E);
+            if (q < full) c[k] = load_vec<T, E>(x + q * E);
         }
         sum_up(0, xt);
     } else {
         for (int k = 0; k < nq; k++) {
             const int q = threadIdx.x + k * THREADS;
-            if (q < full) c[0] = load_vec(x + q * E);
+            if (q < full) c[0] = load_vec<T, E>(x + q * E);
             sum_up(k, k ? -__builtin_inff() : xt);
         }
     }
@@ -317,7 +277,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     if (threadIdx.x == 0) row_terms(a, r, row, a.partials + row * kSums);
     if (!dx) return;
     const int aq = act >= 0 ? act / E : -1, ai = act % E;
-    auto gradient = [&](int q, const Vec<T>& held) __attribute__((always_inline)) {
+    auto gradient = [&](int q, const Vec<T, E>& held) __attribute__((always_inline)) {
         if (q >= full) return;
         float g[E];
 #pragma unroll
@@ -325,7 +285,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
         if (q == aq)
 #pragma unroll
             for (int i = 0; i < E; i++) g[i] += i == ai ? r.f : 0.0f;
-        Vec<T> out;
+        Vec<T, E> out;
         out.set(g);
         store_vec(dx + q * E, out);
     };
@@ -334,7 +294,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
 #pragma unroll
         for (int k = 0; k < kKeep; k++) gradient(threadIdx.x + k * THREADS, c[k]);
     } else {
-        for (int q = threadIdx.x; q < full; q += THREADS) gradient(q, load_vec(x + q * E));
+        for (int q = threadIdx.x; q < full; q += THREADS) gradient(q, load_vec<T, E>(x + q * E));
     }
     if (tail < a.V) dx[tail] = from_f32<T>(grad_of(r, xt - r.base) + (tail == act ? r.f : 0.0f));
 }

@@ -19,8 +19,83 @@ typedef __bf16 bf16_t;
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
 template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T)v; }
 
-// N consecutive elements moved with one load / store when the address allows it (the caller has checked that it is aligned)
-template <typename T, int N> struct alignas(sizeof(T) * N) Pack { T v[N]; };
+// N consecutive elements (at most 16 bytes), kept as they are stored and moved with one access.  The access is aligned to the element
+// only - rows of an odd width start anywhere -, which the memory takes at the same speed.
+template <int kWords> struct Words;
+#define AG_WORDS(n)                                                                  \
+    template <> struct Words<n> {                                                    \
+        typedef uint32_t any2 __attribute__((ext_vector_type(n), aligned(2)));       \
+        typedef uint32_t any4 __attribute__((ext_vector_type(n), aligned(4)));       \
+    };
+AG_WORDS(2) AG_WORDS(4)
+#undef AG_WORDS
+template <> struct Words<1> {
+    typedef uint32_t any2 __attribute__((aligned(2)));
+    typedef uint32_t any4;
+};
+
+template <typename T, int N> struct Vec {
+    static constexpr int kWords = N * (int)sizeof(T) / 4;
+    uint32_t w[kWords ? kWords : 1];
+    __device__ __forceinline__ float at(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(w[i]);
+        const uint32_t v = w[i / 2];
+        if (__is_same(T, bf16_t)) return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
+        return (float)__builtin_bit_cast(f16_t, (uint16_t)(i & 1 ? v >> 16 : v));
+    }
+    __device__ __forceinline__ void set(const float* x) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < N; k++) w[k] = __float_as_uint(x[k]);
+        } else if constexpr (N == 1) {
+            w[0] = __builtin_bit_cast(uint16_t, from_f32<T>(x[0]));
+        } else {
+            typedef T pair __attribute__((ext_vector_type(2)));
+            typedef float two __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int k = 0; k < kWords; k++) {
+                const two f = {x[2 * k], x[2 * k + 1]};
+                w[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, pair));
+            }
+        }
+    }
+};
+template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
+    constexpr int K = Vec<T, N>::kWords;
+    Vec<T, N> c;
+    if constexpr (K == 0) c.w[0] = *(const uint16_t*)p;
+    else if constexpr (K == 1) {
+        if constexpr (sizeof(T) == 2) c.w[0] = *(const Words<1>::any2*)p;
+        else c.w[0] = *(const uint32_t*)p;
+    } else if constexpr (sizeof(T) == 2) {
+        const auto v = *(const typename Words<K>::any2*)p;
+#pragma unroll
+        for (int k = 0; k < K; k++) c.w[k] = v[k];
+    } else {
+        const auto v = *(const typename Words<K>::any4*)p;
+#pragma unroll
+        for (int k = 0; k < K; k++) c.w[k] = v[k];
+    }
+    return c;
+}
+template <typename T, int N> __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& c) {
+    constexpr int K = Vec<T, N>::kWords;
+    if constexpr (K == 0) *(uint16_t*)p = (uint16_t)c.w[0];
+    else if constexpr (K == 1) {
+        if constexpr (sizeof(T) == 2) *(Words<1>::any2*)p = c.w[0];
+        else *(uint32_t*)p = c.w[0];
+    } else if constexpr (sizeof(T) == 2) {
+        typename Words<K>::any2 v;
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] = c.w[k];
+        *(typename Words<K>::any2*)p = v;
+    } else {
+        typename Words<K>::any4 v;
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] = c.w[k];
+        *(typename Words<K>::any4*)p = v;
+    }
+}
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }       // v_log_f32: 1 ulp

@@ -57,7 +57,7 @@ class _CausalConv(torch.autograd.Function):
         dx, dw = torch.empty(B, T, D, dtype=x.dtype, device=x.device), torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
         ds = None if state is None else torch.empty_like(state)
-        n = lib.ag_causal_conv_workspace_bytes(B, T, D, W)
+        n = lib.ag_causal_conv_workspace_bytes(B, T, D, W, N.AG_DTYPES[x.dtype])
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
         a = _fill(x, weight, bias, state, lengths, resets, ctx.silu)
         g = N.AgConvGrads(ctypes.sizeof(N.AgConvGrads), dy.data_ptr(), ptr(dlast), dy.stride(0), dy.stride(1), dx.data_ptr(), dw.data_ptr(),

@@ -836,7 +836,7 @@ typedef struct ag_conv_grads {
     long long workspace_bytes;
 } ag_conv_grads;
 int ag_causal_conv_fwd(const ag_conv_args* args, void* stream);
-long long ag_causal_conv_workspace_bytes(int B, int T, int D, int W);
+long long ag_causal_conv_workspace_bytes(int B, int T, int D, int W, int dtype);
 int ag_causal_conv_bwd(const ag_conv_args* args, const ag_conv_grads* grads, void* stream);
 /* one step for B sequences: x, y [B, D] (x rows x_sb apart), state_dev [B, W-1, D] moved on in place, resets_dev u8 [B] or NULL */
 int ag_causal_conv_step(const void* x_dev, long long x_sb, void* state_dev, const float* weight_dev, const float* bias_dev,

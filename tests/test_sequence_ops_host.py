@@ -40,7 +40,7 @@ def test_conv_entries_refuse(lib):
     g = N.AgConvGrads(ctypes.sizeof(N.AgConvGrads), p, None, 40, 8, p, p, None, None, p, 0)
     assert lib.ag_causal_conv_bwd(ctypes.byref(a), ctypes.byref(g), None) == -1          # workspace too small
     assert lib.ag_causal_conv_bwd(ctypes.byref(a), None, None) == -1 and lib.ag_causal_conv_fwd(None, None) == -1
-    assert lib.ag_causal_conv_workspace_bytes(2, 5, 8, 4) > 0 and lib.ag_causal_conv_workspace_bytes(2, 5, 8, 9) == 0
+    assert lib.ag_causal_conv_workspace_bytes(2, 5, 8, 4, 0) > 0 and lib.ag_causal_conv_workspace_bytes(2, 5, 8, 9, 0) == 0
     assert lib.ag_causal_conv_step(p, 8, None, p, None, None, p, 0, 2, 8, 4, 1, None) == -1
     assert lib.ag_causal_conv_step(p, 8, p, p, None, None, p, 0, 2, 8, 9, 1, None) == -6
 
