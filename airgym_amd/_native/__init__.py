@@ -169,7 +169,7 @@ class AgTokenLossArgs(ctypes.Structure):
         [(n, ctypes.c_longlong) for n in ("R0", "R1", "s0", "s1")] + \
         [(n, ctypes.c_void_p) for n in ("logits_dev", "actions_dev", "old_logp_dev", "advantages_dev", "ref_logp_dev", "mask_dev")] + \
         [(n, ctypes.c_float) for n in ("e_clip", "kl_coef", "entropy_coef")] + \
-        [(n, ctypes.c_void_p) for n in ("stats_dev", "dlogits_dev", "workspace_dev")] + [("workspace_bytes", ctypes.c_longlong)]
+        [(n, ctypes.c_void_p) for n in ("loss_dev", "stats_dev", "dlogits_dev", "workspace_dev")] + [("workspace_bytes", ctypes.c_longlong)]
 
 
 class AgInputLayerArgs(ctypes.Structure):

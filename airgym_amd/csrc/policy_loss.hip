@@ -362,16 +362,16 @@ __global__ __launch_bounds__(256) void stats_part_kernel(const float* rows, long
 }
 
 template <typename S>
-__global__ __launch_bounds__(256) void stats_kernel(const S* rows, long long n, const float* count, float kl_coef, float ent_coef, float* stats) {
+__global__ __launch_bounds__(256) void stats_kernel(const S* rows, long long n, const float* count, float kl_coef, float ent_coef, float* loss,
+                                                    float* stats) {
     __shared__ double part[4][kSums];
     double s[kSums];
     sum_rows(rows, n, s, part);
     if (threadIdx.x == 0) {
 #pragma unroll
-        for (int k = 0; k < kSums; k++) s[k] /= (double)count[0], stats[1 + k] = (float)s[k];
-        stats[0] = (float)(s[0] + (double)kl_coef * s[1] - (double)ent_coef * s[2]);
-        stats[6] = count[1];
-        stats[7] = 0.0f;
+        for (int k = 0; k < kSums; k++) s[k] /= (double)count[0], stats[k] = (float)s[k];
+        loss[0] = (float)(s[0] + (double)kl_coef * s[1] - (double)ent_coef * s[2]);
+        stats[kSums] = count[1];
     }
 }
 
@@ -441,7 +441,7 @@ extern "C" long long ag_token_policy_loss_workspace_bytes(long long R, int V) {
 
 extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     if (!p || p->struct_size != sizeof(ag_token_loss_args) || !p->logits_dev || !p->actions_dev || !p->old_logp_dev || !p->advantages_dev ||
-        !p->stats_dev || !p->workspace_dev || p->R0 <= 0 || p->R1 <= 0 || p->V <= 0)
+        !p->loss_dev || !p->stats_dev || !p->workspace_dev || p->R0 <= 0 || p->R1 <= 0 || p->V <= 0)
         return AG_ERR_INVALID_ARG;
     if (p->dtype < AG_F32 || p->dtype > AG_F16 || p->R0 > 0x7fffffffLL / p->R1) return AG_ERR_UNSUPPORTED;
     const long long R = p->R0 * p->R1;
@@ -457,9 +457,11 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     const float kl = p->ref_logp_dev ? p->kl_coef : 0.0f;
     if (blocks) {
         hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a.partials, rows, sums);
-        hipLaunchKernelGGL((stats_kernel<double>), dim3(1), dim3(256), 0, (hipStream_t)stream, sums, blocks, count, kl, p->entropy_coef, p->stats_dev);
+        hipLaunchKernelGGL((stats_kernel<double>), dim3(1), dim3(256), 0, (hipStream_t)stream, sums, blocks, count, kl, p->entropy_coef, p->loss_dev,
+                           p->stats_dev);
     } else
-        hipLaunchKernelGGL((stats_kernel<float>), dim3(1), dim3(256), 0, (hipStream_t)stream, a.partials, rows, count, kl, p->entropy_coef, p->stats_dev);
+        hipLaunchKernelGGL((stats_kernel<float>), dim3(1), dim3(256), 0, (hipStream_t)stream, a.partials, rows, count, kl, p->entropy_coef, p->loss_dev,
+                           p->stats_dev);
     return seq_status();
 }
 

@@ -1,17 +1,16 @@
-"""What the wrappers of the sequence operators share: argument checks, element strides, the stream and the device of a call."""
+"""What the wrappers of the sequence operators share: argument checks, the stream and the device of a call.
+
+A step of a rollout is a few microseconds of GPU work, so the checks are plain comparisons and messages are put together only when one
+fails."""
 import contextlib
-import ctypes
 
 import torch
 
 from airgym_amd import _native as N
 
+DTYPES = N.AG_DTYPES
 _SAME = contextlib.nullcontext()
-
-
-def require(ok, what):
-    if not ok:
-        raise ValueError(what)
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else None
 
 
 def on_device_of(t):
@@ -20,59 +19,74 @@ def on_device_of(t):
 
 
 def stream_of(t):
-    return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    """The current stream of t's device as the library takes it."""
+    if _raw_stream is not None:
+        return _raw_stream(t.device.index)
+    return torch.cuda.current_stream(t.device).cuda_stream
 
 
 def ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def activations(name, t, shape, like=None):
-    """t checked against `shape` and, with `like`, against another activation's type and device; its last dimension made dense if it
+def shape_error(name, t, shape):
+    got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    return ValueError(f"{name}: expected {shape}, got {got}")
+
+
+def activation(name, t, shape):
+    """t as the first activation of a call: its type and device are what the others are held to.  Its last dimension is made dense if it
     is not (an expanded channel, a transposed view)."""
-    require(isinstance(t, torch.Tensor) and t.is_cuda, f"{name}: expected a tensor on the GPU")
-    require(t.dtype in N.AG_DTYPES, f"{name}: float32, bfloat16 or float16 expected, got {t.dtype}")
-    require(tuple(t.shape) == tuple(shape), f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    if like is not None:
-        require(t.dtype == like.dtype, f"{name}: expected {like.dtype} like the other activations, got {t.dtype}")
-        require(t.device == like.device, f"{name}: on {t.device}, the other tensors on {like.device}")
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise shape_error(name, t, "a tensor on the GPU")
+    if t.dtype not in DTYPES:
+        raise shape_error(name, t, "float32, bfloat16 or float16")
+    if t.shape != shape:
+        raise shape_error(name, t, list(shape))
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def same_kind(name, t, shape, like):
+    """... and the others."""
+    if not isinstance(t, torch.Tensor) or t.dtype != like.dtype or t.device != like.device or t.shape != shape:
+        raise shape_error(name, t, f"{like.dtype} {list(shape)} on {like.device}, like the other activations")
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def parameter(name, t, shape, device):
-    """A float32 parameter as a dense tensor, or None."""
+    """A float32 parameter or state as a dense tensor, or None."""
     if t is None:
         return None
-    require(isinstance(t, torch.Tensor) and t.device == device, f"{name}: expected a tensor on {device}")
-    require(t.dtype == torch.float32, f"{name}: parameters and states of the scan are float32, got {t.dtype}")
-    require(tuple(t.shape) == tuple(shape), f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-    return t.contiguous()
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.device != device or t.shape != shape:
+        raise shape_error(name, t, f"float32 {list(shape)} on {device}")
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def lengths_of(lengths, batch, device):
     if lengths is None:
         return None
-    require(isinstance(lengths, torch.Tensor) and lengths.dtype == torch.int32 and tuple(lengths.shape) == (batch,)
-            and lengths.device == device, f"lengths: expected int32 [{batch}] on {device}")
+    if not isinstance(lengths, torch.Tensor) or lengths.dtype != torch.int32 or lengths.shape != (batch,) or lengths.device != device:
+        raise shape_error("lengths", lengths, f"int32 [{batch}] on {device}")
     return lengths.contiguous()
 
 
 def flags_of(name, flags, shape, device):
-    """bool or uint8 flags, read through their strides."""
+    """bool or uint8 flags, read through their strides, or None."""
     if flags is None:
         return None
-    require(isinstance(flags, torch.Tensor) and flags.dtype in (torch.bool, torch.uint8) and tuple(flags.shape) == tuple(shape)
-            and flags.device == device, f"{name}: expected bool or uint8 {list(shape)} on {device}")
+    if not isinstance(flags, torch.Tensor) or flags.dtype not in (torch.bool, torch.uint8) or flags.shape != shape or flags.device != device:
+        raise shape_error(name, flags, f"bool or uint8 {list(shape)} on {device}")
     return flags
 
 
 def in_place_state(name, t, shape, dtype, device):
-    require(isinstance(t, torch.Tensor) and t.device == device and t.dtype == dtype and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
-            f"{name}: expected a contiguous {dtype} tensor of shape {list(shape)} on {device} (it is moved on in place)")
-    require(not t.requires_grad, f"{name}: moved on in place, cannot require a gradient")
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.shape != shape or not t.is_contiguous():
+        raise shape_error(name, t, f"contiguous {dtype} {list(shape)} on {device} (it is moved on in place)")
+    if t.requires_grad:
+        raise ValueError(f"{name}: moved on in place, cannot require a gradient")
     return t
 
 
 def no_gradient(what, *tensors):
-    require(not (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)),
-            f"{what} has no backward pass: call it under torch.no_grad(), or the sequence form to train")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no backward pass: call it under torch.no_grad(), or the sequence form to train")

@@ -13,73 +13,75 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from airgym_amd import _native as N
-from airgym_amd.lib.core.native_call import activations, flags_of, on_device_of, ptr, require, stream_of
+from airgym_amd.lib.core.native_call import activation, flags_of, on_device_of, ptr, shape_error, stream_of
 
 STATS = ("policy_loss", "kl", "entropy", "old_kl", "clip_frac", "rows")
+_ARGS = ctypes.sizeof(N.AgTokenLossArgs)
 
 
 def _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, want_grad):
     lib = N.load()
     r0, r1, v = logits.shape
-    stats = torch.empty(8, dtype=torch.float32, device=logits.device)
-    grad = torch.empty(r0, r1, v, dtype=logits.dtype, device=logits.device) if want_grad else None
+    dev = logits.device
+    loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(6, dtype=torch.float32, device=dev)
+    grad = torch.empty((r0, r1, v), dtype=logits.dtype, device=dev) if want_grad else None
     n = lib.ag_token_policy_loss_workspace_bytes(r0 * r1, v)
-    ws = torch.empty(n, dtype=torch.uint8, device=logits.device)
-    a = N.AgTokenLossArgs(ctypes.sizeof(N.AgTokenLossArgs), N.AG_DTYPES[logits.dtype], v, r0, r1, logits.stride(0), logits.stride(1),
-                          logits.data_ptr(), actions.data_ptr(), old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(mask),
-                          *coefs, stats.data_ptr(), ptr(grad), ws.data_ptr(), n)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    a = N.AgTokenLossArgs(_ARGS, N.AG_DTYPES[logits.dtype], v, r0, r1, logits.stride(0), logits.stride(1), logits.data_ptr(),
+                          actions.data_ptr(), old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(mask), *coefs, loss.data_ptr(),
+                          stats.data_ptr(), ptr(grad), ws.data_ptr(), n)
     with on_device_of(logits):
         N.check(lib.ag_token_policy_loss(ctypes.byref(a), stream_of(logits)), "ag_token_policy_loss")
-    return stats, grad
+    return loss, stats, grad
 
 
 class _TokenPolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, coefs):
-        stats, grad = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, ctx.needs_input_grad[0])
+        loss, stats, grad = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, ctx.needs_input_grad[0])
         ctx.save_for_backward(logits, actions, old_logp, advantages, ref_logp, mask)
         ctx.coefs, ctx.grad = coefs, grad
-        loss, rest = stats[0], stats[1:7]
-        ctx.mark_non_differentiable(rest)
-        return loss, rest
+        ctx.mark_non_differentiable(stats)
+        ctx.set_materialize_grads(False)
+        return loss, stats
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dloss, _):
+        if dloss is None:
+            return None, None, None, None, None, None, None
         saved = ctx.saved_tensors
         # the gradient is handed over, not kept: autograd may go on to add to it in place.  A second pass over a retained graph forms
         # it again.
         grad, ctx.grad = ctx.grad, None
         if grad is None:
-            _, grad = _launch(*saved, ctx.coefs, True)
-        scale = dloss.to(torch.float32).contiguous()
+            grad = _launch(*saved, ctx.coefs, True)[2]
         with on_device_of(grad):
-            N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], scale.data_ptr(), stream_of(grad)),
+            N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], dloss.data_ptr(), stream_of(grad)),
                     "ag_scale_by")
         return grad, None, None, None, None, None, None
 
 
 def _rows(logits, actions):
     """logits as [R0, R1, V] (a view where their strides allow), the leading shape and the actions as dense int64."""
-    require(isinstance(logits, torch.Tensor) and logits.dim() >= 2, "logits: expected [..., V]")
-    lead, v = tuple(logits.shape[:-1]), logits.shape[-1]
-    require(v >= 1, "logits: no choices")
-    logits = activations("logits", logits, logits.shape)
-    require(isinstance(actions, torch.Tensor) and actions.dtype == torch.int64 and tuple(actions.shape) == lead
-            and actions.device == logits.device, f"actions: expected int64 {list(lead)} on {logits.device}")
+    if not isinstance(logits, torch.Tensor) or logits.dim() < 2 or logits.shape[-1] < 1:
+        raise shape_error("logits", logits, "[..., V]")
+    lead = logits.shape[:-1]
+    logits = activation("logits", logits, logits.shape)
+    if not isinstance(actions, torch.Tensor) or actions.dtype != torch.int64 or actions.shape != lead or actions.device != logits.device:
+        raise shape_error("actions", actions, f"int64 {list(lead)} on {logits.device}")
     if len(lead) == 1:
         logits = logits.unsqueeze(0)
     elif len(lead) > 2:
-        logits = logits.reshape(-1, lead[-1], v)
+        logits = logits.reshape(-1, lead[-1], logits.shape[-1])
     return logits, lead, actions.contiguous()
 
 
 def _per_row(name, t, lead, device):
-    if t is None:
-        return None
-    require(isinstance(t, torch.Tensor) and t.dtype == torch.float32 and tuple(t.shape) == lead and t.device == device,
-            f"{name}: expected float32 {list(lead)} on {device}")
-    require(not (torch.is_grad_enabled() and t.requires_grad), f"{name}: the loss has gradients for the logits only; detach it")
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != lead or t.device != device:
+        raise shape_error(name, t, f"float32 {list(lead)} on {device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name}: the loss has gradients for the logits only; detach it")
     return t.contiguous()
 
 
@@ -93,13 +95,15 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logp=None, mask=No
     [0, V) in a row that counts gives NaN."""
     logits, lead, actions = _rows(logits, actions)
     dev = logits.device
-    old_logp, advantages, ref_logp = (_per_row(n, t, lead, dev) for n, t in (("old_logp", old_logp), ("advantages", advantages),
-                                                                              ("ref_logp", ref_logp)))
-    require(old_logp is not None and advantages is not None, "old_logp and advantages are needed")
-    mask = flags_of("mask", mask, lead, dev)
-    mask = None if mask is None else mask.contiguous()
-    require(e_clip >= 0.0, f"e_clip: {e_clip} is negative")
-    require(ref_logp is not None or kl_coef == 0.0, "kl_coef: the KL term needs ref_logp")
+    old_logp, advantages = _per_row("old_logp", old_logp, lead, dev), _per_row("advantages", advantages, lead, dev)
+    if ref_logp is not None:
+        ref_logp = _per_row("ref_logp", ref_logp, lead, dev)
+    elif kl_coef != 0.0:
+        raise ValueError("kl_coef: the KL term needs ref_logp")
+    if mask is not None:
+        mask = flags_of("mask", mask, lead, dev).contiguous()
+    if not e_clip >= 0.0:
+        raise ValueError(f"e_clip: {e_clip}")
     if logits.numel() == 0:
         return logits.sum().float(), torch.zeros(6, device=dev)
     return _TokenPolicyLoss.apply(logits, actions, old_logp, advantages, ref_logp, mask, (float(e_clip), float(kl_coef), float(entropy_coef)))
@@ -108,8 +112,8 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logp=None, mask=No
 def action_logp(logits, actions):
     """log softmax(logits)[action] and the entropy of every row, float32 [...]: what a rollout stores as old_logp and what a reference
     policy's logits give as ref_logp.  No gradients.  An action outside [0, V) gives NaN."""
-    require(not (torch.is_grad_enabled() and isinstance(logits, torch.Tensor) and logits.requires_grad),
-            "action_logp has no backward pass: detach the logits (policy_loss trains)")
+    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError("action_logp has no backward pass: detach the logits (policy_loss trains)")
     logits, lead, actions = _rows(logits, actions)
     logp = torch.empty(lead, dtype=torch.float32, device=logits.device)
     entropy = torch.empty_like(logp)

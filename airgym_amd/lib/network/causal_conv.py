@@ -10,14 +10,15 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from airgym_amd import _native as N
-from airgym_amd.lib.core.native_call import (activations, flags_of, in_place_state, lengths_of, no_gradient, on_device_of, parameter, ptr,
-                                             require, stream_of)
+from airgym_amd.lib.core.native_call import (activation as first_activation, flags_of, in_place_state, lengths_of, no_gradient, on_device_of,
+                                             parameter, ptr, same_kind, shape_error, stream_of)
 
 MAX_TAPS = 8
 
 
 def _activation(activation):
-    require(activation in (None, "silu"), f"activation: None or 'silu' expected, got {activation!r}")
+    if activation not in (None, "silu"):
+        raise ValueError(f"activation: None or 'silu' expected, got {activation!r}")
     return int(activation == "silu")
 
 
@@ -52,7 +53,7 @@ class _CausalConv(torch.autograd.Function):
         lib = N.load()
         B, T, D = x.shape
         W = weight.shape[1]
-        dy = torch.zeros(B, T, D, dtype=x.dtype, device=x.device) if dy is None else activations("dy", dy, x.shape, x)
+        dy = torch.zeros(B, T, D, dtype=x.dtype, device=x.device) if dy is None else same_kind("dy", dy, x.shape, x)
         dlast = None if dlast is None else dlast.contiguous()
         dx, dw = torch.empty(B, T, D, dtype=x.dtype, device=x.device), torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
@@ -68,8 +69,8 @@ class _CausalConv(torch.autograd.Function):
 
 
 def _weight(weight, D, device):
-    require(isinstance(weight, torch.Tensor) and weight.dim() == 2, "weight: expected [D, W]")
-    require(2 <= weight.shape[1] <= MAX_TAPS, f"weight: 2 to {MAX_TAPS} taps, got {weight.shape[1]}")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or not 2 <= weight.shape[1] <= MAX_TAPS:
+        raise shape_error("weight", weight, f"[{D}, W] with 2 to {MAX_TAPS} taps")
     return parameter("weight", weight, (D, weight.shape[1]), device)
 
 
@@ -77,12 +78,13 @@ def causal_conv(x, weight, bias=None, *, activation="silu", initial_state=None, 
     """x [B, T, D] (float32, bfloat16 or float16; any batch and time strides), weight [D, W] and bias [D] float32 -> y [B, T, D], and
     with return_state the last W - 1 inputs [B, W - 1, D] (oldest first, x's type) to go on from.  initial_state: the same;
     lengths int32 [B]; resets bool or uint8 [B, T].  Gradients reach x, weight, bias, initial_state, also through the returned state."""
-    require(isinstance(x, torch.Tensor) and x.dim() == 3, "x: expected [B, T, D]")
+    if not isinstance(x, torch.Tensor) or x.dim() != 3:
+        raise shape_error("x", x, "[B, T, D]")
     B, T, D = x.shape
-    x = activations("x", x, x.shape)
+    x = first_activation("x", x, x.shape)
     weight, bias = _weight(weight, D, x.device), parameter("bias", bias, (D,), x.device)
     W = weight.shape[1]
-    state = None if initial_state is None else activations("initial_state", initial_state, (B, W - 1, D), x).contiguous()
+    state = None if initial_state is None else same_kind("initial_state", initial_state, (B, W - 1, D), x).contiguous()
     lengths, resets = lengths_of(lengths, B, x.device), flags_of("resets", resets, (B, T), x.device)
     silu = _activation(activation)
     if x.numel() == 0:
@@ -95,21 +97,23 @@ def causal_conv(x, weight, bias=None, *, activation="silu", initial_state=None, 
 def causal_conv_step(x, state, weight, bias=None, *, activation="silu", resets=None):
     """One step: x [B, D] -> y [B, D]; state [B, W - 1, D] (contiguous, x's type) is moved on in place.  resets [B] clears a row's
     state first.  No gradients."""
-    require(isinstance(x, torch.Tensor) and x.dim() == 2, "x: expected [B, D]")
+    if not isinstance(x, torch.Tensor) or x.dim() != 2:
+        raise shape_error("x", x, "[B, D]")
     B, D = x.shape
     no_gradient("causal_conv_step", x, weight, bias)
-    x = activations("x", x, x.shape)
-    weight, bias = _weight(weight, D, x.device), parameter("bias", bias, (D,), x.device)
-    state = in_place_state("state", state, (B, weight.shape[1] - 1, D), x.dtype, x.device)
-    resets = flags_of("resets", resets, (B,), x.device)
+    x = first_activation("x", x, x.shape)
+    device = x.device
+    weight, bias = _weight(weight, D, device), parameter("bias", bias, (D,), device)
+    W = weight.shape[1]
+    state = in_place_state("state", state, (B, W - 1, D), x.dtype, device)
+    resets = flags_of("resets", resets, (B,), device)
     silu = _activation(activation)
-    y = torch.empty(B, D, dtype=x.dtype, device=x.device)
+    y = torch.empty((B, D), dtype=x.dtype, device=device)
     if x.numel() == 0:
         return y
-    if resets is not None:
+    if resets is not None and not resets.is_contiguous():
         resets = resets.contiguous()
     with on_device_of(x):
         N.check(N.load().ag_causal_conv_step(x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), ptr(bias), ptr(resets),
-                                             y.data_ptr(), N.AG_DTYPES[x.dtype], B, D, weight.shape[1], silu, stream_of(x)),
-                "ag_causal_conv_step")
+                                             y.data_ptr(), N.AG_DTYPES[x.dtype], B, D, W, silu, stream_of(x)), "ag_causal_conv_step")
     return y

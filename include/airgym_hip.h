@@ -896,8 +896,8 @@ int ag_selective_scan_step(const ag_scan_args* args, void* stream);
  * averaged over the rows with mask != 0 (mask NULL: all; none: loss 0, gradients 0).  Rows that do not count are neither read nor
  * checked; their gradient is zero.  An action outside [0, V) in a row that counts makes that row's results NaN.
  * Logits of -inf are choices that are not available: probability 0, gradient 0.
- *   stats_dev [8] = {loss, policy loss, KL term, entropy, KL of the old policy to this one (r - 1 - log r), fraction of rows whose r
- *       left the clip range, rows counted, 0}
+ *   loss_dev [1]; stats_dev [6] = {policy loss, KL term, entropy, KL of the old policy to this one (r - 1 - log r), fraction of rows
+ *       whose r left the clip range, rows counted}
  *   dlogits_dev [R, V] contiguous in the logits' type, or NULL
  *   workspace_dev: ag_token_policy_loss_workspace_bytes(R, V) bytes, 16-byte aligned. */
 typedef struct ag_token_loss_args {
@@ -911,7 +911,8 @@ typedef struct ag_token_loss_args {
     const float* ref_logp_dev;         /* [R] or NULL (no KL term) */
     const unsigned char* mask_dev;     /* u8 [R] or NULL */
     float e_clip, kl_coef, entropy_coef;
-    float* stats_dev;                  /* [8] */
+    float* loss_dev;                   /* [1] */
+    float* stats_dev;                  /* [6] */
     void* dlogits_dev;
     void* workspace_dev;
     long long workspace_bytes;

@@ -24,7 +24,7 @@ def _blocks():
     conv = N.AgConvArgs(ctypes.sizeof(N.AgConvArgs), 0, 2, 5, 8, 4, 1, p, p, None, None, None, None, 40, 8, 0, 0, p, None)
     scan = N.AgScanArgs(ctypes.sizeof(N.AgScanArgs), 0, 2, 5, 8, 16, 1, 1, p, p, None, p, p, p)
     scan.out_dev = scan.state_out_dev = scan.ckpt_dev = p
-    loss = N.AgTokenLossArgs(ctypes.sizeof(N.AgTokenLossArgs), 0, 9, 1, 3, 27, 9, p, p, p, p, None, None, 0.2, 0.0, 0.0, p, p, p, 1 << 20)
+    loss = N.AgTokenLossArgs(ctypes.sizeof(N.AgTokenLossArgs), 0, 9, 1, 3, 27, 9, p, p, p, p, None, None, 0.2, 0.0, 0.0, p, p, p, p, 1 << 20)
     return N, p, conv, scan, loss
 
 
@@ -66,7 +66,7 @@ def test_scan_entries_refuse(lib):
 def test_loss_entries_refuse(lib):
     N, p, _, _, a = _blocks()
     for field, value, rc in [("struct_size", 4, -1), ("logits_dev", None, -1), ("actions_dev", None, -1), ("old_logp_dev", None, -1),
-                             ("stats_dev", None, -1), ("workspace_dev", None, -1), ("workspace_bytes", 4, -1), ("V", 0, -1), ("R0", 0, -1),
+                             ("stats_dev", None, -1), ("loss_dev", None, -1), ("workspace_dev", None, -1), ("workspace_bytes", 4, -1), ("V", 0, -1), ("R0", 0, -1),
                              ("dtype", 5, -6), ("R0", 1 << 31, -6)]:
         old = getattr(a, field)
         setattr(a, field, value)
