@@ -350,6 +350,8 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
     const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
     const unsigned at = (unsigned)d * (unsigned)sizeof(T);
     const long long state = (long long)d * N;
+    const int GN = a.G * N;
+    const unsigned bc_at = brow * GN + p.g * N + bn;                    // in a tile of [T, G, N]
     float A2[4], dA[4], dD = 0.0f, dbias = 0.0f;
     load4(a.A + state, w, N, A2);
     zero4(dA);
@@ -546,16 +548,17 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
             const long long back = (long long)kBack * D * (long long)sizeof(T);
             du -= back, ddelta -= back, dz -= back;
             if (brow < nt && bn < N) {                                  // nt <= 8
-                const auto k = scan_args();
                 const auto g = grad_args();
                 const float vB = brow < nv ? sdBC[0][brow][bn] : 0.0f, vC = brow < nv ? sdBC[1][brow][bn] : 0.0f;
-                const long long i = (((long long)b * T_ + t0 + brow) * k->G + p.g) * N + bn, n = (long long)k->B * T_ * k->G * N;
+                const long long first = ((long long)b * T_ + t0) * GN;
                 if (g->bc_partials) {
-                    g->bc_partials[2 * p.cb * n + i] = vB;
-                    g->bc_partials[(2 * p.cb + 1) * n + i] = vC;
+                    const long long all = (long long)a.B * T_ * GN;
+                    float* part = g->bc_partials + (2 * p.cb * all + first);
+                    part[bc_at] = vB;
+                    (part + all)[bc_at] = vC;
                 } else {
-                    ((T*)g->dB)[i] = from_f32<T>(vB);
-                    ((T*)g->dC)[i] = from_f32<T>(vC);
+                    ((T*)g->dB + first)[bc_at] = from_f32<T>(vB);
+                    ((T*)g->dC + first)[bc_at] = from_f32<T>(vC);
                 }
             }
         }
@@ -621,43 +624,57 @@ template <typename T> struct ScanShared {
 };
 
 // One step: a channel's state is spread over L lanes, four numbers each, so that a wave moves 1 KB of states per access; the states
-// in and out are nearly all of the bytes.
-template <typename T, int L>
+// in and out are nearly all of the bytes.  A thread takes R sequences, all of their loads first.
+template <typename T, int L, int R>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     const unsigned item = (unsigned)(((unsigned long long)blockIdx.x * 256 + threadIdx.x) / L), D = a.D;      // B D < 2^31
     const int part = threadIdx.x % L;
-    const bool live = item < (unsigned)a.B * D;
-    const unsigned b = live ? item / D : 0, d = live ? item - b * D : 0, g = a.G > 1 ? d / (unsigned)a.Dg : 0;
-    const T* Bm = (const T*)a.Bm + (b * a.bb + g * a.bg);
-    const T* Cm = (const T*)a.Cm + (b * a.cb + g * a.cg);
-    const long long row = ((long long)b * D + d) * a.N;
-    float h[4], A[4];
-    zero4(h);
-    const bool cut = a.resets && a.resets[b * a.rb];
-    if (a.s0 && !cut) load4(a.s0 + row, part, a.N, h);
-    load4(a.A + (long long)d * a.N, part, a.N, A);
-    const float uu = to_f32(((const T*)a.u)[b * a.ub + d]);
-    const float raw = to_f32(((const T*)a.delta)[b * a.db + d]) + (a.bias ? a.bias[d] : 0.0f);
-    const float dt = a.softplus ? softplus(raw) : raw;
-    float y = 0.0f;
+    const unsigned first = item / D * R, d = item % D, g = a.G > 1 ? d / (unsigned)a.Dg : 0;
+    float h[R][4], A[4], uu[R], raw[R], zz[R], Bn[R][4], Cn[R][4], y[R];
+    unsigned char cut[R];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const int n = 4 * part + j;
-        if (n >= a.N) break;
-        h[j] = __builtin_fmaf(exp2_hw(dt * (A[j] * kLog2e)), h[j], dt * uu * to_f32(Bm[n]));
-        y = __builtin_fmaf(to_f32(Cm[n]), h[j], y);
+    for (int i = 0; i < R; i++) {
+        const unsigned b = min(first + i, (unsigned)a.B - 1);          // a thread without a sequence reads the last one's and writes nothing
+        const T* Bm = (const T*)a.Bm + (b * a.bb + g * a.bg);
+        const T* Cm = (const T*)a.Cm + (b * a.cb + g * a.cg);
+        zero4(h[i]);
+        if (a.s0) load4(a.s0 + ((long long)b * D + d) * a.N, part, a.N, h[i]);
+        cut[i] = a.resets ? a.resets[b * a.rb] : 0;
+        uu[i] = to_f32(((const T*)a.u)[b * a.ub + d]);
+        raw[i] = to_f32(((const T*)a.delta)[b * a.db + d]);
+        zz[i] = a.z ? to_f32(((const T*)a.z)[b * a.zb + d]) : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int n = 4 * part + j;
+            Bn[i][j] = n < a.N ? to_f32(Bm[n]) : 0.0f;
+            Cn[i][j] = n < a.N ? to_f32(Cm[n]) : 0.0f;
+        }
     }
-    if (live) store4(a.s1 + row, part, a.N, h);
-    if (L > 1) y += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y), 0xB1, 0xf, 0xf, true));
-    if (L > 2) y += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y), 0x4E, 0xf, 0xf, true));
-    if (L > 4) y += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y), 0x141, 0xf, 0xf, true));
-    if (!live || part) return;
-    y = __builtin_fmaf(a.Dskip ? a.Dskip[d] : 0.0f, uu, y);
-    if (a.z) {
-        const float zz = to_f32(((const T*)a.z)[b * a.zb + d]);
-        y *= zz * sigmoid(zz);
+    load4(a.A + (long long)d * a.N, part, a.N, A);
+    const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        if (cut[i]) zero4(h[i]);
+        const float dt = a.softplus ? softplus(raw[i] + bias) : raw[i] + bias;
+        y[i] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            h[i][j] = __builtin_fmaf(exp2_hw(dt * (A[j] * kLog2e)), h[i][j], dt * uu[i] * Bn[i][j]);
+            y[i] = __builtin_fmaf(Cn[i][j], h[i][j], y[i]);
+        }
+        if (L > 1) y[i] += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y[i]), 0xB1, 0xf, 0xf, true));
+        if (L > 2) y[i] += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y[i]), 0x4E, 0xf, 0xf, true));
+        if (L > 4) y[i] += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y[i]), 0x141, 0xf, 0xf, true));
     }
-    ((T*)a.out)[item] = from_f32<T>(y);
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+        if (first + i >= (unsigned)a.B) break;
+        const long long at = (long long)(first + i) * D + d;
+        store4(a.s1 + at * a.N, part, a.N, h[i]);
+        float o = __builtin_fmaf(skip, uu[i], y[i]);
+        if (a.z) o *= zz[i] * sigmoid(zz[i]);
+        if (part == 0) ((T*)a.out)[at] = from_f32<T>(o);
+    }
 }
 
 int groups_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
@@ -790,8 +807,14 @@ extern "C" int ag_selective_scan_step(const ag_scan_args* p, void* stream) {
     const ScanArgs a = device_args(p);
     const int lanes = groups_of(p->N);
     if ((long long)a.B * a.D > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
-    const long long blocks = ((long long)a.B * a.D * lanes + 255) / 256;
-    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, NG>), dim3((unsigned)blocks), dim3(256), 0,
-                                                                  (hipStream_t)stream, a)));
+    // two sequences per thread once that leaves 32 waves per CU
+    const bool two = (long long)a.B * a.D * lanes / 128 >= 8192;
+    const long long blocks = ((long long)(two ? (a.B + 1) / 2 : a.B) * a.D * lanes + 255) / 256;
+    if (two)
+        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, NG, 2>), dim3((unsigned)blocks), dim3(256), 0,
+                                                                      (hipStream_t)stream, a)));
+    else
+        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, NG, 1>), dim3((unsigned)blocks), dim3(256), 0,
+                                                                      (hipStream_t)stream, a)));
     return seq_status();
 }

@@ -261,7 +261,7 @@ def test_a_reset_clears_a_state_that_is_not_finite():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("B,D,N,G", [(1, 1, 1, 1), (3, 6, 3, 2), (5, 130, 16, 1), (2, 64, 8, 1), (3, 33, 32, 1), (2, 48, 13, 3)])
+@pytest.mark.parametrize("B,D,N,G", [(1, 1, 1, 1), (3, 6, 3, 2), (5, 130, 16, 1), (2, 64, 8, 1), (3, 33, 32, 1), (2, 48, 13, 3), (7, 37500, 16, 1)])
 def test_selective_scan_steps_against_float64(B, D, N, G, dtype):
     from airgym_amd.lib.network.selective_scan import selective_scan_step
     T = 5
@@ -423,6 +423,53 @@ def test_policy_loss_scaled_and_backward_twice():
     flat = logits.detach().reshape(21, 300).requires_grad_()
     l2, _ = policy_loss(flat, actions.reshape(21), old.reshape(21), adv.reshape(21), entropy_coef=0.1)
     assert torch.equal(l2, loss) and torch.equal(torch.autograd.grad(l2, flat)[0].view_as(first), first)
+
+
+# ------------------------------------------------------------------------------------------------ far rows, repeats
+def _far(t, gap):
+    """t [2, ...] with its two rows more than 2^32 bytes apart."""
+    n = t[0].numel()
+    big = torch.empty(gap + n, dtype=t.dtype, device="cuda")
+    out = big.as_strided(t.shape, (gap, *t[0].stride()))
+    out.copy_(t)
+    return out
+
+
+def test_rows_further_apart_than_32_bits():
+    from airgym_amd.lib.core.policy_loss import action_logp
+    from airgym_amd.lib.network.causal_conv import causal_conv
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    g, gap = gen(9), 2 ** 31 + 2 ** 10
+    x = torch.randn(2, 37, 48, generator=g).to(torch.bfloat16).cuda()
+    weight = torch.randn(48, 4, generator=g).cuda()
+    far = _far(x, gap).requires_grad_()
+    near = x.clone().requires_grad_()
+    dy = torch.randn(2, 37, 48, generator=g).to(torch.bfloat16).cuda()
+    a, b = causal_conv(far, weight), causal_conv(near, weight)
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, far, dy)[0], torch.autograd.grad(b, near, dy)[0])
+    A, bc = -torch.rand(48, 16, generator=g).cuda(), torch.randn(2, 37, 16, generator=g).to(torch.bfloat16).cuda()
+    a, b = selective_scan(far, far, A, bc, bc), selective_scan(near, near, A, bc, bc)
+    assert torch.equal(a, b)
+    assert torch.equal(torch.autograd.grad(a, far, dy)[0], torch.autograd.grad(b, near, dy)[0])
+    logits, actions = x[:, 0], torch.tensor([3, 40], device="cuda")
+    assert torch.equal(action_logp(_far(logits, gap), actions)[0], action_logp(logits, actions)[0])
+
+
+def test_the_same_inputs_give_the_same_bits():
+    """No atomics: every sum has a fixed order."""
+    t, ln, resets, dy, dlast, _ = scan_case((5, 150, 130, 16, 2, [150, 19, 0, 77, 149], 0.05, True, True, True, True, True), torch.float32)
+    t = {k: torch.nan_to_num(v).cuda().requires_grad_() for k, v in t.items()}
+    from airgym_amd.lib.network.selective_scan import selective_scan
+
+    def once():
+        out, last = selective_scan(*(t[k] for k in NAMES[:-1]), initial_state=t["state"], lengths=ln.cuda(), resets=resets.cuda(), return_state=True)
+        return [out, last, *torch.autograd.grad([out, last], list(t.values()), [torch.nan_to_num(dy).cuda(), dlast.cuda()])]
+
+    first = once()
+    for _ in range(3):
+        for a, b in zip(first, once()):
+            assert torch.equal(a, b)
 
 
 # ------------------------------------------------------------------------------------------------ streams, graphs, refusals
