@@ -329,6 +329,9 @@ class A2CAgent:
                 "num_seqs": self.num_actors * self.num_agents, "value_size": self.value_size,
                 "normalize_value": self.normalize_value, "normalize_input": self.normalize_input}
         self.model = ModelA2CContinuousLogStd(params, keys).to(self.ppo_device)
+        if self.model.has_memory and self.minibatch_size % self.horizon_length:
+            raise ValueError(f"a policy with a memory trains on whole sequences: minibatch_size {self.minibatch_size} is no multiple of "
+                             f"horizon_length {self.horizon_length}")
         self._flatten_parameters()
         self.optimizer = FlatAdam(self.flat_param, self.flat_grad[:-1], self.last_lr, eps=1e-8,
                                   weight_decay=self.weight_decay)
@@ -472,6 +475,10 @@ class A2CAgent:
         self.raw_rewards_buf = torch.zeros(H, N, **f)
         # dones[t] = done entering step t; uint8 like the reference's rollout buffer (lib/core/experience.py:329)
         self.dones_buf = torch.ones(H + 1, N, dtype=torch.uint8, device=dev)
+        # what the policy remembers of each env's episode now, and what it remembered when the rollout began (the update's start)
+        self.memory_state = self.memory_start = None
+        if self.model.has_memory:
+            self.memory_state, self.memory_start = (self.model.memory.initial_state(N, dev) for _ in range(2))
         self.current_rewards = torch.zeros(N, self.value_size, **f)
         self.current_shaped_rewards = torch.zeros(N, self.value_size, **f)
         self.current_lengths = torch.zeros(N, **f)
@@ -507,6 +514,8 @@ class A2CAgent:
         fr, fs = self._fused_rollout, self._fused_step
         if fr is None:
             rollout = "generic: model forward (torch) + env.step per rollout step"
+            if self.model.has_memory:
+                rollout += "; memory: ag_causal_conv_step + ag_selective_scan_step"
         elif fr.chain is not None:
             rollout = ("ag_mlp_chain_forward (whole policy forward, one launch, activations in registers) + "
                        + ("ag_step_rollout_fused" if fr.fuse_tail else "ag_policy_sample + ag_step_rollout + ag_rollout_account"))
@@ -516,6 +525,8 @@ class A2CAgent:
                        + ("ag_step_rollout_fused" if fr.fuse_tail else "ag_policy_sample + ag_step_rollout + ag_rollout_account"))
         if fs is None:
             update = "generic: autograd (torch) + fused PPO loss kernel where supported"
+            if self.model.has_memory:
+                update += "; memory: ag_causal_conv_fwd / _bwd + ag_selective_scan_fwd / _bwd"
         else:
             update = fs.describe_paths()
         return {"rollout_step": rollout, "update": update,
@@ -609,9 +620,9 @@ class A2CAgent:
         return self._obs_at(0)
 
     @torch.no_grad()
-    def get_action_values(self, obs):
+    def get_action_values(self, obs, memory=None):
         self.model.eval()
-        return self.model({"is_train": False, "prev_actions": None, "obs": obs})
+        return self.model({"is_train": False, "prev_actions": None, "obs": obs, "memory": memory})
 
     @torch.no_grad()
     def _rollout_step(self, n):
@@ -621,7 +632,8 @@ class A2CAgent:
         if getattr(self, "_dedup", False):      # the CNN ran when the frame was rendered
             res = self.get_action_values({"observation": self.obs_buf["observation"][n], "cnn_features": self._frame_feat})
         else:
-            res = self.get_action_values(self._obs_at(n))
+            memory = None if self.memory_state is None else {"state": self.memory_state, "resets": self.dones_buf[n]}
+            res = self.get_action_values(self._obs_at(n), memory)
         self.actions_buf[n].copy_(res["actions"])
         self.neglogpacs_buf[n].copy_(res["neglogpacs"])
         self.values_buf[n].copy_(res["values"])
@@ -716,6 +728,9 @@ class A2CAgent:
                 # likewise for the trainable CNN: the features of slot 0's frame were not computed yet (or, after a restore,
                 # come from other weights) - encode it with the weights this rollout runs under
                 self._refresh_frame_features()
+            if self.memory_state is not None:
+                for start, now in zip(self.memory_start, self.memory_state):
+                    start.copy_(now)
             for n in range(H):
                 self._rollout_step(n)
             if fr is not None:
@@ -750,7 +765,10 @@ class A2CAgent:
                 last_values = self.model({"is_train": False, "obs": {"observation": self.obs_buf["observation"][H],
                                                                       "cnn_features": self._frame_feat}})["values"]
             else:
-                last_values = self.model({"is_train": False, "obs": self._obs_at(H)})["values"]
+                memory = None
+                if self.memory_state is not None:      # the next rollout takes this step again: it moves a copy on
+                    memory = {"state": tuple(t.clone() for t in self.memory_state), "resets": self.dones_buf[H]}
+                last_values = self.model({"is_train": False, "obs": self._obs_at(H), "memory": memory})["values"]
             fdones = self.dones_buf[H].float()
             mb_fdones = self.dones_buf[:H].float()
             mb_advs = self._gae(fdones, last_values, mb_fdones)
@@ -809,6 +827,9 @@ class A2CAgent:
             "returns": returns, "actions": batch_dict["actions"], "obs": batch_dict["obses"],
             "dones": batch_dict["dones"], "mu": batch_dict["mus"], "sigma": batch_dict["sigmas"],
         }
+        if self.memory_state is not None:
+            from airgym_amd.lib.network.ssm import RolloutMemory
+            values_dict["memory"] = RolloutMemory(self.memory_start, batch_dict["dones"], self.horizon_length)
         if self._graph_update or self._graph_generic:
             # captured minibatch graphs read fixed addresses: keep the dataset in persistent buffers (dict observations: the
             # state vector is copied, the frame store and its cached index tensors are persistent already)
@@ -892,7 +913,7 @@ class A2CAgent:
     def _loss_and_backward_fused(self, mb):
         """Same quantities as _loss_and_backward, per-row math in one HIP kernel (ag_ppo_loss)."""
         from airgym_amd.lib.core.fused_loss import fused_ppo_loss
-        self.model.trunk(mb["obs"], heads_only=True)
+        self.model.trunk(mb["obs"], heads_only=True, memory=mb.get("memory"))
         loss, stats = fused_ppo_loss(
             self.model.last_heads, self.model.logstd, mb["actions"], mb["old_logp_actions"], mb["advantages"],
             mb["returns"], mb["old_values"], mb["mu"], mb["sigma"], e_clip=self.e_clip, critic_coef=self.critic_coef,
@@ -909,7 +930,7 @@ class A2CAgent:
         """calc_gradients up to backward(), a2c_continuous.py:299-350."""
         if self._fused_loss_ok():
             return self._loss_and_backward_fused(mb)
-        res = self.model({"is_train": True, "prev_actions": mb["actions"], "obs": mb["obs"]})
+        res = self.model({"is_train": True, "prev_actions": mb["actions"], "obs": mb["obs"], "memory": mb.get("memory")})
         a_loss = common_losses.actor_loss(mb["old_logp_actions"], res["prev_neglogp"], mb["advantages"], self.ppo, self.e_clip)
         if self.use_diagnostics:
             with torch.no_grad():

@@ -119,7 +119,7 @@ class FusedMLPStep:
     def supported(agent):
         m = agent.model
         return (str(agent.ppo_device).startswith("cuda") and agent.config.get("use_fused_update", True)
-                and agent._fused_loss_ok() and not m.dict_obs and m.actor_mlp.activation_name == "elu"
+                and agent._fused_loss_ok() and not m.dict_obs and not m.has_memory and m.actor_mlp.activation_name == "elu"
                 and agent.minibatch_size % SPLIT_K == 0 and getattr(agent, "heads_w", None) is not None
                 and all(l.weight.shape[0] % 4 == 0 and l.weight.shape[0] <= 1024 and 256 % (l.weight.shape[0] // 4) == 0
                         for l in m.actor_mlp.layers))
@@ -566,7 +566,7 @@ class FusedRolloutStep:
         sh = agent.rewards_shaper
         return (str(agent.ppo_device).startswith("cuda") and agent.config.get("use_fused_rollout", True)
                 and agent._hip_env is not None and agent._hip_env.task in ("hovering", "tracking")
-                and agent._fused_loss_ok() and not m.dict_obs
+                and agent._fused_loss_ok() and not m.dict_obs and not m.has_memory
                 and m.actor_mlp.activation_name == "elu" and getattr(agent, "heads_w", None) is not None
                 and agent.actions_num in (4, 5) and agent.clip_actions
                 and bool((agent.actions_low == -1).all()) and bool((agent.actions_high == 1).all())

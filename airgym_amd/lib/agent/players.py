@@ -44,6 +44,7 @@ class A2CPlayer:
                 "normalize_input": config.get("normalize_input", False)}
         self.model = ModelA2CContinuousLogStd(params, keys).to(self.device)
         self.model.eval()
+        self.memory_state = self.model.memory.initial_state(self.num_actors, self.device) if self.model.has_memory else None
 
     def restore(self, fn):
         checkpoint = torch_ext.load_checkpoint(fn)
@@ -88,8 +89,15 @@ class A2CPlayer:
         self.model.value_head.load_state_dict({"weight": weights["value_head.weight"], "bias": weights["value_head.bias"]})
 
     @torch.no_grad()
-    def get_action(self, obs, is_deterministic=True):
-        res = self.model({"is_train": False, "prev_actions": None, "obs": obs})
+    def get_action(self, obs, is_deterministic=True, dones=None):
+        """dones [num_actors]: envs whose episode ended with the previous step (a policy with a memory forgets them; None: all of them,
+        the first step after a reset)."""
+        memory = None
+        if self.memory_state is not None:
+            if dones is None:
+                dones = torch.ones(self.num_actors, dtype=torch.uint8, device=self.device)
+            memory = {"state": self.memory_state, "resets": dones if dones.dtype in (torch.bool, torch.uint8) else dones != 0}
+        res = self.model({"is_train": False, "prev_actions": None, "obs": obs, "memory": memory})
         action = res["mus"] if is_deterministic else res["actions"]
         if self.clip_actions:
             return rescale_actions(self.actions_low, self.actions_high, torch.clamp(action, -1.0, 1.0))
@@ -103,8 +111,9 @@ class A2CPlayer:
         steps = torch.zeros(n, device=self.device)
         acc = torch.zeros(3, dtype=torch.float64, device=self.device)      # games, sum reward, sum steps
         games_played, sum_rewards, sum_steps = 0, 0.0, 0.0
+        done = None
         for it in range(self.max_steps):
-            action = self.get_action(obs, self.is_deterministic)
+            action = self.get_action(obs, self.is_deterministic, done)
             obs, r, done, info = self.env.step(action)
             cr += r
             steps += 1

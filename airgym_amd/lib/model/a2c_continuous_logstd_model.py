@@ -5,6 +5,10 @@ lib/model/base_model.py:5-35).
   dict obs   :  image -> RunningMeanStd['image'] -> CNN -> cat(observation, features) ->
                 RunningMeanStd['observation'] (over the 16+feature_dim concat, a2c_continuous_logstd_model.py:71-75,
                 157-161) -> MLP -> heads
+  memory     :  `network.memory` {units, states, taps} puts a selective state space layer (lib/network/ssm.py) between the normaliser
+                and the MLP of a vector-observation policy: obs -> RunningMeanStd -> SelectiveMemory -> MLP -> heads.  Calls then carry
+                `memory` = {state, resets}: one step (resets [N]; the state moves on in place) or sequences (resets [rows, steps],
+                obs env-major)
   heads      :  mu Linear (x0.1 init), value_head Linear (x0.1 init), logstd parameter (init 0)
 
 State-dict keys are the reference's (`actor_mlp.layers.*`, `actor_cnn.features.*`, `actor_cnn.fc.*`, `mu.*`, `logstd`,
@@ -39,6 +43,11 @@ class ModelA2CContinuousLogStd(nn.Module):
         self.dict_obs = isinstance(input_shape, dict)
         if (self.has_cnn or self.has_vae) != self.dict_obs:
             raise ValueError("a 'cnn' / 'vae' network block needs dict observations {image, observation} and vice versa")
+        if self.has_memory:
+            if self.dict_obs:
+                raise NotImplementedError("a 'memory' network block needs vector observations")
+            from airgym_amd.lib.network.ssm import SelectiveMemory
+            self.memory = SelectiveMemory(input_shape[0], **self.memory_cfg)
         self._frozen = []            # frozen encoders: NOT registered, so they stay out of parameters() / state_dict()
         if self.has_vae:
             # a2c_continuous_logstd_model.py:32-35,45-48,114-126: frozen VAE means take the CNN features' place
@@ -94,6 +103,9 @@ class ModelA2CContinuousLogStd(nn.Module):
         self.has_cnn = "cnn" in params
         self.has_resnet = "resnet" in params
         self.has_vae = "vae" in params
+        self.has_memory = params.get("memory") is not None
+        if self.has_memory:
+            self.memory_cfg = {k: v for k, v in params["memory"].items() if k != "name"}
         if self.has_cnn:
             self.feature_dim = params["cnn"]["output_dim"]
         if self.has_vae:
@@ -162,8 +174,17 @@ class ModelA2CContinuousLogStd(nn.Module):
             enc.encoder._apply(fn, *a, **k)
         return super()._apply(fn, *a, **k)
 
+    def _remember(self, x, memory):
+        """x [M, D] through the memory layer: one step of M envs (resets [M]) or whole sequences, env-major (resets [rows, steps])."""
+        if memory is None:
+            raise ValueError("this policy has a memory: call it with memory = {'state', 'resets'}")
+        resets = memory["resets"]
+        if resets.dim() == 1:
+            return self.memory.step(x, memory["state"], resets)
+        return self.memory(x.view(*resets.shape, -1), memory["state"], resets).reshape(x.shape)
+
     # ---- forward
-    def trunk(self, obs, heads_only=False):
+    def trunk(self, obs, heads_only=False, memory=None):
         if self.dict_obs and self.has_vae:
             if "latent" in obs:       # features of the frozen encoder computed once, when the image was rendered (agent cache)
                 feat = obs["latent"]
@@ -197,6 +218,8 @@ class ModelA2CContinuousLogStd(nn.Module):
                 c_out = a_out
         else:
             norm_out = self.norm_obs(obs)
+            if self.has_memory:
+                norm_out = self._remember(norm_out, memory)
             a_out = self.actor_mlp(norm_out)
             c_out = self.critic_mlp(norm_out) if self.separate else a_out
         if not self.separate:
@@ -224,7 +247,7 @@ class ModelA2CContinuousLogStd(nn.Module):
     def forward(self, input_dict):
         is_train = input_dict.get("is_train", True)
         prev_actions = input_dict.get("prev_actions", None)
-        mu, logstd, value = self.trunk(input_dict["obs"])
+        mu, logstd, value = self.trunk(input_dict["obs"], memory=input_dict.get("memory"))
         sigma = torch.exp(logstd)
         if is_train:
             # Normal(mu, sigma).entropy() = 0.5 + 0.5 log(2 pi) + log sigma

@@ -57,7 +57,7 @@ class _CausalConv(torch.autograd.Function):
         dlast = None if dlast is None else dlast.contiguous()
         dx, dw = torch.empty(B, T, D, dtype=x.dtype, device=x.device), torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
-        ds = None if state is None else torch.empty_like(state)
+        ds = torch.empty_like(state) if ctx.needs_input_grad[3] else None
         n = lib.ag_causal_conv_workspace_bytes(B, T, D, W, N.AG_DTYPES[x.dtype])
         ws = torch.empty(n, dtype=torch.uint8, device=x.device)
         a = _fill(x, weight, bias, state, lengths, resets, ctx.silu)
@@ -117,3 +117,23 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", resets=N
         N.check(N.load().ag_causal_conv_step(x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), ptr(bias), ptr(resets),
                                              y.data_ptr(), N.AG_DTYPES[x.dtype], B, D, W, silu, stream_of(x)), "ag_causal_conv_step")
     return y
+
+
+def causal_conv_torch(x, weight, bias=None, *, activation="silu", initial_state=None, resets=None, return_state=False):
+    """The same convolution out of torch ops, step by step (any device; autograd derives the backward): the path of CPU tensors."""
+    B, T, D = x.shape
+    W = weight.shape[1]
+    window = list(x.new_zeros(W - 1, B, D) if initial_state is None else initial_state.unbind(1))
+    ys = []
+    for t in range(T):
+        if resets is not None:
+            cut = (resets[:, t] != 0)[:, None]
+            window = [torch.where(cut, torch.zeros_like(w), w) for w in window]
+        window.append(x[:, t])
+        p = sum(w * weight[:, k] for k, w in enumerate(window))
+        if bias is not None:
+            p = p + bias
+        ys.append(p * torch.sigmoid(p) if activation == "silu" else p)
+        window.pop(0)
+    y = torch.stack(ys, 1)
+    return (y, torch.stack(window, 1)) if return_state else y

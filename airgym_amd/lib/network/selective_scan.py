@@ -74,7 +74,8 @@ class _SelectiveScan(torch.autograd.Function):
 
         dout = torch.zeros(b, T, d, dtype=u.dtype, device=u.device) if dout is None else same_kind("dout", dout, u.shape, u)
         dlast = None if dlast is None else dlast.contiguous()
-        du, ddelta, dA, dB, dC, dD, dz, dbias, dstate = (like(t) for t in (u, delta, A, B, C, D, z, bias, state))
+        du, ddelta, dA, dB, dC, dD, dz, dbias, dstate = (like(t) for t in (u, delta, A, B, C, D, z, bias,
+                                                                               state if ctx.needs_input_grad[8] else None))
         bytes_ = lib.ag_selective_scan_workspace_bytes(b, T, d, n, G, 1)
         ws = _workspace(bytes_, u.device)
         a = _fill(u, delta, A, B, C, D, z, bias, state, lengths, resets, ctx.softplus)
@@ -161,3 +162,23 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     with on_device_of(u):
         N.check(N.load().ag_selective_scan_step(ctypes.byref(a), stream_of(u)), "ag_selective_scan_step")
     return out
+
+
+def selective_scan_torch(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, initial_state=None, resets=None, return_state=False):
+    """The same scan (one group, softplus) out of torch ops, step by step (any device; autograd derives the backward): the path of CPU
+    tensors."""
+    b, T, d = u.shape
+    h = u.new_zeros(b, d, A.shape[1]) if initial_state is None else initial_state
+    dt = torch.nn.functional.softplus(delta if delta_bias is None else delta + delta_bias)
+    ys = []
+    for t in range(T):
+        if resets is not None:
+            h = torch.where((resets[:, t] != 0)[:, None, None], torch.zeros_like(h), h)
+        h = torch.exp(dt[:, t, :, None] * A) * h + (dt[:, t] * u[:, t])[..., None] * B[:, t, None]
+        ys.append((h * C[:, t, None]).sum(-1))
+    y = torch.stack(ys, 1)
+    if D is not None:
+        y = y + D * u
+    if z is not None:
+        y = y * z * torch.sigmoid(z)
+    return (y, h) if return_state else y
