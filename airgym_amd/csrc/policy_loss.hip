@@ -19,7 +19,7 @@ constexpr int kSums = 5;               // policy loss, KL term, entropy, KL of t
 
 struct LossArgs {
     const void* logits; const long long* actions; const float *old_logp, *adv, *ref_logp; const unsigned char* mask;
-    void* dlogits; const float* count;
+    void* dlogits; const float* count; // {max(rows that count, 1), rows that count}, or NULL: all R
     float* partials;                   // [workgroups, kSums] sums of the rows' terms
     float *logp, *entropy;             // the log-probability form: these instead
     long long R1, s0, s1, R;
@@ -62,7 +62,7 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, bool inf, f
     const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
     float f = plain >= held || plain != plain ? plain : 0.0f;
     if (a.ref_logp) f -= a.kl_coef * expm1f(a.ref_logp[row] - r.lp);
-    const float n = 1.0f / a.count[0];
+    const float n = 1.0f / (a.count ? a.count[0] : (float)a.R);
     r.f = f * n;
     r.ent = a.entropy_coef * n;
     return r;
@@ -299,31 +299,25 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     if (tail < a.V) dx[tail] = from_f32<T>(grad_of(r, xt - r.base) + (tail == act ? r.f : 0.0f));
 }
 
-// {max(rows that count, 1), rows that count}
 __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, long long R, float* count) {
     __shared__ int part[16];
     int c = 0;
-    if (mask) {
-        const long long head = (16 - ((uintptr_t)mask & 15)) & 15, n16 = R > head ? (R - head) / 16 : 0;
-        const uint4* m = (const uint4*)(mask + head);
-        for (long long i = threadIdx.x; i < n16; i += 1024) {
-            const uint4 v = m[i];
-            const unsigned q[4] = {v.x, v.y, v.z, v.w};
+    const long long head = (16 - ((uintptr_t)mask & 15)) & 15, n16 = R > head ? (R - head) / 16 : 0;
+    const uint4* m = (const uint4*)(mask + head);
+    for (long long i = threadIdx.x; i < n16; i += 1024) {
+        const uint4 v = m[i];
+        const unsigned q[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int k = 0; k < 4; k++) {      // bytes that are not zero: bit 7 of (b | (b & 0x7f) + 0x7f)
-                const unsigned nz = (q[k] | ((q[k] & 0x7f7f7f7fu) + 0x7f7f7f7fu)) & 0x80808080u;
-                c += __popc(nz);
-            }
-        }
-        if (threadIdx.x < head && threadIdx.x < R) c += mask[threadIdx.x] != 0;
-        const long long tail = head + n16 * 16 + threadIdx.x;      // at most 15 bytes
-        if (tail < R) c += mask[tail] != 0;
+        for (int k = 0; k < 4; k++) c += __popc((q[k] | ((q[k] & 0x7f7f7f7fu) + 0x7f7f7f7fu)) & 0x80808080u);      // bytes that are not zero
     }
+    if (threadIdx.x < head && threadIdx.x < R) c += mask[threadIdx.x] != 0;
+    const long long tail = head + n16 * 16 + threadIdx.x;      // at most 15 bytes
+    if (tail < R) c += mask[tail] != 0;
     for (int o = 32; o; o >>= 1) c += __shfl_xor(c, o);
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = c;
     __syncthreads();
     if (threadIdx.x == 0) {
-        long long s = mask ? 0 : R;
+        int s = 0;
         for (int i = 0; i < 16; i++) s += part[i];
         count[0] = s > 0 ? (float)s : 1.0f;
         count[1] = (float)s;
@@ -332,7 +326,7 @@ __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, 
 
 // The rows' terms summed in a fixed order, in double: kStatsRows of them per workgroup, then those sums by one workgroup (which, for
 // few rows, takes the terms themselves).  One workgroup over 65 536 rows took 45 us, the two stages take 7.
-constexpr int kStatsRows = 1024;
+constexpr int kStatsRows = 2048;
 
 template <typename S>
 __device__ __forceinline__ void sum_rows(const S* rows, long long n, double* s, double (*part)[kSums]) {
@@ -362,16 +356,16 @@ __global__ __launch_bounds__(256) void stats_part_kernel(const float* rows, long
 }
 
 template <typename S>
-__global__ __launch_bounds__(256) void stats_kernel(const S* rows, long long n, const float* count, float kl_coef, float ent_coef, float* loss,
+__global__ __launch_bounds__(256) void stats_kernel(const S* rows, long long n, const float* count, long long R, float kl_coef, float ent_coef, float* loss,
                                                     float* stats) {
     __shared__ double part[4][kSums];
     double s[kSums];
     sum_rows(rows, n, s, part);
     if (threadIdx.x == 0) {
 #pragma unroll
-        for (int k = 0; k < kSums; k++) s[k] /= (double)count[0], stats[k] = (float)s[k];
+        for (int k = 0; k < kSums; k++) s[k] /= count ? (double)count[0] : (double)R, stats[k] = (float)s[k];
         loss[0] = (float)(s[0] + (double)kl_coef * s[1] - (double)ent_coef * s[2]);
-        stats[kSums] = count[1];
+        stats[kSums] = count ? count[1] : (float)R;
     }
 }
 
@@ -449,18 +443,19 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     float* count = (float*)p->workspace_dev;                 // 4 floats, then the stages' sums, then the rows' terms
     const long long blocks = stats_blocks(partial_rows(R, p->V));
     double* sums = (double*)(count + 4);
-    const LossArgs a{p->logits_dev, p->actions_dev, p->old_logp_dev, p->advantages_dev, p->ref_logp_dev, p->mask_dev, p->dlogits_dev, count,
+    const LossArgs a{p->logits_dev, p->actions_dev, p->old_logp_dev, p->advantages_dev, p->ref_logp_dev, p->mask_dev, p->dlogits_dev,
+                     p->mask_dev ? count : nullptr,
                      (float*)(sums + blocks * kSums), nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef, p->entropy_coef};
-    hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p->mask_dev, R, count);
+    if (a.count) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p->mask_dev, R, count);
     long long rows = 0;
     AG_FOR_DTYPE(p->dtype, rows = launch_rows<T>(a, stream));
     const float kl = p->ref_logp_dev ? p->kl_coef : 0.0f;
     if (blocks) {
         hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a.partials, rows, sums);
-        hipLaunchKernelGGL((stats_kernel<double>), dim3(1), dim3(256), 0, (hipStream_t)stream, sums, blocks, count, kl, p->entropy_coef, p->loss_dev,
+        hipLaunchKernelGGL((stats_kernel<double>), dim3(1), dim3(256), 0, (hipStream_t)stream, sums, blocks, a.count, R, kl, p->entropy_coef, p->loss_dev,
                            p->stats_dev);
     } else
-        hipLaunchKernelGGL((stats_kernel<float>), dim3(1), dim3(256), 0, (hipStream_t)stream, a.partials, rows, count, kl, p->entropy_coef, p->loss_dev,
+        hipLaunchKernelGGL((stats_kernel<float>), dim3(1), dim3(256), 0, (hipStream_t)stream, a.partials, rows, a.count, R, kl, p->entropy_coef, p->loss_dev,
                            p->stats_dev);
     return seq_status();
 }
