@@ -29,23 +29,25 @@ struct ConvGradArgs {
     int groups;                        // workgroups along the runs = rows of partial parameter gradients
 };
 
-// the W-1 inputs before step t0 as the convolution sees them there: the state's before step 0, zero from the last reset backwards
+// the W-1 inputs before step t0 as the convolution sees them there: the state's before step 0, zero from the last reset backwards, and
+// zero behind the sequence's end, whatever stands there
 template <typename T, int W, int VEC>
-__device__ __forceinline__ void load_window(const ConvArgs& a, int b, int t0, int d, float (*win)[VEC]) {
+__device__ __forceinline__ void load_window(const ConvArgs& a, int b, int t0, int len, int d, float (*win)[VEC]) {
 #pragma unroll
     for (int j = 0; j < W - 1; j++) {
         const int t = t0 - (W - 1) + j;
+        const bool there = t < 0 ? a.s0 != nullptr : t < len;
         Vec<T, VEC> c;
-        if (t >= 0) {
+        if (t >= 0 && there) {
             c = load_vec<T, VEC>((const T*)a.x + (b * a.xb + t * a.xt + d));
             if (a.resets && a.resets[b * a.rb + t * a.rt])
 #pragma unroll
                 for (int i = 0; i < j; i++)
 #pragma unroll
                     for (int v = 0; v < VEC; v++) win[i][v] = 0.0f;
-        } else if (a.s0) c = load_vec<T, VEC>((const T*)a.s0 + (((long long)b * (W - 1) + (t + W - 1)) * a.D + d));
+        } else if (there) c = load_vec<T, VEC>((const T*)a.s0 + (((long long)b * (W - 1) + (t + W - 1)) * a.D + d));
 #pragma unroll
-        for (int v = 0; v < VEC; v++) win[j][v] = t >= 0 || a.s0 ? c.at(v) : 0.0f;
+        for (int v = 0; v < VEC; v++) win[j][v] = there ? c.at(v) : 0.0f;
     }
 }
 
@@ -72,52 +74,50 @@ __global__ __launch_bounds__(kThreads) void conv_fwd_kernel(ConvArgs a) {
     T* y = (T*)a.y + ((long long)b * a.T * a.D + d);
     float w[W][VEC], bias[VEC], win[W][VEC];
     load_taps<T, W, VEC>(a, d, w, bias);
-    if (t0 < tv || (len == 0 && t0 == 0)) load_window<T, W, VEC>(a, b, min(t0, len), d, win);
-    for (int t = t0; t < tv; t += kAhead) {
+    if (t0 < tv || (len == 0 && t0 == 0)) load_window<T, W, VEC>(a, b, min(t0, len), len, d, win);
+    auto step = [&](int t, const Vec<T, VEC>& c, unsigned char cut) __attribute__((always_inline)) {
+        float p[VEC];
+        if (a.resets)
+#pragma unroll
+            for (int j = 0; j < W - 1; j++)
+#pragma unroll
+                for (int v = 0; v < VEC; v++) win[j][v] = cut ? 0.0f : win[j][v];
+#pragma unroll
+        for (int v = 0; v < VEC; v++) {
+            win[W - 1][v] = c.at(v);
+            p[v] = bias[v];
+#pragma unroll
+            for (int k = 0; k < W; k++) p[v] = __builtin_fmaf(w[k][v], win[k][v], p[v]);
+        }
+        if (a.silu)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) p[v] *= sigmoid(p[v]);
+        Vec<T, VEC> o;
+        o.set(p);
+        store_vec<T, VEC>(y + (long long)t * a.D, o);
+#pragma unroll
+        for (int j = 0; j < W - 1; j++)
+#pragma unroll
+            for (int v = 0; v < VEC; v++) win[j][v] = win[j + 1][v];
+    };
+    const unsigned char* flags = a.resets ? a.resets + b * a.rb : nullptr;
+    int t = t0;
+    for (; t + kAhead <= tv; t += kAhead) {
         Vec<T, VEC> c[kAhead];
         unsigned char cut[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
-            cut[i] = 0;
-            if (t + i < tv) {
-                c[i] = load_vec<T, VEC>(x + (t + i) * a.xt);
-                if (a.resets) cut[i] = a.resets[b * a.rb + (t + i) * a.rt];
-            }
+            c[i] = load_vec<T, VEC>(x + (t + i) * a.xt);
+            cut[i] = flags ? flags[(t + i) * a.rt] : 0;
         }
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            if (t + i >= tv) break;
-            float p[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; v++) {
-                win[W - 1][v] = c[i].at(v);
-                p[v] = bias[v];
-            }
-            if (cut[i])
-#pragma unroll
-                for (int j = 0; j < W - 1; j++)
-#pragma unroll
-                    for (int v = 0; v < VEC; v++) win[j][v] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < W; k++)
-#pragma unroll
-                for (int v = 0; v < VEC; v++) p[v] = __builtin_fmaf(w[k][v], win[k][v], p[v]);
-            if (a.silu)
-#pragma unroll
-                for (int v = 0; v < VEC; v++) p[v] *= sigmoid(p[v]);
-            Vec<T, VEC> o;
-            o.set(p);
-            store_vec<T, VEC>(y + (long long)(t + i) * a.D, o);
-#pragma unroll
-            for (int j = 0; j < W - 1; j++)
-#pragma unroll
-                for (int v = 0; v < VEC; v++) win[j][v] = win[j + 1][v];
-        }
+        for (int i = 0; i < kAhead; i++) step(t + i, c[i], cut[i]);
     }
+    for (; t < tv; t++) step(t, load_vec<T, VEC>(x + t * a.xt), flags ? flags[t * a.rt] : 0);
     const float none[VEC] = {};
     Vec<T, VEC> zero;
     zero.set(none);
-    for (int t = max(t0, tv); t < t1; t++) store_vec<T, VEC>(y + (long long)t * a.D, zero);
+    for (t = max(t0, tv); t < t1; t++) store_vec<T, VEC>(y + (long long)t * a.D, zero);
     // the run that holds the last step (the first run of an empty sequence) leaves the state behind
     if (a.s1 && (len == 0 ? t0 == 0 : (t0 < len && len <= t0 + a.run))) {
         T* s1 = (T*)a.s1 + ((long long)b * (W - 1) * a.D + d);
@@ -159,77 +159,77 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGrad
             for (int j = 0; j < W; j++)
 #pragma unroll
                 for (int v = 0; v < VEC; v++) acc[j][v] = 0.0f;
-            load_window<T, W, VEC>(a, b, t0, d, win);      // beyond the length: read but not used (dp = 0 there)
-            int alive = W;                         // taps that reach back over no reset since the run's start
+            load_window<T, W, VEC>(a, b, t0, len, d, win);
+            const unsigned char* flags = a.resets ? a.resets + b * a.rb : nullptr;
+            const int some = min(len, t1 + W - 1);         // steps from here on have x = dy = 0: they add nothing
+            int alive = W;                                 // taps that reach back over no reset since the run's start
             for (int t = t0; t < t1 + W - 1; t += kAhead) {
                 Vec<T, VEC> cx[kAhead], cg[kAhead];
                 unsigned char cut[kAhead];
 #pragma unroll
                 for (int i = 0; i < kAhead; i++) {
+                    const float none[VEC] = {};
                     cut[i] = 0;
-                    if (t + i < min(len, t1 + W - 1)) {
+                    if (t + i < some) {
                         cx[i] = load_vec<T, VEC>(x + (t + i) * a.xt);
                         cg[i] = load_vec<T, VEC>(dy + (t + i) * g.dyt);
-                        if (a.resets) cut[i] = a.resets[b * a.rb + (t + i) * a.rt];
-                    }
+                        if (flags) cut[i] = flags[(t + i) * a.rt];
+                    } else cx[i].set(none), cg[i].set(none);
                 }
+                // No branch changes a window from here on: each would cost the copies that join its two sides.
 #pragma unroll
                 for (int i = 0; i < kAhead; i++) {
                     const int ti = t + i;
-                    if (ti >= t1 + W - 1) break;
+                    float dp[VEC], mine[VEC];
+                    if (flags) {
+                        alive = cut[i] ? 1 : alive;
 #pragma unroll
-                    for (int v = 0; v < VEC; v++) win[W - 1][v] = 0.0f;
-                    if (ti < len) {
-                        float p[VEC], dp[VEC];
-                        if (cut[i]) {
-                            alive = 1;
+                        for (int j = 0; j < W - 1; j++)
 #pragma unroll
-                            for (int j = 0; j < W - 1; j++)
+                            for (int v = 0; v < VEC; v++) win[j][v] = cut[i] ? 0.0f : win[j][v];
+                    }
 #pragma unroll
-                                for (int v = 0; v < VEC; v++) win[j][v] = 0.0f;
-                        }
+                    for (int v = 0; v < VEC; v++) win[W - 1][v] = cx[i].at(v), dp[v] = cg[i].at(v);
+                    if (a.silu)
 #pragma unroll
                         for (int v = 0; v < VEC; v++) {
-                            win[W - 1][v] = cx[i].at(v);
-                            p[v] = bias[v];
-                            dp[v] = cg[i].at(v);
+                            float p = bias[v];
+#pragma unroll
+                            for (int k = 0; k < W; k++) p = __builtin_fmaf(w[k][v], win[k][v], p);
+                            const float s = sigmoid(p);
+                            dp[v] *= s * __builtin_fmaf(p, 1.0f - s, 1.0f);
                         }
-                        if (a.silu) {
 #pragma unroll
-                            for (int k = 0; k < W; k++)
+                    for (int v = 0; v < VEC; v++) {
+                        mine[v] = ti < t1 ? dp[v] : 0.0f;
+                        dw[W][v] += mine[v];
 #pragma unroll
-                                for (int v = 0; v < VEC; v++) p[v] = __builtin_fmaf(w[k][v], win[k][v], p[v]);
-#pragma unroll
-                            for (int v = 0; v < VEC; v++) {
-                                const float s = sigmoid(p[v]);
-                                dp[v] *= s * (1.0f + p[v] * (1.0f - s));
-                            }
-                        }
-                        if (ti < t1) {
-#pragma unroll
-                            for (int v = 0; v < VEC; v++) {
-                                dw[W][v] += dp[v];
-#pragma unroll
-                                for (int k = 0; k < W; k++) dw[k][v] = __builtin_fmaf(dp[v], win[k][v], dw[k][v]);
-                            }
-                        }
+                        for (int k = 0; k < W; k++) dw[k][v] = __builtin_fmaf(mine[v], win[k][v], dw[k][v]);
+                    }
+                    if (flags) {
 #pragma unroll
                         for (int k = 0; k < W; k++)
-                            if (k >= W - alive)
 #pragma unroll
-                                for (int v = 0; v < VEC; v++) acc[k][v] = __builtin_fmaf(w[k][v], dp[v], acc[k][v]);
-                        alive = min(alive + 1, W);
+                            for (int v = 0; v < VEC; v++) acc[k][v] = __builtin_fmaf(w[k][v], k >= W - alive ? dp[v] : 0.0f, acc[k][v]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < W; k++)
+#pragma unroll
+                            for (int v = 0; v < VEC; v++) acc[k][v] = __builtin_fmaf(w[k][v], dp[v], acc[k][v]);
                     }
+                    alive = ti < len ? min(alive + 1, W) : alive;
                     const int done = ti - (W - 1);         // this input has met every step that reads it
-                    if (g.ds1 && ti >= len && done < len && len - 1 - done < alive - 1) {      // ... and is part of the state left behind
+                    if (g.ds1 && ti >= len && done < len && len - 1 - done < alive - 1 && ti - len < W - 1) {
+                        // ... and is part of the state left behind
                         const auto c = load_vec<T, VEC>((const T*)g.ds1 + (((long long)b * (W - 1) + (ti - len)) * a.D + d));
 #pragma unroll
                         for (int v = 0; v < VEC; v++) acc[0][v] += c.at(v);
                     }
                     Vec<T, VEC> o;
                     o.set(acc[0]);
-                    if (done >= t0) store_vec<T, VEC>(dx + (long long)done * a.D, o);
-                    else if (t0 == 0 && g.ds0) store_vec<T, VEC>((T*)g.ds0 + (((long long)b * (W - 1) + ti) * a.D + d), o);
+                    if (done >= t0) {
+                        if (done < t1) store_vec<T, VEC>(dx + (long long)done * a.D, o);
+                    } else if (t0 == 0 && g.ds0) store_vec<T, VEC>((T*)g.ds0 + (((long long)b * (W - 1) + ti) * a.D + d), o);
 #pragma unroll
                     for (int v = 0; v < VEC; v++) {
 #pragma unroll
@@ -294,7 +294,7 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(const T* x, long lo
 struct Plan { int vec, lx, ly, nx, run, runs; };
 Plan plan_of(long long B, int T, int D, int wide) {
     Plan p;
-    // 16 bytes per access (8 for the backward's 16-bit types, which carry gradients too); channels that do not divide move two or one
+    // what one access should hold (16 bytes in the forward); channels that do not divide move two or one
     p.vec = D % wide == 0 ? wide : D % 2 == 0 ? 2 : 1;
     const int dv = D / p.vec;
     p.lx = dv < kThreads ? dv : kThreads;
@@ -311,7 +311,9 @@ Plan plan_of(long long B, int T, int D, int wide) {
 }
 
 constexpr int wide_fwd(int size) { return 16 / size; }
-constexpr int wide_bwd(int) { return 4; }
+// the backward holds 4 W + 1 rows of VEC in registers: four channels up to five taps, then two (W = 8 at 64 x 1000 x 512: 158 us with two,
+// 194 with four)
+constexpr int wide_bwd(int W) { return W <= 5 ? 4 : 2; }
 
 // workgroups along the runs in the backward, each with one row of partial gradients
 int grad_groups(const Plan& p, long long B) {
@@ -370,8 +372,7 @@ extern "C" int ag_causal_conv_fwd(const ag_conv_args* p, void* stream) {
 
 extern "C" long long ag_causal_conv_workspace_bytes(int B, int T, int D, int W, int dtype) {
     if (B <= 0 || T <= 0 || D <= 0 || W < 2 || W > 8 || dtype < AG_F32 || dtype > AG_F16) return 0;
-    const int size = dtype == AG_F32 ? 4 : 2;
-    return (long long)grad_groups(plan_of(B, T, D, wide_bwd(size)), B) * D * (W + 1) * (long long)sizeof(float);
+    return (long long)grad_groups(plan_of(B, T, D, wide_bwd(W)), B) * D * (W + 1) * (long long)sizeof(float);
 }
 
 extern "C" int ag_causal_conv_bwd(const ag_conv_args* p, const ag_conv_grads* q, void* stream) {
@@ -379,13 +380,12 @@ extern "C" int ag_causal_conv_bwd(const ag_conv_args* p, const ag_conv_grads* q,
     if (!q || q->struct_size != sizeof(ag_conv_grads) || !q->dy_dev || !q->dx_dev || !q->dweight_dev || !q->workspace_dev)
         return AG_ERR_INVALID_ARG;
     if (q->workspace_bytes < ag_causal_conv_workspace_bytes(p->B, p->T, p->D, p->W, p->dtype)) return AG_ERR_INVALID_ARG;
-    const int size = p->dtype == AG_F32 ? 4 : 2;
-    const Plan l = plan_of(p->B, p->T, p->D, wide_bwd(size));
+    const Plan l = plan_of(p->B, p->T, p->D, wide_bwd(p->W));
     const ConvArgs a = device_args(p, l);
     const ConvGradArgs g{q->dy_dev, q->dstate_out_dev, q->dx_dev, q->dstate_dev, (float*)q->workspace_dev, q->dy_sb, q->dy_st,
                          grad_groups(l, a.B)};
     const dim3 grid((unsigned)(g.groups * l.nx));
-    AG_FOR_DTYPE(p->dtype, AG_FOR_TAPS(p->W, AG_FOR_VEC(l.vec, wide_bwd(sizeof(T)), hipLaunchKernelGGL((conv_bwd_kernel<T, W, VEC>), grid,
+    AG_FOR_DTYPE(p->dtype, AG_FOR_TAPS(p->W, AG_FOR_VEC(l.vec, wide_bwd(W), hipLaunchKernelGGL((conv_bwd_kernel<T, W, VEC>), grid,
                                                                                      dim3(kThreads), 0, (hipStream_t)stream, a, g))));
     launch_sum_rows(g.partials, g.groups, (long long)a.D * (p->W + 1), ConvParams{q->dweight_dev, q->dbias_dev, p->W}, stream);
     return seq_status();
