@@ -153,14 +153,16 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGrad
             const int len = seq_len(a.lengths, b, a.T);
             const T* x = (const T*)a.x + (b * a.xb + d);
             const T* dy = (const T*)g.dy + (b * g.dyb + d);
-            T* dx = (T*)g.dx + ((long long)b * a.T * a.D + d);
+            // the group's rows; the gradient written at step t is that of step t-W+1
+            const T *px = x + t0 * a.xt, *pg = dy + t0 * g.dyt;
+            T* dx = (T*)g.dx + (((long long)b * a.T + t0 - (W - 1)) * a.D + d);
+            const unsigned char* flags = a.resets ? a.resets + (b * a.rb + t0 * a.rt) : nullptr;
             float win[W][VEC], acc[W][VEC];        // inputs and their gradients, oldest first
 #pragma unroll
             for (int j = 0; j < W; j++)
 #pragma unroll
                 for (int v = 0; v < VEC; v++) acc[j][v] = 0.0f;
             load_window<T, W, VEC>(a, b, t0, len, d, win);
-            const unsigned char* flags = a.resets ? a.resets + b * a.rb : nullptr;
             const int some = min(len, t1 + W - 1);         // steps from here on have x = dy = 0: they add nothing
             int alive = W;                                 // taps that reach back over no reset since the run's start
             for (int t = t0; t < t1 + W - 1; t += kAhead) {
@@ -171,17 +173,19 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGrad
                     const float none[VEC] = {};
                     cut[i] = 0;
                     if (t + i < some) {
-                        cx[i] = load_vec<T, VEC>(x + (t + i) * a.xt);
-                        cg[i] = load_vec<T, VEC>(dy + (t + i) * g.dyt);
-                        if (flags) cut[i] = flags[(t + i) * a.rt];
+                        cx[i] = load_vec<T, VEC>(px + i * a.xt);
+                        cg[i] = load_vec<T, VEC>(pg + i * g.dyt);
+                        if (flags) cut[i] = flags[i * a.rt];
                     } else cx[i].set(none), cg[i].set(none);
                 }
+                px += kAhead * a.xt, pg += kAhead * g.dyt;
+                if (flags) flags += kAhead * a.rt;
                 // No branch changes a window from here on: each would cost the copies that join its two sides.
 #pragma unroll
                 for (int i = 0; i < kAhead; i++) {
                     const int ti = t + i;
                     float dp[VEC], mine[VEC];
-                    if (flags) {
+                    if (a.resets) {
                         alive = cut[i] ? 1 : alive;
 #pragma unroll
                         for (int j = 0; j < W - 1; j++)
@@ -206,7 +210,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGrad
 #pragma unroll
                         for (int k = 0; k < W; k++) dw[k][v] = __builtin_fmaf(mine[v], win[k][v], dw[k][v]);
                     }
-                    if (flags) {
+                    if (a.resets) {
 #pragma unroll
                         for (int k = 0; k < W; k++)
 #pragma unroll
@@ -228,7 +232,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGrad
                     Vec<T, VEC> o;
                     o.set(acc[0]);
                     if (done >= t0) {
-                        if (done < t1) store_vec<T, VEC>(dx + (long long)done * a.D, o);
+                        if (done < t1) store_vec<T, VEC>(dx + (long long)i * a.D, o);
                     } else if (t0 == 0 && g.ds0) store_vec<T, VEC>((T*)g.ds0 + (((long long)b * (W - 1) + ti) * a.D + d), o);
 #pragma unroll
                     for (int v = 0; v < VEC; v++) {
@@ -237,6 +241,7 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a, ConvGrad
                         acc[W - 1][v] = 0.0f;
                     }
                 }
+                dx += (long long)kAhead * a.D;
             }
         }
     // the workgroup's runs added up in order; one row of partial gradients [groups, D, W + 1]
