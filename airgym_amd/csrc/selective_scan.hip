@@ -3,8 +3,8 @@
 //   dt = softplus(delta + bias);  h_t = exp(dt A) h_{t-1} + dt B_t u_t;  y_t = C_t . h_t + D u_t;  out = y z sigmoid(z)
 //   (per channel d a state of N numbers; B_t, C_t shared by the channels of a group; h := 0 before a step flagged as a reset)
 //
-// Layout.  A workgroup owns 64 consecutive channels of one group and walks along time in tiles; wave w owns states 4w .. 4w+3 of all
-// 64 channels (lane = channel), so N = 16 is four waves.  What does not depend on the state index - softplus, the products dt u, the
+// Layout.  A workgroup owns 64 consecutive channels of one group and walks along time in tiles; wave w owns S states of all 64 channels
+// (lane = channel): four waves of 1, 2 or 4 states up to N = 16, eight waves of 4 beyond.  What does not depend on the state index - softplus, the products dt u, the
 // gate - is formed once per (step, channel) by whichever wave stages that row and goes through LDS; per (step, channel, state) there
 // remain one multiply, one v_exp_f32, one multiply and two FMAs.  The sums over states (y, and in the backward the two sums behind du
 // and ddelta) are joined through LDS, in a fixed order.
@@ -107,44 +107,73 @@ template <typename T> __device__ __forceinline__ T get(const Rows& x, int r, uns
 }
 template <typename T> __device__ __forceinline__ void put(char* base, unsigned bytes, T v) { *(T*)(base + bytes) = v; }
 
-// a lane's four states in a row of N, zero where there are none: one access where the row is whole
+// a lane's S states (the w-th S of a row of N), zero where there are none: one access where the row is whole
+typedef float two_any4 __attribute__((ext_vector_type(2), aligned(4)));
 typedef float four_any4 __attribute__((ext_vector_type(4), aligned(4)));
-__device__ __forceinline__ void load4(const float* row, int w, int N, float* x) {
-    if (N % 4 == 0 && 4 * w < N) {
+template <int S> __device__ __forceinline__ void load_states(const float* row, int w, int N, float* x) {
+    if (S == 4 && N % 4 == 0 && 4 * w < N) {
         const four_any4 v = *(const four_any4*)(row + 4 * w);
-        x[0] = v[0], x[1] = v[1], x[2] = v[2], x[3] = v[3];
+#pragma unroll
+        for (int j = 0; j < S; j++) x[j] = v[j];
+    } else if (S == 2 && N % 2 == 0 && 2 * w < N) {
+        const two_any4 v = *(const two_any4*)(row + 2 * w);
+#pragma unroll
+        for (int j = 0; j < S; j++) x[j] = v[j];
     } else
 #pragma unroll
-        for (int j = 0; j < 4; j++) x[j] = 4 * w + j < N ? row[4 * w + j] : 0.0f;
+        for (int j = 0; j < S; j++) x[j] = S * w + j < N ? row[S * w + j] : 0.0f;
 }
-__device__ __forceinline__ void store4(float* row, int w, int N, const float* x) {
-    if (N % 4 == 0 && 4 * w < N) *(four_any4*)(row + 4 * w) = four_any4{x[0], x[1], x[2], x[3]};
-    else
+template <int S> __device__ __forceinline__ void store_states(float* row, int w, int N, const float* x) {
+    if (S == 4 && N % 4 == 0 && 4 * w < N) {
+        four_any4 v;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (4 * w + j < N) row[4 * w + j] = x[j];
+        for (int j = 0; j < S; j++) v[j] = x[j];
+        *(four_any4*)(row + 4 * w) = v;
+    } else if (S == 2 && N % 2 == 0 && 2 * w < N) {
+        two_any4 v;
+#pragma unroll
+        for (int j = 0; j < S; j++) v[j] = x[j];
+        *(two_any4*)(row + 2 * w) = v;
+    } else
+#pragma unroll
+        for (int j = 0; j < S; j++)
+            if (S * w + j < N) row[S * w + j] = x[j];
 }
-__device__ __forceinline__ void zero4(float* x) { x[0] = x[1] = x[2] = x[3] = 0.0f; }
+template <int S> __device__ __forceinline__ void clear(float* x) {
+#pragma unroll
+    for (int j = 0; j < S; j++) x[j] = 0.0f;
+}
+// S neighbouring numbers of an LDS row
+template <int S> __device__ __forceinline__ void read_row(const float* row, float* x) {
+    if constexpr (S == 4) {
+        const float4 v = *(const float4*)row;
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    } else if constexpr (S == 2) {
+        const float2 v = *(const float2*)row;
+        x[0] = v.x, x[1] = v.y;
+    } else x[0] = row[0];
+}
 
 // state (or gradient of a state) that chunk `chunk` starts from, folded over the chunks first .. last - 1 (step +-1) before it
+template <int S>
 __device__ __forceinline__ void fold_chunks(const ScanArgs& a, int b, int d, int w, int first, int last, int step, const float* A2, float* h) {
 #pragma unroll 1                       // eight at a time took the registers of a sixth workgroup per CU
     for (int c = first; c != last; c += step) {
         const long long at = ((long long)b * a.chunks + c) * a.D + d;
         const float sum = a.chunk_dt[at];
-        float x[4];
-        load4(a.chunk_h + at * a.N, w, a.N, x);
+        float x[S];
+        load_states<S>(a.chunk_h + at * a.N, w, a.N, x);
 #pragma unroll
-        for (int j = 0; j < 4; j++) h[j] = (sum == sum ? exp2_hw(sum * A2[j]) * h[j] : 0.0f) + x[j];
+        for (int j = 0; j < S; j++) h[j] = (sum == sum ? exp2_hw(sum * A2[j]) * h[j] : 0.0f) + x[j];
     }
 }
 
 // kStates: the first pass over chunks (every chunk but the last; no outputs but chunk_h and chunk_dt).  Otherwise the scan itself.
 // A workgroup takes every `rows`-th sequence; while a tile is worked on, the next one's inputs - of the same sequence or the next - are
 // on their way.
-template <typename T, int NG, bool kStates>
-__global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(ScanArgs a) {
-    constexpr int kRows = kTile / NG, kWide = 4 * NG;
+template <typename T, int NG, int S, bool kStates>
+__global__ __launch_bounds__(kLanes* NG, 6) void scan_fwd_kernel(ScanArgs a) {
+    constexpr int kRows = kTile / NG, kWide = S * NG;
     __shared__ float2 sdt[kTile][kLanes];                               // dt, dt u
     __shared__ float sy[kStates ? 1 : NG][kTile][kLanes];
     __shared__ alignas(16) float sB[kTile][kWide], sC[kTile][kWide];
@@ -155,10 +184,10 @@ __global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(Sc
     const bool gate = !kStates && a.z, soft = a.softplus, ckpt = !kStates && a.ckpt;
     const int from = p.chunk * a.steps, to = min(from + a.steps, T_);
 
-    float A2[4];
-    load4(a.A + (long long)d * N, w, N, A2);
+    float A2[S];
+    load_states<S>(a.A + (long long)d * N, w, N, A2);
 #pragma unroll
-    for (int j = 0; j < 4; j++) A2[j] *= kLog2e;
+    for (int j = 0; j < S; j++) A2[j] *= kLog2e;
     const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
     const unsigned at = (unsigned)d * (unsigned)sizeof(T);
     const long long state = (long long)d * N;                          // of the lane's channel
@@ -183,7 +212,7 @@ __global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(Sc
             }
         }
         rB = rC = from_f32<T>(0.0f);
-        if (brow < nv && bn < N) {
+        if ((S == 4 || brow < kTile) && brow < nv && bn < N) {
             rB = get<T>(Bm, brow, bn * (unsigned)sizeof(T));
             if (!kStates) rC = get<T>(Cm, brow, bn * (unsigned)sizeof(T));
         }
@@ -203,11 +232,11 @@ __global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(Sc
             sequence(b);
             load(end - from);
         }
-        float h[4];
-        zero4(h);
+        float h[S];
+        clear<S>(h);
         if (!kStates) {
-            if (k1->s0) load4(k1->s0 + (long long)b * D * N + state, w, N, h);
-            if (p.chunk && from < end) fold_chunks(a, b, d, w, 0, p.chunk, 1, A2, h);
+            if (k1->s0) load_states<S>(k1->s0 + (long long)b * D * N + state, w, N, h);
+            if (p.chunk && from < end) fold_chunks<S>(a, b, d, w, 0, p.chunk, 1, A2, h);
         }
         for (int t0 = from; t0 < end; t0 += kTile) {
             const int nv = min(kTile, end - t0);
@@ -226,8 +255,10 @@ __global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(Sc
                 if (kStates) total += dt;
                 sdt[r][lane] = make_float2(dt, dt * uu[k]);
             }
-            sB[brow][bn] = to_f32(rB);
-            if (!kStates) sC[brow][bn] = to_f32(rC);
+            if (S == 4 || brow < kTile) {
+                sB[brow][bn] = to_f32(rB);
+                if (!kStates) sC[brow][bn] = to_f32(rC);
+            }
             const unsigned cut = reset_bits(scan_args(), b, t0, nv, lane);
             any_cut |= cut != 0;
             __syncthreads();
@@ -242,19 +273,20 @@ __global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(Sc
             for (int r = 0; r < kTile; r++) {                           // steps behind nv have dt = 0: they change nothing
                 if (r % 4 == 0 && r >= nv) break;
                 if (r % kBack == 0 && ckpt) {
-                    if (t0 + r && p.live) store4(ck, w, N, h);
+                    if (t0 + r && p.live) store_states<S>(ck, w, N, h);
                     ck += (long long)D * N;
                 }
-                AG_RARE(cut >> r & 1) zero4(h);
+                AG_RARE(cut >> r & 1) clear<S>(h);
                 const float2 q = sdt[r][lane];
-                const float4 Bv = *(const float4*)&sB[r][4 * w];
-                const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w};
+                float Bn[S], Cn[S], y = 0.0f;
+                read_row<S>(&sB[r][S * w], Bn);
+                if (!kStates) read_row<S>(&sC[r][S * w], Cn);
 #pragma unroll
-                for (int j = 0; j < 4; j++) h[j] = __builtin_fmaf(exp2_hw(q.x * A2[j]), h[j], q.y * B4[j]);
-                if (!kStates) {
-                    const float4 Cv = *(const float4*)&sC[r][4 * w];
-                    sy[w][r][lane] = __builtin_fmaf(Cv.x, h[0], Cv.y * h[1]) + __builtin_fmaf(Cv.z, h[2], Cv.w * h[3]);
+                for (int j = 0; j < S; j++) {
+                    h[j] = __builtin_fmaf(exp2_hw(q.x * A2[j]), h[j], q.y * Bn[j]);
+                    if (!kStates) y = j ? __builtin_fmaf(Cn[j], h[j], y) : Cn[j] * h[j];
                 }
+                if (!kStates) sy[w][r][lane] = y;
             }
             __syncthreads();
             if (!kStates) {
@@ -278,7 +310,7 @@ __global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(Sc
             __syncthreads();
             if (!p.live) return;
             const long long row = ((long long)b * a.chunks + p.chunk) * D + d;
-            store4(k2->chunk_h + row * N, w, N, h);
+            store_states<S>(k2->chunk_h + row * N, w, N, h);
             if (w == 0) {
                 float s = 0.0f;
                 for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
@@ -292,7 +324,7 @@ __global__ __launch_bounds__(kLanes* NG, NG < 4 ? 1 : 6) void scan_fwd_kernel(Sc
             for (int t = max(from, end) + w; t < to; t += NG) put(out + (long long)t * D * (long long)sizeof(T), at, from_f32<T>(0.0f));
         }
         if (k2->s1 && (len ? from < len && len <= to : p.chunk == 0))   // the chunk with the last step
-            store4(k2->s1 + (long long)b * D * N + state, w, N, h);
+            store_states<S>(k2->s1 + (long long)b * D * N + state, w, N, h);
     }
 }
 
@@ -329,13 +361,13 @@ __device__ __forceinline__ int sum_lanes8_order(int lane) {
 // The states of a tile of 8 steps are run again from the state the forward left before it and kept, with the decays, in registers;
 // tiles are walked backwards.  16 steps per tile took 326 registers (one wave per SIMD) and five times as long.  A workgroup takes
 // every `rows`-th sequence, so that dA, dD and the bias gradient stay in registers meanwhile.
-// dB and dC are sums over channels, that is over lanes: two steps' four values at a time, transposed on the way.
+// dB and dC are sums over channels, that is over lanes: eight values (8 / S steps') at a time, transposed on the way.
 
 // kCarry: the first pass over chunks (every chunk but the first): what the chunk hands back to the one before when nothing reaches it
 // from behind, and its sum of dt.
-template <typename T, int NG, bool kCarry>
-__global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd_kernel(ScanArgs a, ScanGradArgs q) {
-    constexpr int kRows = kBack / NG, kWide = 4 * NG;
+template <typename T, int NG, int S, bool kCarry>
+__global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(ScanArgs a, ScanGradArgs q) {
+    constexpr int kRows = kBack / NG, kWide = S * NG, kSteps = 8 / S;
     __shared__ float2 sdt[kBack][kLanes];                               // dt, dt u
     __shared__ float sdy[kBack][kLanes];
     __shared__ float sy[kCarry ? 1 : NG][kBack][kLanes], ss1[kCarry ? 1 : NG][kBack][kLanes], ss2[kCarry ? 1 : NG][kBack][kLanes];
@@ -346,21 +378,21 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
     const bool gate = a.z, soft = a.softplus;
     const int from = p.chunk * a.steps, to = min(from + a.steps, T_), last = from + (to - from - 1) / kBack * kBack;
-    // 8 rows of B and of C: half of the threads have one of each
+    // 8 rows of B and of C: a thread has one of each, or none
     const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
     const unsigned at = (unsigned)d * (unsigned)sizeof(T);
     const long long state = (long long)d * N;
     const int GN = a.G * N;
     const unsigned bc_at = brow * GN + p.g * N + bn;                    // in a tile of [T, G, N]
-    float A2[4], dA[4], dD = 0.0f, dbias = 0.0f;
-    load4(a.A + state, w, N, A2);
-    zero4(dA);
+    float A2[S], dA[S], dD = 0.0f, dbias = 0.0f;
+    load_states<S>(a.A + state, w, N, A2);
+    clear<S>(dA);
 #pragma unroll
-    for (int j = 0; j < 4; j++) A2[j] *= kLog2e;
+    for (int j = 0; j < S; j++) A2[j] *= kLog2e;
 
     Rows u, delta, z, dout, Bm, Cm;
     T ru[kRows], rd[kRows], rz[kRows], rg[kRows], rB, rC;
-    float start[4];
+    float start[S];
     auto sequence = [&](int b) __attribute__((always_inline)) {        // its last tile in this chunk
         const auto k = scan_args();
         const auto g = grad_args();
@@ -390,9 +422,9 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
         }
         if (!kCarry && nv > 0) {
             const auto k = scan_args();
-            if (t0) load4(k->ckpt + ((long long)b * ((T_ - 1) / kBack) + t0 / kBack - 1) * D * N + state, w, N, start);
-            else if (k->s0) load4(k->s0 + (long long)b * D * N + state, w, N, start);
-            else zero4(start);
+            if (t0) load_states<S>(k->ckpt + ((long long)b * ((T_ - 1) / kBack) + t0 / kBack - 1) * D * N + state, w, N, start);
+            else if (k->s0) load_states<S>(k->s0 + (long long)b * D * N + state, w, N, start);
+            else clear<S>(start);
         }
         if (!kCarry) u.move(-kBack), Bm.move(-kBack);
         delta.move(-kBack), dout.move(-kBack), Cm.move(-kBack);
@@ -410,19 +442,19 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
         const long long o = ((long long)b * T_ + last) * D * (long long)sizeof(T);
         char *du = (char*)g1->du + o, *ddelta = (char*)g1->ddelta + o, *dz = (char*)g1->dz + o;
         const int next_b = b + q.rows, next_len = next_b < a.B ? seq_len(k1->lengths, next_b, T_) : 0;
-        float carry[4];                                                 // a_{t+1} g_{t+1}
-        zero4(carry);
+        float carry[S];                                                 // a_{t+1} g_{t+1}
+        clear<S>(carry);
         if (!kCarry) {
-            if (g1->ds1 && p.live) load4(g1->ds1 + (long long)b * D * N + state, w, N, carry);
-            fold_chunks(a, b, d, w, a.chunks - 1, p.chunk, -1, A2, carry);
+            if (g1->ds1 && p.live) load_states<S>(g1->ds1 + (long long)b * D * N + state, w, N, carry);
+            fold_chunks<S>(a, b, d, w, a.chunks - 1, p.chunk, -1, A2, carry);
         }
         float total = 0.0f;
         bool any_cut = false;
         for (int t0 = last; t0 >= from; t0 -= kBack) {
             const int nv = max(0, min(kBack, len - t0)), nt = min(kBack, T_ - t0);
-            float uu[kRows], dts[kRows], sg[kRows], zz[kRows], sz[kRows], go[kRows], now[4];
+            float uu[kRows], dts[kRows], sg[kRows], zz[kRows], sz[kRows], go[kRows], now[S];
 #pragma unroll
-            for (int j = 0; j < 4; j++) now[j] = p.live ? start[j] : 0.0f;
+            for (int j = 0; j < S; j++) now[j] = p.live ? start[j] : 0.0f;
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
                 const int r = w + k * NG;
@@ -458,67 +490,71 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
             if (kCarry) {
 #pragma unroll
                 for (int r = kBack - 1; r >= 0; r--) {
-                    const float4 Cv = *(const float4*)&sBC[1][r][4 * w];
-                    const float C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w}, dy = sdy[r][lane], dt = sdt[r][lane].x;
+                    const float dy = sdy[r][lane], dt = sdt[r][lane].x;
+                    float Cn[S];
+                    read_row<S>(&sBC[1][r][S * w], Cn);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) carry[j] = exp2_hw(dt * A2[j]) * __builtin_fmaf(C4[j], dy, carry[j]);
-                    AG_RARE(cut >> r & 1) zero4(carry);
+                    for (int j = 0; j < S; j++) carry[j] = exp2_hw(dt * A2[j]) * __builtin_fmaf(Cn[j], dy, carry[j]);
+                    AG_RARE(cut >> r & 1) clear<S>(carry);
                 }
                 __syncthreads();
                 continue;
             }
             if (nv) {
-                float h[kBack][4], e[kBack][4], v[8], sums = 0.0f;      // h[r]: the state step r starts from
-                const int order = sum_lanes8_order(lane), odd = order >> 2, mine = lane & 3;
+                float h[kBack][S], e[kBack][S], v[8], sums = 0.0f;      // h[r]: the state step r starts from
+                // kSteps steps' values are summed at a time; lane 8g + i keeps the i-th sum
+                const int order = sum_lanes8_order(lane), step = order / S, mine = lane % S;
 #pragma unroll
                 for (int r = 0; r < kBack; r++) {      // steps behind nv have dt = dy = 0: decay 1, no input
-                    AG_RARE(cut >> r & 1) zero4(now);
+                    AG_RARE(cut >> r & 1) clear<S>(now);
                     const float2 s = sdt[r][lane];
                     const float dy = sdy[r][lane];
-                    const float4 Bv = *(const float4*)&sBC[0][r][4 * w], Cv = *(const float4*)&sBC[1][r][4 * w];
-                    const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
+                    float Bn[S], Cn[S];
+                    read_row<S>(&sBC[0][r][S * w], Bn);
+                    read_row<S>(&sBC[1][r][S * w], Cn);
                     float y = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
+                    for (int j = 0; j < S; j++) {
                         h[r][j] = now[j];
                         e[r][j] = exp2_hw(s.x * A2[j]);
-                        now[j] = __builtin_fmaf(e[r][j], now[j], s.y * B4[j]);
-                        y = __builtin_fmaf(C4[j], now[j], y);
-                        v[(r & 1) * 4 + j] = dy * now[j];
+                        now[j] = __builtin_fmaf(e[r][j], now[j], s.y * Bn[j]);
+                        y = __builtin_fmaf(Cn[j], now[j], y);
+                        v[r % kSteps * S + j] = dy * now[j];
                     }
                     sy[w][r][lane] = y;
-                    if (r & 1) {
+                    if (r % kSteps == kSteps - 1) {
                         const float x = sum_lanes8(v, lane);
-                        sums = mine == r >> 1 ? x : sums;
+                        sums = mine == r / kSteps ? x : sums;
                     }
                 }
-                if (!(lane & 4)) sdBC[1][2 * mine + odd][4 * w + (order & 3)] = sums;
+                if ((lane & 7) < S) sdBC[1][kSteps * mine + step][S * w + order % S] = sums;
 #pragma unroll
                 for (int r = kBack - 1; r >= 0; r--) {
                     const float2 s = sdt[r][lane];
                     const float dy = sdy[r][lane];
-                    const float4 Bv = *(const float4*)&sBC[0][r][4 * w], Cv = *(const float4*)&sBC[1][r][4 * w];
-                    const float B4[4] = {Bv.x, Bv.y, Bv.z, Bv.w}, C4[4] = {Cv.x, Cv.y, Cv.z, Cv.w};
+                    float Bn[S], Cn[S];
+                    read_row<S>(&sBC[0][r][S * w], Bn);
+                    read_row<S>(&sBC[1][r][S * w], Cn);
                     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float gr = __builtin_fmaf(C4[j], dy, carry[j]);
-                        v[(r & 1) * 4 + j] = gr * s.y;
-                        s1 = __builtin_fmaf(gr, B4[j], s1);
+                    for (int j = 0; j < S; j++) {
+                        const float gr = __builtin_fmaf(Cn[j], dy, carry[j]);
+                        v[r % kSteps * S + j] = gr * s.y;
+                        s1 = __builtin_fmaf(gr, Bn[j], s1);
                         carry[j] = e[r][j] * gr;
                         const float qq = carry[j] * h[r][j];
                         s2 = __builtin_fmaf(qq, A2[j], s2);
                         dA[j] = __builtin_fmaf(qq, s.x, dA[j]);
                     }
-                    AG_RARE(cut >> r & 1) zero4(carry);                 // h[r] is 0 there already
+                    AG_RARE(cut >> r & 1) clear<S>(carry);                 // h[r] is 0 there already
                     ss1[w][r][lane] = s1;
                     ss2[w][r][lane] = s2;
-                    if (!(r & 1)) {
+                    if (r % kSteps == 0) {
                         const float x = sum_lanes8(v, lane);
-                        sums = mine == r >> 1 ? x : sums;
+                        sums = mine == r / kSteps ? x : sums;
                     }
                 }
-                if (!(lane & 4)) sdBC[0][2 * mine + odd][4 * w + (order & 3)] = sums;
+                if ((lane & 7) < S) sdBC[0][kSteps * mine + step][S * w + order % S] = sums;
             }
             __syncthreads();
 #pragma unroll
@@ -571,7 +607,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
             __syncthreads();
             if (p.live) {
                 const long long row = ((long long)b * k2->chunks + p.chunk) * D + d;
-                store4(k2->chunk_h + row * N, w, N, carry);
+                store_states<S>(k2->chunk_h + row * N, w, N, carry);
                 if (w == 0) {
                     float s = 0.0f;
                     for (int v = 0; v < NG; v++) s += sums[v * kLanes + lane];
@@ -580,7 +616,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
             }
             __syncthreads();
         } else if (g2->ds0 && p.live && p.chunk == 0)
-            store4(g2->ds0 + (long long)b * D * N + state, w, N, carry);
+            store_states<S>(g2->ds0 + (long long)b * D * N + state, w, N, carry);
     }
     if (kCarry) return;
     // this workgroup's row of partial parameter gradients: [rows chunks, D, N + 2]
@@ -591,8 +627,8 @@ __global__ __launch_bounds__(kLanes* NG, kCarry || NG < 4 ? 1 : 3) void scan_bwd
     __syncthreads();
     if (!p.live) return;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (4 * w + j < N) part[4 * w + j] = dA[j];
+    for (int j = 0; j < S; j++)
+        if (S * w + j < N) part[S * w + j] = dA[j];
     if (w == 0) {
         float s = 0.0f, t = 0.0f;
 #pragma unroll
@@ -637,8 +673,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
         const unsigned b = min(first + i, (unsigned)a.B - 1);          // a thread without a sequence reads the last one's and writes nothing
         const T* Bm = (const T*)a.Bm + (b * a.bb + g * a.bg);
         const T* Cm = (const T*)a.Cm + (b * a.cb + g * a.cg);
-        zero4(h[i]);
-        if (a.s0) load4(a.s0 + ((long long)b * D + d) * a.N, part, a.N, h[i]);
+        clear<4>(h[i]);
+        if (a.s0) load_states<4>(a.s0 + ((long long)b * D + d) * a.N, part, a.N, h[i]);
         cut[i] = a.resets ? a.resets[b * a.rb] : 0;
         uu[i] = to_f32(((const T*)a.u)[b * a.ub + d]);
         raw[i] = to_f32(((const T*)a.delta)[b * a.db + d]);
@@ -650,11 +686,11 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
             Cn[i][j] = n < a.N ? to_f32(Cm[n]) : 0.0f;
         }
     }
-    load4(a.A + (long long)d * a.N, part, a.N, A);
+    load_states<4>(a.A + (long long)d * a.N, part, a.N, A);
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
 #pragma unroll
     for (int i = 0; i < R; i++) {
-        if (cut[i]) zero4(h[i]);
+        if (cut[i]) clear<4>(h[i]);
         const float dt = a.softplus ? softplus(raw[i] + bias) : raw[i] + bias;
         y[i] = 0.0f;
 #pragma unroll
@@ -670,14 +706,14 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     for (int i = 0; i < R; i++) {
         if (first + i >= (unsigned)a.B) break;
         const long long at = (long long)(first + i) * D + d;
-        store4(a.s1 + at * a.N, part, a.N, h[i]);
+        store_states<4>(a.s1 + at * a.N, part, a.N, h[i]);
         float o = __builtin_fmaf(skip, uu[i], y[i]);
         if (a.z) o *= zz[i] * sigmoid(zz[i]);
         if (part == 0) ((T*)a.out)[at] = from_f32<T>(o);
     }
 }
 
-int groups_of(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
+int step_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 int channel_blocks(int D, int G) { return (D / G + kLanes - 1) / kLanes; }
 
 // Chunks of time.  1536 workgroups are six per CU, what the forward's registers let in and two rounds of the backward; where sequences
@@ -732,14 +768,24 @@ long long chunk_floats(int B, int T, int D, int N, int G) {
 
 }  // namespace
 
-#define AG_FOR_STATES(N_, CALL)                                    \
-    do {                                                           \
-        switch (groups_of(N_)) {                                   \
-            case 1: { constexpr int NG = 1; CALL; } break;         \
-            case 2: { constexpr int NG = 2; CALL; } break;         \
-            case 4: { constexpr int NG = 4; CALL; } break;         \
-            default: { constexpr int NG = 8; CALL; } break;        \
-        }                                                          \
+// Four waves up to 16 states, eight beyond; 1, 2 or 4 states per lane.  (One or two waves of four states a lane for N <= 8 would have to
+// stage all rows themselves: 4096 x 24 x 256 f32, forward and backward, took 523 and 533 us at N = 8 and 4 against 601 at N = 16.)
+#define AG_FOR_STATES(N_, CALL)                                                  \
+    do {                                                                         \
+        if (N_ <= 4) { constexpr int NG = 4, S = 1; CALL; }                      \
+        else if (N_ <= 8) { constexpr int NG = 4, S = 2; CALL; }                 \
+        else if (N_ <= 16) { constexpr int NG = 4, S = 4; CALL; }                \
+        else { constexpr int NG = 8, S = 4; CALL; }                              \
+    } while (0)
+
+#define AG_FOR_LANES(N_, CALL)                                                   \
+    do {                                                                         \
+        switch (step_lanes(N_)) {                                                \
+            case 1: { constexpr int L = 1; CALL; } break;                        \
+            case 2: { constexpr int L = 2; CALL; } break;                        \
+            case 4: { constexpr int L = 4; CALL; } break;                        \
+            default: { constexpr int L = 8; CALL; } break;                       \
+        }                                                                        \
     } while (0)
 
 extern "C" long long ag_selective_scan_ckpt_floats(int B, int T, int D, int N) {
@@ -769,34 +815,34 @@ extern "C" int ag_selective_scan_fwd(const ag_scan_args* p, void* stream) {
     }
     const dim3 grid((unsigned)((long long)a.rows * a.chunks * a.G * a.nb));
     if (a.chunks > 1)
-        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, true>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
-    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
+        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, S, true>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
+    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_fwd_kernel<T, NG, S, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a)));
     return seq_status();
 }
 
-extern "C" int ag_selective_scan_bwd(const ag_scan_args* p, const ag_scan_grads* s, void* stream) {
+extern "C" int ag_selective_scan_bwd(const ag_scan_args* p, const ag_scan_grads* r, void* stream) {
     if (const int rc = check(p)) return rc;
-    if (!s || s->struct_size != sizeof(ag_scan_grads) || !s->dout_dev || !s->du_dev || !s->ddelta_dev || !s->dBm_dev || !s->dCm_dev ||
-        !s->dA_dev || !s->workspace_dev || (p->z_dev != nullptr) != (s->dz_dev != nullptr) || (p->T > kBack && !p->ckpt_dev))
+    if (!r || r->struct_size != sizeof(ag_scan_grads) || !r->dout_dev || !r->du_dev || !r->ddelta_dev || !r->dBm_dev || !r->dCm_dev ||
+        !r->dA_dev || !r->workspace_dev || (p->z_dev != nullptr) != (r->dz_dev != nullptr) || (p->T > kBack && !p->ckpt_dev))
         return AG_ERR_INVALID_ARG;
-    if (s->workspace_bytes < ag_selective_scan_workspace_bytes(p->B, p->T, p->D, p->N, p->G, 1)) return AG_ERR_INVALID_ARG;
-    if (s->dout_st > (0xffffffffLL / 4 - p->D) / kTile) return AG_ERR_UNSUPPORTED;
+    if (r->workspace_bytes < ag_selective_scan_workspace_bytes(p->B, p->T, p->D, p->N, p->G, 1)) return AG_ERR_INVALID_ARG;
+    if (r->dout_st > (0xffffffffLL / 4 - p->D) / kTile) return AG_ERR_UNSUPPORTED;
     ScanArgs a = device_args(p);
-    a.chunk_h = (float*)s->workspace_dev;
+    a.chunk_h = (float*)r->workspace_dev;
     a.chunk_dt = a.chunk_h + (long long)a.B * a.chunks * a.D * a.N;
     float* params = a.chunk_h + chunk_floats(a.B, a.T, a.D, a.N, a.G);
     const int rows = grad_rows(a.B, a.D, a.G);
     float* bc = a.nb > 1 ? params + (long long)rows * a.chunks * a.D * (a.N + 2) : nullptr;
-    const ScanGradArgs q{s->dout_dev, s->dout_sb, s->dout_st, s->dstate_out_dev, s->du_dev, s->ddelta_dev, s->dz_dev, s->dBm_dev, s->dCm_dev,
-                         s->dstate_in_dev, params, bc, rows};
+    const ScanGradArgs q{r->dout_dev, r->dout_sb, r->dout_st, r->dstate_out_dev, r->du_dev, r->ddelta_dev, r->dz_dev, r->dBm_dev, r->dCm_dev,
+                         r->dstate_in_dev, params, bc, rows};
     const dim3 grid((unsigned)((long long)rows * a.chunks * a.G * a.nb));
     if (a.chunks > 1)
-        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_bwd_kernel<T, NG, true>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a, q)));
-    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_bwd_kernel<T, NG, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a, q)));
-    launch_sum_rows(params, rows * a.chunks, (long long)a.D * (a.N + 2), ScanParams{s->dA_dev, s->dDskip_dev, s->ddelta_bias_dev, a.N}, stream);
+        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_bwd_kernel<T, NG, S, true>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a, q)));
+    AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_bwd_kernel<T, NG, S, false>), grid, dim3(kLanes * NG), 0, (hipStream_t)stream, a, q)));
+    launch_sum_rows(params, rows * a.chunks, (long long)a.D * (a.N + 2), ScanParams{r->dA_dev, r->dDskip_dev, r->ddelta_bias_dev, a.N}, stream);
     if (bc) {
         const long long n = (long long)a.B * a.T * a.G * a.N;
-        AG_FOR_DTYPE(p->dtype, launch_sum_rows(bc, a.nb, 2 * n, ScanShared<T>{(T*)s->dBm_dev, (T*)s->dCm_dev, n}, stream));
+        AG_FOR_DTYPE(p->dtype, launch_sum_rows(bc, a.nb, 2 * n, ScanShared<T>{(T*)r->dBm_dev, (T*)r->dCm_dev, n}, stream));
     }
     return seq_status();
 }
@@ -805,16 +851,16 @@ extern "C" int ag_selective_scan_step(const ag_scan_args* p, void* stream) {
     if (const int rc = check(p)) return rc;
     if (p->T != 1 || !p->out_dev || !p->state_out_dev) return AG_ERR_INVALID_ARG;
     const ScanArgs a = device_args(p);
-    const int lanes = groups_of(p->N);
+    const int lanes = step_lanes(p->N);
     if ((long long)a.B * a.D > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
     // two sequences per thread once that leaves 32 waves per CU
     const bool two = (long long)a.B * a.D * lanes / 128 >= 8192;
     const long long blocks = ((long long)(two ? (a.B + 1) / 2 : a.B) * a.D * lanes + 255) / 256;
     if (two)
-        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, NG, 2>), dim3((unsigned)blocks), dim3(256), 0,
+        AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, 2>), dim3((unsigned)blocks), dim3(256), 0,
                                                                       (hipStream_t)stream, a)));
     else
-        AG_FOR_DTYPE(p->dtype, AG_FOR_STATES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, NG, 1>), dim3((unsigned)blocks), dim3(256), 0,
+        AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, 1>), dim3((unsigned)blocks), dim3(256), 0,
                                                                       (hipStream_t)stream, a)));
     return seq_status();
 }
