@@ -66,14 +66,13 @@ __device__ __forceinline__ Place place_of(const ScanArgs& a) {
     return p;
 }
 
-// reset flags of nv steps from t0 as a wave-uniform bit mask
+// reset flags of nv steps from t0, one per lane (requested with the tile's other inputs, used a tile later)
 template <typename A>
-__device__ __forceinline__ unsigned reset_bits(A a, int b, int t0, int nv, int lane) {
-    const unsigned char* resets = a->resets;
-    if (!resets) return 0;
-    const bool f = lane < nv && resets[b * a->rb + (t0 + lane) * a->rt] != 0;
-    return __builtin_amdgcn_readfirstlane((unsigned)__ballot(f));
+__device__ __forceinline__ unsigned char reset_flag(A a, int b, int t0, int nv, int lane) {
+    return lane < nv ? a->resets[b * a->rb + (t0 + lane) * a->rt] : 0;
 }
+// ... and as a wave-uniform bit mask
+__device__ __forceinline__ unsigned reset_bits(unsigned char flag) { return __builtin_amdgcn_readfirstlane((unsigned)__ballot(flag != 0)); }
 
 // a branch that stays one: a select in its place would cost every step what only a reset needs
 #define AG_RARE(cond) if (__builtin_expect(cond, 0)) if (([]() __attribute__((always_inline)) { asm volatile(""); }(), true))
@@ -191,8 +190,10 @@ __global__ __launch_bounds__(kLanes* NG, 6) void scan_fwd_kernel(ScanArgs a) {
     const int brow = threadIdx.x / kWide, bn = threadIdx.x % kWide;
     const unsigned at = (unsigned)d * (unsigned)sizeof(T);
     const long long state = (long long)d * N;                          // of the lane's channel
+    const bool flagged = a.resets;
     Rows u, delta, z, Bm, Cm;
-    T ru[kRows], rd[kRows], rz[kRows], rB, rC;
+    T ru[kRows] = {}, rd[kRows] = {}, rz[kRows] = {}, rB, rC;
+    unsigned char rF = 0;
     auto sequence = [&](int b) __attribute__((always_inline)) {        // its first tile in this chunk
         const auto k = scan_args();
         u.set(k->u, b * k->ub + from * k->ut, k->ut, sizeof(T));
@@ -201,7 +202,9 @@ __global__ __launch_bounds__(kLanes* NG, 6) void scan_fwd_kernel(ScanArgs a) {
         Bm.set(k->Bm, b * k->bb + p.g * k->bg + from * k->bt, k->bt, sizeof(T));
         if (!kStates) Cm.set(k->Cm, b * k->cb + p.g * k->cg + from * k->ct, k->ct, sizeof(T));
     };
-    auto load = [&](int nv) __attribute__((always_inline)) {           // a tile's rows, as they are stored; then on to the next tile's
+    // a tile's rows, as they are stored; then on to the next tile's
+    auto load = [&](int b, int t0, int nv) __attribute__((always_inline)) {
+        if (flagged) rF = reset_flag(scan_args(), b, t0, min(nv, kTile), lane);
 #pragma unroll
         for (int k = 0; k < kRows; k++) {
             const int r = w + k * NG;
@@ -230,7 +233,7 @@ __global__ __launch_bounds__(kLanes* NG, 6) void scan_fwd_kernel(ScanArgs a) {
         float* ck = k1->ckpt + ((long long)b * ((T_ - 1) / kBack) + from / kBack - 1) * D * N + state;
         if (from < end && loaded != b) {
             sequence(b);
-            load(end - from);
+            load(b, from, end - from);
         }
         float h[S];
         clear<S>(h);
@@ -240,35 +243,36 @@ __global__ __launch_bounds__(kLanes* NG, 6) void scan_fwd_kernel(ScanArgs a) {
         }
         for (int t0 = from; t0 < end; t0 += kTile) {
             const int nv = min(kTile, end - t0);
-            float uu[kRows], zz[kRows];
+            float dt[kRows], uu[kRows], zz[kRows];
+#pragma unroll
+            for (int k = 0; k < kRows; k++) dt[k] = to_f32(rd[k]) + bias;
+            if (soft)
+#pragma unroll
+                for (int k = 0; k < kRows; k++) dt[k] = softplus(dt[k]);
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
                 const int r = w + k * NG;
-                float dt = 0.0f;
-                uu[k] = zz[k] = 0.0f;
-                if (r < nv) {
-                    uu[k] = to_f32(ru[k]);
-                    dt = to_f32(rd[k]) + bias;
-                    if (soft) dt = softplus(dt);
-                    if (gate) zz[k] = to_f32(rz[k]);
-                }
-                if (kStates) total += dt;
-                sdt[r][lane] = make_float2(dt, dt * uu[k]);
+                dt[k] = r < nv ? dt[k] : 0.0f;                          // (a row that was not loaded holds an older one)
+                uu[k] = r < nv ? to_f32(ru[k]) : 0.0f;
+                zz[k] = to_f32(rz[k]);
+                if (kStates) total += dt[k];
+                sdt[r][lane] = make_float2(dt[k], dt[k] * uu[k]);
             }
             if (S == 4 || brow < kTile) {
                 sB[brow][bn] = to_f32(rB);
                 if (!kStates) sC[brow][bn] = to_f32(rC);
             }
-            const unsigned cut = reset_bits(scan_args(), b, t0, nv, lane);
+            const unsigned cut = reset_bits(rF);
             any_cut |= cut != 0;
             __syncthreads();
-            int next = end - t0 - kTile;
+            int next = end - t0 - kTile, next_b = b, next_t = t0 + kTile;
             if (!kStates && next <= 0 && b + a.rows < a.B) {
-                loaded = b + a.rows;
-                sequence(loaded);
-                next = min(to, seq_len(scan_args()->lengths, loaded, T_)) - from;
+                loaded = next_b = b + a.rows;
+                next_t = from;
+                sequence(next_b);
+                next = min(to, seq_len(scan_args()->lengths, next_b, T_)) - from;
             }
-            if (next > 0) load(next);
+            if (next > 0) load(next_b, next_t, next);
 #pragma unroll
             for (int r = 0; r < kTile; r++) {                           // steps behind nv have dt = 0: they change nothing
                 if (r % 4 == 0 && r >= nv) break;
@@ -290,15 +294,20 @@ __global__ __launch_bounds__(kLanes* NG, 6) void scan_fwd_kernel(ScanArgs a) {
             }
             __syncthreads();
             if (!kStates) {
+                float y[kRows];
+#pragma unroll
+                for (int k = 0; k < kRows; k++) {
+                    y[k] = skip * uu[k];
+#pragma unroll
+                    for (int v = 0; v < NG; v++) y[k] += sy[v][w + k * NG][lane];      // (rows behind nv: whatever is there, not stored)
+                }
+                if (gate)
+#pragma unroll
+                    for (int k = 0; k < kRows; k++) y[k] *= zz[k] * sigmoid(zz[k]);
 #pragma unroll
                 for (int k = 0; k < kRows; k++) {
                     const int r = w + k * NG;
-                    if (r >= nv) break;
-                    float y = skip * uu[k];
-#pragma unroll
-                    for (int v = 0; v < NG; v++) y += sy[v][r][lane];
-                    if (gate) y *= zz[k] * sigmoid(zz[k]);
-                    if (p.live) put(out, r * (D * (unsigned)sizeof(T)) + at, from_f32<T>(y));
+                    if (r < nv && p.live) put(out, r * (D * (unsigned)sizeof(T)) + at, from_f32<T>(y[k]));
                 }
                 out += (long long)kTile * D * (long long)sizeof(T);
             }
@@ -390,8 +399,10 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
 #pragma unroll
     for (int j = 0; j < S; j++) A2[j] *= kLog2e;
 
+    const bool flagged = a.resets;
     Rows u, delta, z, dout, Bm, Cm;
-    T ru[kRows], rd[kRows], rz[kRows], rg[kRows], rB, rC;
+    T ru[kRows] = {}, rd[kRows] = {}, rz[kRows] = {}, rg[kRows] = {}, rB, rC;
+    unsigned char rF = 0;
     float start[S];
     auto sequence = [&](int b) __attribute__((always_inline)) {        // its last tile in this chunk
         const auto k = scan_args();
@@ -405,6 +416,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
     };
     // a tile's inputs as they are stored, and the state it starts from (nv <= 0: nothing); then on to the tile before
     auto load = [&](int b, int t0, int nv) __attribute__((always_inline)) {
+        if (flagged) rF = reset_flag(scan_args(), b, t0, min(nv, kBack), lane);
 #pragma unroll
         for (int k = 0; k < kRows; k++) {
             const int r = w + k * NG;
@@ -481,7 +493,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
                 if (!kCarry) sBC[0][brow][bn] = to_f32(rB);
                 sBC[1][brow][bn] = to_f32(rC);
             }
-            const unsigned cut = reset_bits(scan_args(), b, t0, nv, lane);
+            const unsigned cut = reset_bits(rF);
             any_cut |= cut != 0;
             __syncthreads();
             const bool same = t0 > from;
@@ -568,7 +580,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
                 }
                 float dy = go[k], dzv = 0.0f;
                 if (gate) {
-                    dzv = go[k] * y * (sz[k] * (1.0f + zz[k] * (1.0f - sz[k])));
+                    dzv = go[k] * y * (sz[k] * __builtin_fmaf(zz[k], 1.0f - sz[k], 1.0f));
                     dy *= zz[k] * sz[k];
                 }
                 const float draw = __builtin_fmaf(uu[k], s1, s2 * kLn2) * sg[k];      // s2 was summed with A log2(e)
@@ -679,12 +691,17 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
         uu[i] = to_f32(((const T*)a.u)[b * a.ub + d]);
         raw[i] = to_f32(((const T*)a.delta)[b * a.db + d]);
         zz[i] = a.z ? to_f32(((const T*)a.z)[b * a.zb + d]) : 0.0f;
+        if (a.N % 4 == 0 && 4 * part < a.N) {
+            const auto vB = load_vec<T, 4>(Bm + 4 * part), vC = load_vec<T, 4>(Cm + 4 * part);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int n = 4 * part + j;
-            Bn[i][j] = n < a.N ? to_f32(Bm[n]) : 0.0f;
-            Cn[i][j] = n < a.N ? to_f32(Cm[n]) : 0.0f;
-        }
+            for (int j = 0; j < 4; j++) Bn[i][j] = vB.at(j), Cn[i][j] = vC.at(j);
+        } else
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int n = 4 * part + j;
+                Bn[i][j] = n < a.N ? to_f32(Bm[n]) : 0.0f;
+                Cn[i][j] = n < a.N ? to_f32(Cm[n]) : 0.0f;
+            }
     }
     load_states<4>(a.A + (long long)d * a.N, part, a.N, A);
     const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
