@@ -40,7 +40,8 @@ __device__ __forceinline__ Sums join(Sums a, Sums b) {
 }
 
 template <typename T> __device__ __forceinline__ const T* row_of(const LossArgs& a, long long row) {
-    return (const T*)a.logits + (row / a.R1) * a.s0 + (row % a.R1) * a.s1;
+    const unsigned i = (unsigned)row / (unsigned)a.R1;         // R0 R1 < 2^31
+    return (const T*)a.logits + i * a.s0 + (row - (long long)i * a.R1) * a.s1;
 }
 
 // what a row's sums say: base and logarithm of the softmax, entropy, log-probability, and the two factors of its gradient
@@ -371,19 +372,40 @@ __global__ __launch_bounds__(256) void stats_kernel(const S* rows, long long n, 
 
 template <typename T>
 __global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const float* scale) {
+    constexpr int E = 16 / sizeof(T);
     const float g = scale[0];
     if (g == 1.0f) return;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) x[i] = from_f32<T>(to_f32(x[i]) * g);
+    const long long full = n / E, step = (long long)gridDim.x * 256, i0 = (long long)blockIdx.x * 256 + threadIdx.x;
+    for (long long i = i0; i < full; i += step) {
+        auto c = load_vec<T, E>(x + i * E);
+        float v[E];
+#pragma unroll
+        for (int k = 0; k < E; k++) v[k] = c.at(k) * g;
+        c.set(v);
+        store_vec<T, E>(x + i * E, c);
+    }
+    if (full * E + i0 < n) x[full * E + i0] = from_f32<T>(to_f32(x[full * E + i0]) * g);
 }
 
 }  // namespace
 
-// Which form takes a row of V logits.  Short rows (V <= 8 lanes' worth of a wave's 64) share a wave; beyond, a workgroup holds the
-// row: 256 threads while 8 accesses of 16 bytes per thread suffice, 1024 threads up to 16 of them, and what is longer is read twice.
+// Which form takes a row of V logits.  Up to 128 of them, 1 to 16 lanes share a wave with other rows; beyond, a workgroup holds the row
+// in accesses of 16 bytes: one wave up to 8 KB, 256 threads up to 32 KB, 1024 threads up to 256 KB; what is longer is read twice.
 static int short_lanes(int V) {
     int l = 1;
-    while (l * kPerLane < V) l *= 2;
+    while (l <= kShortLanes && l * kPerLane < V) l *= 2;
     return l;
+}
+
+// accesses of a row
+static long long accesses(int V, int size) { return ((long long)V * size + 15) / 16; }
+
+// V up to 2^30 (element indexes run a workgroup past the row's end) and all rows in one launch
+static bool launchable(long long R0, long long R1, int V, int dtype) {
+    if (V > 1 << 30 || R0 > 0x7fffffffLL / R1) return false;
+    const int lanes = short_lanes(V);
+    const long long q = accesses(V, dtype == AG_F32 ? 4 : 2), threads = lanes <= kShortLanes ? lanes : q <= 512 ? 64 : q <= 2048 ? 256 : 1024;
+    return R0 * R1 <= kMaxThreads / threads - kShortThreads;
 }
 
 template <typename T>
@@ -398,14 +420,12 @@ static long long launch_rows(const LossArgs& a, void* stream) {
             case 2: hipLaunchKernelGGL((token_loss_short_kernel<T, 2>), grid, block, 0, st, a); break;
             case 4: hipLaunchKernelGGL((token_loss_short_kernel<T, 4>), grid, block, 0, st, a); break;
             case 8: hipLaunchKernelGGL((token_loss_short_kernel<T, 8>), grid, block, 0, st, a); break;
-            case 16: hipLaunchKernelGGL((token_loss_short_kernel<T, 16>), grid, block, 0, st, a); break;
-            case 32: hipLaunchKernelGGL((token_loss_short_kernel<T, 32>), grid, block, 0, st, a); break;
-            default: hipLaunchKernelGGL((token_loss_short_kernel<T, 64>), grid, block, 0, st, a); break;
+            default: hipLaunchKernelGGL((token_loss_short_kernel<T, 16>), grid, block, 0, st, a); break;
         }
         return grid.x;
     }
     const dim3 grid((unsigned)a.R);
-    const int q = (int)(((long long)a.V * sizeof(T) + 15) / 16);       // accesses per row
+    const long long q = accesses(a.V, sizeof(T));
     if (q <= 64) hipLaunchKernelGGL((token_loss_kernel<T, 64, 1>), grid, dim3(64), 0, st, a);
     else if (q <= 128) hipLaunchKernelGGL((token_loss_kernel<T, 64, 2>), grid, dim3(64), 0, st, a);
     else if (q <= 256) hipLaunchKernelGGL((token_loss_kernel<T, 64, 4>), grid, dim3(64), 0, st, a);
@@ -437,7 +457,7 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     if (!p || p->struct_size != sizeof(ag_token_loss_args) || !p->logits_dev || !p->actions_dev || !p->old_logp_dev || !p->advantages_dev ||
         !p->loss_dev || !p->stats_dev || !p->workspace_dev || p->R0 <= 0 || p->R1 <= 0 || p->V <= 0)
         return AG_ERR_INVALID_ARG;
-    if (p->dtype < AG_F32 || p->dtype > AG_F16 || p->R0 > 0x7fffffffLL / p->R1) return AG_ERR_UNSUPPORTED;
+    if (p->dtype < AG_F32 || p->dtype > AG_F16 || !launchable(p->R0, p->R1, p->V, p->dtype)) return AG_ERR_UNSUPPORTED;
     const long long R = p->R0 * p->R1;
     if (p->workspace_bytes < ag_token_policy_loss_workspace_bytes(R, p->V)) return AG_ERR_INVALID_ARG;
     float* count = (float*)p->workspace_dev;                 // 4 floats, then the stages' sums, then the rows' terms
@@ -463,7 +483,7 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
 extern "C" int ag_token_logp(const void* logits, long long R0, long long R1, long long s0, long long s1, int V, int dtype,
                              const long long* actions, float* logp, float* entropy, void* stream) {
     if (!logits || !actions || !logp || R0 <= 0 || R1 <= 0 || V <= 0) return AG_ERR_INVALID_ARG;
-    if (dtype < AG_F32 || dtype > AG_F16 || R0 > 0x7fffffffLL / R1) return AG_ERR_UNSUPPORTED;
+    if (dtype < AG_F32 || dtype > AG_F16 || !launchable(R0, R1, V, dtype)) return AG_ERR_UNSUPPORTED;
     const LossArgs a{logits, actions, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, logp, entropy, R1, s0, s1, R0 * R1, V,
                      0.0f, 0.0f, 0.0f};
     AG_FOR_DTYPE(dtype, (void)launch_rows<T>(a, stream));
@@ -473,7 +493,7 @@ extern "C" int ag_token_logp(const void* logits, long long R0, long long R1, lon
 extern "C" int ag_scale_by(void* x, long long n, int dtype, const float* scale, void* stream) {
     if (!x || !scale || n <= 0) return AG_ERR_INVALID_ARG;
     if (dtype < AG_F32 || dtype > AG_F16) return AG_ERR_UNSUPPORTED;
-    const long long blocks = (n + 255) / 256;
+    const long long blocks = (n / 4 + 255) / 256 + 1;
     AG_FOR_DTYPE(dtype, hipLaunchKernelGGL((scale_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, (hipStream_t)stream,
                                            (T*)x, n, scale));
     return seq_status();

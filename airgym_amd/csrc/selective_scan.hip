@@ -4,11 +4,10 @@
 //   (per channel d a state of N numbers; B_t, C_t shared by the channels of a group; h := 0 before a step flagged as a reset)
 //
 // Layout.  A workgroup owns 64 consecutive channels of one group and walks along time in tiles; wave w owns S states of all 64 channels
-// (lane = channel): four waves of 1, 2 or 4 states up to N = 16, eight waves of 4 beyond.  What does not depend on the state index - softplus, the products dt u, the
-// gate - is formed once per (step, channel) by whichever wave stages that row and goes through LDS; per (step, channel, state) there
-// remain one multiply, one v_exp_f32, one multiply and two FMAs.  The sums over states (y, and in the backward the two sums behind du
-// and ddelta) are joined through LDS, in a fixed order.
-// The vector ALU bounds these kernels (v_exp_f32 takes four issue slots of the eight per state), the bytes come second.
+// (lane = channel): four waves of 1, 2 or 4 states up to N = 16, eight waves of 4 beyond.  What does not depend on the state index -
+// softplus, the products dt u, the gate - is formed once per (step, channel) by whichever wave stages that row and goes through LDS; per
+// (step, channel, state) there remain one multiply, one v_exp_f32, one multiply and two FMAs.  The sums over states (y, and in the
+// backward the two sums behind du and ddelta) are joined through LDS, in a fixed order.
 // Few rows.  When sequences and channels alone do not fill the chip, time is cut into chunks: a first pass finds what each chunk makes
 // of a zero state (backward: of a zero gradient) and the sum of its time steps - exp(A sum dt) is the chunk's decay -, the main pass
 // starts each chunk from those of the chunks before (behind) it.
@@ -735,8 +734,8 @@ int channel_blocks(int D, int G) { return (D / G + kLanes - 1) / kLanes; }
 
 // Chunks of time.  1536 workgroups are six per CU, what the forward's registers let in and two rounds of the backward; where sequences
 // and channels give fewer, time is cut so that there are about that many, in chunks of at least 64 steps (a multiple of 16).  Measured
-// at B = 8, T = 2047, D = 2048, bf16, ragged: 1024 workgroups 235 + 530 us (forward + backward), 1536 200 + 510, 3072 195 + 508; at B = 1,
-// T = 4096, D = 2048, where each chunk has more chunks before it to start from: 88, 100 and 98 us.
+// at B = 8, T = 2047, D = 2048, bf16, ragged: 1024 workgroups 235 + 530 us (forward + backward), 1536 200 + 510, twice as many 195 + 508;
+// at B = 1, T = 4096, D = 2048, where each chunk has more chunks before it to start from: 88, 100 and 98 us.
 struct Chunks { int count, steps; };
 Chunks chunks_of(int B, int T, int D, int G) {
     const long long blocks = (long long)B * G * channel_blocks(D, G);
@@ -760,11 +759,13 @@ int check(const ag_scan_args* p) {
         return AG_ERR_INVALID_ARG;
     if (p->B <= 0 || p->T <= 0 || p->D <= 0 || p->G <= 0 || p->N <= 0 || p->D % p->G) return AG_ERR_INVALID_ARG;
     if (p->N > 32 || p->dtype < AG_F32 || p->dtype > AG_F16) return AG_ERR_UNSUPPORTED;
+    if (p->u_st < 0 || p->delta_st < 0 || p->z_st < 0 || p->b_st < 0 || p->c_st < 0) return AG_ERR_INVALID_ARG;
     // a lane's offset within a tile's rows has 32 bits
     const long long most = (0xffffffffLL / 4 - p->D) / kTile;
     if (p->D > most || p->u_st > most || p->delta_st > most || p->z_st > most || p->b_st > most || p->c_st > most) return AG_ERR_UNSUPPORTED;
-    // the grid, with time in chunks: about 1536 or B G channel blocks (or one per sequence and 64 channels)
-    if ((long long)p->B * p->G * channel_blocks(p->D, p->G) > 0x7fffffffLL - 4096) return AG_ERR_UNSUPPORTED;
+    // the grid: rows_of or chunks_of make it some thousands of workgroups of up to 512 threads, but one per block of channels at least;
+    // with it G N (at most 32 G) times a tile's steps stays within 32 bits
+    if (p->T > kMaxSteps || (long long)p->G * channel_blocks(p->D, p->G) > 1 << 21) return AG_ERR_UNSUPPORTED;
     return AG_OK;
 }
 
@@ -843,6 +844,7 @@ extern "C" int ag_selective_scan_bwd(const ag_scan_args* p, const ag_scan_grads*
         !r->dA_dev || !r->workspace_dev || (p->z_dev != nullptr) != (r->dz_dev != nullptr) || (p->T > kBack && !p->ckpt_dev))
         return AG_ERR_INVALID_ARG;
     if (r->workspace_bytes < ag_selective_scan_workspace_bytes(p->B, p->T, p->D, p->N, p->G, 1)) return AG_ERR_INVALID_ARG;
+    if (r->dout_st < 0) return AG_ERR_INVALID_ARG;
     if (r->dout_st > (0xffffffffLL / 4 - p->D) / kTile) return AG_ERR_UNSUPPORTED;
     ScanArgs a = device_args(p);
     a.chunk_h = (float*)r->workspace_dev;
@@ -872,7 +874,8 @@ extern "C" int ag_selective_scan_step(const ag_scan_args* p, void* stream) {
     if ((long long)a.B * a.D > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
     // two sequences per thread once that leaves 32 waves per CU
     const bool two = (long long)a.B * a.D * lanes / 128 >= 8192;
-    const long long blocks = ((long long)(two ? (a.B + 1) / 2 : a.B) * a.D * lanes + 255) / 256;
+    const long long blocks = ((long long)(two ? (a.B + 1LL) / 2 : a.B) * a.D * lanes + 255) / 256;
+    if (blocks > kMaxThreads / 256) return AG_ERR_UNSUPPORTED;
     if (two)
         AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, 2>), dim3((unsigned)blocks), dim3(256), 0,
                                                                       (hipStream_t)stream, a)));

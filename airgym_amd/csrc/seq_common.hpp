@@ -10,6 +10,9 @@
 
 namespace {
 
+constexpr long long kMaxThreads = 0xffffffffLL;      // of one launch
+constexpr int kMaxSteps = 1 << 30;                   // of a sequence: step indexes run a little past its end
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -150,15 +153,15 @@ __global__ __launch_bounds__(64 * Parts) void sum_rows_kernel(const float* table
     out(i, s);
 }
 
-// ... and of a table of few rows: a column per thread
+// ... and of a table of few rows: a column per thread (several, where columns outnumber what a launch can hold)
 template <typename Out>
 __global__ __launch_bounds__(256) void sum_few_rows_kernel(const float* table, int rows, long long n, Out out) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float s = 0.0f;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+        float s = 0.0f;
 #pragma unroll 8
-    for (int r = 0; r < rows; r++) s += table[(long long)r * n + i];
-    out(i, s);
+        for (int r = 0; r < rows; r++) s += table[(long long)r * n + i];
+        out(i, s);
+    }
 }
 
 // At 256 columns x 1024 rows the split rows take 5 us where a column per thread took 236; at 3 M columns x 4 rows the plain form takes
@@ -166,7 +169,8 @@ __global__ __launch_bounds__(256) void sum_few_rows_kernel(const float* table, i
 template <typename Out>
 inline void launch_sum_rows(const float* table, int rows, long long n, Out out, void* stream) {
     if (rows <= 4 || n >= (1 << 18)) {
-        hipLaunchKernelGGL((sum_few_rows_kernel<Out>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, (hipStream_t)stream, table, rows, n, out);
+        const long long blocks = (n + 255) / 256, most = kMaxThreads / 256;
+        hipLaunchKernelGGL((sum_few_rows_kernel<Out>), dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, (hipStream_t)stream, table, rows, n, out);
         return;
     }
     const dim3 grid((unsigned)((n + 63) / 64));

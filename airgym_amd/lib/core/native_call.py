@@ -87,6 +87,16 @@ def in_place_state(name, t, shape, dtype, device):
     return t
 
 
+def moved_on(state):
+    """state was written by a kernel: autograd learns of it as of any in-place change (a graph that saved it refuses its backward)."""
+    if not state.is_inference():
+        torch.autograd.graph.increment_version(state)
+
+
+def wants_gradient(*tensors):
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+
+
 def no_gradient(what, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if wants_gradient(*tensors):
         raise ValueError(f"{what} has no backward pass: call it under torch.no_grad(), or the sequence form to train")

@@ -13,7 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from airgym_amd import _native as N
-from airgym_amd.lib.core.native_call import activation, flags_of, on_device_of, ptr, shape_error, stream_of
+from airgym_amd.lib.core.native_call import activation, flags_of, on_device_of, ptr, shape_error, stream_of, wants_gradient
 
 STATS = ("policy_loss", "kl", "entropy", "old_kl", "clip_frac", "rows")
 _ARGS = ctypes.sizeof(N.AgTokenLossArgs)
@@ -37,8 +37,8 @@ def _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, want_g
 
 class _TokenPolicyLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, coefs):
-        loss, stats, grad = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, ctx.needs_input_grad[0])
+    def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, coefs, train):
+        loss, stats, grad = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, train)
         ctx.save_for_backward(logits, actions, old_logp, advantages, ref_logp, mask)
         ctx.coefs, ctx.grad = coefs, grad
         ctx.mark_non_differentiable(stats)
@@ -49,7 +49,7 @@ class _TokenPolicyLoss(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dloss, _):
         if dloss is None:
-            return None, None, None, None, None, None, None
+            return (None,) * 8
         saved = ctx.saved_tensors
         # the gradient is handed over, not kept: autograd may go on to add to it in place.  A second pass over a retained graph forms
         # it again.
@@ -59,7 +59,7 @@ class _TokenPolicyLoss(torch.autograd.Function):
         with on_device_of(grad):
             N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], dloss.data_ptr(), stream_of(grad)),
                     "ag_scale_by")
-        return grad, None, None, None, None, None, None
+        return (grad,) + (None,) * 7
 
 
 def _rows(logits, actions):
@@ -106,7 +106,8 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logp=None, mask=No
         raise ValueError(f"e_clip: {e_clip}")
     if logits.numel() == 0:
         return logits.sum().float(), torch.zeros(6, device=dev)
-    return _TokenPolicyLoss.apply(logits, actions, old_logp, advantages, ref_logp, mask, (float(e_clip), float(kl_coef), float(entropy_coef)))
+    return _TokenPolicyLoss.apply(logits, actions, old_logp, advantages, ref_logp, mask, (float(e_clip), float(kl_coef), float(entropy_coef)),
+                                  wants_gradient(logits))
 
 
 def action_logp(logits, actions):

@@ -10,8 +10,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from airgym_amd import _native as N
-from airgym_amd.lib.core.native_call import (activation as first_activation, flags_of, in_place_state, lengths_of, no_gradient, on_device_of,
-                                             parameter, ptr, same_kind, shape_error, stream_of)
+from airgym_amd.lib.core.native_call import (activation as first_activation, flags_of, in_place_state, lengths_of, moved_on, no_gradient,
+                                             on_device_of, parameter, ptr, same_kind, shape_error, stream_of)
 
 MAX_TAPS = 8
 
@@ -116,6 +116,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", resets=N
     with on_device_of(x):
         N.check(N.load().ag_causal_conv_step(x.data_ptr(), x.stride(0), state.data_ptr(), weight.data_ptr(), ptr(bias), ptr(resets),
                                              y.data_ptr(), N.AG_DTYPES[x.dtype], B, D, W, silu, stream_of(x)), "ag_causal_conv_step")
+    moved_on(state)
     return y
 
 

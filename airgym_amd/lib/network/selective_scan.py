@@ -12,8 +12,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from airgym_amd import _native as N
-from airgym_amd.lib.core.native_call import (activation, flags_of, in_place_state, lengths_of, no_gradient, on_device_of, parameter, ptr,
-                                             same_kind, shape_error, stream_of)
+from airgym_amd.lib.core.native_call import (activation, flags_of, in_place_state, lengths_of, moved_on, no_gradient, on_device_of, parameter,
+                                             ptr, same_kind, shape_error, stream_of, wants_gradient)
 
 MAX_STATES = 32
 _ARGS, _GRADS = ctypes.sizeof(N.AgScanArgs), ctypes.sizeof(N.AgScanGrads)
@@ -29,20 +29,25 @@ def _fill(u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus):
                         *u.stride()[:2], *delta.stride()[:2], z_sb, z_st, *B.stride()[:3], *C.stride()[:3], r_sb, r_st)
 
 
+def _near_rows(t):
+    """t with its steps less than 2^25 elements apart: a tile's rows are addressed with 32 bits."""
+    return t if t is None or t.stride(1) < 1 << 25 else t.contiguous()
+
+
 def _workspace(n, device):
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 class _SelectiveScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus, want_state):
+    def forward(ctx, u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus, want_state, train):
         lib = N.load()
         b, T, d = u.shape
         n = A.shape[1]
         out = torch.empty(b, T, d, dtype=u.dtype, device=u.device)
         last = torch.empty(b, d, n, dtype=torch.float32, device=u.device) if want_state else None
         ckpt = None
-        if any(ctx.needs_input_grad):
+        if train:
             ckpt = torch.empty(lib.ag_selective_scan_ckpt_floats(b, T, d, n), dtype=torch.float32, device=u.device)
         bytes_ = lib.ag_selective_scan_workspace_bytes(b, T, d, n, B.shape[2], 0)
         ws = _workspace(bytes_, u.device)
@@ -64,7 +69,7 @@ class _SelectiveScan(torch.autograd.Function):
         b, T, d = u.shape
         n, G = A.shape[1], B.shape[2]
 
-        dout = torch.zeros(b, T, d, dtype=u.dtype, device=u.device) if dout is None else same_kind("dout", dout, u.shape, u)
+        dout = torch.zeros(b, T, d, dtype=u.dtype, device=u.device) if dout is None else _near_rows(same_kind("dout", dout, u.shape, u))
         dlast = None if dlast is None else dlast.contiguous()
         du, ddelta, dz, dB, dC = u.new_empty(u.shape), u.new_empty(u.shape), None if z is None else u.new_empty(u.shape), \
             u.new_empty(B.shape), u.new_empty(B.shape)
@@ -79,7 +84,7 @@ class _SelectiveScan(torch.autograd.Function):
                           ptr(ws), bytes_)
         with on_device_of(u):
             N.check(lib.ag_selective_scan_bwd(ctypes.byref(a), ctypes.byref(g), stream_of(u)), "ag_selective_scan_bwd")
-        return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate, None, None, None, None
+        return du, ddelta, dA, dB, dC, dD, dz, dbias, dstate, None, None, None, None, None
 
 
 def _parameters(A, D, delta_bias, d, device):
@@ -122,7 +127,9 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_
         out = u.clone()
         last = torch.zeros(b, d, A.shape[1], dtype=torch.float32, device=u.device) if state is None else state.clone()
     else:
-        out, last = _SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, state, lengths, resets, int(bool(delta_softplus)), return_state)
+        u, delta, z, B, C = (_near_rows(t) for t in (u, delta, z, B, C))
+        out, last = _SelectiveScan.apply(u, delta, A, B, C, D, z, delta_bias, state, lengths, resets, int(bool(delta_softplus)), return_state,
+                                         wants_gradient(u, delta, A, B, C, D, z, delta_bias, state))
     return (out, last) if return_state else out
 
 
@@ -155,6 +162,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
                      0 if resets is None else resets.stride(0), 0, out.data_ptr(), at)
     with on_device_of(u):
         N.check(N.load().ag_selective_scan_step(ctypes.byref(a), stream_of(u)), "ag_selective_scan_step")
+    moved_on(state)
     return out
 
 

@@ -800,7 +800,11 @@ int ag_planning_last_step_rendered(ag_handle h);
  * [B, T, ...] with element strides for batch and time (the channel stride is 1), so a [T, B, ...] rollout buffer is read where it
  * lies.  lengths_dev int32 [B] (or NULL = T everywhere; clamped to [0, T]): steps from there on are not read, their outputs and
  * gradients are zero and they leave the state alone.  resets_dev u8 [B, T] (or NULL): a non-zero flag clears the state BEFORE that
- * step (an episode ended there).  B, T >= 1; all pointers are device pointers on the current device. */
+ * step (an episode ended there).  B, T >= 1; all pointers are device pointers on the current device.  Apart from the step forms' state
+ * no output may overlap an input (state_out is not state_in).
+ * Refused as AG_ERR_UNSUPPORTED: T above 2^30; a scan whose time strides reach 2^26 - D / 16 elements or whose channels make more than
+ * 2^21 blocks of 64; rows of more than 2^30 logits; launches of more than 2^32 threads (one per 16 steps and channel group in the
+ * convolution, per channel and sequence in the step forms, 1 to 1024 per row of logits). */
 typedef enum ag_dtype { AG_F32 = 0, AG_BF16 = 1, AG_F16 = 2 } ag_dtype;
 
 /* Causal depthwise convolution of W taps, 2 <= W <= 8:

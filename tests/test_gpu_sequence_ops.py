@@ -123,7 +123,7 @@ def test_causal_conv_reads_time_major_buffers_and_flags_where_they_lie():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("B,D,W", [(1, 1, 2), (3, 5, 8), (130, 65, 4), (7, 256, 3)])
+@pytest.mark.parametrize("B,D,W", [(1, 1, 2), (3, 5, 8), (130, 65, 4), (7, 256, 3), (1030, 256, 4), (2049, 132, 8)])
 def test_causal_conv_steps_are_the_sequence(B, D, W, dtype):
     """The step form does the sequence form's arithmetic: same order of the same operations, so the same bits."""
     from airgym_amd.lib.network.causal_conv import causal_conv, causal_conv_step
@@ -454,6 +454,33 @@ def test_rows_further_apart_than_32_bits():
     assert torch.equal(torch.autograd.grad(a, far, dy)[0], torch.autograd.grad(b, near, dy)[0])
     logits, actions = x[:, 0], torch.tensor([3, 40], device="cuda")
     assert torch.equal(action_logp(_far(logits, gap), actions)[0], action_logp(logits, actions)[0])
+
+
+def test_steps_further_apart_than_a_tile_addresses():
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    g, gap = gen(10), 2 ** 26
+    big = torch.empty(2 * gap + 64, dtype=torch.bfloat16, device="cuda")
+    far = big.as_strided((1, 3, 48), (3 * gap, gap, 1))
+    far.copy_(torch.randn(1, 3, 48, generator=g))
+    A, bc = -torch.rand(48, 16, generator=g).cuda(), torch.randn(1, 3, 16, generator=g).to(torch.bfloat16).cuda()
+    assert torch.equal(selective_scan(far, far, A, bc, bc), selective_scan(far.contiguous(), far.contiguous(), A, bc, bc))
+
+
+def test_a_state_that_a_graph_saved_and_a_step_moved_on_is_noticed():
+    from airgym_amd.lib.network.causal_conv import causal_conv, causal_conv_step
+    from airgym_amd.lib.network.selective_scan import selective_scan, selective_scan_step
+    x, w, s = torch.randn(2, 5, 8).cuda(), torch.randn(8, 4).cuda().requires_grad_(), torch.randn(2, 3, 8).cuda()
+    y = causal_conv(x, w, initial_state=s)
+    with torch.no_grad():
+        causal_conv_step(x[:, 0], s, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    A, bc, h = -torch.rand(8, 16).cuda().requires_grad_(), torch.randn(2, 5, 16).cuda(), torch.randn(2, 8, 16).cuda()
+    y = selective_scan(x, x, A, bc, bc, initial_state=h)
+    with torch.no_grad():
+        selective_scan_step(x[:, 0], x[:, 0], A, bc[:, 0], bc[:, 0], h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
 
 
 def test_the_same_inputs_give_the_same_bits():

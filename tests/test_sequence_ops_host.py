@@ -32,7 +32,7 @@ def test_conv_entries_refuse(lib):
     N, p, a, _, _ = _blocks()
     fwd = lambda: lib.ag_causal_conv_fwd(ctypes.byref(a), None)      # noqa: E731
     for field, value, rc in [("struct_size", 4, -1), ("x_dev", None, -1), ("weight_dev", None, -1), ("y_dev", None, -1), ("B", 0, -1), ("T", 0, -1),
-                             ("D", -1, -1), ("W", 1, -6), ("W", 9, -6), ("dtype", 3, -6), ("dtype", -1, -6)]:
+                             ("D", -1, -1), ("T", (1 << 30) + 1, -6), ("W", 1, -6), ("W", 9, -6), ("dtype", 3, -6), ("dtype", -1, -6)]:
         old = getattr(a, field)
         setattr(a, field, value)
         assert fwd() == rc, field
@@ -48,7 +48,7 @@ def test_conv_entries_refuse(lib):
 def test_scan_entries_refuse(lib):
     N, p, _, a, _ = _blocks()
     for field, value, rc in [("struct_size", 4, -1), ("u_dev", None, -1), ("delta_dev", None, -1), ("Bm_dev", None, -1), ("A_dev", None, -1),
-                             ("out_dev", None, -1), ("B", 0, -1), ("T", 0, -1), ("G", 3, -1), ("G", 0, -1), ("N", 33, -6), ("N", 0, -1), ("dtype", 7, -6)]:
+                             ("out_dev", None, -1), ("B", 0, -1), ("T", 0, -1), ("T", (1 << 30) + 1, -6), ("u_st", -1, -1), ("b_st", 1 << 26, -6), ("D", 1 << 28, -6), ("G", 3, -1), ("G", 0, -1), ("N", 33, -6), ("N", 0, -1), ("dtype", 7, -6)]:
         old = getattr(a, field)
         setattr(a, field, value)
         assert lib.ag_selective_scan_fwd(ctypes.byref(a), None) == rc, field
@@ -66,13 +66,17 @@ def test_scan_entries_refuse(lib):
 def test_loss_entries_refuse(lib):
     N, p, _, _, a = _blocks()
     for field, value, rc in [("struct_size", 4, -1), ("logits_dev", None, -1), ("actions_dev", None, -1), ("old_logp_dev", None, -1),
-                             ("stats_dev", None, -1), ("loss_dev", None, -1), ("workspace_dev", None, -1), ("workspace_bytes", 4, -1), ("V", 0, -1), ("R0", 0, -1),
+                             ("stats_dev", None, -1), ("loss_dev", None, -1), ("workspace_dev", None, -1), ("workspace_bytes", 4, -1), ("V", 0, -1), ("V", 2147483647, -6), ("R0", 0, -1),
                              ("dtype", 5, -6), ("R0", 1 << 31, -6)]:
         old = getattr(a, field)
         setattr(a, field, value)
         assert lib.ag_token_policy_loss(ctypes.byref(a), None) == rc, field
         setattr(a, field, old)
     assert lib.ag_token_logp(p, 1, 3, 27, 9, 9, 0, None, p, p, None) == -1 and lib.ag_token_logp(p, 1, 3, 27, 9, 9, 4, p, p, p, None) == -6
+    # 64 threads per row of 129 to 2048 float32 logits, 1024 beyond 8192: more than one launch holds
+    assert lib.ag_token_logp(p, 1 << 26, 1, 200, 200, 200, 0, p, p, p, None) == -6
+    assert lib.ag_token_logp(p, 1 << 22, 1, 9000, 9000, 9000, 0, p, p, p, None) == -6
+    assert lib.ag_token_policy_loss_workspace_bytes(3, 2147483647) > 0
     assert lib.ag_scale_by(p, 0, 0, p, None) == -1 and lib.ag_scale_by(p, 4, 9, p, None) == -6
 
 
