@@ -20,7 +20,7 @@ constexpr int kSums = 5;               // policy loss, KL term, entropy, KL of t
 struct LossArgs {
     const void* logits; const long long* actions; const float *old_logp, *adv, *ref_logp; const unsigned char* mask;
     void* dlogits; const float* count; // {max(rows that count, 1), rows that count}, or NULL: all R
-    float* partials;                   // [workgroups, kSums] sums of the rows' terms
+    float4* rows;                      // [R] what the statistics need of a row: its action's logit, the base, the two sums
     float *logp, *entropy;             // the log-probability form: these instead
     long long R1, s0, s1, R;
     int V;
@@ -69,18 +69,6 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, bool inf, f
     return r;
 }
 
-// the row's share of the statistics (one lane needs it)
-__device__ __forceinline__ void row_terms(const LossArgs& a, const Row& r, long long row, float* term) {
-    const float adv = a.adv[row], moved = r.lp - a.old_logp[row], ratio = expf(moved);
-    const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
-    term[0] = plain != plain ? plain : fmaxf(plain, held);
-    const float d = a.ref_logp ? a.ref_logp[row] - r.lp : 0.0f;
-    term[1] = expm1f(d) - d;
-    term[2] = r.H;
-    term[3] = expm1f(moved) - moved;
-    term[4] = ratio < 1.0f - a.e_clip || ratio > 1.0f + a.e_clip ? 1.0f : 0.0f;
-}
-
 // f (delta - p) + ent p (log p + H) without the delta, from d = x - base
 __device__ __forceinline__ float grad_of(const Row& r, float d) {
     if (r.inf) d = fmaxf(d, kFloor);
@@ -101,11 +89,10 @@ constexpr int kShortThreads = 256, kPerLane = 8, kShortLanes = 16;
 template <typename T, int L>
 __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArgs a) {
     constexpr int kRows = kShortThreads / L;
-    __shared__ float part[kShortThreads / 64][kSums];
     const int l = threadIdx.x % L;
     const long long row = (long long)blockIdx.x * kRows + threadIdx.x / L;
     const bool there = row < a.R, on = there && !(a.mask && !a.mask[row]);
-    float x[kPerLane], xa = __builtin_nanf(""), t[kSums] = {0, 0, 0, 0, 0};
+    float x[kPerLane], xa = __builtin_nanf("");
     Row r;
     int act = -1;
     if (on) {
@@ -140,9 +127,8 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
                 a.logp[row] = r.lp;
                 if (a.entropy) a.entropy[row] = r.H;
             }
-        } else if (l == 0) row_terms(a, r, row, t);
+        } else if (l == 0) a.rows[row] = float4{xa, base, v.s, v.t};
     }
-    if (a.logp) return;
     if (a.dlogits && there) {
         T* dx = (T*)a.dlogits + row * a.V;
 #pragma unroll
@@ -154,19 +140,6 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
                 dx[j] = from_f32<T>(g);
             }
         }
-    }
-#pragma unroll
-    for (int k = 0; k < kSums; k++) {
-#pragma unroll
-        for (int o = 32; o; o >>= 1) t[k] += __shfl_xor(t[k], o);
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6][k] = t[k];
-    }
-    __syncthreads();
-    if (threadIdx.x < kSums) {
-        float s = part[0][threadIdx.x];
-#pragma unroll
-        for (int i = 1; i < kShortThreads / 64; i++) s += part[i][threadIdx.x];
-        a.partials[(long long)blockIdx.x * kSums + threadIdx.x] = s;
     }
 }
 
@@ -189,7 +162,6 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
             for (int q = threadIdx.x; q < full; q += THREADS) store_vec(dx + q * E, zero);
             if (tail < a.V) dx[tail] = from_f32<T>(0.0f);
         }
-        if (threadIdx.x < kSums) a.partials[row * kSums + threadIdx.x] = 0.0f;
         return;
     }
     const long long av = a.actions[row];
@@ -275,7 +247,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
         }
         return;
     }
-    if (threadIdx.x == 0) row_terms(a, r, row, a.partials + row * kSums);
+    if (threadIdx.x == 0) a.rows[row] = float4{xa, r.base, v.s, v.t};
     if (!dx) return;
     const int aq = act >= 0 ? act / E : -1, ai = act % E;
     auto gradient = [&](int q, const Vec<T, E>& held) __attribute__((always_inline)) {
@@ -325,17 +297,32 @@ __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, 
     }
 }
 
-// The rows' terms summed in a fixed order, in double: kStatsRows of them per workgroup, then those sums by one workgroup (which, for
-// few rows, takes the terms themselves).  One workgroup over 65 536 rows took 45 us, the two stages take 7.
-constexpr int kStatsRows = 2048;
+// The loss and its statistics: the rows' terms formed and summed in double, in an order that R alone fixes.  The terms cancel - the
+// advantages have both signs -, so that float32's last bits of a log-probability of -10 would be the loss's fifth digit.  A row per
+// thread: three double functions a row are work for all lanes here, and would stall a workgroup per row up there.
+constexpr int kStatsThreads = 256, kStatsBlocks = 1024, kOneStage = 512, kOneStageRows = 1024;
 
-template <typename S>
-__device__ __forceinline__ void sum_rows(const S* rows, long long n, double* s, double (*part)[kSums]) {
-#pragma unroll
-    for (int k = 0; k < kSums; k++) s[k] = 0.0;
-    for (long long i = threadIdx.x; i < n; i += 256)
-#pragma unroll
-        for (int k = 0; k < kSums; k++) s[k] += (double)rows[i * kSums + k];
+__device__ __forceinline__ void add_row(const LossArgs& a, long long row, double* s) {
+    if (a.mask && !a.mask[row]) return;
+    const float4 v = a.rows[row];
+    // the sums' exponentials are those of (x - m) (1 + tilt), log2(e) being a float there: log S is off by tilt times the mean x - m
+    constexpr double tilt = (double)kLog2e / 1.4426950408889634074 - 1.0;
+    const double mean = (double)v.w / v.z, logS = log((double)v.z) - tilt * mean, lp = ((double)v.x - v.y) - logS, adv = a.adv[row], moved = lp - a.old_logp[row], up = expm1(moved);
+    const double ratio = 1.0 + up, low = 1.0 - (double)a.e_clip, high = 1.0 + (double)a.e_clip;
+    const double held = -adv * fmin(fmax(ratio, low), high), plain = -adv * ratio;
+    s[0] += plain != plain ? plain : fmax(plain, held);
+    if (a.ref_logp) {
+        const double d = a.ref_logp[row] - lp;
+        s[1] += expm1(d) - d;
+    }
+    s[2] += logS - mean;
+    s[3] += up - moved;
+    s[4] += ratio < low || ratio > high ? 1.0 : 0.0;
+}
+
+template <int THREADS>
+__device__ __forceinline__ void sum_block(double* s) {
+    __shared__ double part[THREADS / 64][kSums];
 #pragma unroll
     for (int k = 0; k < kSums; k++) {
         for (int o = 32; o; o >>= 1) s[k] += __shfl_xor(s[k], o);
@@ -343,30 +330,37 @@ __device__ __forceinline__ void sum_rows(const S* rows, long long n, double* s, 
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < kSums; k++) s[k] = ((part[0][k] + part[1][k]) + part[2][k]) + part[3][k];
+    for (int k = 0; k < kSums; k++) {
+        s[k] = part[0][k];
+#pragma unroll
+        for (int i = 1; i < THREADS / 64; i++) s[k] += part[i][k];
+    }
 }
 
-__global__ __launch_bounds__(256) void stats_part_kernel(const float* rows, long long n, double* out) {
-    __shared__ double part[4][kSums];
-    double s[kSums];
-    const long long first = (long long)blockIdx.x * kStatsRows;
-    sum_rows(rows + first * kSums, min((long long)kStatsRows, n - first), s, part);
+__global__ __launch_bounds__(kStatsThreads) void stats_part_kernel(LossArgs a, double* out) {
+    double s[kSums] = {0, 0, 0, 0, 0};
+    for (long long i = (long long)blockIdx.x * kStatsThreads + threadIdx.x; i < a.R; i += (long long)gridDim.x * kStatsThreads) add_row(a, i, s);
+    sum_block<kStatsThreads>(s);
     if (threadIdx.x == 0)
 #pragma unroll
-        for (int k = 0; k < kSums; k++) out[(long long)blockIdx.x * kSums + k] = s[k];
+        for (int k = 0; k < kSums; k++) out[blockIdx.x * kSums + k] = s[k];
 }
 
-template <typename S>
-__global__ __launch_bounds__(256) void stats_kernel(const S* rows, long long n, const float* count, long long R, float kl_coef, float ent_coef, float* loss,
-                                                    float* stats) {
-    __shared__ double part[4][kSums];
-    double s[kSums];
-    sum_rows(rows, n, s, part);
+// parts: the first stage's sums of `blocks` workgroups; NULL (few rows): the rows themselves
+__global__ __launch_bounds__(kOneStage) void stats_kernel(LossArgs a, const double* parts, int blocks, float* loss, float* stats) {
+    double s[kSums] = {0, 0, 0, 0, 0};
+    if (parts) {
+        for (int i = threadIdx.x; i < blocks; i += kOneStage)
+#pragma unroll
+            for (int k = 0; k < kSums; k++) s[k] += parts[i * kSums + k];
+    } else
+        for (long long i = threadIdx.x; i < a.R; i += kOneStage) add_row(a, i, s);
+    sum_block<kOneStage>(s);
     if (threadIdx.x == 0) {
 #pragma unroll
-        for (int k = 0; k < kSums; k++) s[k] /= count ? (double)count[0] : (double)R, stats[k] = (float)s[k];
-        loss[0] = (float)(s[0] + (double)kl_coef * s[1] - (double)ent_coef * s[2]);
-        stats[kSums] = count ? count[1] : (float)R;
+        for (int k = 0; k < kSums; k++) s[k] /= a.count ? (double)a.count[0] : (double)a.R, stats[k] = (float)s[k];
+        loss[0] = (float)(s[0] + (double)a.kl_coef * s[1] - (double)a.entropy_coef * s[2]);
+        stats[kSums] = a.count ? a.count[1] : (float)a.R;
     }
 }
 
@@ -409,7 +403,7 @@ static bool launchable(long long R0, long long R1, int V, int dtype) {
 }
 
 template <typename T>
-static long long launch_rows(const LossArgs& a, void* stream) {
+static void launch_rows(const LossArgs& a, void* stream) {
     const hipStream_t st = (hipStream_t)stream;
     const int lanes = short_lanes(a.V);
     if (lanes <= kShortLanes) {
@@ -422,7 +416,7 @@ static long long launch_rows(const LossArgs& a, void* stream) {
             case 8: hipLaunchKernelGGL((token_loss_short_kernel<T, 8>), grid, block, 0, st, a); break;
             default: hipLaunchKernelGGL((token_loss_short_kernel<T, 16>), grid, block, 0, st, a); break;
         }
-        return grid.x;
+        return;
     }
     const dim3 grid((unsigned)a.R);
     const long long q = accesses(a.V, sizeof(T));
@@ -436,21 +430,17 @@ static long long launch_rows(const LossArgs& a, void* stream) {
     else if (q <= 8192) hipLaunchKernelGGL((token_loss_kernel<T, 1024, 8>), grid, dim3(1024), 0, st, a);
     else if (q <= 16384) hipLaunchKernelGGL((token_loss_kernel<T, 1024, 16>), grid, dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((token_loss_kernel<T, 1024, 0>), grid, dim3(1024), 0, st, a);
-    return a.R;
 }
 
-static long long partial_rows(long long R, int V) {
-    const int lanes = short_lanes(V);
-    return lanes <= kShortLanes ? (R * lanes + kShortThreads - 1) / kShortThreads : R;
+// workgroups of the statistics' first stage; 0: one stage
+static int stats_blocks(long long R) {
+    const long long blocks = (R + kStatsThreads - 1) / kStatsThreads;
+    return R <= kOneStageRows ? 0 : (int)(blocks < kStatsBlocks ? blocks : kStatsBlocks);
 }
-
-// workgroups of the first stage of the statistics; 0: one stage
-static long long stats_blocks(long long rows) { return rows > kStatsRows ? (rows + kStatsRows - 1) / kStatsRows : 0; }
 
 extern "C" long long ag_token_policy_loss_workspace_bytes(long long R, int V) {
     if (R <= 0 || V <= 0) return 0;
-    const long long rows = partial_rows(R, V);
-    return 16 + stats_blocks(rows) * kSums * (long long)sizeof(double) + rows * kSums * (long long)sizeof(float);
+    return 16 + R * (long long)sizeof(float4) + stats_blocks(R) * kSums * (long long)sizeof(double);
 }
 
 extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
@@ -460,23 +450,17 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     if (p->dtype < AG_F32 || p->dtype > AG_F16 || !launchable(p->R0, p->R1, p->V, p->dtype)) return AG_ERR_UNSUPPORTED;
     const long long R = p->R0 * p->R1;
     if (p->workspace_bytes < ag_token_policy_loss_workspace_bytes(R, p->V)) return AG_ERR_INVALID_ARG;
-    float* count = (float*)p->workspace_dev;                 // 4 floats, then the stages' sums, then the rows' terms
-    const long long blocks = stats_blocks(partial_rows(R, p->V));
-    double* sums = (double*)(count + 4);
+    float* count = (float*)p->workspace_dev;                 // 4 floats, then the rows' sums, then the first stage's
+    float4* rows = (float4*)(count + 4);
+    const int blocks = stats_blocks(R);
+    double* parts = blocks ? (double*)(rows + R) : nullptr;
     const LossArgs a{p->logits_dev, p->actions_dev, p->old_logp_dev, p->advantages_dev, p->ref_logp_dev, p->mask_dev, p->dlogits_dev,
-                     p->mask_dev ? count : nullptr,
-                     (float*)(sums + blocks * kSums), nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef, p->entropy_coef};
+                     p->mask_dev ? count : nullptr, rows, nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef,
+                     p->entropy_coef};
     if (a.count) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p->mask_dev, R, count);
-    long long rows = 0;
-    AG_FOR_DTYPE(p->dtype, rows = launch_rows<T>(a, stream));
-    const float kl = p->ref_logp_dev ? p->kl_coef : 0.0f;
-    if (blocks) {
-        hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a.partials, rows, sums);
-        hipLaunchKernelGGL((stats_kernel<double>), dim3(1), dim3(256), 0, (hipStream_t)stream, sums, blocks, a.count, R, kl, p->entropy_coef, p->loss_dev,
-                           p->stats_dev);
-    } else
-        hipLaunchKernelGGL((stats_kernel<float>), dim3(1), dim3(256), 0, (hipStream_t)stream, a.partials, rows, a.count, R, kl, p->entropy_coef, p->loss_dev,
-                           p->stats_dev);
+    AG_FOR_DTYPE(p->dtype, launch_rows<T>(a, stream));
+    if (blocks) hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(kStatsThreads), 0, (hipStream_t)stream, a, parts);
+    hipLaunchKernelGGL(stats_kernel, dim3(1), dim3(kOneStage), 0, (hipStream_t)stream, a, parts, blocks, p->loss_dev, p->stats_dev);
     return seq_status();
 }
 
@@ -486,7 +470,7 @@ extern "C" int ag_token_logp(const void* logits, long long R0, long long R1, lon
     if (dtype < AG_F32 || dtype > AG_F16 || !launchable(R0, R1, V, dtype)) return AG_ERR_UNSUPPORTED;
     const LossArgs a{logits, actions, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, logp, entropy, R1, s0, s1, R0 * R1, V,
                      0.0f, 0.0f, 0.0f};
-    AG_FOR_DTYPE(dtype, (void)launch_rows<T>(a, stream));
+    AG_FOR_DTYPE(dtype, launch_rows<T>(a, stream));
     return seq_status();
 }
 
