@@ -21,14 +21,14 @@ _ARGS = ctypes.sizeof(N.AgTokenLossArgs)
 
 def _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, want_grad):
     lib = N.load()
-    r0, r1, v = logits.shape
     dev = logits.device
     loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(6, dtype=torch.float32, device=dev)
-    grad = torch.empty((r0, r1, v), dtype=logits.dtype, device=dev) if want_grad else None
+    grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
+    logits, r0, r1, v, s0, s1 = _table(logits)
     n = lib.ag_token_policy_loss_workspace_bytes(r0 * r1, v)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    a = N.AgTokenLossArgs(_ARGS, N.AG_DTYPES[logits.dtype], v, r0, r1, logits.stride(0), logits.stride(1), logits.data_ptr(),
-                          actions.data_ptr(), old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(mask), *coefs, loss.data_ptr(),
+    a = N.AgTokenLossArgs(_ARGS, N.AG_DTYPES[logits.dtype], v, r0, r1, s0, s1, logits.data_ptr(), actions.data_ptr(),
+                          old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(mask), *coefs, loss.data_ptr(),
                           stats.data_ptr(), ptr(grad), ws.data_ptr(), n)
     with on_device_of(logits):
         N.check(lib.ag_token_policy_loss(ctypes.byref(a), stream_of(logits)), "ag_token_policy_loss")
@@ -50,12 +50,11 @@ class _TokenPolicyLoss(torch.autograd.Function):
     def backward(ctx, dloss, _):
         if dloss is None:
             return (None,) * 8
-        saved = ctx.saved_tensors
         # the gradient is handed over, not kept: autograd may go on to add to it in place.  A second pass over a retained graph forms
         # it again.
         grad, ctx.grad = ctx.grad, None
         if grad is None:
-            grad = _launch(*saved, ctx.coefs, True)[2]
+            grad = _launch(*ctx.saved_tensors, ctx.coefs, True)[2]
         with on_device_of(grad):
             N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], dloss.data_ptr(), stream_of(grad)),
                     "ag_scale_by")
@@ -63,18 +62,24 @@ class _TokenPolicyLoss(torch.autograd.Function):
 
 
 def _rows(logits, actions):
-    """logits as [R0, R1, V] (a view where their strides allow), the leading shape and the actions as dense int64."""
+    """logits with dense rows, their leading shape and the actions as dense int64."""
     if not isinstance(logits, torch.Tensor) or logits.dim() < 2 or logits.shape[-1] < 1:
         raise shape_error("logits", logits, "[..., V]")
     lead = logits.shape[:-1]
     logits = activation("logits", logits, logits.shape)
     if not isinstance(actions, torch.Tensor) or actions.dtype != torch.int64 or actions.shape != lead or actions.device != logits.device:
         raise shape_error("actions", actions, f"int64 {list(lead)} on {logits.device}")
-    if len(lead) == 1:
-        logits = logits.unsqueeze(0)
-    elif len(lead) > 2:
-        logits = logits.reshape(-1, lead[-1], logits.shape[-1])
     return logits, lead, actions.contiguous()
+
+
+def _table(logits):
+    """logits [..., V] as R0 x R1 rows: a tensor that holds them, R0, R1, V and the two strides."""
+    if logits.dim() == 2:
+        (r, v), (s, _) = logits.shape, logits.stride()
+        return logits, 1, r, v, 0, s
+    if logits.dim() > 3:
+        logits = logits.reshape(-1, *logits.shape[-2:])
+    return logits, *logits.shape, *logits.stride()[:2]
 
 
 def _per_row(name, t, lead, device):
@@ -119,8 +124,8 @@ def action_logp(logits, actions):
     logp = torch.empty(lead, dtype=torch.float32, device=logits.device)
     entropy = torch.empty_like(logp)
     if logits.numel():
-        r0, r1, v = logits.shape
+        logits, r0, r1, v, s0, s1 = _table(logits)
         with on_device_of(logits):
-            N.check(N.load().ag_token_logp(logits.data_ptr(), r0, r1, logits.stride(0), logits.stride(1), v, N.AG_DTYPES[logits.dtype],
-                                           actions.data_ptr(), logp.data_ptr(), entropy.data_ptr(), stream_of(logits)), "ag_token_logp")
+            N.check(N.load().ag_token_logp(logits.data_ptr(), r0, r1, s0, s1, v, N.AG_DTYPES[logits.dtype], actions.data_ptr(),
+                                           logp.data_ptr(), entropy.data_ptr(), stream_of(logits)), "ag_token_logp")
     return logp, entropy

@@ -19,14 +19,21 @@ MAX_STATES = 32
 _ARGS, _GRADS = ctypes.sizeof(N.AgScanArgs), ctypes.sizeof(N.AgScanGrads)
 
 
+def _groups(t, lead=2):
+    """Groups of a B or C ([..., G, N], or [..., N]: one) and its leading and group strides."""
+    return (t.shape[lead], t.stride()[:lead + 1]) if t.dim() == lead + 2 else (1, (*t.stride()[:lead], 0))
+
+
 def _fill(u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus):
     """The argument block of sequences [B, T, ...]."""
     b, T, d = u.shape
     z_sb, z_st = (0, 0) if z is None else z.stride()[:2]
     r_sb, r_st = (0, 0) if resets is None else resets.stride()
-    return N.AgScanArgs(_ARGS, N.AG_DTYPES[u.dtype], b, T, d, A.shape[1], B.shape[2], softplus, u.data_ptr(), delta.data_ptr(), ptr(z),
+    G, b_strides = _groups(B)
+    _, c_strides = _groups(C)
+    return N.AgScanArgs(_ARGS, N.AG_DTYPES[u.dtype], b, T, d, A.shape[1], G, softplus, u.data_ptr(), delta.data_ptr(), ptr(z),
                         B.data_ptr(), C.data_ptr(), A.data_ptr(), ptr(D), ptr(bias), ptr(state), ptr(lengths), ptr(resets),
-                        *u.stride()[:2], *delta.stride()[:2], z_sb, z_st, *B.stride()[:3], *C.stride()[:3], r_sb, r_st)
+                        *u.stride()[:2], *delta.stride()[:2], z_sb, z_st, *b_strides, *c_strides, r_sb, r_st)
 
 
 def _near_rows(t):
@@ -49,7 +56,7 @@ class _SelectiveScan(torch.autograd.Function):
         ckpt = None
         if train:
             ckpt = torch.empty(lib.ag_selective_scan_ckpt_floats(b, T, d, n), dtype=torch.float32, device=u.device)
-        bytes_ = lib.ag_selective_scan_workspace_bytes(b, T, d, n, B.shape[2], 0)
+        bytes_ = lib.ag_selective_scan_workspace_bytes(b, T, d, n, _groups(B)[0], 0)
         ws = _workspace(bytes_, u.device)
         a = _fill(u, delta, A, B, C, D, z, bias, state, lengths, resets, softplus)
         a.out_dev, a.state_out_dev, a.workspace_dev, a.workspace_bytes = out.data_ptr(), ptr(last), ptr(ws), bytes_
@@ -67,12 +74,12 @@ class _SelectiveScan(torch.autograd.Function):
         u, delta, A, B, C, D, z, bias, state, lengths, resets, ckpt = ctx.saved_tensors
         lib = N.load()
         b, T, d = u.shape
-        n, G = A.shape[1], B.shape[2]
+        n, G = A.shape[1], _groups(B)[0]
 
         dout = torch.zeros(b, T, d, dtype=u.dtype, device=u.device) if dout is None else _near_rows(same_kind("dout", dout, u.shape, u))
         dlast = None if dlast is None else dlast.contiguous()
         du, ddelta, dz, dB, dC = u.new_empty(u.shape), u.new_empty(u.shape), None if z is None else u.new_empty(u.shape), \
-            u.new_empty(B.shape), u.new_empty(B.shape)
+            u.new_empty(B.shape), u.new_empty(C.shape)
         dA, dD, dbias = torch.empty_like(A), None if D is None else torch.empty_like(D), None if bias is None else torch.empty_like(bias)
         dstate = torch.empty_like(state) if ctx.needs_input_grad[8] else None
         bytes_ = lib.ag_selective_scan_workspace_bytes(b, T, d, n, G, 1)
@@ -94,11 +101,11 @@ def _parameters(A, D, delta_bias, d, device):
 
 
 def _shared(name, t, lead, n, u):
-    """B or C as [..., G, N]; [..., N] is one group."""
+    """B or C, [..., G, N] or [..., N]: one group."""
     if not isinstance(t, torch.Tensor) or t.dim() not in (len(lead) + 1, len(lead) + 2):
         raise shape_error(name, t, f"{[*lead, 'G', n]} or {[*lead, n]}")
     if t.dim() == len(lead) + 1:
-        t = t.unsqueeze(-2)
+        return same_kind(name, t, (*lead, n), u)
     groups = t.shape[-2]
     if groups < 1 or u.shape[-1] % groups:
         raise ValueError(f"{name}: {u.shape[-1]} channels do not split into {groups} groups")
@@ -119,7 +126,7 @@ def selective_scan(u, delta, A, B, C, D=None, z=None, delta_bias=None, *, delta_
     z = None if z is None else same_kind("z", z, u.shape, u)
     A, D, delta_bias = _parameters(A, D, delta_bias, d, u.device)
     B, C = _shared("B", B, (b, T), A.shape[1], u), _shared("C", C, (b, T), A.shape[1], u)
-    if B.shape != C.shape:
+    if _groups(B)[0] != _groups(C)[0]:
         raise ValueError(f"B and C: {list(B.shape)} and {list(C.shape)}")
     state = parameter("initial_state", initial_state, (b, d, A.shape[1]), u.device)
     lengths, resets = lengths_of(lengths, b, u.device), flags_of("resets", resets, (b, T), u.device)
@@ -147,16 +154,16 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
     A, D, delta_bias = _parameters(A, D, delta_bias, d, device)
     n = A.shape[1]
     B, C = _shared("B", B, (b,), n, u), _shared("C", C, (b,), n, u)
-    if B.shape != C.shape:
+    (groups, (b_sb, b_sg)), (c_groups, (c_sb, c_sg)) = _groups(B, 1), _groups(C, 1)
+    if groups != c_groups:
         raise ValueError(f"B and C: {list(B.shape)} and {list(C.shape)}")
     state = in_place_state("state", state, (b, d, n), torch.float32, device)
     resets = flags_of("resets", resets, (b,), device)
     out = torch.empty((b, d), dtype=u.dtype, device=device)
     if u.numel() == 0:
         return out
-    (b_sb, b_sg, _), (c_sb, c_sg, _) = B.stride(), C.stride()
     at = state.data_ptr()
-    a = N.AgScanArgs(_ARGS, N.AG_DTYPES[u.dtype], b, 1, d, n, B.shape[1], int(bool(delta_softplus)), u.data_ptr(), delta.data_ptr(), ptr(z),
+    a = N.AgScanArgs(_ARGS, N.AG_DTYPES[u.dtype], b, 1, d, n, groups, int(bool(delta_softplus)), u.data_ptr(), delta.data_ptr(), ptr(z),
                      B.data_ptr(), C.data_ptr(), A.data_ptr(), ptr(D), ptr(delta_bias), at, None, ptr(resets), u.stride(0), 0,
                      delta.stride(0), 0, 0 if z is None else z.stride(0), 0, b_sb, 0, b_sg, c_sb, 0, c_sg,
                      0 if resets is None else resets.stride(0), 0, out.data_ptr(), at)

@@ -456,6 +456,43 @@ def test_rows_further_apart_than_32_bits():
     assert torch.equal(action_logp(_far(logits, gap), actions)[0], action_logp(logits, actions)[0])
 
 
+def test_one_group_with_and_without_its_dimension():
+    from airgym_amd.lib.network.selective_scan import selective_scan, selective_scan_step
+    g = gen(12)
+    u, A = torch.randn(3, 21, 40, generator=g).cuda(), -torch.rand(40, 16, generator=g).cuda()
+    B, C, dy = (torch.randn(3, 21, n, generator=g).cuda() for n in (16, 16, 40))
+    got = []
+    for wide in ((False, False), (True, False), (False, True), (True, True)):
+        b, c = (t.clone().requires_grad_() for t in (B, C))
+        y = selective_scan(u, u, A, *(t.unsqueeze(2) if w else t for t, w in zip((b, c), wide)))
+        got.append((y.detach(), *torch.autograd.grad(y, (b, c), dy)))
+        state = torch.zeros(3, 40, 16, device="cuda")
+        step = [selective_scan_step(u[:, 0], u[:, 0], A, *(t[:, 0].unsqueeze(1) if w else t[:, 0] for t, w in zip((B, C), wide)), state)]
+        got[-1] += (step[0], state)
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+    with pytest.raises(ValueError, match="B and C"):
+        selective_scan(u, u, A, B, C.unsqueeze(2).expand(-1, -1, 2, -1))
+
+
+def test_loss_over_any_leading_shape_and_after_its_inputs_moved_on():
+    from airgym_amd.lib.core.policy_loss import action_logp, policy_loss
+    g = gen(13)
+    x = torch.randn(2, 3, 4, 7, generator=g).cuda()
+    actions = torch.randint(0, 7, (2, 3, 4), generator=g).cuda()
+    old, adv = (torch.randn(2, 3, 4, generator=g).cuda() * 0.1 for _ in range(2))
+    got = []
+    for lead in ((24,), (6, 4), (2, 3, 4), (2, 1, 3, 4)):
+        leaf = x.view(*lead, 7).clone().requires_grad_()
+        rest = [t.view(lead).clone() for t in (actions, old, adv)]
+        loss, stats = policy_loss(leaf, *rest, entropy_coef=0.1)
+        rest[1].add_(1.0)                   # the gradient is that of the numbers the loss saw
+        (dx,) = torch.autograd.grad(loss, leaf)
+        got.append((loss.detach(), stats, dx.reshape(24, 7), action_logp(leaf.detach(), rest[0])[0].flatten()))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
 def test_steps_further_apart_than_a_tile_addresses():
     from airgym_amd.lib.network.selective_scan import selective_scan
     g, gap = gen(10), 2 ** 26
