@@ -108,11 +108,25 @@ template <typename T> __device__ __forceinline__ void put(char* base, unsigned b
 // a lane's S states (the w-th S of a row of N), zero where there are none: one access where the row is whole
 typedef float two_any4 __attribute__((ext_vector_type(2), aligned(4)));
 typedef float four_any4 __attribute__((ext_vector_type(4), aligned(4)));
-template <int S> __device__ __forceinline__ void load_states(const float* row, int w, int N, float* x) {
+// x[j] = c[j + by], zero beyond
+__device__ __forceinline__ void shift_down(const float* c, int by, float* x) {
+    x[0] = by == 0 ? c[0] : by == 1 ? c[1] : by == 2 ? c[2] : by == 3 ? c[3] : 0.0f;
+    x[1] = by == 0 ? c[1] : by == 1 ? c[2] : by == 2 ? c[3] : 0.0f;
+    x[2] = by == 0 ? c[2] : by == 1 ? c[3] : 0.0f;
+    x[3] = by == 0 ? c[3] : 0.0f;
+}
+template <int S, bool kOnce = false, bool kTail = false> __device__ __forceinline__ void load_states(const float* row, int w, int N, float* x) {
     if (S == 4 && N % 4 == 0 && 4 * w < N) {
-        const four_any4 v = *(const four_any4*)(row + 4 * w);
+        const four_any4* at = (const four_any4*)(row + 4 * w);
+        const four_any4 v = kOnce ? __builtin_nontemporal_load(at) : *at;
 #pragma unroll
         for (int j = 0; j < S; j++) x[j] = v[j];
+    } else if (kTail) {                                                 // N > 4: the last lane of the row takes its last four, and what it needs of them
+        const int first = min(4 * w, N - 4);
+        const four_any4* at = (const four_any4*)(row + first);
+        const four_any4 v = kOnce ? __builtin_nontemporal_load(at) : *at;
+        const float c[4] = {v[0], v[1], v[2], v[3]};
+        shift_down(c, 4 * w - first, x);
     } else if (S == 2 && N % 2 == 0 && 2 * w < N) {
         const two_any4 v = *(const two_any4*)(row + 2 * w);
 #pragma unroll
@@ -121,12 +135,14 @@ template <int S> __device__ __forceinline__ void load_states(const float* row, i
 #pragma unroll
         for (int j = 0; j < S; j++) x[j] = S * w + j < N ? row[S * w + j] : 0.0f;
 }
-template <int S> __device__ __forceinline__ void store_states(float* row, int w, int N, const float* x) {
-    if (S == 4 && N % 4 == 0 && 4 * w < N) {
+template <int S, bool kOnce = false> __device__ __forceinline__ void store_states(float* row, int w, int N, const float* x) {
+    if (S == 4 && 4 * w + 4 <= N) {
         four_any4 v;
 #pragma unroll
         for (int j = 0; j < S; j++) v[j] = x[j];
-        *(four_any4*)(row + 4 * w) = v;
+        four_any4* at = (four_any4*)(row + 4 * w);
+        if (kOnce) __builtin_nontemporal_store(v, at);
+        else *at = v;
     } else if (S == 2 && N % 2 == 0 && 2 * w < N) {
         two_any4 v;
 #pragma unroll
@@ -671,62 +687,78 @@ template <typename T> struct ScanShared {
 };
 
 // One step: a channel's state is spread over L lanes, four numbers each, so that a wave moves 1 KB of states per access; the states
-// in and out are nearly all of the bytes.  A thread takes R sequences, all of their loads first.
-template <typename T, int L, int R>
+// in and out are nearly all of the bytes, each touched once.
+// kShared: a wave takes up to 64 channels of one sequence and group.  Each lane then also owns one of the channels and forms its time
+// step and its gate, the L rounds over the states fetch them from there, B and C are read once for all of them, and L accesses per lane
+// are in flight.  Otherwise a wave's 64 / L channels lie anywhere.  kTail: N is above 4 and no multiple of it.
+// Bytes bound it: 4096 x 512, N = 16, float32 takes 52 us = 5.8 TB/s, bfloat16 52 us = 5.4 TB/s (an in-place product over the states
+// alone 48 us).  The states are marked as used once: with plain accesses the float32 step took 59 us, without sharing 61.
+template <typename T, int L, bool kShared, bool kTail>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
-    const unsigned item = (unsigned)(((unsigned long long)blockIdx.x * 256 + threadIdx.x) / L), D = a.D;      // B D < 2^31
-    const int part = threadIdx.x % L;
-    const unsigned first = item / D * R, d = item % D, g = a.G > 1 ? d / (unsigned)a.Dg : 0;
-    float h[R][4], A[4], uu[R], raw[R], zz[R], Bn[R][4], Cn[R][4], y[R];
-    unsigned char cut[R];
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        const unsigned b = min(first + i, (unsigned)a.B - 1);          // a thread without a sequence reads the last one's and writes nothing
-        const T* Bm = (const T*)a.Bm + (b * a.bb + g * a.bg);
-        const T* Cm = (const T*)a.Cm + (b * a.cb + g * a.cg);
-        clear<4>(h[i]);
-        if (a.s0) load_states<4>(a.s0 + ((long long)b * D + d) * a.N, part, a.N, h[i]);
-        cut[i] = a.resets ? a.resets[b * a.rb] : 0;
-        uu[i] = to_f32(((const T*)a.u)[b * a.ub + d]);
-        raw[i] = to_f32(((const T*)a.delta)[b * a.db + d]);
-        zz[i] = a.z ? to_f32(((const T*)a.z)[b * a.zb + d]) : 0.0f;
-        if (a.N % 4 == 0 && 4 * part < a.N) {
-            const auto vB = load_vec<T, 4>(Bm + 4 * part), vC = load_vec<T, 4>(Cm + 4 * part);
-#pragma unroll
-            for (int j = 0; j < 4; j++) Bn[i][j] = vB.at(j), Cn[i][j] = vC.at(j);
-        } else
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int n = 4 * part + j;
-                Bn[i][j] = n < a.N ? to_f32(Bm[n]) : 0.0f;
-                Cn[i][j] = n < a.N ? to_f32(Cm[n]) : 0.0f;
-            }
+    constexpr int kRounds = kShared ? L : 1, C = 64 / L;                  // channels of a wave per round
+    const int l = threadIdx.x & 63, part = l % L, mine = kShared ? l / L : 0;        // the lane's channel behind c0 in round 0
+    const unsigned wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), D = a.D;
+    unsigned b, c0, d, g, end;                                            // B D < 2^31
+    if (kShared) {
+        const unsigned per = (unsigned)a.nb * (unsigned)a.G, in = wave % per;
+        b = wave / per, g = in / (unsigned)a.nb;
+        c0 = g * (unsigned)a.Dg + in % (unsigned)a.nb * 64, end = (g + 1) * (unsigned)a.Dg, d = min(c0 + l, end - 1);
+    } else {
+        const unsigned item = wave * C + l / L;
+        b = item / D, d = c0 = item % D, end = D, g = a.G > 1 ? d / (unsigned)a.Dg : 0;
     }
-    load_states<4>(a.A + (long long)d * a.N, part, a.N, A);
-    const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
+    if (b >= (unsigned)a.B) return;
+    const long long row = (long long)b * D + c0;
+    float h[kRounds][4], A[kRounds][4], Bn[4], Cn[4];
 #pragma unroll
-    for (int i = 0; i < R; i++) {
-        if (cut[i]) clear<4>(h[i]);
-        const float dt = a.softplus ? softplus(raw[i] + bias) : raw[i] + bias;
-        y[i] = 0.0f;
+    for (int i = 0; i < kRounds; i++) {
+        clear<4>(h[i]);
+        if (a.s0 && c0 + i * C + mine < end) load_states<4, true, kTail>(a.s0 + (row + i * C + mine) * a.N, part, a.N, h[i]);
+    }
+    const T* Bm = (const T*)a.Bm + (b * a.bb + g * a.bg);
+    const T* Cm = (const T*)a.Cm + (b * a.cb + g * a.cg);
+    const bool cut = a.resets && a.resets[b * a.rb];
+    const float u = to_f32(((const T*)a.u)[b * a.ub + d]), raw = to_f32(((const T*)a.delta)[b * a.db + d]);
+    const float z = a.z ? to_f32(((const T*)a.z)[b * a.zb + d]) : 0.0f;
+    clear<4>(Bn), clear<4>(Cn);
+    if (kTail || a.N % 4 == 0) {
+        const int from = min(4 * part, a.N - 4);
+        const auto vB = load_vec<T, 4>(Bm + from), vC = load_vec<T, 4>(Cm + from);
+        const float cB[4] = {vB.at(0), vB.at(1), vB.at(2), vB.at(3)}, cC[4] = {vC.at(0), vC.at(1), vC.at(2), vC.at(3)};
+        if (kTail) shift_down(cB, 4 * part - from, Bn), shift_down(cC, 4 * part - from, Cn);
+        else if (4 * part < a.N)
+#pragma unroll
+            for (int j = 0; j < 4; j++) Bn[j] = cB[j], Cn[j] = cC[j];
+    } else
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (4 * part + j < a.N) Bn[j] = to_f32(Bm[4 * part + j]), Cn[j] = to_f32(Cm[4 * part + j]);
+#pragma unroll
+    for (int i = 0; i < kRounds; i++) load_states<4, false, kTail>(a.A + (long long)min(c0 + i * C + mine, end - 1) * a.N, part, a.N, A[i]);
+    const float bias = a.bias ? a.bias[d] : 0.0f, skip = a.Dskip ? a.Dskip[d] : 0.0f;
+    const float dt = a.softplus ? softplus(raw + bias) : raw + bias, dtu = dt * u;
+    float y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRounds; i++) {
+        const bool fetch = kShared && L > 1;
+        const float t = fetch ? __shfl(dt, i * C + mine) : dt, tu = fetch ? __shfl(dtu, i * C + mine) : dtu;
+        float p = 0.0f;
+        if (cut) clear<4>(h[i]);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            h[i][j] = __builtin_fmaf(exp2_hw(dt * (A[j] * kLog2e)), h[i][j], dt * uu[i] * Bn[i][j]);
-            y[i] = __builtin_fmaf(Cn[i][j], h[i][j], y[i]);
+            h[i][j] = __builtin_fmaf(exp2_hw(t * (A[i][j] * kLog2e)), h[i][j], tu * Bn[j]);
+            p = __builtin_fmaf(Cn[j], h[i][j], p);
         }
-        if (L > 1) y[i] += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y[i]), 0xB1, 0xf, 0xf, true));
-        if (L > 2) y[i] += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y[i]), 0x4E, 0xf, 0xf, true));
-        if (L > 4) y[i] += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(y[i]), 0x141, 0xf, 0xf, true));
+        if (c0 + i * C + mine < end) store_states<4, true>(a.s1 + (row + i * C + mine) * a.N, part, a.N, h[i]);
+        if (L > 1) p += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(p), 0xB1, 0xf, 0xf, true));
+        if (L > 2) p += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(p), 0x4E, 0xf, 0xf, true));
+        if (L > 4) p += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(p), 0x141, 0xf, 0xf, true));
+        const float q = fetch ? __shfl(p, l % C * L) : p;                 // a round's channels are its lanes L, 2 L, ...
+        y = !kShared || l / C == i ? q : y;
     }
-#pragma unroll
-    for (int i = 0; i < R; i++) {
-        if (first + i >= (unsigned)a.B) break;
-        const long long at = (long long)(first + i) * D + d;
-        store_states<4>(a.s1 + at * a.N, part, a.N, h[i]);
-        float o = __builtin_fmaf(skip, uu[i], y[i]);
-        if (a.z) o *= zz[i] * sigmoid(zz[i]);
-        if (part == 0) ((T*)a.out)[at] = from_f32<T>(o);
-    }
+    float o = __builtin_fmaf(skip, u, y);
+    if (a.z) o *= z * sigmoid(z);
+    if (kShared ? c0 + l < end : part == 0) ((T*)a.out)[(long long)b * D + d] = from_f32<T>(o);
 }
 
 int step_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
@@ -872,15 +904,16 @@ extern "C" int ag_selective_scan_step(const ag_scan_args* p, void* stream) {
     const ScanArgs a = device_args(p);
     const int lanes = step_lanes(p->N);
     if ((long long)a.B * a.D > 0x7fffffffLL) return AG_ERR_UNSUPPORTED;
-    // two sequences per thread once that leaves 32 waves per CU
-    const bool two = (long long)a.B * a.D * lanes / 128 >= 8192;
-    const long long blocks = ((long long)(two ? (a.B + 1LL) / 2 : a.B) * a.D * lanes + 255) / 256;
+    // where the channels of a group fill the lanes of its waves to four fifths and more (4096 x 512 in 16 groups of 32 channels: 69 us
+    // not shared; 4096 x 500: 53 us shared, 69 us not)
+    const bool shared = a.nb * 64LL * 4 <= a.Dg * 5LL, tail = a.N > 4 && a.N % 4;
+    const long long waves = shared ? (long long)a.B * a.G * a.nb : ((long long)a.B * a.D * lanes + 63) / 64, blocks = (waves + 3) / 4;
     if (blocks > kMaxThreads / 256) return AG_ERR_UNSUPPORTED;
-    if (two)
-        AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, 2>), dim3((unsigned)blocks), dim3(256), 0,
-                                                                      (hipStream_t)stream, a)));
-    else
-        AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, 1>), dim3((unsigned)blocks), dim3(256), 0,
-                                                                      (hipStream_t)stream, a)));
+    const dim3 grid((unsigned)blocks), block(256);
+    const hipStream_t st = (hipStream_t)stream;
+    if (shared && tail) AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, true, (L > 1)>), grid, block, 0, st, a)));
+    else if (shared) AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, true, false>), grid, block, 0, st, a)));
+    else if (tail) AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, false, (L > 1)>), grid, block, 0, st, a)));
+    else AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, false, false>), grid, block, 0, st, a)));
     return seq_status();
 }

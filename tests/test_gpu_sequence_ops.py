@@ -261,7 +261,10 @@ def test_a_reset_clears_a_state_that_is_not_finite():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("B,D,N,G", [(1, 1, 1, 1), (3, 6, 3, 2), (5, 130, 16, 1), (2, 64, 8, 1), (3, 33, 32, 1), (2, 48, 13, 3), (7, 37500, 16, 1)])
+@pytest.mark.parametrize("B,D,N,G", [(1, 1, 1, 1), (3, 6, 3, 2), (5, 130, 16, 1), (2, 64, 8, 1), (3, 33, 32, 1), (2, 48, 13, 3), (7, 37500, 16, 1), (3, 128, 16, 2),
+                                     (2, 64, 32, 1), (5, 192, 3, 1), (5, 128, 13, 1), (5, 64, 7, 1), (5, 64, 26, 1),
+                                     (3, 70, 5, 1), (3, 180, 16, 3), (2, 120, 8, 2), (2, 61, 29, 1),
+                                     (3, 64, 12, 1), (3, 70, 20, 1), (2, 64, 24, 1), (2, 40, 28, 2), (3, 64, 1, 1), (3, 64, 2, 1), (3, 64, 6, 1)])
 def test_selective_scan_steps_against_float64(B, D, N, G, dtype):
     from airgym_amd.lib.network.selective_scan import selective_scan_step
     T = 5
