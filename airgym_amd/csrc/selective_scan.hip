@@ -693,7 +693,7 @@ template <typename T> struct ScanShared {
 // are in flight.  Otherwise a wave's 64 / L channels lie anywhere.  kTail: N is above 4 and no multiple of it.
 // Bytes bound it: 4096 x 512, N = 16, float32 takes 52 us = 5.8 TB/s, bfloat16 52 us = 5.4 TB/s (an in-place product over the states
 // alone 48 us).  The states are marked as used once: with plain accesses the float32 step took 59 us, without sharing 61.
-template <typename T, int L, bool kShared, bool kTail>
+template <typename T, int L, bool kShared, bool kTail, bool kOnce>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     constexpr int kRounds = kShared ? L : 1, C = 64 / L;                  // channels of a wave per round
     const int l = threadIdx.x & 63, part = l % L, mine = kShared ? l / L : 0;        // the lane's channel behind c0 in round 0
@@ -713,7 +713,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
 #pragma unroll
     for (int i = 0; i < kRounds; i++) {
         clear<4>(h[i]);
-        if (a.s0 && c0 + i * C + mine < end) load_states<4, true, kTail>(a.s0 + (row + i * C + mine) * a.N, part, a.N, h[i]);
+        if (a.s0 && c0 + i * C + mine < end) load_states<4, kOnce, kTail>(a.s0 + (row + i * C + mine) * a.N, part, a.N, h[i]);
     }
     const T* Bm = (const T*)a.Bm + (b * a.bb + g * a.bg);
     const T* Cm = (const T*)a.Cm + (b * a.cb + g * a.cg);
@@ -749,7 +749,7 @@ __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
             h[i][j] = __builtin_fmaf(exp2_hw(t * (A[i][j] * kLog2e)), h[i][j], tu * Bn[j]);
             p = __builtin_fmaf(Cn[j], h[i][j], p);
         }
-        if (c0 + i * C + mine < end) store_states<4, true>(a.s1 + (row + i * C + mine) * a.N, part, a.N, h[i]);
+        if (c0 + i * C + mine < end) store_states<4, kOnce>(a.s1 + (row + i * C + mine) * a.N, part, a.N, h[i]);
         if (L > 1) p += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(p), 0xB1, 0xf, 0xf, true));
         if (L > 2) p += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(p), 0x4E, 0xf, 0xf, true));
         if (L > 4) p += __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(p), 0x141, 0xf, 0xf, true));
@@ -909,11 +909,21 @@ extern "C" int ag_selective_scan_step(const ag_scan_args* p, void* stream) {
     const bool shared = a.nb * 64LL * 4 <= a.Dg * 5LL, tail = a.N > 4 && a.N % 4;
     const long long waves = shared ? (long long)a.B * a.G * a.nb : ((long long)a.B * a.D * lanes + 63) / 64, blocks = (waves + 3) / 4;
     if (blocks > kMaxThreads / 256) return AG_ERR_UNSUPPORTED;
+    // a state of 134 MB (4096 x 512, N = 16, float32) moved on again and again: 47 us plain, 50 as used once, with 34 MB of other work between
+    // the steps 59 and 62, with 134 MB of it 54 and 51; of 268 MB 99 and 95, with 34 MB 124 and 112; of 67 MB 26.5 and 26.9
+    const bool once = (long long)a.B * a.D * a.N * 4 >= kCached;
     const dim3 grid((unsigned)blocks), block(256);
-    const hipStream_t st = (hipStream_t)stream;
-    if (shared && tail) AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, true, (L > 1)>), grid, block, 0, st, a)));
-    else if (shared) AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, true, false>), grid, block, 0, st, a)));
-    else if (tail) AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, false, (L > 1)>), grid, block, 0, st, a)));
-    else AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, false, false>), grid, block, 0, st, a)));
+#define AG_STEP(SHARED, TAIL, ONCE)                                                                                              \
+    AG_FOR_DTYPE(p->dtype, AG_FOR_LANES(p->N, hipLaunchKernelGGL((scan_step_kernel<T, L, SHARED, (TAIL && L > 1), ONCE>), grid, block, 0, \
+                                                                 (hipStream_t)stream, a)))
+    if (shared && tail && once) AG_STEP(true, true, true);
+    else if (shared && tail) AG_STEP(true, true, false);
+    else if (shared && once) AG_STEP(true, false, true);
+    else if (shared) AG_STEP(true, false, false);
+    else if (tail && once) AG_STEP(false, true, true);
+    else if (tail) AG_STEP(false, true, false);
+    else if (once) AG_STEP(false, false, true);
+    else AG_STEP(false, false, false);
+#undef AG_STEP
     return seq_status();
 }

@@ -13,6 +13,10 @@ namespace {
 constexpr long long kMaxThreads = 0xffffffffLL;      // of one launch
 constexpr int kMaxSteps = 1 << 30;                   // of a sequence: step indexes run a little past its end
 
+// The last-level cache holds 256 MB.  What a call reads or writes of a buffer below half of that may still be there for the next kernel;
+// what it touches of a larger one will mostly be gone by then and only drives out the rest: from here on it is marked as used once.
+constexpr long long kCached = 128LL << 20;
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -63,42 +67,47 @@ template <typename T, int N> struct Vec {
         }
     }
 };
-template <typename T, int N> __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
+// kOnce: nothing reads this again before it has left the caches (a hint to them, nothing else)
+#define AG_LOAD(P, p) (kOnce ? __builtin_nontemporal_load((const P*)(p)) : *(const P*)(p))
+#define AG_STORE(P, p, v) (kOnce ? __builtin_nontemporal_store(v, (P*)(p)) : (void)(*(P*)(p) = v))
+template <typename T, int N, bool kOnce = false> __device__ __forceinline__ Vec<T, N> load_vec(const T* p) {
     constexpr int K = Vec<T, N>::kWords;
     Vec<T, N> c;
-    if constexpr (K == 0) c.w[0] = *(const uint16_t*)p;
+    if constexpr (K == 0) c.w[0] = AG_LOAD(uint16_t, p);
     else if constexpr (K == 1) {
-        if constexpr (sizeof(T) == 2) c.w[0] = *(const Words<1>::any2*)p;
-        else c.w[0] = *(const uint32_t*)p;
+        if constexpr (sizeof(T) == 2) c.w[0] = AG_LOAD(Words<1>::any2, p);
+        else c.w[0] = AG_LOAD(uint32_t, p);
     } else if constexpr (sizeof(T) == 2) {
-        const auto v = *(const typename Words<K>::any2*)p;
+        const auto v = AG_LOAD(typename Words<K>::any2, p);
 #pragma unroll
         for (int k = 0; k < K; k++) c.w[k] = v[k];
     } else {
-        const auto v = *(const typename Words<K>::any4*)p;
+        const auto v = AG_LOAD(typename Words<K>::any4, p);
 #pragma unroll
         for (int k = 0; k < K; k++) c.w[k] = v[k];
     }
     return c;
 }
-template <typename T, int N> __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& c) {
+template <typename T, int N, bool kOnce = false> __device__ __forceinline__ void store_vec(T* p, const Vec<T, N>& c) {
     constexpr int K = Vec<T, N>::kWords;
-    if constexpr (K == 0) *(uint16_t*)p = (uint16_t)c.w[0];
+    if constexpr (K == 0) AG_STORE(uint16_t, p, (uint16_t)c.w[0]);
     else if constexpr (K == 1) {
-        if constexpr (sizeof(T) == 2) *(Words<1>::any2*)p = c.w[0];
-        else *(uint32_t*)p = c.w[0];
+        if constexpr (sizeof(T) == 2) AG_STORE(Words<1>::any2, p, c.w[0]);
+        else AG_STORE(uint32_t, p, c.w[0]);
     } else if constexpr (sizeof(T) == 2) {
         typename Words<K>::any2 v;
 #pragma unroll
         for (int k = 0; k < K; k++) v[k] = c.w[k];
-        *(typename Words<K>::any2*)p = v;
+        AG_STORE(typename Words<K>::any2, p, v);
     } else {
         typename Words<K>::any4 v;
 #pragma unroll
         for (int k = 0; k < K; k++) v[k] = c.w[k];
-        *(typename Words<K>::any4*)p = v;
+        AG_STORE(typename Words<K>::any4, p, v);
     }
 }
+#undef AG_LOAD
+#undef AG_STORE
 
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }      // v_exp_f32: 1 ulp
 __device__ __forceinline__ float log2_hw(float x) { return __builtin_amdgcn_logf(x); }       // v_log_f32: 1 ulp
