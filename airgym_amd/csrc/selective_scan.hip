@@ -73,8 +73,18 @@ __device__ __forceinline__ unsigned char reset_flag(A a, int b, int t0, int nv, 
 // ... and as a wave-uniform bit mask
 __device__ __forceinline__ unsigned reset_bits(unsigned char flag) { return __builtin_amdgcn_readfirstlane((unsigned)__ballot(flag != 0)); }
 
-// a branch that stays one: a select in its place would cost every step what only a reset needs
+// Resets are rare.  In the forward a reset is a branch that stays one: a select in its place would cost every step what only a reset
+// needs.  The backward's tiles are written out twice, with and without them: a branch per step would keep every step's reads from LDS
+// behind the step before (first pass 111 -> 100 us, main pass 390 -> 377 us at 8 x 2047 x 2048 bf16, the two at 4096 x 24 x 256 f32 with a
+// reset in every 24 steps 443 -> 426 us; the forward, with 80 registers, only spills).
 #define AG_RARE(cond) if (__builtin_expect(cond, 0)) if (([]() __attribute__((always_inline)) { asm volatile(""); }(), true))
+template <bool B> struct Flag { static constexpr bool value = B; };
+// x, or zeros (whatever x is); keep is wave-uniform
+template <int S> __device__ __forceinline__ void keep_if(bool keep, float* x) {
+    const unsigned mask = keep ? ~0u : 0u;
+#pragma unroll
+    for (int j = 0; j < S; j++) x[j] = __uint_as_float(__float_as_uint(x[j]) & mask);
+}
 
 // Addresses.  A row's base is wave-uniform and moves on by scalar adds; a lane adds 32 bits of its own (the host has checked that a
 // tile of rows stays below 4 GB).  The argument block is read again, by scalar loads, where a sequence starts: all of its pointers and
@@ -394,6 +404,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
     constexpr int kRows = kBack / NG, kWide = S * NG, kSteps = 8 / S;
     __shared__ float2 sdt[kBack][kLanes];                               // dt, dt u
     __shared__ float sdy[kBack][kLanes];
+    __shared__ float skeep[3][kCarry ? 1 : kBack][kLanes];              // u, softplus' slope, what turns y into the gate's gradient
     __shared__ float sy[kCarry ? 1 : NG][kBack][kLanes], ss1[kCarry ? 1 : NG][kBack][kLanes], ss2[kCarry ? 1 : NG][kBack][kLanes];
     __shared__ alignas(16) float sBC[2][kBack][kWide], sdBC[2][kBack][kWide];
     const Place p = place_of(a);
@@ -479,30 +490,29 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
         bool any_cut = false;
         for (int t0 = last; t0 >= from; t0 -= kBack) {
             const int nv = max(0, min(kBack, len - t0)), nt = min(kBack, T_ - t0);
-            float uu[kRows], dts[kRows], sg[kRows], zz[kRows], sz[kRows], go[kRows], now[S];
+            float now[S];
 #pragma unroll
             for (int j = 0; j < S; j++) now[j] = p.live ? start[j] : 0.0f;
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
                 const int r = w + k * NG;
-                uu[k] = dts[k] = sg[k] = zz[k] = go[k] = 0.0f;
-                sz[k] = 1.0f;
-                float dy = 0.0f;
+                float dt = 0.0f, dy = 0.0f, uu = 0.0f, slope = 0.0f, dg = 0.0f;
                 if (r < nv && p.live) {
-                    if (!kCarry) uu[k] = to_f32(ru[k]);
-                    dts[k] = to_f32(rd[k]) + bias;
-                    sg[k] = 1.0f;
-                    if (soft) dts[k] = softplus(dts[k], sg[k]);
-                    go[k] = dy = to_f32(rg[k]);
+                    if (!kCarry) uu = to_f32(ru[k]);
+                    dt = to_f32(rd[k]) + bias;
+                    slope = 1.0f;
+                    if (soft) dt = softplus(dt, slope);
+                    dy = to_f32(rg[k]);
                     if (gate) {
-                        zz[k] = to_f32(rz[k]);
-                        sz[k] = sigmoid(zz[k]);
-                        dy *= zz[k] * sz[k];
+                        const float zz = to_f32(rz[k]), sz = sigmoid(zz);
+                        dg = dy * sz * __builtin_fmaf(zz, 1.0f - sz, 1.0f);
+                        dy *= sz * zz;
                     }
                 }
-                sdt[r][lane] = make_float2(dts[k], dts[k] * uu[k]);
+                sdt[r][lane] = make_float2(dt, dt * uu);
                 sdy[r][lane] = dy;
-                if (kCarry) total += dts[k];
+                if (!kCarry) skeep[0][r][lane] = uu, skeep[1][r][lane] = slope, skeep[2][r][lane] = dg;
+                if (kCarry) total += dt;
             }
             if (brow < kBack) {
                 if (!kCarry) sBC[0][brow][bn] = to_f32(rB);
@@ -515,7 +525,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
             if (!same && next_b < a.B) sequence(next_b);
             load(same ? b : next_b, same ? t0 - kBack : last, same ? len - t0 + kBack : next_len - last);
             if (kCarry) {
-                auto back = [&](bool cuts) __attribute__((always_inline)) {
+                auto back = [&](auto kCut) __attribute__((always_inline)) {
 #pragma unroll
                     for (int r = kBack - 1; r >= 0; r--) {
                         const float dy = sdy[r][lane], dt = sdt[r][lane].x;
@@ -523,23 +533,21 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
                         read_row<S>(&sBC[1][r][S * w], Cn);
 #pragma unroll
                         for (int j = 0; j < S; j++) carry[j] = exp2_hw(dt * A2[j]) * __builtin_fmaf(Cn[j], dy, carry[j]);
-                        if (cuts && (cut >> r & 1)) clear<S>(carry);
+                        if (kCut.value) keep_if<S>(!(cut >> r & 1), carry);
                     }
                 };
-                // Written out twice: the branches of the resets would keep every step's reads from LDS behind the step before (8 x 2047 x
-                // 2048 bf16: 111 us, this way 99).  The main pass's tiles have no registers for reading ahead: no gain there.
-                if (cut) back(true);
-                else back(false);
+                if (cut) back(Flag<true>{});
+                else back(Flag<false>{});
                 __syncthreads();
                 continue;
             }
-            if (nv) {
+            auto tile = [&](auto kCut) __attribute__((always_inline)) {
                 float h[kBack][S], e[kBack][S], v[8], sums = 0.0f;      // h[r]: the state step r starts from
                 // kSteps steps' values are summed at a time; lane 8g + i keeps the i-th sum
                 const int order = sum_lanes8_order(lane), step = order / S, mine = lane % S;
 #pragma unroll
                 for (int r = 0; r < kBack; r++) {      // steps behind nv have dt = dy = 0: decay 1, no input
-                    AG_RARE(cut >> r & 1) clear<S>(now);
+                    if (kCut.value) keep_if<S>(!(cut >> r & 1), now);
                     const float2 s = sdt[r][lane];
                     const float dy = sdy[r][lane];
                     float Bn[S], Cn[S];
@@ -551,7 +559,7 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
                         h[r][j] = now[j];
                         e[r][j] = exp2_hw(s.x * A2[j]);
                         now[j] = __builtin_fmaf(e[r][j], now[j], s.y * Bn[j]);
-                        y = __builtin_fmaf(Cn[j], now[j], y);
+                        y = j ? __builtin_fmaf(Cn[j], now[j], y) : Cn[j] * now[j];
                         v[r % kSteps * S + j] = dy * now[j];
                     }
                     sy[w][r][lane] = y;
@@ -560,6 +568,9 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
                         sums = mine == r / kSteps ? x : sums;
                     }
                 }
+                // nothing is moved across: with both passes' reads ahead of the first the kernel keeps 46 registers in memory (780 us
+                // where it takes 426)
+                __builtin_amdgcn_sched_barrier(0);
                 if ((lane & 7) < S) sdBC[1][kSteps * mine + step][S * w + order % S] = sums;
 #pragma unroll
                 for (int r = kBack - 1; r >= 0; r--) {
@@ -573,13 +584,13 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
                     for (int j = 0; j < S; j++) {
                         const float gr = __builtin_fmaf(Cn[j], dy, carry[j]);
                         v[r % kSteps * S + j] = gr * s.y;
-                        s1 = __builtin_fmaf(gr, Bn[j], s1);
+                        s1 = j ? __builtin_fmaf(gr, Bn[j], s1) : gr * Bn[j];
                         carry[j] = e[r][j] * gr;
                         const float qq = carry[j] * h[r][j];
-                        s2 = __builtin_fmaf(qq, A2[j], s2);
+                        s2 = j ? __builtin_fmaf(qq, A2[j], s2) : qq * A2[j];
                         dA[j] = __builtin_fmaf(qq, s.x, dA[j]);
                     }
-                    AG_RARE(cut >> r & 1) clear<S>(carry);                 // h[r] is 0 there already
+                    if (kCut.value) keep_if<S>(!(cut >> r & 1), carry);     // h[r] is 0 there already
                     ss1[w][r][lane] = s1;
                     ss2[w][r][lane] = s2;
                     if (r % kSteps == 0) {
@@ -587,31 +598,33 @@ __global__ __launch_bounds__(kLanes* NG, kCarry ? 1 : 3) void scan_bwd_kernel(Sc
                         sums = mine == r / kSteps ? x : sums;
                     }
                 }
+                __builtin_amdgcn_sched_barrier(0);
                 if ((lane & 7) < S) sdBC[0][kSteps * mine + step][S * w + order % S] = sums;
+            };
+            if (nv) {
+                if (cut) tile(Flag<true>{});
+                else tile(Flag<false>{});
             }
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < kRows; k++) {
                 const int r = w + k * NG;
                 if (r >= nt) break;
-                float y = skip * uu[k], s1 = 0.0f, s2 = 0.0f;
+                const float uu = skeep[0][r][lane];
+                float y = skip * uu, s1 = 0.0f, s2 = 0.0f;
                 if (r < nv) {
 #pragma unroll
                     for (int v = 0; v < NG; v++) y += sy[v][r][lane], s1 += ss1[v][r][lane], s2 += ss2[v][r][lane];
                 }
-                float dy = go[k], dzv = 0.0f;
-                if (gate) {
-                    dzv = go[k] * y * (sz[k] * __builtin_fmaf(zz[k], 1.0f - sz[k], 1.0f));
-                    dy *= zz[k] * sz[k];
-                }
-                const float draw = __builtin_fmaf(uu[k], s1, s2 * kLn2) * sg[k];      // s2 was summed with A log2(e)
+                const float dy = sdy[r][lane], dt = sdt[r][lane].x;
+                const float draw = __builtin_fmaf(uu, s1, s2 * kLn2) * skeep[1][r][lane];      // s2 was summed with A log2(e)
                 if (p.live) {
                     const unsigned i = r * (D * (unsigned)sizeof(T)) + at;
-                    put(du, i, from_f32<T>(__builtin_fmaf(dts[k], s1, skip * dy)));
+                    put(du, i, from_f32<T>(__builtin_fmaf(dt, s1, skip * dy)));
                     put(ddelta, i, from_f32<T>(draw));
-                    if (gate) put(dz, i, from_f32<T>(dzv));
+                    if (gate) put(dz, i, from_f32<T>(skeep[2][r][lane] * y));
                 }
-                dD = __builtin_fmaf(dy, uu[k], dD);
+                dD = __builtin_fmaf(dy, uu, dD);
                 dbias += draw;
             }
             const long long back = (long long)kBack * D * (long long)sizeof(T);
