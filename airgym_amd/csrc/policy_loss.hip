@@ -9,7 +9,7 @@
 // Every wave sums against a maximum of its own and the waves' results are joined.  Memory bounds it: about 20 issue slots per element
 // are some 2 T elements/s over the chip, more than arrives.
 // Logits of -inf have probability 0.  Their infinite log-probability would meet it as 0 times inf: a wave that finds its second sum
-// NaN forms it again with the log-probability held at -1e30, and so does the gradient.
+// NaN forms it again with the log-probability held at -1e30; the gradient holds it there always.
 #include "seq_common.hpp"
 
 namespace {
@@ -27,15 +27,17 @@ struct LossArgs {
     float e_clip, kl_coef, entropy_coef;
 };
 
-struct Sums { float m, s, t; };        // maximum, sum e^{x-m}, sum e^{x-m} (x-m)
+struct Sums { float m, s, t; };        // with y = (x - m) log2(e), m the maximum: m, sum 2^y, sum 2^y y
 
+// (x - m first: with y as one FMA, x log2(e) - c, the rounding of c would be all of y where every logit of a row is a mask's -1e30)
 __device__ __forceinline__ float safe_max(float m) { return m == -__builtin_inff() ? 0.0f : m; }
+__device__ __forceinline__ float shifted(float x, float base) { return (x - base) * kLog2e; }
 
 __device__ __forceinline__ Sums join(Sums a, Sums b) {
     const float m = fmaxf(a.m, b.m), base = safe_max(m);
-    const float da = fmaxf(a.m - base, kFloor), db = fmaxf(b.m - base, kFloor);
-    const float ea = exp_hw(da), eb = exp_hw(db);
-    // t shifts with the base: sum e^{x-m} (x-m) = e^{a.m-m} (a.t + (a.m-m) a.s)
+    const float da = fmaxf(shifted(a.m, base), kFloor), db = fmaxf(shifted(b.m, base), kFloor);
+    const float ea = exp2_hw(da), eb = exp2_hw(db);
+    // t shifts with the base: sum 2^(y + da) (y + da) = 2^da (t + da s)
     return Sums{m, a.s * ea + b.s * eb, ea * (a.t + da * a.s) + eb * (b.t + db * b.s)};
 }
 
@@ -44,20 +46,18 @@ template <typename T> __device__ __forceinline__ const T* row_of(const LossArgs&
     return (const T*)a.logits + i * a.s0 + (row - (long long)i * a.R1) * a.s1;
 }
 
-// what a row's sums say: base and logarithm of the softmax, entropy, log-probability, and the two factors of its gradient
+// what a row's sums say: base and log2 of the softmax's sum, entropy, log-probability, and the factors of its gradient
 struct Row {
-    float base, logS, H, lp, f, ent;
-    bool inf;                          // some logits are -inf
+    float base, lS, H, lp, f, k, ent;  // p (ent log2 p + k), and f for the action
 };
 
-__device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, bool inf, float xa, long long row) {
+__device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, float xa, long long row) {
     Row r;
-    r.inf = inf;
     r.base = safe_max(v.m);
-    r.logS = log2_hw(v.s) * kLn2;
-    r.H = r.logS - v.t / v.s;
-    r.lp = (xa - r.base) - r.logS;
-    r.f = r.ent = 0.0f;
+    r.lS = log2_hw(v.s);
+    r.H = (r.lS - v.t / v.s) * kLn2;
+    r.lp = (xa - r.base) - r.lS * kLn2;
+    r.f = r.k = r.ent = 0.0f;
     if (a.logp) return r;
     const float adv = a.adv[row], ratio = expf(r.lp - a.old_logp[row]);
     const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
@@ -65,22 +65,22 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, bool inf, f
     if (a.ref_logp) f -= a.kl_coef * expm1f(a.ref_logp[row] - r.lp);
     const float n = 1.0f / (a.count ? a.count[0] : (float)a.R);
     r.f = f * n;
-    r.ent = a.entropy_coef * n;
+    r.ent = a.entropy_coef * n * kLn2;
+    r.k = __builtin_fmaf(a.entropy_coef * n, r.H, -r.f);
     return r;
 }
 
-// f (delta - p) + ent p (log p + H) without the delta, from d = x - base
-__device__ __forceinline__ float grad_of(const Row& r, float d) {
-    if (r.inf) d = fmaxf(d, kFloor);
-    const float p = exp2_hw((d - r.logS) * kLog2e);
-    return p * __builtin_fmaf(r.ent, d + (r.H - r.logS), -r.f);
+// f (delta - p) + ent p (log p + H) without the delta
+__device__ __forceinline__ float grad_of(const Row& r, float x) {
+    const float q = fmaxf(__builtin_fmaf(x - r.base, kLog2e, -r.lS), kFloor);      // log2 p
+    return exp2_hw(q) * __builtin_fmaf(r.ent, q, r.k);
 }
 
 // one element's share of the sums
 __device__ __forceinline__ void add_to(Sums& v, float x, float base) {
-    const float d = x - base, e = exp_hw(d);
+    const float y = shifted(x, base), e = exp2_hw(y);
     v.s += e;
-    v.t = __builtin_fmaf(e, d, v.t);
+    v.t = __builtin_fmaf(e, y, v.t);
 }
 
 // ---- short rows: L lanes of a wave per row, up to 8 elements a lane ------------------------------------------------------
@@ -99,35 +99,35 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
         const T* p = row_of<T>(a, row);
         const long long av = a.actions[row];
         act = av >= 0 && av < a.V ? (int)av : -1;
-        Sums v{-__builtin_inff(), 0.0f, 0.0f};
+        float m = -__builtin_inff();
 #pragma unroll
         for (int k = 0; k < kPerLane; k++) {
             const int j = l + k * L;
             x[k] = j < a.V ? to_f32(p[j]) : -__builtin_inff();
-            v.m = fmaxf(v.m, x[k]);
+            m = fmaxf(m, x[k]);
         }
         if (act >= 0) xa = to_f32(p[act]);
 #pragma unroll
-        for (int o = L / 2; o; o >>= 1) v.m = fmaxf(v.m, __shfl_xor(v.m, o));
-        const float base = safe_max(v.m);
-        bool inf = false;
+        for (int o = L / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        Sums v{m, 0.0f, 0.0f};
+        const float base = safe_max(m);
 #pragma unroll
         for (int k = 0; k < kPerLane; k++)
             if (l + k * L < a.V) {
-                const float d = x[k] - base, e = exp_hw(d);
-                inf |= d == -__builtin_inff();
+                const float y = shifted(x[k], base), e = exp2_hw(y);
                 v.s += e;
-                v.t = __builtin_fmaf(e, fmaxf(d, kFloor), v.t);
+                v.t = __builtin_fmaf(e, fmaxf(y, kFloor), v.t);
             }
 #pragma unroll
         for (int o = L / 2; o; o >>= 1) v.s += __shfl_xor(v.s, o), v.t += __shfl_xor(v.t, o);
-        r = finish_row(a, v, inf, xa, row);
+        r = finish_row(a, v, xa, row);
+        if (!a.logp && l == 0) a.rows[row] = float4{xa, r.base, v.s, v.t};
         if (a.logp) {
             if (l == 0) {
                 a.logp[row] = r.lp;
                 if (a.entropy) a.entropy[row] = r.H;
             }
-        } else if (l == 0) a.rows[row] = float4{xa, base, v.s, v.t};
+        }
     }
     if (a.dlogits && there) {
         T* dx = (T*)a.dlogits + row * a.V;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
             const int j = l + k * L;
             if (j < a.V) {
                 float g = 0.0f;
-                if (on) g = grad_of(r, x[k] - r.base) + (j == act ? r.f : 0.0f);
+                if (on) g = grad_of(r, x[k]) + (j == act ? r.f : 0.0f);
                 dx[j] = from_f32<T>(g);
             }
         }
@@ -150,7 +150,6 @@ template <typename T, int THREADS, int NV, bool kOnceIn, bool kOnceOut>
 __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     constexpr int E = 16 / sizeof(T), kWaves = THREADS / 64, kKeep = NV ? NV : 1;
     __shared__ Sums part[kWaves];
-    __shared__ int has_inf[kWaves];
     const long long row = blockIdx.x;
     const T* x = row_of<T>(a, row);
     T* dx = a.dlogits ? (T*)a.dlogits + row * a.V : nullptr;
@@ -170,7 +169,6 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     const float xa = act >= 0 ? to_f32(x[act]) : __builtin_nanf("");
     Vec<T, E> c[kKeep];
     Sums v{-__builtin_inff(), 0.0f, 0.0f};
-    bool inf = false;
     // The row stays as it came: without this the compiler keeps the 16-bit types' float forms from one pass over it to the next, two
     // registers for one.
     auto as_it_came = [&]() __attribute__((always_inline)) {
@@ -195,8 +193,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
             if ((k0 + k) * THREADS + (int)threadIdx.x < full)
 #pragma unroll
                 for (int i = 0; i < E; i++) add_to(u, c[k].at(i), base);
-        if (u.t != u.t) {              // some x - base are -inf (or NaN, which stays)
-            inf = true;
+        if (u.t != u.t) {              // some y are -inf (or NaN, which stays)
             u.t = 0.0f;
             as_it_came();
 #pragma unroll
@@ -204,15 +201,14 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
                 if ((k0 + k) * THREADS + (int)threadIdx.x < full)
 #pragma unroll
                     for (int i = 0; i < E; i++) {
-                        const float d = c[k].at(i) - base;
-                        u.t = __builtin_fmaf(exp_hw(d), fmaxf(d, kFloor), u.t);
+                        const float y = shifted(c[k].at(i), base);
+                        u.t = __builtin_fmaf(exp2_hw(y), fmaxf(y, kFloor), u.t);
                     }
         }
         if (k0 == 0 && tail < a.V) {
-            const float d = xt - base, e = exp_hw(d);
-            inf |= d == -__builtin_inff();
+            const float y = shifted(xt, base), e = exp2_hw(y);
             u.s += e;
-            u.t = __builtin_fmaf(e, fmaxf(d, kFloor), u.t);
+            u.t = __builtin_fmaf(e, fmaxf(y, kFloor), u.t);
         }
 #pragma unroll
         for (int o = 32; o; o >>= 1) u.s += __shfl_xor(u.s, o), u.t += __shfl_xor(u.t, o);
@@ -233,14 +229,12 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
             sum_up(k, k ? -__builtin_inff() : xt);
         }
     }
-    const bool any = __any(inf);
-    if (lane == 0) part[w] = v, has_inf[w] = any;
+    if (lane == 0) part[w] = v;
     __syncthreads();
     v = part[lane % kWaves];
-    const bool row_inf = __any(has_inf[lane % kWaves]);
 #pragma unroll
     for (int o = kWaves / 2; o; o >>= 1) v = join(v, Sums{__shfl_xor(v.m, o), __shfl_xor(v.s, o), __shfl_xor(v.t, o)});
-    const Row r = finish_row(a, v, row_inf, xa, row);
+    const Row r = finish_row(a, v, xa, row);
     if (a.logp) {
         if (threadIdx.x == 0) {
             a.logp[row] = r.lp;
@@ -255,7 +249,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
         if (q >= full) return;
         float g[E];
 #pragma unroll
-        for (int i = 0; i < E; i++) g[i] = grad_of(r, held.at(i) - r.base);
+        for (int i = 0; i < E; i++) g[i] = grad_of(r, held.at(i));
         if (q == aq)
 #pragma unroll
             for (int i = 0; i < E; i++) g[i] += i == ai ? r.f : 0.0f;
@@ -270,7 +264,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     } else {
         for (int q = threadIdx.x; q < full; q += THREADS) gradient(q, load_vec<T, E>(x + q * E));
     }
-    if (tail < a.V) dx[tail] = from_f32<T>(grad_of(r, xt - r.base) + (tail == act ? r.f : 0.0f));
+    if (tail < a.V) dx[tail] = from_f32<T>(grad_of(r, xt) + (tail == act ? r.f : 0.0f));
 }
 
 __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, long long R, float* count) {
@@ -306,9 +300,10 @@ constexpr int kStatsThreads = 256, kStatsBlocks = 1024, kOneStage = 512, kOneSta
 __device__ __forceinline__ void add_row(const LossArgs& a, long long row, double* s) {
     if (a.mask && !a.mask[row]) return;
     const float4 v = a.rows[row];
-    // the sums' exponentials are those of (x - m) (1 + tilt), log2(e) being a float there: log S is off by tilt times the mean x - m
-    constexpr double tilt = (double)kLog2e / 1.4426950408889634074 - 1.0;
-    const double mean = (double)v.w / v.z, logS = log((double)v.z) - tilt * mean, lp = ((double)v.x - v.y) - logS, adv = a.adv[row], moved = lp - a.old_logp[row], up = expm1(moved);
+    // The sums are those of the softmax of x (1 + tilt), log2(e) being a float: log S is off by tilt times the mean x - base.
+    constexpr double ln2 = 0.6931471805599453094, tilt = (double)kLog2e * ln2 - 1.0;
+    const double mean = (double)v.w / v.z * ln2, logS = log((double)v.z) - tilt * mean;
+    const double lp = ((double)v.x - v.y) - logS, adv = a.adv[row], moved = lp - a.old_logp[row], up = expm1(moved);
     const double ratio = 1.0 + up, low = 1.0 - (double)a.e_clip, high = 1.0 + (double)a.e_clip;
     const double held = -adv * fmin(fmax(ratio, low), high), plain = -adv * ratio;
     s[0] += plain != plain ? plain : fmax(plain, held);
