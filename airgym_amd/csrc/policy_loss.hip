@@ -19,13 +19,53 @@ constexpr int kSums = 5;               // policy loss, KL term, entropy, KL of t
 
 struct LossArgs {
     const void* logits; const long long* actions; const float *old_logp, *adv, *ref_logp; const unsigned char* mask;
-    void* dlogits; const float* count; // {max(rows that count, 1), rows that count}, or NULL: all R
+    void* dlogits; const float* count; // {max(rows that count, 1), rows that count, 1 / the first}, or NULL: all R
     float4* rows;                      // [R] what the statistics need of a row: its action's logit, the base, the two sums
     float *logp, *entropy;             // the log-probability form: these instead
     long long R1, s0, s1, R;
     int V;
-    float e_clip, kl_coef, entropy_coef;
+    float e_clip, kl_coef, entropy_coef, inv_R;
 };
+
+// x of the lane that differs in bit 0, 1 (of a lane's four), 2 (mirrored within eight), 3 (within sixteen): no LDS, one instruction
+template <int kCtrl> __device__ __forceinline__ float across(float x) {
+    return __uint_as_float(__builtin_amdgcn_mov_dpp(__float_as_uint(x), kCtrl, 0xf, 0xf, true));
+}
+// op over each L lanes in a row, in all of them; 64: the wave, all of whose lanes are here
+template <int L, typename Op> __device__ __forceinline__ float over_lanes(float x, Op op) {
+    if (L > 1) x = op(x, across<0xB1>(x));
+    if (L > 2) x = op(x, across<0x4E>(x));
+    if (L > 4) x = op(x, across<0x141>(x));
+    if (L > 8) x = op(x, across<0x140>(x));
+    if (L > 16) {
+        const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    if (L > 32) {
+        const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = op(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    }
+    return x;
+}
+template <int L> __device__ __forceinline__ float max_over(float x) { return over_lanes<L>(x, [](float a, float b) { return fmaxf(a, b); }); }
+template <int L> __device__ __forceinline__ float sum_over(float x) { return over_lanes<L>(x, [](float a, float b) { return a + b; }); }
+
+// e^x to about 2 ulp: 2^y, y = x log2(e) rounded, times 1 + what the rounding and log2(e)'s own left out.  A row's factors are formed by
+// every lane of its waves, so that the general functions' tables of cases were most of a short row's work.
+__device__ __forceinline__ float exp_near(float x) {
+    const float y = x * kLog2e, r = exp2_hw(y), lost = __builtin_fmaf(x, 1.925963e-8f, __builtin_fmaf(x, kLog2e, -y));
+    return __builtin_fabsf(x) < 128.0f ? r * __builtin_fmaf(lost, kLn2, 1.0f) : r;
+}
+// e^x - 1: below 0.35 by its series, whose next term is below 2^-26 of the sum
+__device__ __forceinline__ float expm1_near(float x) {
+    float p = 1.0f / 5040.0f;
+    p = __builtin_fmaf(p, x, 1.0f / 720.0f);
+    p = __builtin_fmaf(p, x, 1.0f / 120.0f);
+    p = __builtin_fmaf(p, x, 1.0f / 24.0f);
+    p = __builtin_fmaf(p, x, 1.0f / 6.0f);
+    p = __builtin_fmaf(p, x, 0.5f);
+    return __builtin_fabsf(x) < 0.35f ? __builtin_fmaf(p * x, x, x) : exp_near(x) - 1.0f;
+}
 
 struct Sums { float m, s, t; };        // with y = (x - m) log2(e), m the maximum: m, sum 2^y, sum 2^y y
 
@@ -55,15 +95,15 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, float xa, l
     Row r;
     r.base = safe_max(v.m);
     r.lS = log2_hw(v.s);
-    r.H = (r.lS - v.t / v.s) * kLn2;
+    r.H = (r.lS - v.t * rcp_hw(v.s)) * kLn2;
     r.lp = (xa - r.base) - r.lS * kLn2;
     r.f = r.k = r.ent = 0.0f;
     if (a.logp) return r;
-    const float adv = a.adv[row], ratio = expf(r.lp - a.old_logp[row]);
+    const float adv = a.adv[row], ratio = exp_near(r.lp - a.old_logp[row]);
     const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
     float f = plain >= held || plain != plain ? plain : 0.0f;
-    if (a.ref_logp) f -= a.kl_coef * expm1f(a.ref_logp[row] - r.lp);
-    const float n = 1.0f / (a.count ? a.count[0] : (float)a.R);
+    if (a.ref_logp) f -= a.kl_coef * expm1_near(a.ref_logp[row] - r.lp);
+    const float n = a.count ? a.count[2] : a.inv_R;
     r.f = f * n;
     r.ent = a.entropy_coef * n * kLn2;
     r.k = __builtin_fmaf(a.entropy_coef * n, r.H, -r.f);
@@ -84,7 +124,7 @@ __device__ __forceinline__ void add_to(Sums& v, float x, float base) {
 }
 
 // ---- short rows: L lanes of a wave per row, up to 8 elements a lane ------------------------------------------------------
-constexpr int kShortThreads = 256, kPerLane = 8, kShortLanes = 16;
+constexpr int kShortThreads = 256, kPerLane = 8, kShortLanes = 32;
 
 template <typename T, int L>
 __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArgs a) {
@@ -107,8 +147,7 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
             m = fmaxf(m, x[k]);
         }
         if (act >= 0) xa = to_f32(p[act]);
-#pragma unroll
-        for (int o = L / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        m = max_over<L>(m);
         Sums v{m, 0.0f, 0.0f};
         const float base = safe_max(m);
 #pragma unroll
@@ -118,8 +157,7 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
                 v.s += e;
                 v.t = __builtin_fmaf(e, fmaxf(y, kFloor), v.t);
             }
-#pragma unroll
-        for (int o = L / 2; o; o >>= 1) v.s += __shfl_xor(v.s, o), v.t += __shfl_xor(v.t, o);
+        v.s = sum_over<L>(v.s), v.t = sum_over<L>(v.t);
         r = finish_row(a, v, xa, row);
         if (!a.logp && l == 0) a.rows[row] = float4{xa, r.base, v.s, v.t};
         if (a.logp) {
@@ -183,8 +221,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
             if ((k0 + k) * THREADS + (int)threadIdx.x < full)
 #pragma unroll
                 for (int i = 0; i < E; i++) m = fmaxf(m, c[k].at(i));
-#pragma unroll
-        for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+        m = max_over<64>(m);
         Sums u{m, 0.0f, 0.0f};
         const float base = safe_max(m);
         as_it_came();
@@ -210,8 +247,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
             u.s += e;
             u.t = __builtin_fmaf(e, fmaxf(y, kFloor), u.t);
         }
-#pragma unroll
-        for (int o = 32; o; o >>= 1) u.s += __shfl_xor(u.s, o), u.t += __shfl_xor(u.t, o);
+        u.s = sum_over<64>(u.s), u.t = sum_over<64>(u.t);
         v = NV ? u : join(v, u);
     };
     const float xt = tail < a.V ? to_f32(x[tail]) : -__builtin_inff();
@@ -289,6 +325,7 @@ __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, 
         for (int i = 0; i < 16; i++) s += part[i];
         count[0] = s > 0 ? (float)s : 1.0f;
         count[1] = (float)s;
+        count[2] = 1.0f / count[0];
     }
 }
 
@@ -379,7 +416,8 @@ __global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const flo
 
 }  // namespace
 
-// Which form takes a row of V logits.  Up to 128 of them, 1 to 16 lanes share a wave with other rows; beyond, a workgroup holds the row
+// Which form takes a row of V logits.  Up to 256 of them, 1 to 32 lanes share a wave with other rows (65536 x 129 float32: 26 us with the
+// gradient where a wave per row takes 37; at 256 34 and 38, at 512 a wave per row moves 4.5 TB/s); beyond, a workgroup holds the row
 // in accesses of 16 bytes: one wave up to 8 KB, 256 threads up to 32 KB, 1024 threads up to 256 KB; what is longer is read twice.
 static int short_lanes(int V) {
     int l = 1;
@@ -427,7 +465,8 @@ static void launch_rows(const LossArgs& a, void* stream) {
             case 2: hipLaunchKernelGGL((token_loss_short_kernel<T, 2>), grid, block, 0, st, a); break;
             case 4: hipLaunchKernelGGL((token_loss_short_kernel<T, 4>), grid, block, 0, st, a); break;
             case 8: hipLaunchKernelGGL((token_loss_short_kernel<T, 8>), grid, block, 0, st, a); break;
-            default: hipLaunchKernelGGL((token_loss_short_kernel<T, 16>), grid, block, 0, st, a); break;
+            case 16: hipLaunchKernelGGL((token_loss_short_kernel<T, 16>), grid, block, 0, st, a); break;
+            default: hipLaunchKernelGGL((token_loss_short_kernel<T, 32>), grid, block, 0, st, a); break;
         }
         return;
     }
@@ -464,7 +503,7 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     double* parts = blocks ? (double*)(rows + R) : nullptr;
     const LossArgs a{p->logits_dev, p->actions_dev, p->old_logp_dev, p->advantages_dev, p->ref_logp_dev, p->mask_dev, p->dlogits_dev,
                      p->mask_dev ? count : nullptr, rows, nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef,
-                     p->entropy_coef};
+                     p->entropy_coef, 1.0f / (float)R};
     if (a.count) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p->mask_dev, R, count);
     AG_FOR_DTYPE(p->dtype, launch_rows<T>(a, stream));
     if (blocks) hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(kStatsThreads), 0, (hipStream_t)stream, a, parts);
@@ -477,7 +516,7 @@ extern "C" int ag_token_logp(const void* logits, long long R0, long long R1, lon
     if (!logits || !actions || !logp || R0 <= 0 || R1 <= 0 || V <= 0) return AG_ERR_INVALID_ARG;
     if (dtype < AG_F32 || dtype > AG_F16 || !launchable(R0, R1, V, dtype)) return AG_ERR_UNSUPPORTED;
     const LossArgs a{logits, actions, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, logp, entropy, R1, s0, s1, R0 * R1, V,
-                     0.0f, 0.0f, 0.0f};
+                     0.0f, 0.0f, 0.0f, 0.0f};
     AG_FOR_DTYPE(dtype, launch_rows<T>(a, stream));
     return seq_status();
 }

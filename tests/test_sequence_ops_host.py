@@ -73,8 +73,8 @@ def test_loss_entries_refuse(lib):
         assert lib.ag_token_policy_loss(ctypes.byref(a), None) == rc, field
         setattr(a, field, old)
     assert lib.ag_token_logp(p, 1, 3, 27, 9, 9, 0, None, p, p, None) == -1 and lib.ag_token_logp(p, 1, 3, 27, 9, 9, 4, p, p, p, None) == -6
-    # 64 threads per row of 129 to 2048 float32 logits, 1024 beyond 8192: more than one launch holds
-    assert lib.ag_token_logp(p, 1 << 26, 1, 200, 200, 200, 0, p, p, p, None) == -6
+    # 64 threads per row of 257 to 2048 float32 logits, 1024 beyond 8192: more than one launch holds
+    assert lib.ag_token_logp(p, 1 << 26, 1, 300, 300, 300, 0, p, p, p, None) == -6
     assert lib.ag_token_logp(p, 1 << 22, 1, 9000, 9000, 9000, 0, p, p, p, None) == -6
     assert lib.ag_token_policy_loss_workspace_bytes(3, 2147483647) > 0
     assert lib.ag_scale_by(p, 0, 0, p, None) == -1 and lib.ag_scale_by(p, 4, 9, p, None) == -6
