@@ -69,10 +69,11 @@ def policy_loss(logits, actions, old_logp, adv, ref_logp, mask, e_clip, kl_coef,
             continue
         rows += 1
         on = logits[r] > -float("inf")
-        x = logits[r][on]
+        top = logits[r][on].max().detach()        # shifts nothing, but log V beside a row of -3e38 is lost in any number format
+        x = logits[r][on] - top
         lse = torch.logsumexp(x, 0)
         H = -(torch.exp(x - lse) * (x - lse)).sum()
-        lp = logits[r, actions[r]] - lse
+        lp = (logits[r, actions[r]] - top) - lse
         ratio = torch.exp(lp - old_logp[r])
         pol = torch.maximum(-adv[r] * ratio, -adv[r] * ratio.clamp(1 - e_clip, 1 + e_clip))
         kl = zero

@@ -330,7 +330,7 @@ def test_gradients_against_differences():
 
 
 # ------------------------------------------------------------------------------------------------ clipped policy loss
-LOSS = [(1, 1), (1, 2), (3, 5), (70, 21), (64, 64), (33, 257), (5, 1000), (7, 4099), (3, 33001)]
+LOSS = [(1, 1), (1, 2), (3, 5), (70, 21), (64, 64), (9, 129), (10, 200), (6, 256), (33, 257), (9, 700), (5, 1000), (7, 4099), (3, 33001)]
 
 
 def loss_case(R, V, dtype, masked, minus_inf, seed=0):
@@ -386,6 +386,86 @@ def test_policy_loss_and_gradient(R, V, masked, minus_inf, dtype):
     ls = torch.log_softmax(logits[on].double(), 1)
     close("logp", lp, ls.gather(1, actions[on][:, None])[:, 0], n, 20)
     close("entropy", H, -(ls.exp() * ls.clamp(min=-1e30)).sum(1), n, 20)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("V", [6, 150, 1500])
+def test_logits_at_a_mask_s_lowest_value(V, dtype):
+    """Choices masked with a finite lowest number instead of -inf, rows of nothing else among them: those are uniform."""
+    from airgym_amd.lib.core.policy_loss import action_logp, policy_loss
+    t = DTYPES[dtype]
+    low = [torch.finfo(t).min, -1e30 if t != torch.float16 else -6e4, -1e9 if t != torch.float16 else -3e4]
+    logits = torch.randn(6, V, generator=gen(V)).to(t)
+    for r in range(3):
+        logits[r, ::2] = low[r]
+        logits[3 + r] = low[r]
+    actions = torch.tensor([1, 3, 5, 0, 2, 4])
+    old = torch.log_softmax(logits.double(), 1).gather(1, actions[:, None])[:, 0].float()
+    adv = torch.tensor([1.0, -1.0, 0.5, 2.0, -0.5, 1.5])
+    x = logits.double().requires_grad_()
+    loss64, stats64 = ref.policy_loss(x, actions, old.double(), adv.double(), None, None, e_clip=0.2, kl_coef=0.0, entropy_coef=0.01)
+    (g64,) = torch.autograd.grad(loss64, x)
+    leaf = logits.cuda().requires_grad_()
+    loss, stats = policy_loss(leaf, actions.cuda(), old.cuda(), adv.cuda(), entropy_coef=0.01)
+    (g,) = torch.autograd.grad(loss, leaf)
+    n, size = 20 * 3 + 2 * 17 + V / 256 + 60, 3 * 3 * 10           # as above
+    close("loss", loss, loss64.detach(), n, size)
+    close("stats", stats[[0, 2, 3, 5]], stats64[[0, 2, 3, 5]], n, size)
+    close("dlogits", g, g64, n, size / 6)
+    lp, H = action_logp(leaf.detach(), actions.cuda())
+    ls = torch.log_softmax(logits.double(), 1)
+    close("logp", lp, ls.gather(1, actions[:, None])[:, 0], n, 20)
+    close("entropy", H, -(ls.exp() * ls).sum(1), n, 20)
+
+
+@pytest.mark.parametrize("R,V,dtype", [(1024, 33000, "f32"), (1024, 65536, "f32"), (1024, 66001, "f32"), (262144, 300, "f32"),
+                                       (4096, 33000, "bf16")])
+def test_loss_beyond_what_the_caches_hold_is_that_of_its_parts(R, V, dtype):
+    """Buffers from 128 and 256 MiB on are read and written past the caches; a quarter of the rows is four times their share exactly."""
+    from airgym_amd.lib.core.policy_loss import action_logp, policy_loss
+    g = torch.Generator("cuda").manual_seed(R + V)
+    logits = torch.randn(R, V, generator=g, device="cuda").to(DTYPES[dtype]).requires_grad_()
+    actions = torch.randint(0, V, (R,), generator=g, device="cuda")
+    lp, H = action_logp(logits.detach(), actions)
+    adv = torch.randn(R, generator=g, device="cuda")
+    old = lp + 0.1 * torch.randn(R, generator=g, device="cuda")
+    (whole,) = torch.autograd.grad(policy_loss(logits, actions, old, adv, entropy_coef=0.01)[0], logits)
+    for first in range(0, R, R // 4):
+        rows = slice(first, first + R // 4)
+        part = logits.detach()[rows].requires_grad_()
+        (grad,) = torch.autograd.grad(policy_loss(part, actions[rows], old[rows], adv[rows], entropy_coef=0.01)[0], part)
+        assert torch.equal(whole[rows] * 4, grad)
+        plp, pH = action_logp(part.detach(), actions[rows])
+        assert torch.equal(plp, lp[rows]) and torch.equal(pH, H[rows])
+
+
+@pytest.mark.parametrize("N", [16, 13, 32])
+def test_steps_of_states_beyond_what_the_caches_hold_are_those_of_their_parts(N):
+    from airgym_amd.lib.network.causal_conv import causal_conv_step
+    from airgym_amd.lib.network.selective_scan import selective_scan_step
+    g = torch.Generator("cuda").manual_seed(N)
+    for D in (2048, 2000 if N == 16 else 1000):
+        B = (128 << 20) // (D * N * 4) // 4 * 4 + 4
+
+        def rand(*shape):
+            return torch.randn(*shape, generator=g, device="cuda")
+
+        u, Bm, C, A, state = rand(B, D), rand(B, N), rand(B, N), -rand(D, N).abs(), rand(B, D, N)
+        parts = state.clone()
+        whole = selective_scan_step(u, u, A, Bm, C, state, u[0], u)
+        for rows in (slice(i * B // 4, (i + 1) * B // 4) for i in range(4)):
+            out = selective_scan_step(u[rows], u[rows], A, Bm[rows], C[rows], parts[rows], u[0], u[rows])
+            assert torch.equal(out, whole[rows])
+        assert torch.equal(parts, state)
+        for t in (torch.float32, torch.bfloat16):
+            W, D2 = 8, D - (N == 13)
+            B = (128 << 20) // (D2 * (W - 1) * (4 if t == torch.float32 else 2)) // 4 * 4 + 4
+            x, w, state = rand(B, D2).to(t), rand(D2, W), rand(B, W - 1, D2).to(t)
+            parts = state.clone()
+            whole = causal_conv_step(x, state, w)
+            for rows in (slice(i * B // 4, (i + 1) * B // 4) for i in range(4)):
+                assert torch.equal(causal_conv_step(x[rows], parts[rows], w), whole[rows])
+            assert torch.equal(parts, state)
 
 
 def test_policy_loss_of_rows_that_do_not_count_at_all():
