@@ -169,7 +169,8 @@ class AgTokenLossArgs(ctypes.Structure):
         [(n, ctypes.c_longlong) for n in ("R0", "R1", "s0", "s1")] + \
         [(n, ctypes.c_void_p) for n in ("logits_dev", "actions_dev", "old_logp_dev", "advantages_dev", "ref_logp_dev", "mask_dev")] + \
         [(n, ctypes.c_float) for n in ("e_clip", "kl_coef", "entropy_coef")] + \
-        [(n, ctypes.c_void_p) for n in ("loss_dev", "stats_dev", "dlogits_dev", "workspace_dev")] + [("workspace_bytes", ctypes.c_longlong)]
+        [(n, ctypes.c_void_p) for n in ("loss_dev", "stats_dev", "dlogits_dev", "workspace_dev")] + \
+        [("workspace_bytes", ctypes.c_longlong), ("dlogits_unit_dev", ctypes.c_void_p)]
 
 
 class AgInputLayerArgs(ctypes.Structure):
@@ -335,7 +336,7 @@ SYMBOLS = [
     ("ag_selective_scan_step", ctypes.c_int, [ctypes.POINTER(AgScanArgs), _P]),
     ("ag_token_policy_loss_workspace_bytes", ctypes.c_longlong, [ctypes.c_longlong, ctypes.c_int]),
     ("ag_token_policy_loss", ctypes.c_int, [ctypes.POINTER(AgTokenLossArgs), _P]),
-    ("ag_scale_by", ctypes.c_int, [_P, ctypes.c_longlong, ctypes.c_int, _P, _P]),
+    ("ag_scale_by", ctypes.c_int, [_P, ctypes.c_longlong, ctypes.c_int, _P, _P, _P]),
     ("ag_token_logp", ctypes.c_int, [_P] + [ctypes.c_longlong] * 4 + [ctypes.c_int, ctypes.c_int, _P, _P, _P, _P]),
 ]
 

@@ -26,7 +26,12 @@ struct LossArgs {
     long long R1, s0, s1, R;
     int V;
     float e_clip, kl_coef, entropy_coef, inv_R;
+    float* unit;                       // the gradient is stored divided by this power of two, or NULL
 };
+
+// 1 / rows that count, and the power of two at or below it
+__device__ __forceinline__ float share_of(const LossArgs& a) { return a.count ? a.count[2] : a.inv_R; }
+__device__ __forceinline__ float unit_of(float share) { return __uint_as_float(__float_as_uint(share) & 0x7f800000u); }
 
 // x of the lane that differs in bit 0, 1 (of a lane's four), 2 (mirrored within eight), 3 (within sixteen): no LDS, one instruction
 template <int kCtrl> __device__ __forceinline__ float across(float x) {
@@ -104,7 +109,8 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, float xa, l
     const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
     float f = plain >= held || plain != plain ? plain : 0.0f;
     if (a.ref_logp) f -= a.kl_coef * expm1_near(a.ref_logp[row] - r.lp);
-    const float n = a.count ? a.count[2] : a.inv_R;
+    float n = share_of(a);
+    if (a.unit) n /= unit_of(n);       // exact
     r.f = f * n;
     r.ent = a.entropy_coef * n * kLn2;
     r.k = __builtin_fmaf(a.entropy_coef * n, r.H, -r.f);
@@ -395,13 +401,15 @@ __global__ __launch_bounds__(kOneStage) void stats_kernel(LossArgs a, const doub
         for (int k = 0; k < kSums; k++) s[k] /= a.count ? (double)a.count[0] : (double)a.R, stats[k] = (float)s[k];
         loss[0] = (float)(s[0] + (double)a.kl_coef * s[1] - (double)a.entropy_coef * s[2]);
         stats[kSums] = a.count ? a.count[1] : (float)a.R;
+        if (a.unit) a.unit[0] = unit_of(share_of(a));
     }
 }
 
+// The gradient of a loss that is not the graph's root: a second rounding in the 16-bit types, unless the factor is a power of two.
 template <typename T>
-__global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const float* scale) {
+__global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const float* scale, const float* unit) {
     constexpr int E = 16 / sizeof(T);
-    const float g = scale[0];
+    const float g = unit ? scale[0] * unit[0] : scale[0];
     if (g == 1.0f) return;
     const long long full = n / E, step = (long long)gridDim.x * 256, i0 = (long long)blockIdx.x * 256 + threadIdx.x;
     for (long long i = i0; i < full; i += step) {
@@ -504,7 +512,7 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     double* parts = blocks ? (double*)(rows + R) : nullptr;
     const LossArgs a{p->logits_dev, p->actions_dev, p->old_logp_dev, p->advantages_dev, p->ref_logp_dev, p->mask_dev, p->dlogits_dev,
                      p->mask_dev ? count : nullptr, rows, nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef,
-                     p->entropy_coef, 1.0f / (float)R};
+                     p->entropy_coef, 1.0f / (float)R, p->dlogits_unit_dev};
     if (a.count) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p->mask_dev, R, count);
     AG_FOR_DTYPE(p->dtype, launch_rows<T>(a, stream));
     if (blocks) hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(kStatsThreads), 0, (hipStream_t)stream, a, parts);
@@ -517,16 +525,16 @@ extern "C" int ag_token_logp(const void* logits, long long R0, long long R1, lon
     if (!logits || !actions || !logp || R0 <= 0 || R1 <= 0 || V <= 0) return AG_ERR_INVALID_ARG;
     if (dtype < AG_F32 || dtype > AG_F16 || !launchable(R0, R1, V, dtype)) return AG_ERR_UNSUPPORTED;
     const LossArgs a{logits, actions, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, logp, entropy, R1, s0, s1, R0 * R1, V,
-                     0.0f, 0.0f, 0.0f, 0.0f};
+                     0.0f, 0.0f, 0.0f, 0.0f, nullptr};
     AG_FOR_DTYPE(dtype, launch_rows<T>(a, stream));
     return seq_status();
 }
 
-extern "C" int ag_scale_by(void* x, long long n, int dtype, const float* scale, void* stream) {
+extern "C" int ag_scale_by(void* x, long long n, int dtype, const float* scale, const float* unit, void* stream) {
     if (!x || !scale || n <= 0) return AG_ERR_INVALID_ARG;
     if (dtype < AG_F32 || dtype > AG_F16) return AG_ERR_UNSUPPORTED;
     const long long blocks = (n / 4 + 255) / 256 + 1;
     AG_FOR_DTYPE(dtype, hipLaunchKernelGGL((scale_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, (hipStream_t)stream,
-                                           (T*)x, n, scale));
+                                           (T*)x, n, scale, unit));
     return seq_status();
 }

@@ -6,7 +6,8 @@ Gaussian head, for a policy that answers with a choice - a discrete head, a toke
 
 averaged over the rows that `mask` counts.  exp(d) - d - 1 is the non-negative estimate of KL(policy || reference) from the action
 taken.  One pass writes the loss and its gradient: a forward under autograd already holds d loss / d logits, the backward only scales
-it (by nothing at all if the loss is the graph's root)."""
+it (by nothing at all if the loss is the graph's root).  A mean over many rows has gradients below float16's range: for such logits the
+forward's gradient is that of about one row, and the backward brings in the rest together with whatever the loss was scaled by."""
 import ctypes
 
 import torch
@@ -24,23 +25,24 @@ def _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, want_g
     dev = logits.device
     loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(6, dtype=torch.float32, device=dev)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
+    unit = torch.empty((), dtype=torch.float32, device=dev) if want_grad and logits.dtype == torch.float16 else None
     logits, r0, r1, v, s0, s1 = _table(logits)
     n = lib.ag_token_policy_loss_workspace_bytes(r0 * r1, v)
     ws = torch.empty(n, dtype=torch.uint8, device=dev)
     a = N.AgTokenLossArgs(_ARGS, N.AG_DTYPES[logits.dtype], v, r0, r1, s0, s1, logits.data_ptr(), actions.data_ptr(),
                           old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(mask), *coefs, loss.data_ptr(),
-                          stats.data_ptr(), ptr(grad), ws.data_ptr(), n)
+                          stats.data_ptr(), ptr(grad), ws.data_ptr(), n, ptr(unit))
     with on_device_of(logits):
         N.check(lib.ag_token_policy_loss(ctypes.byref(a), stream_of(logits)), "ag_token_policy_loss")
-    return loss, stats, grad
+    return loss, stats, grad, unit
 
 
 class _TokenPolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, coefs, train):
-        loss, stats, grad = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, train)
+        loss, stats, grad, unit = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, train)
         ctx.save_for_backward(logits, actions, old_logp, advantages, ref_logp, mask)
-        ctx.coefs, ctx.grad = coefs, grad
+        ctx.coefs, ctx.grad, ctx.unit = coefs, grad, unit
         ctx.mark_non_differentiable(stats)
         ctx.set_materialize_grads(False)
         return loss, stats
@@ -52,12 +54,12 @@ class _TokenPolicyLoss(torch.autograd.Function):
             return (None,) * 8
         # the gradient is handed over, not kept: autograd may go on to add to it in place.  A second pass over a retained graph forms
         # it again.
-        grad, ctx.grad = ctx.grad, None
+        grad, unit, ctx.grad = ctx.grad, ctx.unit, None
         if grad is None:
-            grad = _launch(*ctx.saved_tensors, ctx.coefs, True)[2]
+            _, _, grad, unit = _launch(*ctx.saved_tensors, ctx.coefs, True)
         with on_device_of(grad):
-            N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], dloss.data_ptr(), stream_of(grad)),
-                    "ag_scale_by")
+            N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], dloss.data_ptr(), ptr(unit),
+                                           stream_of(grad)), "ag_scale_by")
         return (grad,) + (None,) * 7
 
 

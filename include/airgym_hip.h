@@ -902,7 +902,9 @@ int ag_selective_scan_step(const ag_scan_args* args, void* stream);
  * Logits of -inf are choices that are not available: probability 0, gradient 0.
  *   loss_dev [1]; stats_dev [6] = {policy loss, KL term, entropy, KL of the old policy to this one (r - 1 - log r), fraction of rows
  *       whose r left the clip range, rows counted}
- *   dlogits_dev [R, V] contiguous in the logits' type, or NULL
+ *   dlogits_dev [R, V] contiguous in the logits' type, or NULL.  With dlogits_unit_dev (f32 [1]) it holds the gradient divided by that
+ *       number, which the call writes: the power of two at or below 1 / rows counted.  A mean over many rows leaves float16's range, and
+ *       what is lost there no loss scale brings back: ag_scale_by takes unit and scale together.
  *   workspace_dev: ag_token_policy_loss_workspace_bytes(R, V) bytes, 16-byte aligned. */
 typedef struct ag_token_loss_args {
     uint32_t struct_size;              /* = sizeof(ag_token_loss_args), ABI guard */
@@ -920,11 +922,13 @@ typedef struct ag_token_loss_args {
     void* dlogits_dev;
     void* workspace_dev;
     long long workspace_bytes;
+    float* dlogits_unit_dev;           /* [1] or NULL */
 } ag_token_loss_args;
 long long ag_token_policy_loss_workspace_bytes(long long R, int V);
 int ag_token_policy_loss(const ag_token_loss_args* args, void* stream);
-/* x *= *scale_dev in place over n elements; a factor of exactly 1 touches nothing (the gradient of a loss that is the graph's root) */
-int ag_scale_by(void* x_dev, long long n, int dtype, const float* scale_dev, void* stream);
+/* x *= *scale_dev * *unit_dev (NULL: 1) in place over n elements; a factor of exactly 1 touches nothing (the gradient of a loss that is
+ * the graph's root) */
+int ag_scale_by(void* x_dev, long long n, int dtype, const float* scale_dev, const float* unit_dev, void* stream);
 /* log-probability of each row's action and the row's entropy: logp_dev, entropy_dev f32 [R] (entropy NULL: not written) */
 int ag_token_logp(const void* logits_dev, long long R0, long long R1, long long s0, long long s1, int V, int dtype,
                   const long long* actions_dev, float* logp_dev, float* entropy_dev, void* stream);

@@ -508,6 +508,34 @@ def test_policy_loss_scaled_and_backward_twice():
     assert torch.equal(l2, loss) and torch.equal(torch.autograd.grad(l2, flat)[0].view_as(first), first)
 
 
+@pytest.mark.parametrize("V", [11, 900])
+@pytest.mark.parametrize("masked", [False, True])
+def test_policy_loss_in_half_precision_under_a_loss_scale(V, masked):
+    """The mean over 30000 rows takes most gradients below float16's smallest numbers (6e-8); scaled by 2^15 they are back."""
+    from airgym_amd.lib.core.policy_loss import policy_loss
+    R, scale = 30000, 2.0 ** 15
+    g = torch.Generator("cuda").manual_seed(V)
+    logits = torch.randn(R, V, generator=g, device="cuda").half()
+    actions = torch.randint(0, V, (R,), generator=g, device="cuda")
+    adv = torch.randn(R, generator=g, device="cuda")
+    mask = torch.rand(R, generator=g, device="cuda") < 0.7 if masked else None
+    old = torch.log_softmax(logits.double(), 1).gather(1, actions[:, None])[:, 0].float()        # ratio one: f = -A
+    leaf = logits.clone().requires_grad_()
+    (got,) = torch.autograd.grad(scale * policy_loss(leaf, actions, old, adv, mask=mask)[0], leaf)
+    on = torch.ones(R, dtype=torch.bool, device="cuda") if mask is None else mask
+    p = torch.softmax(logits.double(), 1)
+    want = p * adv.double()[:, None]
+    want.scatter_add_(1, actions[:, None], -adv.double()[:, None])
+    want = torch.where(on[:, None], want, 0.0) * (scale / int(on.sum()))
+    # 60 roundings on the way to p and f (sizes: p <= 1, |f| <= largest |A|), then one in float16
+    n, size = 60 + 20 * 3 + V / 256, float(adv.abs().max()) * scale / int(on.sum())
+    close("dlogits", got, want.cpu(), n, size)
+    again = logits.clone().requires_grad_()
+    loss, _ = policy_loss(again, actions, old, adv, mask=mask)
+    first = torch.autograd.grad(scale * loss, again, retain_graph=True)[0]
+    assert torch.equal(first, got) and torch.equal(torch.autograd.grad(scale * loss, again)[0], got)
+
+
 # ------------------------------------------------------------------------------------------------ far rows, repeats
 def _far(t, gap):
     """t [2, ...] with its two rows more than 2^32 bytes apart."""

@@ -77,7 +77,7 @@ def test_loss_entries_refuse(lib):
     assert lib.ag_token_logp(p, 1 << 26, 1, 300, 300, 300, 0, p, p, p, None) == -6
     assert lib.ag_token_logp(p, 1 << 22, 1, 9000, 9000, 9000, 0, p, p, p, None) == -6
     assert lib.ag_token_policy_loss_workspace_bytes(3, 2147483647) > 0
-    assert lib.ag_scale_by(p, 0, 0, p, None) == -1 and lib.ag_scale_by(p, 4, 9, p, None) == -6
+    assert lib.ag_scale_by(p, 0, 0, p, None, None) == -1 and lib.ag_scale_by(p, 4, 9, p, None, None) == -6
 
 
 def test_argument_blocks_match_the_header(tmp_path):
