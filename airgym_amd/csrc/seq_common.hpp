@@ -167,8 +167,13 @@ template <typename Out>
 __global__ __launch_bounds__(256) void sum_few_rows_kernel(const float* table, int rows, long long n, Out out) {
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
         float s = 0.0f;
-#pragma unroll 8
-        for (int r = 0; r < rows; r++) s += table[(long long)r * n + i];
+        for (int r = 0; r < rows; r += 4) {                     // four rows' loads at a time, added in order
+            float v[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = r + k < rows ? table[(long long)(r + k) * n + i] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) s += v[k];
+        }
         out(i, s);
     }
 }
