@@ -687,6 +687,44 @@ def test_all_operators_together_on_another_stream():
         assert torch.equal(a, b), k
 
 
+def test_two_streams_and_two_graphs_at_once():
+    """Calls in flight together share no workspace: each side's results are those it has alone."""
+    sides = [_together_inputs(seed) for seed in (6, 7)]
+    streams = [torch.cuda.Stream() for _ in sides]
+
+    def once(p, data):
+        loss, stats = _together(data[0], p, *data[1:])
+        return [loss.detach(), stats, *torch.autograd.grad(loss, list(p.values()))]
+
+    alone = [once(*side) for side in sides]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(3):
+        for k, (side, stream) in enumerate(zip(sides, streams)):
+            with torch.cuda.stream(stream):
+                got[k].append(once(*side))
+    torch.cuda.synchronize()
+    for k in range(2):
+        for run in got[k]:
+            assert all(torch.equal(a, b) for a, b in zip(alone[k], run))
+    del got
+    graphs = []
+    for side in sides:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = once(*side)
+        graphs.append((graph, out))
+    for _ in range(3):
+        for (graph, out), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                for t in out:
+                    t.zero_()
+                graph.replay()
+        torch.cuda.synchronize()
+        for (_, out), want in zip(graphs, alone):
+            assert all(torch.equal(a, b) for a, b in zip(want, out))
+
+
 def test_all_operators_together_captured_and_replayed():
     """Forward and backward as one graph; every replay against the eager result on the same inputs, with eager work in between."""
     p, data = _together_inputs(1)
