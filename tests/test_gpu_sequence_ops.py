@@ -159,6 +159,9 @@ SCAN = [  # B, T, D, N, G, lengths, resets, state, z, D, bias, softplus
     (2, 260, 9, 3, 1, [129, 260], 0.01, True, True, True, True, True),
     (1, 129, 8, 32, 1, None, 0.05, False, False, True, True, True),
     (2, 192, 8, 4, 1, [65, 192], 0.0, True, True, True, False, False),
+    (4, 700, 40, 16, 1, [700, 0, 5, 333], 0.02, True, True, True, True, True),
+    (3, 515, 70, 13, 1, [16, 515, 257], 0.0, True, True, True, True, True),
+    (2, 400, 20, 32, 2, [1, 400], 0.01, True, False, True, True, True),
 ]
 NAMES = ("u", "delta", "A", "B", "C", "D", "z", "bias", "state")
 
