@@ -830,9 +830,10 @@ int step_lanes(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : 8; }
 int channel_blocks(int D, int G) { return (D / G + kLanes - 1) / kLanes; }
 
 // Chunks of time.  1536 workgroups are six per CU, what the forward's registers let in and two rounds of the backward; where sequences
-// and channels give fewer, time is cut so that there are about that many, in chunks of at least 64 steps (a multiple of 16).  Measured
-// at B = 8, T = 2047, D = 2048, bf16, ragged: 1024 workgroups 235 + 530 us (forward + backward), 1536 200 + 510, twice as many 195 + 508;
-// at B = 1, T = 4096, D = 2048, where each chunk has more chunks before it to start from: 88, 100 and 98 us.
+// and channels give fewer, time is cut so that there are about that many, in chunks of at least 64 steps (a multiple of 16).  Forward and
+// backward in bf16 with 768, 1024, 1536, 2304 and twice 1536 workgroups: 785, 722, 657, 652 and 646 us at B = 8, T = 2047, D = 2048 with lengths
+// drawn evenly; 864, 914, 833, 857 and 853 in full length; 263, 268, 279, 291 and 290 at B = 1, T = 4096, where each chunk has more chunks
+// before it to start from.
 int chunks_of(int B, int T, int D, int G) {
     const long long blocks = (long long)B * G * channel_blocks(D, G);
     const long long want = (1536 + blocks - 1) / blocks;
