@@ -108,7 +108,7 @@ def causal_conv_step(x, state, weight, bias=None, *, activation="silu", resets=N
     state = in_place_state("state", state, (B, W - 1, D), x.dtype, device)
     resets = flags_of("resets", resets, (B,), device)
     silu = _activation(activation)
-    y = torch.empty((B, D), dtype=x.dtype, device=device)
+    y = torch.empty_like(x) if x.is_contiguous() else torch.empty((B, D), dtype=x.dtype, device=device)      # (half a microsecond apart)
     if x.numel() == 0:
         return y
     if resets is not None and not resets.is_contiguous():

@@ -159,7 +159,7 @@ def selective_scan_step(u, delta, A, B, C, state, D=None, z=None, delta_bias=Non
         raise ValueError(f"B and C: {list(B.shape)} and {list(C.shape)}")
     state = in_place_state("state", state, (b, d, n), torch.float32, device)
     resets = flags_of("resets", resets, (b,), device)
-    out = torch.empty((b, d), dtype=u.dtype, device=device)
+    out = torch.empty_like(u) if u.is_contiguous() else torch.empty((b, d), dtype=u.dtype, device=device)
     if u.numel() == 0:
         return out
     at = state.data_ptr()
