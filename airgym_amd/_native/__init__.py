@@ -28,6 +28,7 @@ AG_FLAG_STAGGER_PHASE = 1 << 3
 AG_NUM_REWARD_TERMS = 11
 
 AG_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # ag_dtype
+AG_TOKEN_KEPT_ROW_FLOATS = 8
 
 AG_ERR_UNKNOWN_TASK = -2
 AG_ERR_UNKNOWN_CTL = -3
@@ -170,7 +171,7 @@ class AgTokenLossArgs(ctypes.Structure):
         [(n, ctypes.c_void_p) for n in ("logits_dev", "actions_dev", "old_logp_dev", "advantages_dev", "ref_logp_dev", "mask_dev")] + \
         [(n, ctypes.c_float) for n in ("e_clip", "kl_coef", "entropy_coef")] + \
         [(n, ctypes.c_void_p) for n in ("loss_dev", "stats_dev", "dlogits_dev", "workspace_dev")] + \
-        [("workspace_bytes", ctypes.c_longlong), ("dlogits_unit_dev", ctypes.c_void_p)]
+        [("workspace_bytes", ctypes.c_longlong), ("kept_rows_dev", ctypes.c_void_p)]
 
 
 class AgInputLayerArgs(ctypes.Structure):
@@ -336,7 +337,8 @@ SYMBOLS = [
     ("ag_selective_scan_step", ctypes.c_int, [ctypes.POINTER(AgScanArgs), _P]),
     ("ag_token_policy_loss_workspace_bytes", ctypes.c_longlong, [ctypes.c_longlong, ctypes.c_int]),
     ("ag_token_policy_loss", ctypes.c_int, [ctypes.POINTER(AgTokenLossArgs), _P]),
-    ("ag_scale_by", ctypes.c_int, [_P, ctypes.c_longlong, ctypes.c_int, _P, _P, _P]),
+    ("ag_scale_by", ctypes.c_int, [_P, ctypes.c_longlong, ctypes.c_int, _P, _P]),
+    ("ag_token_policy_grad", ctypes.c_int, [_P, _P, ctypes.c_longlong, ctypes.c_int, ctypes.c_int, _P, _P]),
     ("ag_token_logp", ctypes.c_int, [_P] + [ctypes.c_longlong] * 4 + [ctypes.c_int, ctypes.c_int, _P, _P, _P, _P]),
 ]
 

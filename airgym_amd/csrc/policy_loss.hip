@@ -9,6 +9,9 @@
 // Every wave sums against a maximum of its own and the waves' results are joined.  Memory bounds it in float32: 8192 x 32000 with the
 // gradient takes 365 us = 5.7 TB/s, the log-probabilities alone 172 us = 6.1 TB/s.  In the 16-bit types the two exponentials and some 15
 // other instructions per element bound it as much: 8192 x 32000 bfloat16 takes 224 us = 4.7 TB/s, the vector pipe busy for 85 % of it.
+// float16 logits under autograd are the exception: a row's factors span more than their type does - a mean over many rows is below 6e-8 where
+// a single row's ratio may be above 65504 -, so that their gradient cannot be rounded before what the loss is scaled by is known.  The
+// forward leaves a copy of the logits and each row's factors, the backward forms the gradient in the copy's place, rounded once.
 // Logits of -inf have probability 0.  Their infinite log-probability would meet it as 0 times inf: a wave that finds its second sum
 // NaN forms it again with the log-probability held at -1e30; the gradient holds it there always.
 #include "seq_common.hpp"
@@ -18,6 +21,11 @@ namespace {
 constexpr float kFloor = -1e30f;
 constexpr int kSums = 5;               // policy loss, KL term, entropy, KL of the old policy, clipped
 
+// what a row's gradient is formed from later: `act` < 0 is an action out of range, kUncounted a row that does not count
+struct KeptRow { float base, lS, f, k, ent; int act, pad[2]; };
+static_assert(sizeof(KeptRow) == AG_TOKEN_KEPT_ROW_FLOATS * sizeof(float), "a row of kept_rows_dev");
+constexpr int kUncounted = -2;
+
 struct LossArgs {
     const void* logits; const long long* actions; const float *old_logp, *adv, *ref_logp; const unsigned char* mask;
     void* dlogits; const float* count; // {max(rows that count, 1), rows that count, 1 / the first}, or NULL: all R
@@ -26,12 +34,13 @@ struct LossArgs {
     long long R1, s0, s1, R;
     int V;
     float e_clip, kl_coef, entropy_coef, inv_R;
-    float* unit;                       // the gradient is stored divided by this power of two, or NULL
+    KeptRow* kept;                     // [R], float16: dlogits gets the logits themselves, this what their gradient takes besides; or NULL
 };
 
-// 1 / rows that count, and the power of two at or below it
+// 1 / rows that count
 __device__ __forceinline__ float share_of(const LossArgs& a) { return a.count ? a.count[2] : a.inv_R; }
-__device__ __forceinline__ float unit_of(float share) { return __uint_as_float(__float_as_uint(share) & 0x7f800000u); }
+// whether the logits are kept for a later gradient (compiled for float16 only)
+template <typename T> __device__ __forceinline__ bool keeps(const LossArgs& a) { return __is_same(T, f16_t) && a.kept; }
 
 // x of the lane that differs in bit 0, 1 (of a lane's four), 2 (mirrored within eight), 3 (within sixteen): no LDS, one instruction
 template <int kCtrl> __device__ __forceinline__ float across(float x) {
@@ -109,8 +118,7 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, float xa, l
     const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
     float f = plain >= held || plain != plain ? plain : 0.0f;
     if (a.ref_logp) f -= a.kl_coef * expm1_near(a.ref_logp[row] - r.lp);
-    float n = share_of(a);
-    if (a.unit) n /= unit_of(n);       // exact
+    const float n = share_of(a);
     r.f = f * n;
     r.ent = a.entropy_coef * n * kLn2;
     r.k = __builtin_fmaf(a.entropy_coef * n, r.H, -r.f);
@@ -118,7 +126,7 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, float xa, l
 }
 
 // f (delta - p) + ent p (log p + H) without the delta
-__device__ __forceinline__ float grad_of(const Row& r, float x) {
+template <typename R> __device__ __forceinline__ float grad_of(const R& r, float x) {
     const float q = fmaxf(__builtin_fmaf(x - r.base, kLog2e, -r.lS), kFloor);      // log2 p
     return exp2_hw(q) * __builtin_fmaf(r.ent, q, r.k);
 }
@@ -174,6 +182,7 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
             }
         }
     }
+    if (keeps<T>(a) && there && l == 0) a.kept[row] = on ? KeptRow{r.base, r.lS, r.f, r.k, r.ent, act, {0, 0}} : KeptRow{0, 0, 0, 0, 0, kUncounted, {0, 0}};
     if (a.dlogits && there) {
         T* dx = (T*)a.dlogits + row * a.V;
 #pragma unroll
@@ -181,7 +190,7 @@ __global__ __launch_bounds__(kShortThreads) void token_loss_short_kernel(LossArg
             const int j = l + k * L;
             if (j < a.V) {
                 float g = 0.0f;
-                if (on) g = grad_of(r, x[k]) + (j == act ? r.f : 0.0f);
+                if (on) g = keeps<T>(a) ? x[k] : grad_of(r, x[k]) + (j == act ? r.f : 0.0f);
                 dx[j] = from_f32<T>(g);
             }
         }
@@ -202,6 +211,10 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     const int full = a.V / E, nq = NV ? NV : (full + THREADS - 1) / THREADS;      // whole accesses of the row, per thread
     const int tail = full * E + threadIdx.x;                                        // the elements behind them: one per thread
     if (a.mask && !a.mask[row]) {
+        if (keeps<T>(a)) {
+            if (threadIdx.x == 0) a.kept[row] = KeptRow{0, 0, 0, 0, 0, kUncounted, {0, 0}};
+            return;
+        }
         const Vec<T, E> zero{{0, 0, 0, 0}};
         if (dx) {
             for (int q = threadIdx.x; q < full; q += THREADS) store_vec<T, E, kOnceOut>(dx + q * E, zero);
@@ -285,11 +298,18 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
         }
         return;
     }
-    if (threadIdx.x == 0) a.rows[row] = float4{xa, r.base, v.s, v.t};
+    if (threadIdx.x == 0) {
+        a.rows[row] = float4{xa, r.base, v.s, v.t};
+        if (keeps<T>(a)) a.kept[row] = KeptRow{r.base, r.lS, r.f, r.k, r.ent, act, {0, 0}};
+    }
     if (!dx) return;
     const int aq = act >= 0 ? act / E : -1, ai = act % E;
     auto gradient = [&](int q, const Vec<T, E>& held) __attribute__((always_inline)) {
         if (q >= full) return;
+        if (keeps<T>(a)) {
+            store_vec<T, E, kOnceOut>(dx + q * E, held);
+            return;
+        }
         float g[E];
 #pragma unroll
         for (int i = 0; i < E; i++) g[i] = grad_of(r, held.at(i));
@@ -307,7 +327,7 @@ __global__ __launch_bounds__(THREADS) void token_loss_kernel(LossArgs a) {
     } else {
         for (int q = threadIdx.x; q < full; q += THREADS) gradient(q, load_vec<T, E>(x + q * E));
     }
-    if (tail < a.V) dx[tail] = from_f32<T>(grad_of(r, xt) + (tail == act ? r.f : 0.0f));
+    if (tail < a.V) dx[tail] = from_f32<T>(keeps<T>(a) ? xt : grad_of(r, xt) + (tail == act ? r.f : 0.0f));
 }
 
 __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, long long R, float* count) {
@@ -401,15 +421,15 @@ __global__ __launch_bounds__(kOneStage) void stats_kernel(LossArgs a, const doub
         for (int k = 0; k < kSums; k++) s[k] /= a.count ? (double)a.count[0] : (double)a.R, stats[k] = (float)s[k];
         loss[0] = (float)(s[0] + (double)a.kl_coef * s[1] - (double)a.entropy_coef * s[2]);
         stats[kSums] = a.count ? a.count[1] : (float)a.R;
-        if (a.unit) a.unit[0] = unit_of(share_of(a));
     }
 }
 
-// The gradient of a loss that is not the graph's root: a second rounding in the 16-bit types, unless the factor is a power of two.
+// The gradient of a loss that is not the graph's root: in bfloat16 a second rounding, unless the factor is a power of two.  (float16 has
+// the kernel below.)
 template <typename T>
-__global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const float* scale, const float* unit) {
+__global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const float* scale) {
     constexpr int E = 16 / sizeof(T);
-    const float g = unit ? scale[0] * unit[0] : scale[0];
+    const float g = scale[0];
     if (g == 1.0f) return;
     const long long full = n / E, step = (long long)gridDim.x * 256, i0 = (long long)blockIdx.x * 256 + threadIdx.x;
     for (long long i = i0; i < full; i += step) {
@@ -421,6 +441,40 @@ __global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const flo
         store_vec<T, E>(x + i * E, c);
     }
     if (full * E + i0 < n) x[full * E + i0] = from_f32<T>(to_f32(x[full * E + i0]) * g);
+}
+
+// The gradient of kept logits, in their place, times the loss's factor: rounded once.  A thread takes 16 bytes at a time wherever the rows'
+// borders lie, and moves on by a fixed number of rows and columns, so that it divides once.  Its bytes bound it.
+__global__ __launch_bounds__(256) void kept_grad_kernel(f16_t* x, const KeptRow* rows, long long n, int V, const float* scale) {
+    constexpr int E = 16 / sizeof(f16_t);
+    const float g = scale[0];
+    const long long step = (long long)gridDim.x * 256 * E, rows_on = step / V;
+    const int cols_on = (int)(step - rows_on * V);
+    long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * E, row = i / V;
+    int col = (int)(i - row * V);
+    for (; i < n; i += step, row += rows_on, col += cols_on) {         // (col + cols_on < 2^31: V is at most 2^30)
+        if (col >= V) col -= V, row++;
+        const int m = n - i < E ? (int)(n - i) : E;
+        Vec<f16_t, E> c;
+        if (m == E) c = load_vec<f16_t, E>(x + i);
+        float v[E];
+        long long at = row;
+        int j = col;
+        KeptRow r = rows[at];
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            if (k >= m) break;
+            if (j == V) j = 0, r = rows[++at];                          // k < m: the row is there
+            const float e = m == E ? c.at(k) : to_f32(x[i + k]);
+            v[k] = r.act == kUncounted ? 0.0f : (grad_of(r, e) + (j == r.act ? r.f : 0.0f)) * g;
+            j++;
+        }
+        if (m == E) {
+            c.set(v);
+            store_vec<f16_t, E>(x + i, c);
+        } else
+            for (int k = 0; k < m; k++) x[i + k] = from_f32<f16_t>(v[k]);
+    }
 }
 
 }  // namespace
@@ -504,6 +558,7 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
         !p->loss_dev || !p->stats_dev || !p->workspace_dev || p->R0 <= 0 || p->R1 <= 0 || p->V <= 0)
         return AG_ERR_INVALID_ARG;
     if (p->dtype < AG_F32 || p->dtype > AG_F16 || !launchable(p->R0, p->R1, p->V, p->dtype)) return AG_ERR_UNSUPPORTED;
+    if (p->kept_rows_dev && (p->dtype != AG_F16 || !p->dlogits_dev)) return AG_ERR_INVALID_ARG;
     const long long R = p->R0 * p->R1;
     if (p->workspace_bytes < ag_token_policy_loss_workspace_bytes(R, p->V)) return AG_ERR_INVALID_ARG;
     float* count = (float*)p->workspace_dev;                 // 4 floats, then the rows' sums, then the first stage's
@@ -512,7 +567,7 @@ extern "C" int ag_token_policy_loss(const ag_token_loss_args* p, void* stream) {
     double* parts = blocks ? (double*)(rows + R) : nullptr;
     const LossArgs a{p->logits_dev, p->actions_dev, p->old_logp_dev, p->advantages_dev, p->ref_logp_dev, p->mask_dev, p->dlogits_dev,
                      p->mask_dev ? count : nullptr, rows, nullptr, nullptr, p->R1, p->s0, p->s1, R, p->V, p->e_clip, p->kl_coef,
-                     p->entropy_coef, 1.0f / (float)R, p->dlogits_unit_dev};
+                     p->entropy_coef, 1.0f / (float)R, (KeptRow*)p->kept_rows_dev};
     if (a.count) hipLaunchKernelGGL(count_kernel, dim3(1), dim3(1024), 0, (hipStream_t)stream, p->mask_dev, R, count);
     AG_FOR_DTYPE(p->dtype, launch_rows<T>(a, stream));
     if (blocks) hipLaunchKernelGGL(stats_part_kernel, dim3((unsigned)blocks), dim3(kStatsThreads), 0, (hipStream_t)stream, a, parts);
@@ -530,11 +585,20 @@ extern "C" int ag_token_logp(const void* logits, long long R0, long long R1, lon
     return seq_status();
 }
 
-extern "C" int ag_scale_by(void* x, long long n, int dtype, const float* scale, const float* unit, void* stream) {
+extern "C" int ag_scale_by(void* x, long long n, int dtype, const float* scale, void* stream) {
     if (!x || !scale || n <= 0) return AG_ERR_INVALID_ARG;
     if (dtype < AG_F32 || dtype > AG_F16) return AG_ERR_UNSUPPORTED;
     const long long blocks = (n / 4 + 255) / 256 + 1;
     AG_FOR_DTYPE(dtype, hipLaunchKernelGGL((scale_kernel<T>), dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, (hipStream_t)stream,
-                                           (T*)x, n, scale, unit));
+                                           (T*)x, n, scale));
+    return seq_status();
+}
+
+extern "C" int ag_token_policy_grad(void* x, const float* kept_rows, long long R, int V, int dtype, const float* scale, void* stream) {
+    if (!x || !kept_rows || !scale || R <= 0 || V <= 0) return AG_ERR_INVALID_ARG;
+    if (dtype != AG_F16 || !launchable(1, R, V, dtype)) return AG_ERR_UNSUPPORTED;
+    const long long n = R * V, blocks = (n / 8 + 255) / 256 + 1;
+    hipLaunchKernelGGL(kept_grad_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, (hipStream_t)stream, (f16_t*)x,
+                       (const KeptRow*)kept_rows, n, V, scale);
     return seq_status();
 }

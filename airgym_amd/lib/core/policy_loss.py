@@ -6,8 +6,9 @@ Gaussian head, for a policy that answers with a choice - a discrete head, a toke
 
 averaged over the rows that `mask` counts.  exp(d) - d - 1 is the non-negative estimate of KL(policy || reference) from the action
 taken.  One pass writes the loss and its gradient: a forward under autograd already holds d loss / d logits, the backward only scales
-it (by nothing at all if the loss is the graph's root).  A mean over many rows has gradients below float16's range: for such logits the
-forward's gradient is that of about one row, and the backward brings in the rest together with whatever the loss was scaled by."""
+it (by nothing at all if the loss is the graph's root; bfloat16 gradients are rounded a second time by any factor that is no power of two).
+float16 holds neither the gradients of a mean over many rows nor those of a single row with a large ratio: for such logits the forward
+keeps a copy of the logits, and the backward forms the gradient in its place, together with whatever the loss was scaled by."""
 import ctypes
 
 import torch
@@ -18,6 +19,7 @@ from airgym_amd.lib.core.native_call import activation, flags_of, on_device_of, 
 
 STATS = ("policy_loss", "kl", "entropy", "old_kl", "clip_frac", "rows")
 _ARGS = ctypes.sizeof(N.AgTokenLossArgs)
+_KEPT = 4 * N.AG_TOKEN_KEPT_ROW_FLOATS
 
 
 def _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, want_grad):
@@ -25,24 +27,25 @@ def _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, want_g
     dev = logits.device
     loss, stats = torch.empty((), dtype=torch.float32, device=dev), torch.empty(6, dtype=torch.float32, device=dev)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=dev) if want_grad else None
-    unit = torch.empty((), dtype=torch.float32, device=dev) if want_grad and logits.dtype == torch.float16 else None
     logits, r0, r1, v, s0, s1 = _table(logits)
     n = lib.ag_token_policy_loss_workspace_bytes(r0 * r1, v)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    keep = r0 * r1 * _KEPT if want_grad and logits.dtype == torch.float16 else 0
+    ws = torch.empty(keep + n, dtype=torch.uint8, device=dev)         # the rows that are kept first
+    at = ws.data_ptr()
     a = N.AgTokenLossArgs(_ARGS, N.AG_DTYPES[logits.dtype], v, r0, r1, s0, s1, logits.data_ptr(), actions.data_ptr(),
                           old_logp.data_ptr(), advantages.data_ptr(), ptr(ref_logp), ptr(mask), *coefs, loss.data_ptr(),
-                          stats.data_ptr(), ptr(grad), ws.data_ptr(), n, ptr(unit))
+                          stats.data_ptr(), ptr(grad), at + keep, n, at if keep else None)
     with on_device_of(logits):
         N.check(lib.ag_token_policy_loss(ctypes.byref(a), stream_of(logits)), "ag_token_policy_loss")
-    return loss, stats, grad, unit
+    return loss, stats, grad, ws if keep else None
 
 
 class _TokenPolicyLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, old_logp, advantages, ref_logp, mask, coefs, train):
-        loss, stats, grad, unit = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, train)
+        loss, stats, grad, kept = _launch(logits, actions, old_logp, advantages, ref_logp, mask, coefs, train)
         ctx.save_for_backward(logits, actions, old_logp, advantages, ref_logp, mask)
-        ctx.coefs, ctx.grad, ctx.unit = coefs, grad, unit
+        ctx.coefs, ctx.grad, ctx.kept = coefs, grad, kept
         ctx.mark_non_differentiable(stats)
         ctx.set_materialize_grads(False)
         return loss, stats
@@ -54,12 +57,16 @@ class _TokenPolicyLoss(torch.autograd.Function):
             return (None,) * 8
         # the gradient is handed over, not kept: autograd may go on to add to it in place.  A second pass over a retained graph forms
         # it again.
-        grad, unit, ctx.grad = ctx.grad, ctx.unit, None
+        grad, kept, ctx.grad, ctx.kept = ctx.grad, ctx.kept, None, None
         if grad is None:
-            _, _, grad, unit = _launch(*ctx.saved_tensors, ctx.coefs, True)
+            _, _, grad, kept = _launch(*ctx.saved_tensors, ctx.coefs, True)
+        lib, dtype = N.load(), N.AG_DTYPES[grad.dtype]
         with on_device_of(grad):
-            N.check(N.load().ag_scale_by(grad.data_ptr(), grad.numel(), N.AG_DTYPES[grad.dtype], dloss.data_ptr(), ptr(unit),
-                                           stream_of(grad)), "ag_scale_by")
+            if kept is None:
+                N.check(lib.ag_scale_by(grad.data_ptr(), grad.numel(), dtype, dloss.data_ptr(), stream_of(grad)), "ag_scale_by")
+            else:
+                N.check(lib.ag_token_policy_grad(grad.data_ptr(), kept.data_ptr(), grad.numel() // grad.shape[-1], grad.shape[-1], dtype,
+                                                 dloss.data_ptr(), stream_of(grad)), "ag_token_policy_grad")
         return (grad,) + (None,) * 7
 
 

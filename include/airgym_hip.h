@@ -902,9 +902,10 @@ int ag_selective_scan_step(const ag_scan_args* args, void* stream);
  * Logits of -inf are choices that are not available: probability 0, gradient 0.
  *   loss_dev [1]; stats_dev [6] = {policy loss, KL term, entropy, KL of the old policy to this one (r - 1 - log r), fraction of rows
  *       whose r left the clip range, rows counted}
- *   dlogits_dev [R, V] contiguous in the logits' type, or NULL.  With dlogits_unit_dev (f32 [1]) it holds the gradient divided by that
- *       number, which the call writes: the power of two at or below 1 / rows counted.  A mean over many rows leaves float16's range, and
- *       what is lost there no loss scale brings back: ag_scale_by takes unit and scale together.
+ *   dlogits_dev [R, V] contiguous in the logits' type, or NULL.  With kept_rows_dev (float16 only) it gets the logits of the rows that count
+ *       instead, and kept_rows_dev what their gradient takes besides: ag_token_policy_grad forms it in their place.  A mean over many rows is
+ *       below float16's range and a single row's ratio may be above it, so that the type cannot hold the gradient before it is known what
+ *       the loss is scaled by.
  *   workspace_dev: ag_token_policy_loss_workspace_bytes(R, V) bytes, 16-byte aligned. */
 typedef struct ag_token_loss_args {
     uint32_t struct_size;              /* = sizeof(ag_token_loss_args), ABI guard */
@@ -922,13 +923,16 @@ typedef struct ag_token_loss_args {
     void* dlogits_dev;
     void* workspace_dev;
     long long workspace_bytes;
-    float* dlogits_unit_dev;           /* [1] or NULL */
+    float* kept_rows_dev;              /* [R, AG_TOKEN_KEPT_ROW_FLOATS], 16-byte aligned, or NULL */
 } ag_token_loss_args;
+#define AG_TOKEN_KEPT_ROW_FLOATS 8
 long long ag_token_policy_loss_workspace_bytes(long long R, int V);
 int ag_token_policy_loss(const ag_token_loss_args* args, void* stream);
-/* x *= *scale_dev * *unit_dev (NULL: 1) in place over n elements; a factor of exactly 1 touches nothing (the gradient of a loss that is
- * the graph's root) */
-int ag_scale_by(void* x_dev, long long n, int dtype, const float* scale_dev, const float* unit_dev, void* stream);
+/* x *= *scale_dev in place over n elements; a factor of exactly 1 touches nothing (the gradient of a loss that is the graph's root) */
+int ag_scale_by(void* x_dev, long long n, int dtype, const float* scale_dev, void* stream);
+/* x_dev [R, V], the kept logits of a loss with kept_rows_dev (dtype AG_F16), becomes their gradient times *scale_dev, rounded once; zero in the
+ * rows that did not count */
+int ag_token_policy_grad(void* x_dev, const float* kept_rows_dev, long long R, int V, int dtype, const float* scale_dev, void* stream);
 /* log-probability of each row's action and the row's entropy: logp_dev, entropy_dev f32 [R] (entropy NULL: not written) */
 int ag_token_logp(const void* logits_dev, long long R0, long long R1, long long s0, long long s1, int V, int dtype,
                   const long long* actions_dev, float* logp_dev, float* entropy_dev, void* stream);
