@@ -90,13 +90,13 @@ class A2CPlayer:
 
     @torch.no_grad()
     def get_action(self, obs, is_deterministic=True, dones=None):
-        """dones [num_actors]: envs whose episode ended with the previous step (a policy with a memory forgets them; None: all of them,
-        the first step after a reset)."""
+        """dones [num_actors]: envs whose episode ended with the previous step, all of them after a reset of the envs: a policy with a
+        memory forgets those before this step (None: none)."""
         memory = None
         if self.memory_state is not None:
-            if dones is None:
-                dones = torch.ones(self.num_actors, dtype=torch.uint8, device=self.device)
-            memory = {"state": self.memory_state, "resets": dones if dones.dtype in (torch.bool, torch.uint8) else dones != 0}
+            if dones is not None and dones.dtype not in (torch.bool, torch.uint8):
+                dones = dones != 0
+            memory = {"state": self.memory_state, "resets": dones}
         res = self.model({"is_train": False, "prev_actions": None, "obs": obs, "memory": memory})
         action = res["mus"] if is_deterministic else res["actions"]
         if self.clip_actions:
@@ -111,7 +111,7 @@ class A2CPlayer:
         steps = torch.zeros(n, device=self.device)
         acc = torch.zeros(3, dtype=torch.float64, device=self.device)      # games, sum reward, sum steps
         games_played, sum_rewards, sum_steps = 0, 0.0, 0.0
-        done = None
+        done = torch.ones(n, dtype=torch.uint8, device=self.device)      # the envs were reset: nothing of an earlier run is remembered
         for it in range(self.max_steps):
             action = self.get_action(obs, self.is_deterministic, done)
             obs, r, done, info = self.env.step(action)

@@ -7,7 +7,7 @@ lib/model/base_model.py:5-35).
                 157-161) -> MLP -> heads
   memory     :  `network.memory` {units, states, taps} puts a selective state space layer (lib/network/ssm.py) between the normaliser
                 and the MLP of a vector-observation policy: obs -> RunningMeanStd -> SelectiveMemory -> MLP -> heads.  Calls then carry
-                `memory` = {state, resets}: one step (resets [N]; the state moves on in place) or sequences (resets [rows, steps],
+                `memory` = {state, resets}: one step (resets [N] or None; the state moves on in place) or sequences (resets [rows, steps],
                 obs env-major)
   heads      :  mu Linear (x0.1 init), value_head Linear (x0.1 init), logstd parameter (init 0)
 
@@ -175,11 +175,11 @@ class ModelA2CContinuousLogStd(nn.Module):
         return super()._apply(fn, *a, **k)
 
     def _remember(self, x, memory):
-        """x [M, D] through the memory layer: one step of M envs (resets [M]) or whole sequences, env-major (resets [rows, steps])."""
+        """x [M, D] through the memory layer: one step of M envs (resets [M] or None) or whole sequences, env-major (resets [rows, steps])."""
         if memory is None:
             raise ValueError("this policy has a memory: call it with memory = {'state', 'resets'}")
         resets = memory["resets"]
-        if resets.dim() == 1:
+        if resets is None or resets.dim() == 1:
             return self.memory.step(x, memory["state"], resets)
         return self.memory(x.view(*resets.shape, -1), memory["state"], resets).reshape(x.shape)
 

@@ -1,0 +1,65 @@
+"""When a policy's memory is kept and when it is cleared: the player's calls, checkpoints.  CPU."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import _stub_env
+from airgym_amd.lib.agent.a2c_continuous import A2CAgent
+from airgym_amd.lib.agent.players import A2CPlayer
+
+_stub_env.register()
+
+
+def params(**kw):
+    p = _stub_env.ppo_params(**kw)
+    p["network"]["memory"] = {"units": 24, "states": 5, "taps": 3}
+    p["config"]["player"] = {"games_num": 10 ** 6, "max_steps": 9, "print_stats": False}
+    return p
+
+
+def test_player_s_plain_call_remembers():
+    """get_action(obs), step after step, is the sequence; `dones` forgets the envs it names and no others."""
+    torch.manual_seed(0)
+    player = A2CPlayer(params(num_actors=6))
+    m, n = player.model, 6
+    obs = torch.randn(7, n, player.obs_shape[0])
+    resets = torch.zeros(n, 7, dtype=torch.bool)
+    resets[2, 4] = resets[5, 4] = True
+    got = []
+    for t in range(7):
+        got.append(player.get_action(obs[t], dones=resets[:, t]) if t == 4 else player.get_action(obs[t]))
+    with torch.no_grad():
+        flat = obs.transpose(0, 1).reshape(7 * n, -1)
+        mu, _, _ = m.trunk(flat, memory={"state": m.memory.initial_state(n), "resets": resets})
+    want = torch.clamp(mu, -1.0, 1.0).view(n, 7, -1)
+    # one float32 computation in two orders: 24 channels, 32 units, 7 steps
+    for t in range(7):
+        assert torch.allclose(got[t], want[:, t], rtol=0, atol=1e-5), t
+    alone = A2CPlayer(params(num_actors=6))
+    alone.model.load_state_dict(m.state_dict())
+    assert not torch.allclose(alone.get_action(obs[6]), got[6], rtol=0, atol=1e-4)
+
+
+def test_player_s_run_starts_without_a_memory_of_the_run_before():
+    torch.manual_seed(0)
+    p = params(num_actors=6)
+    player = A2CPlayer(p)
+    seen = []
+    first = player.get_action
+
+    def spy(obs, is_deterministic=True, dones=None):
+        seen.append((obs.clone(), first(obs, is_deterministic, dones)))
+        return seen[-1][1]
+
+    player.get_action = spy
+    player.run()
+    assert player.memory_state[1].abs().max() > 0
+    player.run()
+    assert len(seen) == 18
+    fresh = A2CPlayer(p)
+    fresh.model.load_state_dict(player.model.state_dict())
+    obs, action = seen[9]                   # the second run's first step
+    assert torch.allclose(fresh.get_action(obs), action, rtol=0, atol=1e-6)
