@@ -30,6 +30,7 @@ import torch.distributed as dist
 from airgym_amd.lib.core import collectives, common_losses, schedulers, torch_ext
 from airgym_amd.lib.core.datasets import PPODataset
 from airgym_amd.lib.model.a2c_continuous_logstd_model import ModelA2CContinuousLogStd
+from airgym_amd.lib.network.ssm import RolloutMemory, forget
 from airgym_amd.lib.utils import vecenv
 from airgym_amd.lib.utils.tr_helpers import DefaultRewardsShaper
 
@@ -828,7 +829,6 @@ class A2CAgent:
             "dones": batch_dict["dones"], "mu": batch_dict["mus"], "sigma": batch_dict["sigmas"],
         }
         if self.memory_state is not None:
-            from airgym_amd.lib.network.ssm import RolloutMemory
             values_dict["memory"] = RolloutMemory(self.memory_start, batch_dict["dones"], self.horizon_length)
         if self._graph_update or self._graph_generic:
             # captured minibatch graphs read fixed addresses: keep the dataset in persistent buffers (dict observations: the
@@ -1342,6 +1342,8 @@ class A2CAgent:
             self.optimizer.load_state_dict(opt, self._optimizer_layout())
         self.last_mean_rewards = weights.get("last_mean_rewards", -100500)
         self.vec_env.set_env_state(weights.get("env_state"))
+        # what a live agent remembers came from other weights, and is of other episodes than a restored env's
+        forget(getattr(self, "memory_state", None))
         self._restored_noise_counter = weights.get("rollout_noise_counter")
         fr = getattr(self, "_fused_rollout", None)
         if fr is not None and self._restored_noise_counter is not None:

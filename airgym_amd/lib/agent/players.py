@@ -11,6 +11,7 @@ import torch
 from airgym_amd.lib.agent.a2c_continuous import rescale_actions
 from airgym_amd.lib.core import torch_ext
 from airgym_amd.lib.model.a2c_continuous_logstd_model import ModelA2CContinuousLogStd
+from airgym_amd.lib.network.ssm import forget
 from airgym_amd.lib.utils import vecenv
 
 
@@ -58,6 +59,7 @@ class A2CPlayer:
         leaves the encoder at its initialisation.  Unlike the reference's bare `except:` the fallback is taken
         only for the case it was written for (encoder keys missing); any other mismatch still raises."""
         weights = checkpoint["model"]
+        forget(self.memory_state)          # it came from other weights
         try:
             self.model.load_state_dict(weights)
             return

@@ -75,6 +75,12 @@ class SelectiveMemory(nn.Module):
         return torch.addmm(x, y, self.out_proj.weight.t())
 
 
+def forget(state):
+    """Clears a state (initial_state) where it lies; None: nothing to clear."""
+    for t in state or ():
+        t.zero_()
+
+
 class RolloutMemory:
     """What the update needs of a rollout's memory, per minibatch: slicing the flattened batch (env-major, whole sequences) gives the
     state each of its sequences started from and where episodes ended inside."""

@@ -2,7 +2,6 @@
 import os
 import sys
 
-import pytest
 import torch
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
@@ -63,3 +62,32 @@ def test_player_s_run_starts_without_a_memory_of_the_run_before():
     fresh.model.load_state_dict(player.model.state_dict())
     obs, action = seen[9]                   # the second run's first step
     assert torch.allclose(fresh.get_action(obs), action, rtol=0, atol=1e-6)
+
+
+def _trained(tmp_path, **kw):
+    torch.manual_seed(1)
+    agent = A2CAgent("run", params(num_actors=16, horizon=8, **kw))
+    agent.init_tensors()
+    agent.obs = agent.env_reset()
+    agent.play_steps()
+    fn = str(tmp_path / "ck")
+    agent.save(fn)
+    return agent, fn if os.path.exists(fn) else fn + ".pth"
+
+
+def test_a_restore_into_a_live_agent_does_not_keep_another_policy_s_memory(tmp_path):
+    """The envs go on with their own episodes; what was remembered of them came from the weights that are gone."""
+    _, fn = _trained(tmp_path)
+    live = A2CAgent("run", params(num_actors=16, horizon=8))
+    live.init_tensors()
+    live.obs = live.env_reset()
+    live.play_steps()
+    places = [t.data_ptr() for t in live.memory_state]
+    assert live.memory_state[1].abs().max() > 0
+    live.restore(fn)
+    assert not any(t.any() for t in live.memory_state)
+    assert [t.data_ptr() for t in live.memory_state] == places          # captured rollouts read them there
+    player = A2CPlayer(params(num_actors=16))
+    player.get_action(torch.randn(16, player.obs_shape[0]))
+    player.restore(fn)
+    assert not any(t.any() for t in player.memory_state)
