@@ -101,6 +101,15 @@ def wants_gradient(*tensors):
     return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
+def nothing(x, *inputs):
+    """An empty output like x, which has no elements; all of the inputs that want a gradient get one of zero."""
+    y = x.new_empty(x.shape)
+    for t in (x, *inputs):
+        if wants_gradient(t):
+            y = y + t.sum().to(y.dtype)
+    return y
+
+
 def no_gradient(what, *tensors):
     if wants_gradient(*tensors):
         raise ValueError(f"{what} has no backward pass: call it under torch.no_grad(), or the sequence form to train")

@@ -1,0 +1,34 @@
+"""The sequence operators at the edges of their arguments: empty batches under autograd."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("B,T,D", [(0, 5, 8), (2, 0, 8), (0, 0, 8), (2, 3, 0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_an_empty_batch_has_gradients_of_zero(B, T, D, dtype):
+    """A step of training on nothing moves nothing - and does not stop the program, whichever of the inputs is trained."""
+    from airgym_amd.lib.network.causal_conv import causal_conv
+    from airgym_amd.lib.network.selective_scan import selective_scan
+
+    def leaf(*shape, t=torch.float32):
+        return torch.randn(*shape, device="cuda").to(t).requires_grad_()
+
+    x, w, b, s = leaf(B, T, D, t=dtype), leaf(D, 4), leaf(D), leaf(B, 3, D, t=dtype)
+    for trained in ([w, b], [x, w, b, s], [x], [s]):
+        args = [t if any(t is v for v in trained) else t.detach() for t in (x, w, b, s)]
+        y, last = causal_conv(*args[:3], initial_state=args[3], return_state=True)
+        assert y.shape == (B, T, D) and y.dtype == dtype and torch.equal(last, args[3]) and y.requires_grad
+        for g in torch.autograd.grad(y.sum(), trained):
+            assert not g.any()
+    u, dl, z, A, Bm, C, Dk, bias, h = (leaf(B, T, D, t=dtype), leaf(B, T, D, t=dtype), leaf(B, T, D, t=dtype), leaf(D, 16), leaf(B, T, 16, t=dtype),
+                                       leaf(B, T, 16, t=dtype), leaf(D), leaf(D), leaf(B, D, 16))
+    for trained in ([A, Dk, bias], [u, dl, A, Bm, C, Dk, z, bias, h], [dl], [h]):
+        a = [t if any(t is v for v in trained) else t.detach() for t in (u, dl, A, Bm, C, Dk, z, bias, h)]
+        y, last = selective_scan(*a[:-1], initial_state=a[-1], return_state=True)
+        assert y.shape == (B, T, D) and y.dtype == dtype and torch.equal(last, a[-1]) and y.requires_grad
+        for g in torch.autograd.grad(y.sum(), trained):
+            assert not g.any()
+    with torch.no_grad():
+        assert not causal_conv(x, w, b).requires_grad and not selective_scan(u, dl, A, Bm, C).requires_grad
