@@ -82,6 +82,9 @@ __device__ __forceinline__ float expm1_near(float x) {
     return __builtin_fabsf(x) < 0.35f ? __builtin_fmaf(p * x, x, x) : exp_near(x) - 1.0f;
 }
 
+// a x, and 0 where a is 0 and x beyond the type: an advantage or a coefficient of exactly zero takes its term out (NaN stays)
+template <typename F> __device__ __forceinline__ F times(F a, F x) { return a == 0 && __builtin_isinf(x) ? (F)0 : a * x; }
+
 struct Sums { float m, s, t; };        // with y = (x - m) log2(e), m the maximum: m, sum 2^y, sum 2^y y
 
 // (x - m first: with y as one FMA, x log2(e) - c, the rounding of c would be all of y where every logit of a row is a mask's -1e30)
@@ -115,9 +118,9 @@ __device__ __forceinline__ Row finish_row(const LossArgs& a, Sums v, float xa, l
     r.f = r.k = r.ent = 0.0f;
     if (a.logp) return r;
     const float adv = a.adv[row], ratio = exp_near(r.lp - a.old_logp[row]);
-    const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = -adv * ratio;
+    const float held = -adv * fminf(fmaxf(ratio, 1.0f - a.e_clip), 1.0f + a.e_clip), plain = times(-adv, ratio);
     float f = plain >= held || plain != plain ? plain : 0.0f;
-    if (a.ref_logp) f -= a.kl_coef * expm1_near(a.ref_logp[row] - r.lp);
+    if (a.ref_logp && a.kl_coef != 0.0f) f -= a.kl_coef * expm1_near(a.ref_logp[row] - r.lp);
     const float n = share_of(a);
     r.f = f * n;
     r.ent = a.entropy_coef * n * kLn2;
@@ -361,6 +364,9 @@ __global__ __launch_bounds__(1024) void count_kernel(const unsigned char* mask, 
 // thread: three double functions a row are work for all lanes here, and would stall a workgroup per row up there.
 constexpr int kStatsThreads = 256, kStatsBlocks = 1024, kOneStage = 512, kOneStageRows = 1024;
 
+// e^x - 1 - x from e^x - 1, infinite at both ends
+__device__ __forceinline__ double beyond(double em1, double x) { return em1 == __builtin_inf() ? em1 : em1 - x; }
+
 __device__ __forceinline__ void add_row(const LossArgs& a, long long row, double* s) {
     if (a.mask && !a.mask[row]) return;
     const float4 v = a.rows[row];
@@ -369,14 +375,14 @@ __device__ __forceinline__ void add_row(const LossArgs& a, long long row, double
     const double mean = (double)v.w / v.z * ln2, logS = log((double)v.z) - tilt * mean;
     const double lp = ((double)v.x - v.y) - logS, adv = a.adv[row], moved = lp - a.old_logp[row], up = expm1(moved);
     const double ratio = 1.0 + up, low = 1.0 - (double)a.e_clip, high = 1.0 + (double)a.e_clip;
-    const double held = -adv * fmin(fmax(ratio, low), high), plain = -adv * ratio;
+    const double held = -adv * fmin(fmax(ratio, low), high), plain = times(-adv, ratio);
     s[0] += plain != plain ? plain : fmax(plain, held);
     if (a.ref_logp) {
         const double d = a.ref_logp[row] - lp;
-        s[1] += expm1(d) - d;
+        s[1] += beyond(expm1(d), d);
     }
     s[2] += logS - mean;
-    s[3] += up - moved;
+    s[3] += beyond(up, moved);
     s[4] += ratio < low || ratio > high ? 1.0 : 0.0;
 }
 
@@ -419,7 +425,7 @@ __global__ __launch_bounds__(kOneStage) void stats_kernel(LossArgs a, const doub
     if (threadIdx.x == 0) {
 #pragma unroll
         for (int k = 0; k < kSums; k++) s[k] /= a.count ? (double)a.count[0] : (double)a.R, stats[k] = (float)s[k];
-        loss[0] = (float)(s[0] + (double)a.kl_coef * s[1] - (double)a.entropy_coef * s[2]);
+        loss[0] = (float)(s[0] + times((double)a.kl_coef, s[1]) - (double)a.entropy_coef * s[2]);
         stats[kSums] = a.count ? a.count[1] : (float)a.R;
     }
 }

@@ -105,8 +105,9 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logp=None, mask=No
     [policy loss, KL term, entropy, KL of the old policy, fraction of clipped rows, rows counted], each a mean over the rows counted.
 
     Rows that do not count are not read: whatever their logits, actions and numbers are, they add nothing and get a gradient of zero.
-    If no row counts, loss, statistics and gradients are zero.  Logits of -inf are choices that are not available.  An action outside
-    [0, V) in a row that counts gives NaN."""
+    If no row counts, loss, statistics and gradients are zero.  Logits of -inf are choices that are not available; a row that counts and
+    has no other, or an action outside [0, V), gives NaN.  A kl_coef or an advantage of exactly zero takes its term out of loss and
+    gradient, also where the term is infinite."""
     logits, lead, actions = _rows(logits, actions)
     dev = logits.device
     old_logp, advantages = _per_row("old_logp", old_logp, lead, dev), _per_row("advantages", advantages, lead, dev)
@@ -126,7 +127,7 @@ def policy_loss(logits, actions, old_logp, advantages, *, ref_logp=None, mask=No
 
 def action_logp(logits, actions):
     """log softmax(logits)[action] and the entropy of every row, float32 [...]: what a rollout stores as old_logp and what a reference
-    policy's logits give as ref_logp.  No gradients.  An action outside [0, V) gives NaN."""
+    policy's logits give as ref_logp.  No gradients.  An action outside [0, V) and a row of nothing but -inf give NaN."""
     if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
         raise ValueError("action_logp has no backward pass: detach the logits (policy_loss trains)")
     logits, lead, actions = _rows(logits, actions)

@@ -899,7 +899,8 @@ int ag_selective_scan_step(const ag_scan_args* args, void* stream);
  *   row loss = max(-A r, -A clip(r, 1 - e_clip, 1 + e_clip)) + kl_coef (exp(d) - d - 1) - entropy_coef H
  * averaged over the rows with mask != 0 (mask NULL: all; none: loss 0, gradients 0).  Rows that do not count are neither read nor
  * checked; their gradient is zero.  An action outside [0, V) in a row that counts makes that row's results NaN.
- * Logits of -inf are choices that are not available: probability 0, gradient 0.
+ * Logits of -inf are choices that are not available: probability 0, gradient 0; a row that counts and has no other gives NaN.
+ * kl_coef = 0 and an advantage of 0 take their terms out of loss and gradient, also where these are infinite.
  *   loss_dev [1]; stats_dev [6] = {policy loss, KL term, entropy, KL of the old policy to this one (r - 1 - log r), fraction of rows
  *       whose r left the clip range, rows counted}
  *   dlogits_dev [R, V] contiguous in the logits' type, or NULL.  With kept_rows_dev (float16 only) it gets the logits of the rows that count

@@ -1,4 +1,4 @@
-"""The sequence operators at the edges of their arguments: empty batches under autograd."""
+"""The sequence operators at the edges of their arguments: empty batches under autograd, factors of exactly zero beside terms that overflow."""
 import pytest
 import torch
 
@@ -32,3 +32,28 @@ def test_an_empty_batch_has_gradients_of_zero(B, T, D, dtype):
             assert not g.any()
     with torch.no_grad():
         assert not causal_conv(x, w, b).requires_grad and not selective_scan(u, dl, A, Bm, C).requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V", [9, 1000])
+def test_a_factor_of_zero_beside_a_term_that_overflows(V, dtype):
+    """ref_logp for the statistics alone (kl_coef = 0) far from the policy, an advantage of zero beside a ratio beyond float32: both add nothing
+    to loss and gradient."""
+    from airgym_amd.lib.core.policy_loss import policy_loss
+    g = torch.Generator("cuda").manual_seed(V)
+    logits = torch.randn(5, V, generator=g, device="cuda").to(dtype)
+    actions = torch.randint(0, V, (5,), generator=g, device="cuda")
+    lp = torch.log_softmax(logits.double(), 1).gather(1, actions[:, None])[:, 0].float()
+    adv = torch.tensor([1.0, -1.0, 0.0, 0.5, 0.0], device="cuda")
+    old, refl = lp.clone(), lp.clone()
+    refl[0], refl[3] = 100.0, float("inf")
+    plain = logits.clone().requires_grad_()
+    want, _ = policy_loss(plain, actions, old, adv, entropy_coef=0.01)
+    (gw,) = torch.autograd.grad(want, plain)
+    old[2], old[4] = lp[2] - 100.0, -float("inf")
+    leaf = logits.clone().requires_grad_()
+    loss, stats = policy_loss(leaf, actions, old, adv, ref_logp=refl, entropy_coef=0.01)
+    (got,) = torch.autograd.grad(loss, leaf)
+    # (the ratio of an advantage of zero is of no consequence: the same sums, the same bits)
+    assert torch.equal(loss, want) and torch.equal(got, gw)
+    assert torch.isinf(stats[1]) and torch.isinf(stats[3])                # what they are
