@@ -154,3 +154,66 @@ def test_half_precision_of_few_rows(R, V):
     (grad,) = torch.autograd.grad(loss, leaf)
     within("dlogits", grad, want["grad"], room_of(want["grad"], want["mag"], want["n"], grad.dtype))
     assert not grad[~want["on"]].any()
+
+
+# ------------------------------------------------------------------------------------------------ every form, element by element
+# rows of 1 to 32 lanes, of one wave, 256 and 1024 threads, and (from 256 KB on) longer than registers hold; a wave's and a pass's elements there
+FORMS = {"f32": [1, 2, 5, 21, 64, 129, 200, 256, 257, 300, 1000, 1500, 2049, 4099, 8193, 9001, 16385, 33001, 65536, 65537, 66001, 70001],
+         "bf16": [3, 129, 257, 1000, 2500, 4099, 16385, 33001, 65537, 131072, 131080, 140003],
+         "f16": [3, 129, 257, 1000, 2500, 4099, 16385, 33001, 65537, 131072, 131080, 140003]}
+HOLES = {"f32": (256, 4096), "bf16": (512, 8192), "f16": (512, 8192)}
+
+
+def check_all(logits, actions, old, adv, refl, mask, factor=None):
+    from airgym_amd.lib.core.policy_loss import action_logp
+    want = formula(logits, actions, old, adv, refl, mask)
+    n, size = want["n"], want["size"]
+    loss, stats, grad = call(logits, actions, old, adv, refl, mask, factor=factor)
+    within("loss", loss, want["loss"], n * U * (size[0] + KL * size[1] + ENT * size[2]) + U * want["loss"].abs())
+    for k in range(5):
+        within(f"statistic {k}", stats[k], want["stats"][k], n * U * size[k] + U * want["stats"][k].abs())
+    assert float(stats[5]) == float(want["stats"][5])
+    f = 1.0 if factor is None else factor
+    room = room_of(want["grad"], want["mag"], n, grad.dtype, f)
+    if factor is not None and grad.dtype != torch.float16:              # rounded before the factor is known, and after
+        room = room + (U if grad.dtype == torch.float32 else torch.finfo(grad.dtype).eps / 2) * (want["grad"] * f).abs()
+    within("dlogits", grad, want["grad"] * f, room)
+    assert not grad[~want["on"]].any()
+    on = want["on"]
+    lp, H = action_logp(logits[on], actions[on])
+    within("logp", lp, want["lp"][on], n * U * torch.ones_like(want["lp"][on]))
+    within("entropy", H, want["H"][on], n * U * (1 + want["Y"] + want["H"][on]))
+    return want, room, f
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype,V", [(d, v) for d, vs in FORMS.items() for v in vs])
+def test_loss_statistics_and_gradient(dtype, V, masked):
+    args = rows(7, V, DTYPES[dtype], masked)
+    want, room, f = check_all(*args)
+    if dtype == "f16":
+        # Without a loss scale the type itself cannot tell: an entropy term ent p (|log p| + H) / rows of the longest rows is about
+        # 0.01 x 20 / (140003 x 7) = 2e-7, and the numbers there are 6e-8 apart.
+        want, room, f = check_all(*args, factor=2.0 ** 15)
+    if V > 2:                           # the bound is narrow enough to miss neither small term
+        for gone in (dict(ent=0.0), dict(kl=0.0)):
+            other = formula(*args, **gone)["grad"]
+            outside = ((other - want["grad"]).abs() * f > room)[want["on"]]
+            few = dtype != "f32" and "kl" in gone
+            assert float(outside.float().mean()) > (0.0 if few else 0.3), (gone, float(outside.float().mean()))
+
+
+@pytest.mark.parametrize("where", ["some", "first wave", "first pass", "last pass", "all but one end"])
+@pytest.mark.parametrize("dtype,V", [(d, v) for d, vs in FORMS.items() for v in vs if v > 8000])
+def test_long_rows_with_choices_that_are_not_available(dtype, V, where):
+    wave, one = HOLES[dtype]
+    last = V // one * one
+    hole = {"some": "some", "first wave": (0, wave), "first pass": (0, one), "last pass": (last - one, V), "all but one end": (0, V - 1)}[where]
+    check_all(*rows(6, V, DTYPES[dtype], masked=where == "first pass", minus_inf=hole))
+
+
+@pytest.mark.parametrize("V", [2, 21, 256, 300, 9001])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_short_rows_with_choices_that_are_not_available_and_a_factor(dtype, V):
+    for masked in (False, True):
+        check_all(*rows(40, V, DTYPES[dtype], masked, minus_inf="some"), factor=0.3)
