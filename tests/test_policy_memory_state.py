@@ -91,3 +91,47 @@ def test_a_restore_into_a_live_agent_does_not_keep_another_policy_s_memory(tmp_p
     player.get_action(torch.randn(16, player.obs_shape[0]))
     player.restore(fn)
     assert not any(t.any() for t in player.memory_state)
+
+
+def test_training_moves_every_parameter_of_the_memory():
+    torch.manual_seed(2)
+    agent = A2CAgent("run", params(num_actors=16, horizon=8, mini_epochs=2, max_epochs=2))
+    before = {k: v.detach().clone() for k, v in agent.model.named_parameters() if k.startswith("memory.")}
+    assert len(before) == 9
+    agent.train()
+    for k, v in agent.model.named_parameters():
+        if k in before:
+            assert torch.isfinite(v).all() and not torch.equal(v, before[k]), k
+
+
+def test_update_sees_a_rollout_whose_episodes_end_inside(monkeypatch):
+    """The env reports ends in the middle of the horizon; the update's sequences still give the rollout's own action means, and would not
+    without the flags."""
+    from airgym_amd.lib.network.ssm import RolloutMemory
+    torch.manual_seed(3)
+    step, calls = _stub_env.OracleVecEnv.step, [0]
+
+    def ends(self, actions):
+        obs, rew, done, info = step(self, actions)
+        calls[0] += 1
+        done = done.clone()
+        done[calls[0] % 8::8] = 1
+        return obs, rew, done, info
+
+    monkeypatch.setattr(_stub_env.OracleVecEnv, "step", ends)
+    agent = A2CAgent("run", params(num_actors=16, horizon=8))
+    agent.init_tensors()
+    agent.obs = agent.env_reset()
+    agent.model.update_stats = False
+    n = agent.batch_size
+    for _ in range(3):
+        batch = agent.play_steps()
+        memory = RolloutMemory(agent.memory_start, batch["dones"], agent.horizon_length)
+        assert int(memory.resets[:, 1:].any(1).sum()) == 14          # of 16: two end with the horizon's last step
+        with torch.no_grad():
+            for first, last in ((0, n), (n // 2, n)):
+                mu, _, _ = agent.model.trunk(batch["obses"][first:last], memory=memory[first:last])
+                assert torch.allclose(mu, batch["mus"][first:last], rtol=0, atol=1e-5)
+            memory.resets = torch.zeros_like(memory.resets)
+            mu, _, _ = agent.model.trunk(batch["obses"], memory=memory[0:n])
+            assert not torch.allclose(mu, batch["mus"], rtol=0, atol=1e-4)
