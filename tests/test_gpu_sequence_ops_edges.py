@@ -57,3 +57,46 @@ def test_a_factor_of_zero_beside_a_term_that_overflows(V, dtype):
     # (the ratio of an advantage of zero is of no consequence: the same sums, the same bits)
     assert torch.equal(loss, want) and torch.equal(got, gw)
     assert torch.isinf(stats[1]) and torch.isinf(stats[3])                # what they are
+
+
+@pytest.mark.parametrize("N", [3, 4, 8, 16, 32])
+def test_a_growing_state_of_zero_stays_zero(N):
+    """A > 0: the growth over a chunk of time is beyond float32, but nothing is there to grow before the first input (behind the last gradient)."""
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    g = torch.Generator().manual_seed(N)
+    T, D, some = 300, 5, 8
+    A = torch.full((D, N), 2.0).cuda()
+    one, Bm, C = torch.ones(2, T, D).cuda(), torch.randn(2, T, N, generator=g).cuda(), torch.randn(2, T, N, generator=g).cuda()
+    u = torch.zeros(2, T, D).cuda()
+    u[:, -some:] = torch.randn(2, some, D, generator=g).cuda()
+    late = slice(T - some, T)
+    whole, last = selective_scan(u, one, A, Bm, C, delta_softplus=False, return_state=True)
+    part, plast = selective_scan(u[:, late], one[:, late], A, Bm[:, late], C[:, late], delta_softplus=False, return_state=True)
+    assert torch.equal(whole[:, late], part) and torch.equal(last, plast) and not whole[:, :-some].any()
+    # ... and backwards in time
+    u = torch.randn(2, T, D, generator=g).cuda()
+    u[:, some:] = 0.0
+    state = torch.zeros(2, D, N).cuda()
+    dy = torch.zeros(2, T, D).cuda()
+    dy[:, :some] = torch.randn(2, some, D, generator=g).cuda()
+    early = slice(0, some)
+    lw, lp = [t.clone().requires_grad_() for t in (u, Bm, state)], [t.clone().requires_grad_() for t in (u[:, early], Bm[:, early], state)]
+    gw = torch.autograd.grad(selective_scan(lw[0], one, A, lw[1], C, initial_state=lw[2], delta_softplus=False), lw, dy)
+    gp = torch.autograd.grad(selective_scan(lp[0], one[:, early], A, lp[1], C[:, early], initial_state=lp[2], delta_softplus=False), lp, dy[:, early])
+    assert torch.equal(gw[2], gp[2]) and torch.equal(gw[0][:, early], gp[0]) and not gw[0][:, some:].any()
+
+
+@pytest.mark.parametrize("T", [6, 150])
+def test_lengths_outside_the_sequence_are_its_ends(T):
+    from airgym_amd.lib.network.causal_conv import causal_conv
+    from airgym_amd.lib.network.selective_scan import selective_scan
+    g = torch.Generator().manual_seed(T)
+    x, dy = torch.randn(3, T, 24, generator=g).cuda().requires_grad_(), torch.randn(3, T, 24, generator=g).cuda()
+    w, A, bc = torch.randn(24, 4, generator=g).cuda(), -torch.rand(24, 16, generator=g).cuda(), torch.randn(3, T, 16, generator=g).cuda()
+    got = []
+    for ln in ([2 ** 31 - 1, -5, T + 1], [T, 0, T]):
+        ln = torch.tensor(ln, dtype=torch.int32, device="cuda")
+        y, last = causal_conv(x, w, lengths=ln, return_state=True)
+        z, h = selective_scan(x, x, A, bc, bc, lengths=ln, return_state=True)
+        got.append([y, last, z, h, torch.autograd.grad(y, x, dy)[0], torch.autograd.grad(z, x, dy)[0]])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
