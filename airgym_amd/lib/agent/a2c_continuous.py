@@ -513,10 +513,11 @@ class A2CAgent:
     def compute_paths(self):
         """{'rollout': ..., 'update': {layer: {forward, dW / backward, dX}}} - what runs for this network / config."""
         fr, fs = self._fused_rollout, self._fused_step
+        cuda = str(self.ppo_device).startswith("cuda")
         if fr is None:
             rollout = "generic: model forward (torch) + env.step per rollout step"
             if self.model.has_memory:
-                rollout += "; memory: ag_causal_conv_step + ag_selective_scan_step"
+                rollout += "; memory: " + ("ag_causal_conv_step + ag_selective_scan_step" if cuda else "torch, step by step")
         elif fr.chain is not None:
             rollout = ("ag_mlp_chain_forward (whole policy forward, one launch, activations in registers) + "
                        + ("ag_step_rollout_fused" if fr.fuse_tail else "ag_policy_sample + ag_step_rollout + ag_rollout_account"))
@@ -527,11 +528,11 @@ class A2CAgent:
         if fs is None:
             update = "generic: autograd (torch) + fused PPO loss kernel where supported"
             if self.model.has_memory:
-                update += "; memory: ag_causal_conv_fwd / _bwd + ag_selective_scan_fwd / _bwd"
+                update += "; memory: " + ("ag_causal_conv_fwd / _bwd + ag_selective_scan_fwd / _bwd" if cuda else "torch, step by step")
         else:
             update = fs.describe_paths()
         return {"rollout_step": rollout, "update": update,
-                "optimizer": "ag_adam_clip_step (HIP)" if self.config.get("use_fused_adam", True) and str(self.ppo_device).startswith("cuda")
+                "optimizer": "ag_adam_clip_step (HIP)" if self.config.get("use_fused_adam", True) and cuda
                 else "FlatAdam (torch)",
                 "minibatch_hip_graphs": bool(getattr(self, "_graph_update", False) or getattr(self, "_graph_generic", False))}
 

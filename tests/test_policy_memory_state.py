@@ -135,3 +135,9 @@ def test_update_sees_a_rollout_whose_episodes_end_inside(monkeypatch):
             memory.resets = torch.zeros_like(memory.resets)
             mu, _, _ = agent.model.trunk(batch["obses"], memory=memory[0:n])
             assert not torch.allclose(mu, batch["mus"], rtol=0, atol=1e-4)
+
+
+def test_paths_on_the_cpu_name_no_kernels():
+    paths = A2CAgent("run", params(num_actors=8, horizon=4)).compute_paths()
+    assert "memory: torch" in paths["rollout_step"] and "memory: torch" in paths["update"]
+    assert not any("ag_" in v for v in (paths["rollout_step"], paths["update"], paths["optimizer"]))
