@@ -138,6 +138,8 @@ def test_update_sees_a_rollout_whose_episodes_end_inside(monkeypatch):
 
 
 def test_paths_on_the_cpu_name_no_kernels():
-    paths = A2CAgent("run", params(num_actors=8, horizon=4)).compute_paths()
+    agent = A2CAgent("run", params(num_actors=8, horizon=4))
+    agent.init_tensors()
+    paths = agent.compute_paths()
     assert "memory: torch" in paths["rollout_step"] and "memory: torch" in paths["update"]
     assert not any("ag_" in v for v in (paths["rollout_step"], paths["update"], paths["optimizer"]))
