@@ -423,7 +423,9 @@ extern "C" int ag_causal_conv_step(const void* x, long long x_sb, void* state, c
     // 5.16 us at 4096 x 256): the weights of a thread's channels are that many more gathered loads in front of the arithmetic.
     const int vec = dtype != AG_F32 && D % 2 == 0 ? 2 : 1;
     const unsigned blocks = (unsigned)(((long long)B * (D / vec) + kThreads - 1) / kThreads);
-    // 402 MB of states (16384 x 2048, W = 4, bfloat16): 134 us plain, 114 us as used once; 50 MB (8192 x 512, float32): 20.6 and 23.1 us
+    // From half of the last-level cache on the states are marked as used once: plain and marked, in us, one batch moved on alone and three in turn,
+    // at D = 2048, W = 4: float32 48 MiB 20.3, 23.1 and 20.2, 23.3; 127 MiB 49.6, 55.7 and 58.8, 55.7; 384 MiB 178, 162 and 178, 166; bfloat16 48 MiB
+    // 23.3, 25.3 and 23.2, 25.6; 192 MiB 101, 88 and 103, 88.  (Between 60 and 128 MiB three in turn gain as well, one alone loses.)
     const bool once = (long long)B * D * (W_ - 1) * (dtype == AG_F32 ? 4 : 2) >= kCached;
 #define AG_STEP(VEC, ONCE)                                                                                                         \
     AG_FOR_DTYPE(dtype, AG_FOR_TAPS(W_, hipLaunchKernelGGL((conv_step_kernel<T, W, VEC, ONCE>), dim3(blocks), dim3(kThreads), 0,     \

@@ -7,8 +7,8 @@
 // Read once, write once: a row is held in registers, 16 bytes per access, between the sums and the gradient - by 1 to 64 lanes of a
 // wave (short rows), by a workgroup of 256 or 1024 threads, or, beyond what registers hold, read a second time from the cache.
 // Every wave sums against a maximum of its own and the waves' results are joined.  Memory bounds it in float32: 8192 x 32000 with the
-// gradient takes 365 us = 5.7 TB/s, the log-probabilities alone 172 us = 6.1 TB/s.  In the 16-bit types the two exponentials and some 15
-// other instructions per element bound it as much: 8192 x 32000 bfloat16 takes 224 us = 4.7 TB/s, the vector pipe busy for 85 % of it.
+// gradient takes 360 us = 5.8 TB/s, the log-probabilities alone 177 us = 5.9 TB/s.  In the 16-bit types the two exponentials and some 15
+// other instructions per element bound it as much: 8192 x 32000 bfloat16 takes 218 us = 4.8 TB/s, the vector pipe busy for 81 % of it.
 // float16 logits under autograd are the exception: a row's factors span more than their type does - a mean over many rows is below 6e-8 where
 // a single row's ratio may be above 65504 -, so that their gradient cannot be rounded before what the loss is scaled by is known.  The
 // forward leaves a copy of the logits and each row's factors, the backward forms the gradient in the copy's place, rounded once.
@@ -450,7 +450,7 @@ __global__ __launch_bounds__(256) void scale_kernel(T* x, long long n, const flo
 }
 
 // The gradient of kept logits, in their place, times the loss's factor: rounded once.  A thread takes 16 bytes at a time wherever the rows'
-// borders lie, and moves on by a fixed number of rows and columns, so that it divides once.  Its bytes bound it.
+// borders lie, and moves on by a fixed number of rows and columns, so that it divides once.  Its bytes bound it: 8191 x 32000 takes 195 us = 5.4 TB/s.
 __global__ __launch_bounds__(256) void kept_grad_kernel(f16_t* x, const KeptRow* rows, long long n, int V, const float* scale) {
     constexpr int E = 16 / sizeof(f16_t);
     const float g = scale[0];

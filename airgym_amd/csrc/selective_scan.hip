@@ -774,7 +774,8 @@ template <typename T> struct ScanShared {
 // step and its gate, the L rounds over the states fetch them from there, B and C are read once for all of them, and L accesses per lane
 // are in flight.  Otherwise a wave's 64 / L channels lie anywhere.  kTail: N is above 4 and no multiple of it.
 // Bytes bound it: 4096 x 512, N = 16, float32 takes 52 us = 5.8 TB/s, bfloat16 52 us = 5.4 TB/s (an in-place product over the states
-// alone 48 us).  The states are marked as used once: with plain accesses the float32 step took 59 us, without sharing 61.
+// alone 48 us).  Large states are marked as used once (the rule and both sides stand where it is chosen); without sharing the float32 step
+// took 61 us.
 template <typename T, int L, bool kShared, bool kTail, bool kOnce>
 __global__ __launch_bounds__(256) void scan_step_kernel(ScanArgs a) {
     constexpr int kRounds = kShared ? L : 1, C = 64 / L;                  // channels of a wave per round
@@ -990,8 +991,10 @@ extern "C" int ag_selective_scan_step(const ag_scan_args* p, void* stream) {
     const bool shared = a.nb * 64LL * 4 <= a.Dg * 5LL, tail = a.N > 4 && a.N % 4;
     const long long waves = shared ? (long long)a.B * a.G * a.nb : ((long long)a.B * a.D * lanes + 63) / 64, blocks = (waves + 3) / 4;
     if (blocks > kMaxThreads / 256) return AG_ERR_UNSUPPORTED;
-    // a state of 134 MB (4096 x 512, N = 16, float32) moved on again and again: 47 us plain, 50 as used once, with 34 MB of other work between
-    // the steps 59 and 62, with 134 MB of it 54 and 51; of 268 MB 99 and 95, with 34 MB 124 and 112; of 67 MB 26.5 and 26.9
+    // From half of the last-level cache on a state is marked as used once.  One state moved on again and again, with nothing between the steps,
+    // pays for it; a state that other work has driven out (here: three batches in turn) gains.  Plain and marked, in us, at N = 16, D = 512:
+    //   float32   64 MiB 27.6, 27.6 and 27.1, 28.8    128 MiB 49.7, 52 and 63.3, 52    192 MiB 72.0, 74.5 and 90.3, 74.5    256 MiB 107, 97 and 117, 97
+    //   bfloat16  64 MiB 28.1, 25.8 and 27.6, 27.4    128 MiB 49.3, 49.8 and 60.8, 50.8    256 MiB 98, 95 and 112, 95
     const bool once = (long long)a.B * a.D * a.N * 4 >= kCached;
     const dim3 grid((unsigned)blocks), block(256);
 #define AG_STEP(SHARED, TAIL, ONCE)                                                                                              \

@@ -1,6 +1,6 @@
 // seq_common.hpp - element types and scalar functions shared by the sequence operators (causal_conv.hip, selective_scan.hip,
 // policy_loss.hip).  Activations come in float32, bfloat16 or float16; every product and sum is formed in float32 and rounded
-// once, to nearest, where a result is stored in its type.
+// once, to nearest, where a result is stored in its type (the policy loss's bfloat16 gradient a second time where the loss is scaled).
 #pragma once
 
 #include <hip/hip_runtime.h>
